@@ -336,6 +336,88 @@ int tqk_dequant_key_block(const tqk_block_desc* d, const uint8_t* packed, const 
 int tqk_dequant_value_block(const tqk_block_desc* d, const uint8_t* packed, const float* norms,
                             const float* pi, const float* vcent, float* out, void* stream);
 
+/*
+ * Projection rows of new tokens made ready for the cache: queries and keys
+ * normalised per head, rotated by position, and queries, keys and values laid
+ * out head-major in the cache's type, in one pass.  A row of qkv holds
+ * [n_q_heads | n_kv_heads | n_kv_heads] heads of head_dim channels.
+ *   x^ = x * rsqrt(mean(x^2) + eps) * (w + weight_offset)   where a weight is given
+ *   pairs (i, i + R/2), or (2i, 2i + 1) when interleaved, of the first R =
+ *   rotary_dim channels turned by position * inv_freq[i] and scaled by
+ *   rope_scale; the other channels pass, and values are converted only.
+ * Computed in fp32 (the angle in 64 bits) and rounded once to out_type.
+ * No counterpart in the reference, whose caches take rotated keys
+ * (turboquant_pro/core.py:986-1009).
+ */
+typedef struct tqk_rope_desc {
+  int32_t batch;
+  int32_t tokens;        /* tokens of every sequence */
+  int32_t n_q_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;      /* 64, 128 or 256 */
+  int32_t rotary_dim;    /* R, a multiple of 16, 0 .. head_dim */
+  int32_t interleaved;   /* 0: pairs (i, i + R/2); 1: pairs (2i, 2i + 1) */
+  int32_t in_type;       /* type of qkv: 0 fp32, 1 fp16, 2 bf16 */
+  int32_t out_type;      /* type of q, k, v: likewise */
+  int32_t weight_type;   /* type of the weights: in_type, or 0 (fp32) */
+  int32_t pos_i64;       /* positions are 0: int32, 1: int64 */
+  int32_t pos_per_token; /* positions [batch][tokens]; 0: [batch], the position of a sequence's first token */
+  int64_t batch_stride;  /* elements of qkv between sequences and between tokens (multiples of 8) */
+  int64_t token_stride;
+  float eps;
+  float weight_offset;   /* added to the weights (1 for weights stored as w - 1) */
+  float rope_scale;      /* factor of the rotated channels (1, or a length extension's) */
+} tqk_rope_desc;
+
+/*
+ * q [batch][n_q_heads][tokens][head_dim], k and v [batch][n_kv_heads][tokens]
+ * [head_dim] (the chunk layout of tqk_append_tokens), all pointers 16-byte
+ * aligned; q_weight, k_weight [head_dim] or null (no norm of that side);
+ * inv_freq [R/2] fp32.
+ */
+int tqk_norm_rope(const tqk_rope_desc* d, const void* qkv, const void* positions,
+                  const float* inv_freq, const void* q_weight, const void* k_weight, void* q,
+                  void* k, void* v, void* stream);
+
+/*
+ * Attention over dense keys and values with a sliding window and a few first
+ * tokens that stay visible.  Query t of sequence b, with m = q_lens[b] queries
+ * and n = kv_lens[b] keys, stands at p = n - m + t and sees the keys j of
+ * [start, p] (start = kv_starts[b]) with j > p - window or j < start + sinks:
+ *   out[b][i][t] = softmax(q[b][i][t] . K^T * sm_scale) V   (kv head i / (Hq / Hkv))
+ * Queries that see nothing, and rows t >= m, get zeros.  Keys and values no
+ * query sees are not read, or count for nothing whatever they hold.
+ * Scores, sums and accumulators are fp32, the weights of the value product of
+ * the inputs' type.  The prefill attention that the reference leaves to its
+ * host framework (turboquant_pro/hf_cache.py:205-214).
+ */
+typedef struct tqk_attn_desc {
+  int32_t batch;
+  int32_t n_q_heads;    /* a multiple of n_kv_heads */
+  int32_t n_kv_heads;
+  int32_t head_dim;     /* 64, 128 or 256 */
+  int32_t q_len;        /* query rows of every sequence */
+  int32_t kv_len;       /* key rows of every sequence */
+  int32_t window;       /* keys a query sees back from itself, itself included; 0: all */
+  int32_t sinks;        /* first tokens that stay visible */
+  int32_t type;         /* 1 fp16, 2 bf16: q, k, v and out */
+  float sm_scale;       /* > 0 */
+  int64_t q_stride[3];  /* elements between sequences, heads and tokens: multiples of 8 */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+} tqk_attn_desc;
+
+/* Bytes of workspace that tqk_attention needs for the current device (0: none;
+ * no initialisation, calls that share one must not overlap). */
+size_t tqk_attention_workspace_bytes(const tqk_attn_desc* d);
+
+/* kv_lens, q_lens, kv_starts [batch] i32 (device) or null (kv_len, q_len, 0 for
+ * every sequence; values outside [0, kv_len], [0, q_len] are clamped to it). */
+int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const void* v,
+                  const int32_t* kv_lens, const int32_t* q_lens, const int32_t* kv_starts, void* out,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

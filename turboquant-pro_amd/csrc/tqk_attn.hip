@@ -1,0 +1,571 @@
+// Attention over dense keys and values with a sliding window and a few first
+// tokens that stay visible (gfx950).
+//
+// Query t of a sequence with m queries and n keys stands at p = n - m + t and
+// sees the keys j of [start, p] with j > p - window or j < start + sinks:
+//   out = sum_j softmax_j(scale q . k_j) v_j
+// by one pass over the visible keys with a running maximum and sum.  A key tile
+// that no row of a workgroup sees is never read.
+//
+// tqk_attn_tiles: prompts and chunks.  The rows of one kv head are its query
+// heads' rows side by side (row = t * heads + head), 32 a wave, 128 a workgroup;
+// 64 keys at a time go through LDS.  Scores are computed transposed, K Q^T, so
+// that a lane holds one row's scores and its running maximum and sum are plain
+// registers, and the weights are already laid out as the operand of V^T P^T (the
+// order of the keys inside a product is free: both operands take the order the
+// scores come in).  V^T comes from LDS by transposing reads.
+// Bound: the matrix cores and, as closely, LDS reads (16 KiB of K and V for
+// 32 x 64 scores a wave).
+#include "tqk_common.h"
+
+namespace {
+
+typedef float f16v_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef short s8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kTileThreads = 256;
+constexpr int kRows = 32;      // rows a wave
+constexpr int kTileRows = 128; // rows a workgroup
+// keys a tile: at head_dim 256 half as many, which leaves the accumulators their registers
+template <int D>
+constexpr int kTileKeys = D == 256 ? 32 : 64;
+constexpr int kMaxKeys = 64;
+// The running maximum follows the scores only when one exceeds it by this much
+// (log2 units): weights stay at most 2^8, far inside fp16's range, and the
+// accumulators are rescaled a few times a row instead of every tile.
+constexpr float kLazy = 8.0f;
+
+struct AttnArgs {
+  tqk_attn_desc d;
+  const void* q;
+  const void* k;
+  const void* v;
+  const int32_t* kv_lens;
+  const int32_t* q_lens;
+  const int32_t* kv_starts;
+  void* out;
+  float* part_ml;   // [split][row][2]: running maximum (log2 units) and sum
+  float* part_acc;  // [split][row][D]
+  int row_tiles;    // row tiles of a (sequence, kv head)
+  int n_splits;
+  long long rows;   // rows of all sequences and heads
+  int compact;      // keys and values hold only the first tiles and those from the first visible one on
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<_Float16> {
+  typedef h8_t v8;
+  static __device__ __forceinline__ f16v_t m32(v8 a, v8 b, f16v_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f4_t m16(v8 a, v8 b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<__bf16> {
+  typedef bf8_t v8;
+  static __device__ __forceinline__ f16v_t m32(v8 a, v8 b, f16v_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f4_t m16(v8 a, v8 b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// whether a 16-bit pattern is an infinity or a NaN
+template <typename T>
+__device__ __forceinline__ bool not_finite2(uint32_t two) {
+  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+  return (two & e) == e || ((two >> 16) & e) == e;
+}
+template <typename T>
+__device__ __forceinline__ bool not_finite(u4_t x) {
+  return not_finite2<T>(x.x) || not_finite2<T>(x.y) || not_finite2<T>(x.z) || not_finite2<T>(x.w);
+}
+
+// the value of the other half-wave's lane with the same l % 32
+__device__ __forceinline__ float other_half(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? (uint32_t)r[0] : (uint32_t)r[1]);
+}
+__device__ __forceinline__ float max_half(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float sum_half(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// What a sequence's queries see.
+struct Seen {
+  int n, m, start, sink_end, window;  // window 0: none
+  __device__ __forceinline__ Seen(const AttnArgs& a, int b) {
+    n = a.kv_lens ? min(max(a.kv_lens[b], 0), a.d.kv_len) : a.d.kv_len;
+    m = a.q_lens ? min(max(a.q_lens[b], 0), a.d.q_len) : a.d.q_len;
+    start = a.kv_starts ? min(max(a.kv_starts[b], 0), n) : 0;
+    sink_end = start + min(a.d.sinks, n - start);
+    window = a.d.window > 0 && a.d.window < n ? a.d.window : 0;
+  }
+  __device__ __forceinline__ int low(int p) const { return window ? max(start, p - window + 1) : start; }
+  __device__ __forceinline__ bool sees(int p, int lo, int j) const {
+    return (j <= p) & ((j >= lo) | ((j < sink_end) & (j >= start)));
+  }
+};
+
+// The key tiles that rows at positions [p_lo, p_hi] see: a run from the first
+// visible tokens' tile, then one up to p_hi's.
+template <int kKeys>
+struct Tiles {
+  int first, n_first, second, n;
+  __device__ __forceinline__ Tiles(const Seen& s, int p_lo, int p_hi) {
+    first = s.start / kKeys;
+    if (p_hi < s.start) {  // nothing
+      n_first = n = second = 0;
+      return;
+    }
+    const int lo = max(s.low(p_lo), s.start);
+    const int sink = min(s.sink_end, p_hi + 1);  // (no row sees past itself)
+    n_first = sink > s.start ? (sink - 1) / kKeys + 1 - first : 0;
+    second = max(lo / kKeys, first + n_first);
+    n = n_first + max(0, p_hi / kKeys + 1 - second);
+  }
+  __device__ __forceinline__ int at(int i) const { return kKeys * (i < n_first ? first + i : second + i - n_first); }
+};
+
+// Rows of a compact key buffer that are left out before position j: whole tiles
+// between the first visible tokens' and the first of the sequence's window.
+__device__ __forceinline__ int compact_gap(const Seen& s) {
+  const int lo = max(s.low(s.n - s.m), 0) / kMaxKeys * kMaxKeys;
+  const int sink = (s.sink_end + kMaxKeys - 1) / kMaxKeys * kMaxKeys;
+  return max(0, lo - sink);
+}
+
+// blockIdx -> item so that consecutive items, which share keys, go to one XCD
+// (workgroups are dealt to the 8 XCDs, each with its own L2, one after another)
+__device__ __forceinline__ int xcd_item(int x, int n) {
+  const int c = x & 7, q = n >> 3, r = n & 7;
+  return c * q + min(c, r) + (x >> 3);
+}
+
+template <int D>
+struct TileGeom {
+  static constexpr int CH = D / 8;  // 16-byte chunks a row
+  // Chunk places in LDS.  K's rows are read 16 bytes a lane, 8 rows at a time
+  // from one column of chunks: the column is turned by the row, so that they
+  // fall in different banks.  V's are read 4 rows x 32 bytes at a time.
+  static __device__ __forceinline__ int k_at(int row, int c) { return (row * CH + (c ^ (row & 7))) * 16; }
+  static __device__ __forceinline__ int v_at(int row, int c) { return (row * CH + (c ^ ((row & 3) << 1))) * 16; }
+};
+
+template <int D, typename T>
+__global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles(AttnArgs a) {
+  typedef typename Mma<T>::v8 v8;
+  constexpr int kKeys = kTileKeys<D>, NU = kKeys / 32;
+  constexpr int CH = D / 8, NST = kKeys * CH / kTileThreads;  // 16-byte chunks a thread stages of K, and of V
+  constexpr int ND = D / 32, NK = D / 16;
+  constexpr int kBytes = kKeys * D * 2;
+  using TG = TileGeom<D>;
+  __shared__ __align__(16) uint8_t k_s[2][kBytes];
+  __shared__ __align__(16) uint8_t v_s[2][kBytes];
+  __shared__ int bad_s[2];  // the tile whose V holds an infinity or a NaN under a mask
+
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
+  const int Hq = a.d.n_q_heads, Hkv = a.d.n_kv_heads, gq = Hq / Hkv;
+  int item = xcd_item(blockIdx.x, gridDim.x);
+  const int split = item % a.n_splits;
+  item /= a.n_splits;
+  const int tile = a.row_tiles - 1 - item % a.row_tiles;  // the last rows, which see most, first
+  item /= a.row_tiles;
+  const int h = item % Hkv, b = item / Hkv;
+  const Seen s(a, b);
+
+  // this lane's row
+  const int row = tile * kTileRows + wave * kRows + ln;
+  const int t = row / gq, qh = h * gq + row % gq;
+  const bool inside = t < a.d.q_len, real = t < s.m;
+  const int p = s.n - s.m + t, lo = s.low(p);
+  // the positions of the workgroup's rows and of the wave's
+  const int t_lo = tile * kTileRows / gq, t_hi = min((tile * kTileRows + kTileRows - 1) / gq, s.m - 1);
+  const int w_lo = (tile * kTileRows + wave * kRows) / gq;
+  const int w_hi = min((tile * kTileRows + wave * kRows + kRows - 1) / gq, s.m - 1);
+  const int p_lo = s.n - s.m + t_lo, p_hi = s.n - s.m + t_hi;
+  const int wp_lo = s.n - s.m + w_lo, wp_hi = s.n - s.m + w_hi;
+  const int b_lo = s.low(p_lo);                           // the first key that a row of the workgroup sees by its window
+  const int wl_lo = s.low(wp_lo), wl_hi = s.low(wp_hi);   // the wave's rows' first and last window start
+
+  const Tiles<kKeys> tiles(s, p_lo, p_hi);
+  int i0 = 0, i1 = t_lo < s.m ? tiles.n : 0;
+  if (a.n_splits > 1) {
+    const int n = i1;
+    i0 = (int)((long long)n * split / a.n_splits);
+    i1 = (int)((long long)n * (split + 1) / a.n_splits);
+  }
+
+  // Q^T as the second operand: row ln, channels 16 ks + 8 lh .. + 7
+  v8 qf[NK];
+  {
+    const T* qp = static_cast<const T*>(a.q) + b * a.d.q_stride[0] + (long long)min(qh, Hq - 1) * a.d.q_stride[1] +
+                  (long long)min(t, a.d.q_len - 1) * a.d.q_stride[2] + 8 * lh;
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) qf[ks] = *reinterpret_cast<const v8*>(qp + 16 * ks);
+  }
+  const float c = a.d.sm_scale * 1.4426950408889634f;  // scores in log2 units
+
+  f16v_t O[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) O[i][r] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;  // (l_run: this lane's keys only)
+
+  // staging: thread tid takes chunks tid + 256 i of the tile, in row order
+  const long long ks_ = a.d.k_stride[2], vs_ = a.d.v_stride[2];
+  const T* const kb = static_cast<const T*>(a.k) + b * a.d.k_stride[0] + h * a.d.k_stride[1];
+  const T* const vb = static_cast<const T*>(a.v) + b * a.d.v_stride[0] + h * a.d.v_stride[1];
+  const int gap = a.compact ? compact_gap(s) : 0;
+  const int sink_rows = (s.sink_end + kMaxKeys - 1) / kMaxKeys * kMaxKeys;
+  u4_t kst[NST], vst[NST];
+  // whether every row of the workgroup sees the whole tile
+  auto whole = [&](int k0) {
+    return k0 + kKeys - 1 <= p_lo && k0 >= s.start && (k0 >= s.low(p_hi) || k0 + kKeys <= s.sink_end);
+  };
+  auto load_tile = [&](int k0) {
+    const int g = k0 >= sink_rows ? gap : 0;
+#pragma unroll
+    for (int i = 0; i < NST; ++i) {
+      const int ch = tid + kTileThreads * i, r = min(k0 + ch / CH, s.n - 1) - g, cc = ch % CH;
+      kst[i] = *reinterpret_cast<const u4_t*>(kb + r * ks_ + 8 * cc);
+      vst[i] = *reinterpret_cast<const u4_t*>(vb + r * vs_ + 8 * cc);
+    }
+  };
+  auto put_tile = [&](int buf, int i_tile, int k0) {
+    if (!whole(k0)) {
+      // values that no row of the workgroup sees count as zero, whatever they
+      // hold (a weight of zero times an infinity is no zero)
+#pragma unroll
+      for (int i = 0; i < NST; ++i) {
+        const int j = k0 + (tid + kTileThreads * i) / CH;
+        if (!s.sees(p_hi, b_lo, j)) vst[i] = u4_t{0u, 0u, 0u, 0u};
+        if (not_finite<T>(vst[i])) bad_s[buf] = i_tile;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NST; ++i) {
+      const int ch = tid + kTileThreads * i, r = ch / CH, cc = ch % CH;
+      *reinterpret_cast<u4_t*>(k_s[buf] + TG::k_at(r, cc)) = kst[i];
+      *reinterpret_cast<u4_t*>(v_s[buf] + TG::v_at(r, cc)) = vst[i];
+    }
+  };
+
+  if (tid < 2) bad_s[tid] = -1;
+  __syncthreads();
+  if (i0 < i1) {
+    load_tile(tiles.at(i0));
+    put_tile(0, i0, tiles.at(i0));
+  }
+  __syncthreads();
+  for (int it = i0; it < i1; ++it) {
+    const int buf = (it - i0) & 1, k0 = tiles.at(it);
+    if (it + 1 < i1) load_tile(tiles.at(it + 1));
+    // (a tile that none of the wave's rows sees: only its staging)
+    if (w_lo < s.m && k0 <= wp_hi && (k0 + kKeys > wl_lo || k0 < s.sink_end)) {
+      // K Q^T: keys k0 + 32 u + 8 (r / 4) + 4 lh + r % 4 of row ln
+      f16v_t S[NU];
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[u][r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+          const v8 kf = *reinterpret_cast<const v8*>(k_s[buf] + TG::k_at(32 * u + ln, 2 * ks + lh));
+          S[u] = Mma<T>::m32(kf, qf[ks], S[u]);
+        }
+      }
+      const bool masked = !(k0 + kKeys - 1 <= wp_lo && k0 >= s.start && (k0 >= wl_hi || k0 + kKeys <= s.sink_end));
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = k0 + 32 * u + 8 * (r / 4) + 4 * lh + r % 4;
+            S[u][r] = s.sees(p, lo, j) ? S[u][r] : -INFINITY;
+          }
+      }
+      float mx = S[0][0];
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[u][r]);
+      mx = max_half(mx) * c;
+      if (__any(mx > m_run + kLazy)) {
+        const float m_new = fmaxf(m_run, mx);
+        const float f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= f;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) O[i][r] *= f;
+      }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          S[u][r] = __builtin_amdgcn_exp2f(fmaf(S[u][r], c, -m_use));
+          l_run += S[u][r];
+        }
+      if (masked && __builtin_expect(bad_s[buf] == it, 0)) {
+        // An infinity or a NaN under a mask: key by key, only into the rows that
+        // see it (the products of a matrix instruction would be NaN in all).
+        float w[16 * NU];
+#pragma unroll
+        for (int r = 0; r < 16 * NU; ++r) w[r] = S[r / 16][r % 16];
+        for (int jj = 0; jj < kKeys; ++jj) {
+          const float mine = w[16 * (jj / 32) + 4 * (jj % 32 / 8) + jj % 4], far = other_half(mine);
+          const float wt = ((jj >> 2) & 1) == lh ? mine : far;
+          const bool vis = s.sees(p, lo, k0 + jj);  // (else the weight is zero)
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+              typedef T v4 __attribute__((ext_vector_type(4)));
+              const int dd = 32 * i + 2 * r + 4 * lh;
+              const v4 x = *reinterpret_cast<const v4*>(v_s[buf] + TG::v_at(jj, dd / 8) + 8 * lh);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) O[i][r + e] = fmaf(wt, vis ? (float)x[e] : 0.f, O[i][r + e]);
+              __builtin_amdgcn_sched_barrier(0);  // (no registers for reads ahead on this path)
+            }
+        }
+      } else {
+        // V^T P^T, 16 keys a product; the weights rounded to the inputs' type
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            v8 pf;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pf[e] = (T)S[u][8 * g + e];
+            // the lane's part of a transposing read: row ln % 16 / 4 of four, channels 4 (ln % 4)
+            const int r0 = 32 * u + 16 * g + 4 * lh + (ln % 16) / 4;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+              const int cc = 4 * i + 2 * (ln / 16) + (ln % 4) / 2;
+              typedef __attribute__((address_space(3))) s4_t* lds4;
+              const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds4)(v_s[buf] + TG::v_at(r0, cc) + 8 * (ln % 2)));
+              const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds4)(v_s[buf] + TG::v_at(r0 + 8, cc) + 8 * (ln % 2)));
+              const s8_t xy = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+              O[i] = Mma<T>::m32(__builtin_bit_cast(v8, xy), pf, O[i]);
+            }
+          }
+      }
+    }
+    if (it + 1 < i1) put_tile(buf ^ 1, it + 1, tiles.at(it + 1));
+    __syncthreads();
+  }
+
+  const float l = sum_half(l_run);
+  if (!inside) return;
+  if (a.n_splits == 1) {
+    // rows that see nothing, and those past the sequence's queries: zero
+    const float inv = real && l != 0.f ? 1.0f / l : 0.f;
+    const bool dead = !real || l == 0.f;
+    T* op = static_cast<T*>(a.out) + b * a.d.o_stride[0] + (long long)qh * a.d.o_stride[1] +
+            (long long)t * a.d.o_stride[2] + 4 * lh;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        v4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(dead ? 0.f : O[i][r + e] * inv);
+        *reinterpret_cast<v4*>(op + 32 * i + 2 * r) = y;
+      }
+  } else {
+    const long long at = (long long)split * a.rows + ((long long)b * Hq + qh) * a.d.q_len + t;
+    if (lh == 0) {
+      a.part_ml[2 * at] = m_run;
+      a.part_ml[2 * at + 1] = real ? l : 0.f;
+    }
+    float* op = a.part_acc + at * D + 4 * lh;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<float4*>(op + 32 * i + 2 * r) = make_float4(O[i][r], O[i][r + 1], O[i][r + 2], O[i][r + 3]);
+  }
+}
+
+// The splits of a row joined: one wave a row, D / 64 channels a lane.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void tqk_attn_join(AttnArgs a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  float M = -INFINITY;
+  for (int s = 0; s < a.n_splits; ++s) {
+    const long long at = s * a.rows + row;
+    if (a.part_ml[2 * at + 1] != 0.f) M = fmaxf(M, a.part_ml[2 * at]);
+  }
+  float l = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s = 0; s < a.n_splits; ++s) {
+    const long long at = s * a.rows + row;
+    const float ls = a.part_ml[2 * at + 1];
+    if (ls == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - M);
+    l = fmaf(ls, f, l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(a.part_acc[at * D + E * lane + e], f, acc[e]);
+  }
+  const int t = (int)(row % a.d.q_len);
+  const long long bh = row / a.d.q_len;
+  T* op = static_cast<T*>(a.out) + bh / a.d.n_q_heads * a.d.o_stride[0] + bh % a.d.n_q_heads * a.d.o_stride[1] +
+          t * a.d.o_stride[2] + E * lane;
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) op[e] = (T)(l != 0.f ? acc[e] * inv : 0.f);
+}
+
+int device_cus() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+  return n;
+}
+
+struct AttnPlan {
+  int row_tiles, n_splits;
+  long long rows, items;
+  size_t ws_bytes;
+};
+
+// Most key tiles that a row tile reads.
+long long most_tiles(const tqk_attn_desc& d) {
+  const int gq = d.n_q_heads / d.n_kv_heads;
+  const long long tokens = d.q_len < kTileRows / gq + 2 ? d.q_len : kTileRows / gq + 2;
+  long long keys = d.kv_len;
+  if (d.window > 0 && d.window < d.kv_len) {
+    keys = (long long)d.window + tokens + d.sinks + 2 * kMaxKeys;
+    if (keys > d.kv_len) keys = d.kv_len;
+  }
+  const int tile = d.head_dim == 256 ? kTileKeys<256> : kTileKeys<128>;
+  return (keys + tile - 1) / tile + 1;
+}
+
+AttnPlan make_plan(const tqk_attn_desc& d) {
+  AttnPlan pl{};
+  const int gq = d.n_q_heads / d.n_kv_heads;
+  pl.rows = (long long)d.batch * d.n_q_heads * d.q_len;
+  pl.row_tiles = (int)(((long long)d.q_len * gq + kTileRows - 1) / kTileRows);
+  const long long pairs = (long long)d.batch * d.n_kv_heads * pl.row_tiles;
+  // Few row tiles: the keys of each are split until the workgroups fill the
+  // chip once (two a CU up to head_dim 128), at least four key tiles a split.
+  const long long slots = (d.head_dim <= 128 ? 2 : 1) * (long long)device_cus();
+  long long splits = 1;
+  if (pairs * 2 <= slots) {
+    splits = slots / pairs;
+    const long long most = most_tiles(d) / 4;
+    if (splits > most) splits = most;
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+  }
+  pl.n_splits = (int)splits;
+  pl.items = pairs * splits;
+  pl.ws_bytes = splits > 1 ? (size_t)splits * pl.rows * (d.head_dim + 2) * sizeof(float) + 256 : 0;
+  return pl;
+}
+
+int check_attn(const tqk_attn_desc* d) {
+  if (!d) return TQK_EINVAL;
+  if (!head_dim_ok(d->head_dim)) return TQK_EUNSUPPORTED;
+  if (d->type != 1 && d->type != 2) return TQK_EUNSUPPORTED;
+  if (d->batch < 0 || d->q_len < 0 || d->kv_len < 0 || d->window < 0 || d->sinks < 0) return TQK_EINVAL;
+  if (d->q_len > (1 << 28) || d->kv_len > (1 << 30)) return TQK_EINVAL;
+  if (d->n_q_heads < 1 || d->n_kv_heads < 1 || d->n_q_heads % d->n_kv_heads) return TQK_EINVAL;
+  if (d->n_q_heads > 1024) return TQK_EUNSUPPORTED;
+  if ((long long)d->q_len * (d->n_q_heads / d->n_kv_heads) > (1LL << 30)) return TQK_EINVAL;
+  if (!(d->sm_scale > 0.f)) return TQK_EINVAL;  // (and not a NaN)
+  for (int i = 0; i < 3; ++i)  // 16-byte accesses
+    if (d->q_stride[i] % 8 || d->k_stride[i] % 8 || d->v_stride[i] % 8 || d->o_stride[i] % 8) return TQK_EINVAL;
+  // (256 threads a workgroup: fewer than 2^32)
+  if (d->batch && d->q_len && make_plan(*d).items > (1LL << 23)) return TQK_EINVAL;
+  return TQK_OK;
+}
+
+template <int D, typename T>
+void launch_tiles(const AttnArgs& a, long long items, hipStream_t st) {
+  hipLaunchKernelGGL((tqk_attn_tiles<D, T>), dim3((unsigned)items), dim3(kTileThreads), 0, st, a);
+  if (a.n_splits > 1)
+    hipLaunchKernelGGL((tqk_attn_join<D, T>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+}
+template <typename T>
+void launch_tiles(const AttnArgs& a, long long items, hipStream_t st) {
+  if (a.d.head_dim == 64)
+    launch_tiles<64, T>(a, items, st);
+  else if (a.d.head_dim == 128)
+    launch_tiles<128, T>(a, items, st);
+  else
+    launch_tiles<256, T>(a, items, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tqk_attention_workspace_bytes(const tqk_attn_desc* d) {
+  if (check_attn(d) != TQK_OK) return 0;
+  if (!d->batch || !d->q_len) return 0;
+  return make_plan(*d).ws_bytes;
+}
+
+int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const void* v,
+                  const int32_t* kv_lens, const int32_t* q_lens, const int32_t* kv_starts, void* out,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_attn(d);
+  if (rc != TQK_OK) return rc;
+  if (!d->batch || !d->q_len) return TQK_OK;
+  if (!q || !out || (d->kv_len && (!k || !v))) return TQK_EINVAL;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) return TQK_EINVAL;
+  const AttnPlan pl = make_plan(*d);
+  if (pl.ws_bytes && (!workspace || workspace_bytes < pl.ws_bytes || ((uintptr_t)workspace & 15)))
+    return TQK_EWORKSPACE;
+  AttnArgs a{};
+  a.d = *d;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.kv_lens = kv_lens;
+  a.q_lens = q_lens;
+  a.kv_starts = kv_starts;
+  a.out = out;
+  a.row_tiles = pl.row_tiles;
+  a.n_splits = pl.n_splits;
+  a.rows = pl.rows;
+  // the accumulators first: 16-byte stores
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = a.part_acc + (size_t)pl.n_splits * pl.rows * d->head_dim;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (d->type == 1)
+    launch_tiles<_Float16>(a, pl.items, st);
+  else
+    launch_tiles<__bf16>(a, pl.items, st);
+  return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+}
+
+}  // extern "C"

@@ -30,6 +30,8 @@ PER_UNIT = {
     "tqk_encode.hip": ["-ffp-contract=off"],
     "tqk_block.hip": ["-ffp-contract=off"],
     "tqk_decode.hip": [],
+    "tqk_rope.hip": [],
+    "tqk_attn.hip": [],
 }
 
 

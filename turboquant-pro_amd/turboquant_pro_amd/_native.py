@@ -29,7 +29,8 @@ EXPORTS = (
     "tqk_version", "tqk_check_desc", "tqk_decode_workspace_bytes", "tqk_decode",
     "tqk_decode_noalloc", "tqk_decode_partials", "tqk_decode_splits", "tqk_decode_merge", "tqk_encode_groups",
     "tqk_append_hot", "tqk_append_tokens", "tqk_dequant_groups", "tqk_dequant_dense", "tqk_encode_key_block", "tqk_encode_value_block",
-    "tqk_dequant_key_block", "tqk_dequant_value_block",
+    "tqk_dequant_key_block", "tqk_dequant_value_block", "tqk_norm_rope", "tqk_attention_workspace_bytes",
+    "tqk_attention",
 )
 
 
@@ -55,6 +56,23 @@ class BlockDesc(ctypes.Structure):
         "outliers_per_channel", "outlier_cap", "input_f32")] + [("dc_mask", ctypes.c_uint32 * 8)]
 
 
+class RopeDesc(ctypes.Structure):
+    """``tqk_rope_desc``: projection rows, their norms, rotation and types."""
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "batch", "tokens", "n_q_heads", "n_kv_heads", "head_dim", "rotary_dim", "interleaved", "in_type", "out_type",
+        "weight_type", "pos_i64", "pos_per_token")] + [
+        ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("eps", ctypes.c_float),
+        ("weight_offset", ctypes.c_float), ("rope_scale", ctypes.c_float)]
+
+
+class AttnDesc(ctypes.Structure):
+    """``tqk_attn_desc``: attention over dense keys and values."""
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "batch", "n_q_heads", "n_kv_heads", "head_dim", "q_len", "kv_len", "window", "sinks", "type")] + [
+        ("sm_scale", ctypes.c_float)] + [(n, ctypes.c_int64 * 3) for n in (
+            "q_stride", "k_stride", "v_stride", "o_stride")]
+
+
 _lib = None
 
 
@@ -64,6 +82,7 @@ def load(path: str) -> ctypes.CDLL:
     l_ = ctypes.CDLL(path)
     vp, i32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
     pd, pp, pb = ctypes.POINTER(CacheDesc), ctypes.POINTER(CachePtrs), ctypes.POINTER(BlockDesc)
+    pr, pa = ctypes.POINTER(RopeDesc), ctypes.POINTER(AttnDesc)
     sig = {
         "tqk_version": ([], ctypes.c_int),
         "tqk_check_desc": ([pd], ctypes.c_int),
@@ -82,6 +101,9 @@ def load(path: str) -> ctypes.CDLL:
         "tqk_encode_value_block": ([pb, vp, vp, vp, vp, vp, vp], ctypes.c_int),
         "tqk_dequant_key_block": ([pb, vp, vp, vp, i32, vp, vp, vp, vp], ctypes.c_int),
         "tqk_dequant_value_block": ([pb, vp, vp, vp, vp, vp, vp], ctypes.c_int),
+        "tqk_norm_rope": ([pr, vp, vp, vp, vp, vp, vp, vp, vp, vp], ctypes.c_int),
+        "tqk_attention_workspace_bytes": ([pa], sz),
+        "tqk_attention": ([pa, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(l_, name)

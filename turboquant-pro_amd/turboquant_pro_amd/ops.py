@@ -1,0 +1,226 @@
+"""The model step's operators around the cache: head norms with the position
+rotation (:func:`norm_rope`) and attention over dense keys and values with a
+sliding window and first tokens that stay visible (:func:`window_attention`).
+
+Both run hand-written gfx950 kernels behind ``include/tqk.h`` on the current
+stream of their tensors' device and have no CPU form.  ``TQKVPool.append_qkv``
+and ``TQKVPool.attend`` are their counterparts on a coded cache.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import _native as N
+from .codebooks import HEAD_DIMS
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _types():
+    torch = _torch()
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _on_gpu(what, *tensors):
+    """The one GPU that every given tensor is on."""
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise RuntimeError(f"{what} runs on a ROCm GPU (gfx950); got a tensor on {dev}")
+    for t in tensors[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+class _on:
+    """Makes ``dev`` the current device for a launch, where it is not."""
+
+    def __init__(self, dev):
+        torch = _torch()
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _stream(dev):
+    return ctypes.c_void_p(_torch().cuda.current_stream(dev).cuda_stream)
+
+
+def _aligned(x):
+    """``x`` with its last dimension contiguous, 16-byte rows and a 16-byte
+    start: itself, or a copy."""
+    el = x.element_size()
+    if (x.stride(-1) == 1 or x.shape[-1] == 1) and x.data_ptr() % 16 == 0 and all(
+            s % 8 == 0 and s * el % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
+        return x
+    return x.contiguous() if not x.is_contiguous() else x.clone()
+
+
+def _check_rope(qkv, n_q_heads, n_kv_heads, inv_freq, positions, q_weight, k_weight, dtype):
+    """Shapes and types of a :func:`norm_rope` call: (B, T, D, out dtype)."""
+    torch = _torch()
+    types = _types()
+    n_q_heads, n_kv_heads = int(n_q_heads), int(n_kv_heads)
+    if n_q_heads < 0 or n_kv_heads < 0 or n_q_heads + n_kv_heads == 0:
+        raise ValueError("norm_rope needs query or key/value heads")
+    heads = n_q_heads + 2 * n_kv_heads
+    if qkv.dim() != 3 or qkv.shape[2] % heads:
+        raise ValueError(f"norm_rope expects (B, T, {heads} * head_dim) rows, got {tuple(qkv.shape)}")
+    B, T, D = int(qkv.shape[0]), int(qkv.shape[1]), int(qkv.shape[2]) // heads
+    if D not in HEAD_DIMS:
+        raise NotImplementedError(f"head_dim {D}: the gfx950 kernels serve {HEAD_DIMS}")
+    dtype = qkv.dtype if dtype is None else dtype
+    if qkv.dtype not in types or dtype not in types:
+        raise ValueError(f"norm_rope takes and gives fp32, fp16 or bf16, not {qkv.dtype} and {dtype}")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
+        raise ValueError("inv_freq is a 1-D fp32 tensor, one frequency for each rotated pair")
+    if 2 * inv_freq.shape[0] > D:
+        raise ValueError(f"{inv_freq.shape[0]} rotated pairs do not fit head_dim {D}")
+    if inv_freq.shape[0] % 8:
+        raise NotImplementedError(f"{inv_freq.shape[0]} rotated pairs: the gfx950 kernel takes multiples of 8")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((B,), (B, T)):
+        raise ValueError(f"positions are int32 or int64 of shape ({B},) (of first tokens) or ({B}, {T}), "
+                         f"not {positions.dtype} {tuple(positions.shape)}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (D,) or w.dtype not in (qkv.dtype, torch.float32)):
+            raise ValueError(f"{name} is ({D},) in the rows' type or fp32, not {tuple(w.shape)} {w.dtype}")
+    return B, T, D, dtype
+
+
+def norm_rope(qkv, n_q_heads: int, n_kv_heads: int, inv_freq, positions, *, q_weight=None, k_weight=None,
+              eps: float = 1e-6, weight_offset: float = 0.0, interleaved: bool = False, rope_scale: float = 1.0,
+              dtype=None):
+    """Queries, keys and values of new tokens from their projection rows.
+
+    ``qkv`` ``(B, T, (Hq + 2 Hkv) * D)`` fp32, fp16 or bf16: the query heads,
+    then the key heads, then the value heads of a token.  Queries are
+    normalised per head by ``x * rsqrt(mean(x^2) + eps) * (q_weight +
+    weight_offset)`` when ``q_weight`` ``(D,)`` is given, keys likewise; then
+    the first ``2 * len(inv_freq)`` channels are rotated by ``position *
+    inv_freq`` in pairs ``(i, i + R/2)`` (``interleaved``: ``(2i, 2i + 1)``)
+    and scaled by ``rope_scale``; values are only converted.  ``positions``:
+    ``(B, T)``, or ``(B,)`` for the position of every sequence's first token
+    (int32 or int64).  Computed in fp32, the angles in 64 bits, and rounded
+    once to ``dtype`` (the rows' by default).
+
+    Returns ``q (B, Hq, T, D)``, ``k`` and ``v`` ``(B, Hkv, T, D)``: what
+    ``TQKVPool.append`` and ``TQKVPool.attend`` take."""
+    torch = _torch()
+    B, T, D, dtype = _check_rope(qkv, n_q_heads, n_kv_heads, inv_freq, positions, q_weight, k_weight, dtype)
+    dev = _on_gpu("norm_rope", qkv, inv_freq, positions, q_weight, k_weight)
+    types = _types()
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        q_weight, k_weight = q_weight.float(), k_weight.float()
+    w = q_weight if q_weight is not None else k_weight
+    qkv, inv_freq, positions = _aligned(qkv), inv_freq.contiguous(), positions.contiguous()
+    q_weight = None if q_weight is None else _aligned(q_weight)
+    k_weight = None if k_weight is None else _aligned(k_weight)
+    q = torch.empty((B, n_q_heads, T, D), dtype=dtype, device=dev)
+    k = torch.empty((B, n_kv_heads, T, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if B * T:
+        d = N.RopeDesc(batch=B, tokens=T, n_q_heads=n_q_heads, n_kv_heads=n_kv_heads, head_dim=D,
+                       rotary_dim=2 * inv_freq.shape[0], interleaved=int(bool(interleaved)), in_type=types[qkv.dtype],
+                       out_type=types[dtype], weight_type=0 if w is None else types[w.dtype],
+                       pos_i64=int(positions.dtype == torch.int64), pos_per_token=int(positions.dim() == 2),
+                       batch_stride=qkv.stride(0) if B > 1 else 0, token_stride=qkv.stride(1) if T > 1 else 0,
+                       eps=eps, weight_offset=weight_offset, rope_scale=rope_scale)
+        with _on(dev):
+            N.check(N.lib().tqk_norm_rope(ctypes.byref(d), qkv.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+                                          None if q_weight is None else q_weight.data_ptr(),
+                                          None if k_weight is None else k_weight.data_ptr(),
+                                          q.data_ptr(), k.data_ptr(), v.data_ptr(), _stream(dev)), "norm_rope")
+    return q, k, v
+
+
+def _window_args(window, sinks):
+    """``window`` (None: 0) and ``sinks`` as whole numbers of the C ABI."""
+    if window is not None and int(window) < 1:
+        raise ValueError("window is at least 1 token (the query's own), or None")
+    if int(sinks) < 0:
+        raise ValueError("sinks is not negative")
+    top = 2 ** 31 - 1  # (a longer window or more sinks than an int32 length: all keys)
+    return 0 if window is None or int(window) > top else int(window), min(int(sinks), top)
+
+
+def _lens(x, B, name):
+    torch = _torch()
+    if x is None:
+        return None
+    if tuple(x.shape) != (B,) or x.dtype != torch.int32:
+        raise ValueError(f"{name} is ({B},) int32, not {tuple(x.shape)} {x.dtype}")
+    return x.contiguous()
+
+
+def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scale: float | None = None,
+                     kv_lens=None, q_lens=None, kv_starts=None, out=None):
+    """Causal attention over dense keys and values with a sliding window and
+    first tokens that stay visible.
+
+    ``q`` ``(B, Hq, T, D)``, ``k`` and ``v`` ``(B, Hkv, L, D)``, fp16 or bf16,
+    any strides; query head i reads kv head ``i // (Hq / Hkv)``.  The queries
+    are a sequence's last: with ``n = kv_lens[b]`` keys (L) and ``m =
+    q_lens[b]`` queries (T), query t stands at ``p = n - m + t`` and sees the
+    keys j of ``[start, p]``, ``start = kv_starts[b]`` (0; a left-padded
+    batch's first tokens), with ``j > p - window`` (every one with None) or
+    ``j < start + sinks``.  Lengths are int32 ``(B,)`` tensors on the device.
+
+    Returns ``(B, Hq, T, D)`` in the inputs' type, ``out`` where given (any
+    strides of whole 16 bytes), else laid out ``(B, T, Hq, D)`` as the output
+    projection reads it.  A query that sees nothing and rows ``t >= m`` get
+    zeros.  ``scale``: ``1/sqrt(D)`` by default, positive."""
+    torch = _torch()
+    types = _types()
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"window_attention expects q (B, Hq, T, D) and k, v (B, Hkv, L, D), got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    B, Hq, T, D = (int(x) for x in q.shape)
+    Hkv, L = int(k.shape[1]), int(k.shape[2])
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hkv} kv heads")
+    if D not in HEAD_DIMS:
+        raise NotImplementedError(f"head_dim {D}: the gfx950 kernels serve {HEAD_DIMS}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v are of one type, not {q.dtype}, {k.dtype} and {v.dtype}")
+    if types.get(q.dtype, 0) == 0:
+        raise NotImplementedError(f"window_attention takes fp16 or bf16, not {q.dtype}")
+    window, sinks = _window_args(window, sinks)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not scale > 0.0 or not math.isfinite(scale):
+        raise ValueError(f"scale is positive and finite, not {scale}")
+    kv_lens, q_lens, kv_starts = (_lens(x, B, n) for x, n in ((kv_lens, "kv_lens"), (q_lens, "q_lens"),
+                                                              (kv_starts, "kv_starts")))
+    if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype):
+        raise ValueError(f"out is {tuple(q.shape)} {q.dtype}, not {tuple(out.shape)} {out.dtype}")
+    dev = _on_gpu("window_attention", q, k, v, kv_lens, q_lens, kv_starts, out)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    if out is None:
+        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev).transpose(1, 2)
+    elif _aligned(out) is not out:
+        raise ValueError("out needs channels side by side, rows of whole 16 bytes and a 16-byte start")
+    if B * T == 0:
+        return out
+    d = N.AttnDesc(batch=B, n_q_heads=Hq, n_kv_heads=Hkv, head_dim=D, q_len=T, kv_len=L, window=window, sinks=sinks,
+                   type=types[q.dtype], sm_scale=scale)
+    for dst, x in ((d.q_stride, q), (d.k_stride, k), (d.v_stride, v), (d.o_stride, out)):
+        dst[:] = [s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape[:3])]
+    lib = N.lib()
+    with _on(dev):
+        need = lib.tqk_attention_workspace_bytes(ctypes.byref(d))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        N.check(lib.tqk_attention(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                  *(None if x is None else x.data_ptr() for x in (kv_lens, q_lens, kv_starts)),
+                                  out.data_ptr(), None if ws is None else ws.data_ptr(), need, _stream(dev)),
+                "window_attention")
+    return out
