@@ -418,6 +418,42 @@ int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const vo
                   const int32_t* kv_lens, const int32_t* q_lens, const int32_t* kv_starts, void* out,
                   void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Attention of the last queries of every sequence over the two-tier cache, with
+ * a sliding window and first tokens that stay visible: query t of sequence b,
+ * with m = q_lens[b] queries and n = seq_lens[b] cached tokens, stands at p = n
+ * - m + t and sees the tokens j of [0, p] with j > p - window or j < sinks.
+ * Only the coded groups that a query sees are read.  Queries with p < 0 and
+ * rows t >= m get zeros.
+ *   q        [batch][n_q_heads][q_len][head_dim] by strides, fp16 (fp32 when input_f32)
+ *   seq_lens [batch] i32 (device), clamped to max_len
+ *   q_lens   [batch] i32 (device) or null (q_len); clamped to [0, q_len]
+ *   out      like q by strides, fp32 or fp16
+ * The windowed form of tqk_decode, for one query (a decode step), a few (a
+ * verification step) or a prompt's chunk.  Few queries are attended in code
+ * space; more than 8 fp16 ones with an fp16 output over keys and values
+ * reconstructed in the workspace (weights and keys rounded to fp16).
+ */
+typedef struct tqk_attend_desc {
+  int32_t batch;        /* at most n_pages of the cache */
+  int32_t q_len;        /* query rows of every sequence */
+  int32_t max_len;      /* the longest sequence */
+  int32_t window;       /* tokens a query sees back from itself, itself included; 0: all */
+  int32_t sinks;        /* first tokens that stay visible */
+  int32_t out_type;     /* 0 fp32, 1 fp16 */
+  int64_t q_stride[3];  /* elements between sequences, heads and queries: multiples of 8 */
+  int64_t o_stride[3];
+} tqk_attend_desc;
+
+/* Bytes of workspace for the current device (no initialisation, 16-byte
+ * aligned; calls that share one must not overlap); 0 for a bad descriptor or
+ * nothing to do. */
+size_t tqk_attend_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t);
+
+int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
+               const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace,
+               size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

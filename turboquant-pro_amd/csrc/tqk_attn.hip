@@ -442,13 +442,6 @@ __global__ __launch_bounds__(256) void tqk_attn_join(AttnArgs a) {
   for (int e = 0; e < E; ++e) op[e] = (T)(l != 0.f ? acc[e] * inv : 0.f);
 }
 
-int device_cus() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 256;
-  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
-  return n;
-}
-
 struct AttnPlan {
   int row_tiles, n_splits;
   long long rows, items;

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/tqk.h"
 
 #define TQK_D 128          // head_dim of the MFMA decode (other head dims run the VALU decode)
@@ -58,6 +60,21 @@ __device__ __forceinline__ float h2f(uint16_t x) {
 }
 __device__ __forceinline__ uint16_t f2h(float x) {  // round to nearest even
   return __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+
+// compute units of the current device (the plan sizes the launch for them),
+// queried once per device and process
+constexpr int kMaxDevices = 64;
+static inline int device_cus() {
+  static std::atomic<int> cus[kMaxDevices];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) return 256;
+  int n = cus[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
+    n = 256;
+  cus[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 // 4-bit nibble bit reversal: the key stream stores each code LSB-first inside

@@ -30,6 +30,7 @@ PER_UNIT = {
     "tqk_encode.hip": ["-ffp-contract=off"],
     "tqk_block.hip": ["-ffp-contract=off"],
     "tqk_decode.hip": [],
+    "tqk_attend.hip": [],
     "tqk_rope.hip": [],
     "tqk_attn.hip": [],
 }

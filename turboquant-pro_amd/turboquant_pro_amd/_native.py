@@ -30,7 +30,7 @@ EXPORTS = (
     "tqk_decode_noalloc", "tqk_decode_partials", "tqk_decode_splits", "tqk_decode_merge", "tqk_encode_groups",
     "tqk_append_hot", "tqk_append_tokens", "tqk_dequant_groups", "tqk_dequant_dense", "tqk_encode_key_block", "tqk_encode_value_block",
     "tqk_dequant_key_block", "tqk_dequant_value_block", "tqk_norm_rope", "tqk_attention_workspace_bytes",
-    "tqk_attention",
+    "tqk_attention", "tqk_attend_workspace_bytes", "tqk_attend",
 )
 
 
@@ -73,6 +73,13 @@ class AttnDesc(ctypes.Structure):
             "q_stride", "k_stride", "v_stride", "o_stride")]
 
 
+class AttendDesc(ctypes.Structure):
+    """``tqk_attend_desc``: windowed attention over the cache."""
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "batch", "q_len", "max_len", "window", "sinks", "out_type")] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "o_stride")]
+
+
 _lib = None
 
 
@@ -82,7 +89,7 @@ def load(path: str) -> ctypes.CDLL:
     l_ = ctypes.CDLL(path)
     vp, i32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
     pd, pp, pb = ctypes.POINTER(CacheDesc), ctypes.POINTER(CachePtrs), ctypes.POINTER(BlockDesc)
-    pr, pa = ctypes.POINTER(RopeDesc), ctypes.POINTER(AttnDesc)
+    pr, pa, pt = ctypes.POINTER(RopeDesc), ctypes.POINTER(AttnDesc), ctypes.POINTER(AttendDesc)
     sig = {
         "tqk_version": ([], ctypes.c_int),
         "tqk_check_desc": ([pd], ctypes.c_int),
@@ -103,6 +110,8 @@ def load(path: str) -> ctypes.CDLL:
         "tqk_dequant_value_block": ([pb, vp, vp, vp, vp, vp, vp], ctypes.c_int),
         "tqk_norm_rope": ([pr, vp, vp, vp, vp, vp, vp, vp, vp, vp], ctypes.c_int),
         "tqk_attention_workspace_bytes": ([pa], sz),
+        "tqk_attend_workspace_bytes": ([pd, pt], sz),
+        "tqk_attend": ([pd, pp, pt, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
         "tqk_attention": ([pa, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

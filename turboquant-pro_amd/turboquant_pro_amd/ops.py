@@ -37,7 +37,7 @@ def _on_gpu(what, *tensors):
     return dev
 
 
-class _on:
+class on_device:
     """Makes ``dev`` the current device for a launch, where it is not."""
 
     def __init__(self, dev):
@@ -53,11 +53,11 @@ class _on:
             self.guard.__exit__(*exc)
 
 
-def _stream(dev):
+def stream_of(dev):
     return ctypes.c_void_p(_torch().cuda.current_stream(dev).cuda_stream)
 
 
-def _aligned(x):
+def aligned(x):
     """``x`` with its last dimension contiguous, 16-byte rows and a 16-byte
     start: itself, or a copy."""
     el = x.element_size()
@@ -123,9 +123,9 @@ def norm_rope(qkv, n_q_heads: int, n_kv_heads: int, inv_freq, positions, *, q_we
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         q_weight, k_weight = q_weight.float(), k_weight.float()
     w = q_weight if q_weight is not None else k_weight
-    qkv, inv_freq, positions = _aligned(qkv), inv_freq.contiguous(), positions.contiguous()
-    q_weight = None if q_weight is None else _aligned(q_weight)
-    k_weight = None if k_weight is None else _aligned(k_weight)
+    qkv, inv_freq, positions = aligned(qkv), inv_freq.contiguous(), positions.contiguous()
+    q_weight = None if q_weight is None else aligned(q_weight)
+    k_weight = None if k_weight is None else aligned(k_weight)
     q = torch.empty((B, n_q_heads, T, D), dtype=dtype, device=dev)
     k = torch.empty((B, n_kv_heads, T, D), dtype=dtype, device=dev)
     v = torch.empty_like(k)
@@ -136,15 +136,15 @@ def norm_rope(qkv, n_q_heads: int, n_kv_heads: int, inv_freq, positions, *, q_we
                        pos_i64=int(positions.dtype == torch.int64), pos_per_token=int(positions.dim() == 2),
                        batch_stride=qkv.stride(0) if B > 1 else 0, token_stride=qkv.stride(1) if T > 1 else 0,
                        eps=eps, weight_offset=weight_offset, rope_scale=rope_scale)
-        with _on(dev):
+        with on_device(dev):
             N.check(N.lib().tqk_norm_rope(ctypes.byref(d), qkv.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
                                           None if q_weight is None else q_weight.data_ptr(),
                                           None if k_weight is None else k_weight.data_ptr(),
-                                          q.data_ptr(), k.data_ptr(), v.data_ptr(), _stream(dev)), "norm_rope")
+                                          q.data_ptr(), k.data_ptr(), v.data_ptr(), stream_of(dev)), "norm_rope")
     return q, k, v
 
 
-def _window_args(window, sinks):
+def window_args(window, sinks):
     """``window`` (None: 0) and ``sinks`` as whole numbers of the C ABI."""
     if window is not None and int(window) < 1:
         raise ValueError("window is at least 1 token (the query's own), or None")
@@ -154,7 +154,7 @@ def _window_args(window, sinks):
     return 0 if window is None or int(window) > top else int(window), min(int(sinks), top)
 
 
-def _lens(x, B, name):
+def lengths_arg(x, B, name):
     torch = _torch()
     if x is None:
         return None
@@ -195,19 +195,19 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
         raise ValueError(f"q, k and v are of one type, not {q.dtype}, {k.dtype} and {v.dtype}")
     if types.get(q.dtype, 0) == 0:
         raise NotImplementedError(f"window_attention takes fp16 or bf16, not {q.dtype}")
-    window, sinks = _window_args(window, sinks)
+    window, sinks = window_args(window, sinks)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not scale > 0.0 or not math.isfinite(scale):
         raise ValueError(f"scale is positive and finite, not {scale}")
-    kv_lens, q_lens, kv_starts = (_lens(x, B, n) for x, n in ((kv_lens, "kv_lens"), (q_lens, "q_lens"),
+    kv_lens, q_lens, kv_starts = (lengths_arg(x, B, n) for x, n in ((kv_lens, "kv_lens"), (q_lens, "q_lens"),
                                                               (kv_starts, "kv_starts")))
     if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype):
         raise ValueError(f"out is {tuple(q.shape)} {q.dtype}, not {tuple(out.shape)} {out.dtype}")
     dev = _on_gpu("window_attention", q, k, v, kv_lens, q_lens, kv_starts, out)
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    q, k, v = aligned(q), aligned(k), aligned(v)
     if out is None:
         out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev).transpose(1, 2)
-    elif _aligned(out) is not out:
+    elif aligned(out) is not out:
         raise ValueError("out needs channels side by side, rows of whole 16 bytes and a 16-byte start")
     if B * T == 0:
         return out
@@ -216,11 +216,11 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
     for dst, x in ((d.q_stride, q), (d.k_stride, k), (d.v_stride, v), (d.o_stride, out)):
         dst[:] = [s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape[:3])]
     lib = N.lib()
-    with _on(dev):
+    with on_device(dev):
         need = lib.tqk_attention_workspace_bytes(ctypes.byref(d))
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         N.check(lib.tqk_attention(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                   *(None if x is None else x.data_ptr() for x in (kv_lens, q_lens, kv_starts)),
-                                  out.data_ptr(), None if ws is None else ws.data_ptr(), need, _stream(dev)),
+                                  out.data_ptr(), None if ws is None else ws.data_ptr(), need, stream_of(dev)),
                 "window_attention")
     return out

@@ -27,6 +27,7 @@ from . import _native as N
 from .formats import (NF4_ZERO_CODE, codes_from_key_rows, key_rows_from_codes, nf4_codes,
                       pack_key_codes, pack_values, tile_value_rows, uniform_codes, unpack_key_codes,
                       unpack_values, untile_value_rows)
+from .ops import aligned, lengths_arg, norm_rope, on_device, stream_of, window_args
 from .codebooks import (HEAD_DIMS, dc_channel_mask, dc_mask_words, group_tokens_for, n_groups_for,
                         outliers_per_channel, random_rotation, rope_averaged_bias, value_codebook)
 
@@ -417,6 +418,74 @@ class TQKVPool:
                                             ws.data_ptr(), need, self._stream()),
                 "tqk_decode_partials")
         return m, l_, acc
+
+    def attend(self, q, *, window: int | None = None, sinks: int = 0, q_lens=None, out=None):
+        """Attention of every sequence's last queries over its cache, with a
+        sliding window and first tokens that stay visible.
+
+        ``q`` ``(B, Hq, T, D)`` in the pool's input type, any strides: the
+        queries of the last T tokens appended (T = 1: a decode step; a few: a
+        verification step; a prompt's chunk).  Query t of a sequence of n
+        cached tokens stands at ``p = n - m + t`` with ``m = q_lens[b]`` (an
+        int32 ``(B,)`` tensor on the device; T by default) and sees the tokens
+        j <= p with ``j > p - window`` (every one with None) or ``j < sinks``.
+        Only the coded groups that a query sees are read.
+
+        Returns ``(B, Hq, T, D)`` in the queries' type (``out`` where given,
+        else laid out ``(B, T, Hq, D)``); rows ``t >= m`` and queries before
+        the first token get zeros."""
+        torch = _torch()
+        B, Hq, D = self.max_batch, self.n_q_heads, self.head_dim
+        if q.dim() != 4 or tuple(q.shape[:2]) != (B, Hq) or q.shape[3] != D or q.dtype != self.dtype:
+            raise ValueError(f"attend expects {self.input_dtype} q of shape ({B}, {Hq}, T, {D}), got {q.dtype} "
+                             f"{tuple(q.shape)}")
+        T = int(q.shape[2])
+        window, sinks = window_args(window, sinks)
+        q_lens = lengths_arg(q_lens, B, "q_lens")
+        if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or aligned(out) is not out):
+            raise ValueError(f"out is {tuple(q.shape)} {q.dtype} with channels side by side, rows of whole 16 bytes "
+                             "and a 16-byte start")
+        for name, x in (("q", q), ("q_lens", q_lens), ("out", out)):
+            if x is not None and x.device != self.kcodes.device:
+                raise ValueError(f"attend: {name} is on {x.device}, the pool on {self.kcodes.device}")
+        self.check()
+        q = aligned(q)
+        if out is None:
+            out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device).transpose(1, 2)
+        if B * T == 0:
+            return out
+        t = N.AttendDesc(batch=B, q_len=T, max_len=max(self.lengths), window=window, sinks=sinks,
+                         out_type=0 if self.f32 else 1)
+        for dst, x in ((t.q_stride, q), (t.o_stride, out)):
+            dst[:] = [s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape[:3])]
+        lib = N.lib()
+        with on_device(q.device):
+            need = lib.tqk_attend_workspace_bytes(ctypes.byref(self.desc), ctypes.byref(t))
+            # (a call's own: calls on several streams and captured graphs share nothing)
+            ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=q.device)
+            N.check(lib.tqk_attend(ctypes.byref(self.desc), ctypes.byref(self.ptrs), ctypes.byref(t), q.data_ptr(),
+                                   self.seq_lens.data_ptr(), None if q_lens is None else q_lens.data_ptr(),
+                                   out.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(q.device)), "tqk_attend")
+        return out
+
+    def append_qkv(self, qkv, inv_freq, *, q_weight=None, k_weight=None, eps: float = 1e-6,
+                   weight_offset: float = 0.0, interleaved: bool = False, rope_scale: float = 1.0, positions=None,
+                   n_new=None):
+        """New tokens from their projection rows ``(B, T, (Hq + 2 Hkv) * D)``:
+        head norms and rotation (:func:`~turboquant_pro_amd.ops.norm_rope`, the
+        positions following each sequence's cached tokens unless given), then
+        :meth:`append` of the keys and values.  Returns the queries ``(B, Hq, T,
+        D)`` for :meth:`attend` in the pool's input type."""
+        if qkv.dim() != 3 or int(qkv.shape[0]) != self.max_batch or \
+                int(qkv.shape[2]) != (self.n_q_heads + 2 * self.n_kv_heads) * self.head_dim:
+            raise ValueError(f"append_qkv expects ({self.max_batch}, T, {self.n_q_heads + 2 * self.n_kv_heads} * "
+                             f"{self.head_dim}) rows, got {tuple(qkv.shape)}")
+        q, k, v = norm_rope(qkv, self.n_q_heads, self.n_kv_heads, inv_freq,
+                            self.seq_lens if positions is None else positions, q_weight=q_weight, k_weight=k_weight,
+                            eps=eps, weight_offset=weight_offset, interleaved=interleaved, rope_scale=rope_scale,
+                            dtype=self.dtype)
+        self.append(k, v, n_new=n_new)
+        return q
 
     # ------------------------------------------------------------------ #
     def dequant_groups(self, items):
