@@ -81,7 +81,7 @@ struct Mma<__bf16> {
 // whether a 16-bit pattern is an infinity or a NaN
 template <typename T>
 __device__ __forceinline__ bool not_finite2(uint32_t two) {
-  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+  constexpr uint32_t e = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
   return (two & e) == e || ((two >> 16) & e) == e;
 }
 template <typename T>
@@ -89,11 +89,25 @@ __device__ __forceinline__ bool not_finite(u4_t x) {
   return not_finite2<T>(x.x) || not_finite2<T>(x.y) || not_finite2<T>(x.z) || not_finite2<T>(x.w);
 }
 
-// the value of the other half-wave's lane with the same l % 32
-__device__ __forceinline__ float other_half(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __builtin_bit_cast(float, (threadIdx.x & 32) ? (uint32_t)r[0] : (uint32_t)r[1]);
+template <typename T>
+__device__ __forceinline__ u4_t only_finite(u4_t x) {
+  constexpr uint32_t e = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((x[i] & e) == e) x[i] &= 0xFFFF0000u;
+    if (((x[i] >> 16) & e) == e) x[i] &= 0xFFFFu;
+  }
+  return x;
+}
+
+// a raw buffer of `bytes` from p on (32-bit data, no swizzle); past it loads give zeros
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const char* p, long long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, (int)bytes, 0x00020000);
+}
+// this wave's loads into LDS are done
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ float max_half(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
@@ -175,9 +189,8 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
   constexpr int ND = D / 32, NK = D / 16;
   constexpr int kBytes = kKeys * D * 2;
   using TG = TileGeom<D>;
-  __shared__ __align__(16) uint8_t k_s[2][kBytes];
-  __shared__ __align__(16) uint8_t v_s[2][kBytes];
-  __shared__ int bad_s[2];  // the tile whose V holds an infinity or a NaN under a mask
+  __shared__ __align__(16) uint8_t k0_s[kBytes], v0_s[kBytes], k1_s[kBytes], v1_s[kBytes];
+  __shared__ int odd_s;  // an infinity or a NaN among the values that only some rows see
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
   const int Hq = a.d.n_q_heads, Hkv = a.d.n_kv_heads, gq = Hq / Hkv;
@@ -228,152 +241,169 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
     for (int r = 0; r < 16; ++r) O[i][r] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;  // (l_run: this lane's keys only)
 
-  // staging: thread tid takes chunks tid + 256 i of the tile, in row order
-  const long long ks_ = a.d.k_stride[2], vs_ = a.d.v_stride[2];
-  const T* const kb = static_cast<const T*>(a.k) + b * a.d.k_stride[0] + h * a.d.k_stride[1];
-  const T* const vb = static_cast<const T*>(a.v) + b * a.d.v_stride[0] + h * a.d.v_stride[1];
+  // A tile goes straight into LDS, 16 bytes a lane and no registers: thread tid
+  // fills places tid + 256 i, rows 256 / CH apart, from the chunk that belongs
+  // there.  The buffer resource starts at the tile's first row and ends with
+  // the last key: rows past it are not read.
+  const long long ks_ = a.d.k_stride[2] * 2, vs_ = a.d.v_stride[2] * 2;
+  const char* const kb = static_cast<const char*>(a.k) + 2 * (b * a.d.k_stride[0] + h * a.d.k_stride[1]);
+  const char* const vb = static_cast<const char*>(a.v) + 2 * (b * a.d.v_stride[0] + h * a.d.v_stride[1]);
   const int gap = a.compact ? compact_gap(s) : 0;
   const int sink_rows = (s.sink_end + kMaxKeys - 1) / kMaxKeys * kMaxKeys;
-  u4_t kst[NST], vst[NST];
+  const int my_row = tid / CH, my_ch = tid % CH;
+  const uint32_t k_off = (uint32_t)my_row * (uint32_t)ks_ + 16u * (uint32_t)(TG::k_at(my_row, my_ch) / 16 % CH);
+  const uint32_t v_off = (uint32_t)my_row * (uint32_t)vs_ + 16u * (uint32_t)(TG::v_at(my_row, my_ch) / 16 % CH);
   // whether every row of the workgroup sees the whole tile
   auto whole = [&](int k0) {
     return k0 + kKeys - 1 <= p_lo && k0 >= s.start && (k0 >= s.low(p_hi) || k0 + kKeys <= s.sink_end);
   };
-  auto load_tile = [&](int k0) {
-    const int g = k0 >= sink_rows ? gap : 0;
+  auto load_tile = [&](uint8_t* kd, uint8_t* vd, int k0) {
+    const long long r0 = k0 - (k0 >= sink_rows ? gap : 0);
+    const long long rows = min(kKeys, s.n - k0);
+    const __amdgpu_buffer_rsrc_t rk = tile_rsrc(kb + r0 * ks_, (rows - 1) * ks_ + 2 * D);
+    const __amdgpu_buffer_rsrc_t rv = tile_rsrc(vb + r0 * vs_, (rows - 1) * vs_ + 2 * D);
 #pragma unroll
     for (int i = 0; i < NST; ++i) {
-      const int ch = tid + kTileThreads * i, r = min(k0 + ch / CH, s.n - 1) - g, cc = ch % CH;
-      kst[i] = *reinterpret_cast<const u4_t*>(kb + r * ks_ + 8 * cc);
-      vst[i] = *reinterpret_cast<const u4_t*>(vb + r * vs_ + 8 * cc);
+      typedef __attribute__((address_space(3))) void* lds;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds)(kd + 1024 * wave + 16 * kTileThreads * i), 16, (int)k_off,
+                                               (int)(i * (kTileThreads / CH) * ks_), 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds)(vd + 1024 * wave + 16 * kTileThreads * i), 16, (int)v_off,
+                                               (int)(i * (kTileThreads / CH) * vs_), 0, 0);
     }
   };
-  auto put_tile = [&](int buf, int i_tile, int k0) {
-    if (!whole(k0)) {
-      // values that no row of the workgroup sees count as zero, whatever they
-      // hold (a weight of zero times an infinity is no zero)
-#pragma unroll
-      for (int i = 0; i < NST; ++i) {
-        const int j = k0 + (tid + kTileThreads * i) / CH;
-        if (!s.sees(p_hi, b_lo, j)) vst[i] = u4_t{0u, 0u, 0u, 0u};
-        if (not_finite<T>(vst[i])) bad_s[buf] = i_tile;
+  // The tile has arrived (every wave waits for its own loads).  Values that no
+  // row of the workgroup sees count as zero, and an infinity or a NaN that some
+  // rows see and others do not is set aside (a weight of zero times one of them
+  // is no zero): a thread mends the chunks that it loaded.
+  auto mend_tile = [&](uint8_t* vd, int k0) {
+    if (whole(k0)) return;
+#pragma unroll 1
+    for (int i = 0; i < NST; ++i) {
+      u4_t* x = reinterpret_cast<u4_t*>(vd + 16 * (tid + kTileThreads * i));
+      const int j = k0 + my_row + i * (kTileThreads / CH);
+      if (!s.sees(p_hi, b_lo, j)) {
+        *x = u4_t{0u, 0u, 0u, 0u};
+      } else if (not_finite<T>(*x)) {
+        *x = only_finite<T>(*x);
+        odd_s = 1;
       }
     }
-#pragma unroll
-    for (int i = 0; i < NST; ++i) {
-      const int ch = tid + kTileThreads * i, r = ch / CH, cc = ch % CH;
-      *reinterpret_cast<u4_t*>(k_s[buf] + TG::k_at(r, cc)) = kst[i];
-      *reinterpret_cast<u4_t*>(v_s[buf] + TG::v_at(r, cc)) = vst[i];
-    }
   };
-
-  if (tid < 2) bad_s[tid] = -1;
-  __syncthreads();
-  if (i0 < i1) {
-    load_tile(tiles.at(i0));
-    put_tile(0, i0, tiles.at(i0));
-  }
-  __syncthreads();
-  for (int it = i0; it < i1; ++it) {
-    const int buf = (it - i0) & 1, k0 = tiles.at(it);
-    if (it + 1 < i1) load_tile(tiles.at(it + 1));
+  auto attend_tile = [&](const uint8_t* k_t, const uint8_t* v_t, int k0) {
     // (a tile that none of the wave's rows sees: only its staging)
-    if (w_lo < s.m && k0 <= wp_hi && (k0 + kKeys > wl_lo || k0 < s.sink_end)) {
-      // K Q^T: keys k0 + 32 u + 8 (r / 4) + 4 lh + r % 4 of row ln
-      f16v_t S[NU];
+    if (!(w_lo < s.m && k0 <= wp_hi && (k0 + kKeys > wl_lo || k0 < s.sink_end))) return;
+    // K Q^T: keys k0 + 32 u + 8 (r / 4) + 4 lh + r % 4 of row ln
+    f16v_t S[NU];
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
+    for (int u = 0; u < NU; ++u) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) S[u][r] = 0.f;
+      for (int r = 0; r < 16; ++r) S[u][r] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-          const v8 kf = *reinterpret_cast<const v8*>(k_s[buf] + TG::k_at(32 * u + ln, 2 * ks + lh));
-          S[u] = Mma<T>::m32(kf, qf[ks], S[u]);
-        }
+      for (int ks = 0; ks < NK; ++ks) {
+        const v8 kf = *reinterpret_cast<const v8*>(k_t + TG::k_at(32 * u + ln, 2 * ks + lh));
+        S[u] = Mma<T>::m32(kf, qf[ks], S[u]);
       }
-      const bool masked = !(k0 + kKeys - 1 <= wp_lo && k0 >= s.start && (k0 >= wl_hi || k0 + kKeys <= s.sink_end));
-      if (masked) {
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = k0 + 32 * u + 8 * (r / 4) + 4 * lh + r % 4;
-            S[u][r] = s.sees(p, lo, j) ? S[u][r] : -INFINITY;
-          }
-      }
-      float mx = S[0][0];
-#pragma unroll
-      for (int u = 0; u < NU; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[u][r]);
-      mx = max_half(mx) * c;
-      if (__any(mx > m_run + kLazy)) {
-        const float m_new = fmaxf(m_run, mx);
-        const float f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-        m_run = m_new;
-        l_run *= f;
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) O[i][r] *= f;
-      }
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    }
+    if (!(k0 + kKeys - 1 <= wp_lo && k0 >= s.start && (k0 >= wl_hi || k0 + kKeys <= s.sink_end))) {
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          S[u][r] = __builtin_amdgcn_exp2f(fmaf(S[u][r], c, -m_use));
-          l_run += S[u][r];
+          const int j = k0 + 32 * u + 8 * (r / 4) + 4 * lh + r % 4;
+          S[u][r] = s.sees(p, lo, j) ? S[u][r] : -INFINITY;
         }
-      if (masked && __builtin_expect(bad_s[buf] == it, 0)) {
-        // An infinity or a NaN under a mask: key by key, only into the rows that
-        // see it (the products of a matrix instruction would be NaN in all).
-        float w[16 * NU];
+    }
+    float mx = S[0][0];
 #pragma unroll
-        for (int r = 0; r < 16 * NU; ++r) w[r] = S[r / 16][r % 16];
-        for (int jj = 0; jj < kKeys; ++jj) {
-          const float mine = w[16 * (jj / 32) + 4 * (jj % 32 / 8) + jj % 4], far = other_half(mine);
-          const float wt = ((jj >> 2) & 1) == lh ? mine : far;
-          const bool vis = s.sees(p, lo, k0 + jj);  // (else the weight is zero)
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int i = 0; i < ND; ++i)
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[u][r]);
+    mx = max_half(mx) * c;
+    if (__any(mx > m_run + kLazy)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= f;
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-              typedef T v4 __attribute__((ext_vector_type(4)));
-              const int dd = 32 * i + 2 * r + 4 * lh;
-              const v4 x = *reinterpret_cast<const v4*>(v_s[buf] + TG::v_at(jj, dd / 8) + 8 * lh);
+      for (int i = 0; i < ND; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) O[i][r + e] = fmaf(wt, vis ? (float)x[e] : 0.f, O[i][r + e]);
-              __builtin_amdgcn_sched_barrier(0);  // (no registers for reads ahead on this path)
-            }
+        for (int r = 0; r < 16; ++r) O[i][r] *= f;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    // V^T P^T, 16 keys a product; the weights rounded to the inputs' type
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        v8 pf;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float w = __builtin_amdgcn_exp2f(fmaf(S[u][8 * g + e], c, -m_use));
+          l_run += w;
+          pf[e] = (T)w;
         }
-      } else {
-        // V^T P^T, 16 keys a product; the weights rounded to the inputs' type
+        // the lane's part of a transposing read: row ln % 16 / 4 of four, channels 4 (ln % 4)
+        const int r0 = 32 * u + 16 * g + 4 * lh + (ln % 16) / 4;
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
+        for (int i = 0; i < ND; ++i) {
+          const int cc = 4 * i + 2 * (ln / 16) + (ln % 4) / 2;
+          typedef __attribute__((address_space(3))) s4_t* lds4;
+          const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_t + TG::v_at(r0, cc) + 8 * (ln % 2)));
+          const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_t + TG::v_at(r0 + 8, cc) + 8 * (ln % 2)));
+          const s8_t xy = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+          O[i] = Mma<T>::m32(__builtin_bit_cast(v8, xy), pf, O[i]);
+        }
+      }
+  };
+
+  if (tid == 0) odd_s = 0;
+  __syncthreads();
+  if (i0 < i1) {
+    load_tile(k0_s, v0_s, tiles.at(i0));
+    wait_loads();
+    mend_tile(v0_s, tiles.at(i0));
+  }
+  __syncthreads();
+  // two tiles a round, each in LDS of its own: one is computed while the next arrives
+  for (int it = i0; it < i1; it += 2) {
+    if (it + 1 < i1) load_tile(k1_s, v1_s, tiles.at(it + 1));
+    attend_tile(k0_s, v0_s, tiles.at(it));
+    if (it + 1 >= i1) break;
+    wait_loads();
+    mend_tile(v1_s, tiles.at(it + 1));
+    __syncthreads();
+    if (it + 2 < i1) load_tile(k0_s, v0_s, tiles.at(it + 2));
+    attend_tile(k1_s, v1_s, tiles.at(it + 1));
+    if (it + 2 < i1) {
+      wait_loads();
+      mend_tile(v0_s, tiles.at(it + 2));
+    }
+    __syncthreads();
+  }
+
+  if (__builtin_expect(odd_s != 0, 0)) {
+    // the infinities and NaN set aside, into the rows that see them (any
+    // positive weight gives the same)
+    for (int it = i0; it < i1; ++it) {
+      const int k0 = tiles.at(it);
+      if (whole(k0)) continue;
+      for (int j = k0; j < min(k0 + kKeys, s.n); ++j) {
+        const bool vis = s.sees(p, lo, j);
+        const T* vr = reinterpret_cast<const T*>(vb + (j - (k0 >= sink_rows ? gap : 0)) * vs_) + 4 * lh;
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            v8 pf;
+        for (int i = 0; i < ND; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pf[e] = (T)S[u][8 * g + e];
-            // the lane's part of a transposing read: row ln % 16 / 4 of four, channels 4 (ln % 4)
-            const int r0 = 32 * u + 16 * g + 4 * lh + (ln % 16) / 4;
+          for (int r = 0; r < 16; r += 4) {
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            const v4 x = *reinterpret_cast<const v4*>(vr + 32 * i + 2 * r);
 #pragma unroll
-            for (int i = 0; i < ND; ++i) {
-              const int cc = 4 * i + 2 * (ln / 16) + (ln % 4) / 2;
-              typedef __attribute__((address_space(3))) s4_t* lds4;
-              const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (lds4)(v_s[buf] + TG::v_at(r0, cc) + 8 * (ln % 2)));
-              const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (lds4)(v_s[buf] + TG::v_at(r0 + 8, cc) + 8 * (ln % 2)));
-              const s8_t xy = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-              O[i] = Mma<T>::m32(__builtin_bit_cast(v8, xy), pf, O[i]);
+            for (int e = 0; e < 4; ++e) {
+              const float y = (float)x[e];
+              O[i][r + e] += vis && !(fabsf(y) < INFINITY) ? y : 0.f;
             }
           }
       }
     }
-    if (it + 1 < i1) put_tile(buf ^ 1, it + 1, tiles.at(it + 1));
-    __syncthreads();
   }
 
   const float l = sum_half(l_run);
@@ -442,6 +472,8 @@ __global__ __launch_bounds__(256) void tqk_attn_join(AttnArgs a) {
   for (int e = 0; e < E; ++e) op[e] = (T)(l != 0.f ? acc[e] * inv : 0.f);
 }
 
+constexpr int64_t kMostStride = 1 << 23;  // elements between tokens of keys and values
+
 struct AttnPlan {
   int row_tiles, n_splits;
   long long rows, items;
@@ -496,6 +528,9 @@ int check_attn(const tqk_attn_desc* d) {
   if (!(d->sm_scale > 0.f)) return TQK_EINVAL;  // (and not a NaN)
   for (int i = 0; i < 3; ++i)  // 16-byte accesses
     if (d->q_stride[i] % 8 || d->k_stride[i] % 8 || d->v_stride[i] % 8 || d->o_stride[i] % 8) return TQK_EINVAL;
+  // (a key tile's rows within 32-bit byte offsets)
+  if (d->k_stride[2] < 0 || d->v_stride[2] < 0 || d->k_stride[2] > kMostStride || d->v_stride[2] > kMostStride)
+    return TQK_EINVAL;
   // (256 threads a workgroup: fewer than 2^32)
   if (d->batch && d->q_len && make_plan(*d).items > (1LL << 23)) return TQK_EINVAL;
   return TQK_OK;
