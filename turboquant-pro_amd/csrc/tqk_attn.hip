@@ -120,13 +120,16 @@ __device__ __forceinline__ float sum_half(float x) {
   return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
+// a number that is the same in every lane, in a scalar register
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // What a sequence's queries see.
 struct Seen {
   int n, m, start, sink_end, window;  // window 0: none
   __device__ __forceinline__ Seen(const AttnArgs& a, int b) {
-    n = a.kv_lens ? min(max(a.kv_lens[b], 0), a.d.kv_len) : a.d.kv_len;
-    m = a.q_lens ? min(max(a.q_lens[b], 0), a.d.q_len) : a.d.q_len;
-    start = a.kv_starts ? min(max(a.kv_starts[b], 0), n) : 0;
+    n = uni(a.kv_lens ? min(max(a.kv_lens[b], 0), a.d.kv_len) : a.d.kv_len);
+    m = uni(a.q_lens ? min(max(a.q_lens[b], 0), a.d.q_len) : a.d.q_len);
+    start = uni(a.kv_starts ? min(max(a.kv_starts[b], 0), n) : 0);
     sink_end = start + min(a.d.sinks, n - start);
     window = a.d.window > 0 && a.d.window < n ? a.d.window : 0;
   }
@@ -153,7 +156,7 @@ struct Tiles {
     second = max(lo / kKeys, first + n_first);
     n = n_first + max(0, p_hi / kKeys + 1 - second);
   }
-  __device__ __forceinline__ int at(int i) const { return kKeys * (i < n_first ? first + i : second + i - n_first); }
+  __device__ __forceinline__ int at(int i) const { return uni(kKeys * (i < n_first ? first + i : second + i - n_first)); }
 };
 
 // Rows of a compact key buffer that are left out before position j: whole tiles
@@ -192,14 +195,14 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
   __shared__ __align__(16) uint8_t k0_s[kBytes], v0_s[kBytes], k1_s[kBytes], v1_s[kBytes];
   __shared__ int odd_s;  // an infinity or a NaN among the values that only some rows see
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
-  const int Hq = a.d.n_q_heads, Hkv = a.d.n_kv_heads, gq = Hq / Hkv;
+  const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, ln = lane & 31, lh = lane >> 5;
+  const int Hq = a.d.n_q_heads, Hkv = a.d.n_kv_heads, gq = uni(Hq / Hkv);
   int item = xcd_item(blockIdx.x, gridDim.x);
-  const int split = item % a.n_splits;
+  const int split = uni(item % a.n_splits);
   item /= a.n_splits;
-  const int tile = a.row_tiles - 1 - item % a.row_tiles;  // the last rows, which see most, first
+  const int tile = uni(a.row_tiles - 1 - item % a.row_tiles);  // the last rows, which see most, first
   item /= a.row_tiles;
-  const int h = item % Hkv, b = item / Hkv;
+  const int h = uni(item % Hkv), b = uni(item / Hkv);
   const Seen s(a, b);
 
   // this lane's row
@@ -208,9 +211,9 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
   const bool inside = t < a.d.q_len, real = t < s.m;
   const int p = s.n - s.m + t, lo = s.low(p);
   // the positions of the workgroup's rows and of the wave's
-  const int t_lo = tile * kTileRows / gq, t_hi = min((tile * kTileRows + kTileRows - 1) / gq, s.m - 1);
-  const int w_lo = (tile * kTileRows + wave * kRows) / gq;
-  const int w_hi = min((tile * kTileRows + wave * kRows + kRows - 1) / gq, s.m - 1);
+  const int t_lo = uni(tile * kTileRows / gq), t_hi = min(uni((tile * kTileRows + kTileRows - 1) / gq), s.m - 1);
+  const int w_lo = uni((tile * kTileRows + wave * kRows) / gq);
+  const int w_hi = min(uni((tile * kTileRows + wave * kRows + kRows - 1) / gq), s.m - 1);
   const int p_lo = s.n - s.m + t_lo, p_hi = s.n - s.m + t_hi;
   const int wp_lo = s.n - s.m + w_lo, wp_hi = s.n - s.m + w_hi;
   const int b_lo = s.low(p_lo);                           // the first key that a row of the workgroup sees by its window
@@ -220,8 +223,8 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
   int i0 = 0, i1 = t_lo < s.m ? tiles.n : 0;
   if (a.n_splits > 1) {
     const int n = i1;
-    i0 = (int)((long long)n * split / a.n_splits);
-    i1 = (int)((long long)n * (split + 1) / a.n_splits);
+    i0 = uni((int)((long long)n * split / a.n_splits));
+    i1 = uni((int)((long long)n * (split + 1) / a.n_splits));
   }
 
   // Q^T as the second operand: row ln, channels 16 ks + 8 lh .. + 7
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
   const long long ks_ = a.d.k_stride[2] * 2, vs_ = a.d.v_stride[2] * 2;
   const char* const kb = static_cast<const char*>(a.k) + 2 * (b * a.d.k_stride[0] + h * a.d.k_stride[1]);
   const char* const vb = static_cast<const char*>(a.v) + 2 * (b * a.d.v_stride[0] + h * a.d.v_stride[1]);
-  const int gap = a.compact ? compact_gap(s) : 0;
+  const int gap = a.compact ? uni(compact_gap(s)) : 0;
   const int sink_rows = (s.sink_end + kMaxKeys - 1) / kMaxKeys * kMaxKeys;
   const int my_row = tid / CH, my_ch = tid % CH;
   const uint32_t k_off = (uint32_t)my_row * (uint32_t)ks_ + 16u * (uint32_t)(TG::k_at(my_row, my_ch) / 16 % CH);
@@ -294,15 +297,19 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
     if (!(w_lo < s.m && k0 <= wp_hi && (k0 + kKeys > wl_lo || k0 < s.sink_end))) return;
     // K Q^T: keys k0 + 32 u + 8 (r / 4) + 4 lh + r % 4 of row ln
     f16v_t S[NU];
+    // (the reads run a few products ahead: a read's latency is several products)
+    constexpr int kAhead = 4;
+    v8 kf[NU * NK];
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) S[u][r] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < NK; ++ks) {
-        const v8 kf = *reinterpret_cast<const v8*>(k_t + TG::k_at(32 * u + ln, 2 * ks + lh));
-        S[u] = Mma<T>::m32(kf, qf[ks], S[u]);
+    for (int i = 0; i < NU * NK + kAhead; ++i) {
+      if (i < NU * NK)
+        kf[i] = *reinterpret_cast<const v8*>(k_t + TG::k_at(32 * (i / NK) + ln, 2 * (i % NK) + lh));
+      if (i >= kAhead) {
+        const int u = (i - kAhead) / NK, ks = (i - kAhead) % NK;
+        if (ks == 0) S[u] = Mma<T>::m32(kf[i - kAhead], qf[ks], f16v_t{});
+        else S[u] = Mma<T>::m32(kf[i - kAhead], qf[ks], S[u]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (!(k0 + kKeys - 1 <= wp_lo && k0 >= s.start && (k0 >= wl_hi || k0 + kKeys <= s.sink_end))) {
 #pragma unroll
