@@ -3,9 +3,10 @@
 //
 // Few queries: every query is an item of its own of the decode kernels (WIN
 // instances of tqk_decode_kernels.h), which read the codes of the groups that
-// it sees and nothing else.  Many queries (fp16 caches): the visible groups are
-// reconstructed once as dense fp16 keys and values in the workspace, and
-// tqk_attention runs over them.
+// it sees and nothing else.  Many queries (fp16 caches): what they see is
+// reconstructed once as dense fp16 keys and values in the workspace, and the
+// kernels of tqk_attention run over it.
+#include "tqk_attn.h"
 #include "tqk_decode_kernels.h"
 
 namespace {
@@ -23,6 +24,239 @@ int most_groups(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   const long long cold = (long long)t->window - (hot > 0 ? hot : 0);
   long long n = ((long long)t->sinks + G - 1) / G + (cold > 0 ? (cold + G - 2) / G + 1 : 0);
   return n < all ? (int)n : all;
+}
+
+// ---- reconstruction of what a chunk's queries see ---------------------------
+// Rows [0, kept.sinks) and from the window on, moved down by kept.gap
+// (tqk_attn.h), 64 tokens of a kv head a step: keys as grid value with the
+// side-list's over it, values as (cent[code] @ Pi) * norm, hot tokens as they
+// are, all in fp16.  Pi in fp16 and the centroids times a power of two near
+// sqrt(D) in fp16 (2^-12 of a value each, as the result's own rounding), summed
+// in fp32 by the matrix cores: the rotation costs a wave 16 products a step where
+// the ordered sums of tqk_dequant_dense took 2 D VALU operations a value.
+// Bound: writing the rows (4 D bytes a token and kv head).
+constexpr int kGather = 64;  // tokens a step
+static_assert(kGather == kMaxKeys, "a step lies on one side of the gap");
+
+struct GatherArgs {
+  tqk_cache_desc d;
+  tqk_cache_ptrs p;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;
+  uint16_t* k;
+  uint16_t* v;
+  int q_len, max_len, window, sinks;
+  int rows;   // rows of a sequence and kv head
+  int steps;  // of kGather rows
+  int units;  // batch * n_kv_heads * steps
+};
+
+template <int VB, int D>
+__global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
+  constexpr int CH = D / 8;                    // 8-channel pieces of a row
+  constexpr int NT = D / 64, NK = D / 32;      // a wave's column tiles, steps of a product
+  constexpr int VROW = D * VB / 8;
+  const tqk_cache_desc& d = a.d;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, ln = lane & 15, lg = lane >> 4;
+  const int G = d.group_tokens, P = d.page_tokens, Hkv = d.n_kv_heads, kb = d.key_bits;
+  const bool polar = d.key_grid == 2;
+  __shared__ __align__(16) uint16_t k_s[kGather][D];
+  __shared__ __align__(16) uint16_t c_s[kGather * D];  // centroids, then rotated values
+  __shared__ int row_s[kGather];   // row in the head's pages; -1: a hot token
+  __shared__ int slot_s[kGather];
+  __shared__ float norm_s[2][kGather];  // value norms, key norms (PolarQuant keys)
+  __shared__ float lev_s[16], cen_s[16];
+  // centroids near 1: a power of two, exact
+  const float up = D == 64 ? 8.f : 16.f, down = 1.f / up;
+  if (tid < 16) lev_s[tid] = key_level(d.key_grid == 1, tid);
+  if (tid < (1 << VB)) cen_s[tid] = a.p.vcent[tid] * up;
+  // Pi: columns e = 16 (NT wave + nt) + ln, rows 32 ks + 8 lg .. + 7 (a row of Pi^T)
+  h8_t pf[NT][NK];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+      const float* r = a.p.pi_t + (size_t)(16 * (NT * wave + nt) + ln) * D + 32 * ks + 8 * lg;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pf[nt][ks][e] = (_Float16)r[e];
+    }
+  // place of a row's 16-byte piece: turned by the row, against bank conflicts
+  auto at = [](int t, int c) { return (t * CH + (c ^ (t & 7))) * 8; };
+
+  for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+    const int step = unit % a.steps, bh = unit / a.steps, h = bh % Hkv, b = bh / Hkv;
+    const int n = min(a.seq_lens[b], a.max_len);
+    const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+    const KeptRows kept(n, m, 0, min(a.sinks, n), a.window);
+    const int r0 = step * kGather, t0 = r0 < kept.sinks ? r0 : r0 + kept.gap;
+    const int nt_ = min(kGather, n - t0);  // tokens of this step
+    if (nt_ <= 0) continue;                // (the same for every thread)
+    const int ng = n_groups_of(n, d.hot_window, G);
+    const size_t head = (size_t)h * d.n_pages * P;
+    const size_t ring = ((size_t)b * Hkv + h) * d.hot_ring;
+    __syncthreads();  // the last step's LDS is read
+    if (tid < kGather) {
+      const int t = t0 + min(tid, nt_ - 1);
+      const bool cold = t < ng * G;
+      row_s[tid] = -1;
+      if (cold) {
+        const int row = a.p.block_table[(size_t)b * d.max_pages_per_seq + t / P] * P + t % P;
+        row_s[tid] = row;
+        slot_s[tid] = a.p.group_table[(size_t)b * d.max_groups_per_seq + t / G];
+        norm_s[0][tid] = a.p.vnorm[head + row] * down;
+        norm_s[1][tid] = polar ? a.p.knorm[head + row] * down : 0.f;
+      }
+    }
+    __syncthreads();
+    uint16_t* const ko = a.k + ((size_t)bh * a.rows + r0) * D;
+    uint16_t* const vo = a.v + ((size_t)bh * a.rows + r0) * D;
+
+    // eight codes of a row from channel 8 c on, 4-bit keys' nibbles in order
+    auto codes8 = [&](const uint8_t* row, int bits, int c, bool key) -> uint32_t {
+      const uint8_t* s = row + c * bits;
+      uint32_t w = 0;
+      if (bits == 4) {
+        w = *reinterpret_cast<const uint32_t*>(s);
+        if (key) w = __builtin_bswap32(__builtin_bitreverse32(w));
+      } else {
+        for (int i = 0; i < bits; ++i) w |= (uint32_t)s[i] << (8 * i);
+      }
+      return w;
+    };
+    auto put_centroids = [&](const uint8_t* rows, int bits, int row_bytes, bool key) {
+      for (int i = tid; i < nt_ * CH; i += kThreads) {
+        const int t = i / CH, c = i % CH;
+        if (row_s[t] < 0) continue;
+        const uint32_t w = codes8(rows + (head + row_s[t]) * row_bytes, bits, c, key);
+        h8_t x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (_Float16)cen_s[(w >> (VB * e)) & ((1 << VB) - 1)];
+        *reinterpret_cast<h8_t*>(c_s + at(t, c)) = x;
+      }
+    };
+    // c_s @ Pi times the norms, back into c_s, then out (hot rows from the ring)
+    auto rotate_out = [&](uint16_t* out, const float* norm, const uint16_t* hot) {
+      __syncthreads();
+      f4_t acc[NT][4];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[nt][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+          const h8_t x = *reinterpret_cast<const h8_t*>(c_s + at(16 * tt + ln, 4 * ks + lg));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)  // transposed: a lane gets four channels of one token
+            acc[nt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf[nt][ks], x, acc[nt][tt], 0, 0, 0);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const float f = norm[16 * tt + ln];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+          h4_t y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = (_Float16)(acc[nt][tt][e] * f);
+          const int ch = 16 * (NT * wave + nt) + 4 * lg;
+          *reinterpret_cast<h4_t*>(c_s + at(16 * tt + ln, ch / 8) + ch % 8) = y;
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < nt_ * CH; i += kThreads) {
+        const int t = i / CH, c = i % CH;
+        const uint4* src = row_s[t] < 0 ? reinterpret_cast<const uint4*>(hot + (ring + (t0 + t) % d.hot_ring) * D + 8 * c)
+                                        : reinterpret_cast<const uint4*>(c_s + at(t, c));
+        *reinterpret_cast<uint4*>(out + (size_t)t * D + 8 * c) = *src;
+      }
+    };
+
+    const uint16_t* const hot_k = static_cast<const uint16_t*>(a.p.hot_k);
+    if (polar) {
+      put_centroids(a.p.kcodes, VB, k_row_bytes(VB, D), true);
+      rotate_out(ko, norm_s[1], hot_k);
+      __syncthreads();
+    } else {
+      for (int i = tid; i < nt_ * CH; i += kThreads) {
+        const int t = i / CH, c = i % CH;
+        if (row_s[t] < 0) {
+          *reinterpret_cast<uint4*>(&k_s[t][8 * c]) =
+              *reinterpret_cast<const uint4*>(hot_k + (ring + (t0 + t) % d.hot_ring) * D + 8 * c);
+          continue;
+        }
+        const uint32_t w = codes8(a.p.kcodes + (head + row_s[t]) * k_row_bytes(kb, D), kb, c, true);
+        const size_t mb = ((size_t)slot_s[t] * Hkv + h) * D + 8 * c;
+        h8_t x;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const float4 sc = *reinterpret_cast<const float4*>(a.p.gscale + mb + e);
+          const float4 mu = *reinterpret_cast<const float4*>(a.p.gmean + mb + e);
+          const float scv[4] = {sc.x, sc.y, sc.z, sc.w}, muv[4] = {mu.x, mu.y, mu.z, mu.w};
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            x[e + f] = (_Float16)fmaf(scv[f], lev_s[(w >> (kb * (e + f))) & ((1u << kb) - 1u)], muv[f]);
+        }
+        *reinterpret_cast<h8_t*>(&k_s[t][8 * c]) = x;
+      }
+    }
+    if (D == TQK_D && v_tiled(G, P, D, 0)) {
+      // unit (lg, c) of a 16-token tile: tokens 4 lg .. + 3 x channels 8 c .. + 7
+      const int tile = tid >> 6, ul = (tid >> 4) & 3, uc = tid & 15;
+      if (16 * tile < nt_ && row_s[16 * tile] >= 0) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(a.p.vcodes + (head + row_s[16 * tile]) * VROW +
+                                                                v_unit_offset(ul, uc, VROW));
+        uint32_t w[VB];
+#pragma unroll
+        for (int i = 0; i < VB; ++i) w[i] = src[i];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          h8_t x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = (_Float16)cen_s[stream_code<VB>(w, 4 * e + t)];
+          *reinterpret_cast<h8_t*>(c_s + at(16 * tile + 4 * ul + t, uc)) = x;
+        }
+      }
+    } else {
+      put_centroids(a.p.vcodes, VB, VROW, false);
+    }
+    if (!polar) {
+      __syncthreads();
+      if (d.outliers_per_channel > 0) {
+        // the side-list entries of the step's tokens, group by group
+        const int end = min(t0 + nt_, ng * G);
+        for (int g = t0 / G; g * G < end; ++g) {
+          const int lo_t = max(t0, g * G), hi_t = min(end, (g + 1) * G);
+          const size_t ob = (size_t)slot_s[lo_t - t0] * Hkv + h;
+          const int32_t* oc = a.p.ocount + ob * TQK_NOB;
+          const int q = (lo_t - g * G) / TQK_OBLK;
+          const int lo = min(q > 0 ? oc[q - 1] : 0, d.outlier_cap);
+          const int hi = min(oc[(hi_t - 1 - g * G) / TQK_OBLK], d.outlier_cap);
+          for (int e = lo + tid; e < hi; e += kThreads) {
+            const uint32_t ent = a.p.oent[ob * d.outlier_cap + e], pos = ent & 0xFFFFu;
+            const int t = g * G + (int)(pos / D);
+            if (t >= lo_t && t < hi_t) k_s[t - t0][pos % D] = (uint16_t)(ent >> 16);
+          }
+        }
+        __syncthreads();
+      }
+      for (int i = tid; i < nt_ * CH; i += kThreads)
+        reinterpret_cast<uint4*>(ko)[i] = reinterpret_cast<const uint4*>(&k_s[0][0])[i];
+    }
+    rotate_out(vo, norm_s[0], static_cast<const uint16_t*>(a.p.hot_v));
+  }
+}
+
+template <int D>
+void launch_gather(const GatherArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.units < 2048 ? a.units : 2048));
+  if (a.d.value_bits == 2)
+    hipLaunchKernelGGL((tqk_gather_seen<2, D>), grid, dim3(kThreads), 0, st, a);
+  else if (a.d.value_bits == 3)
+    hipLaunchKernelGGL((tqk_gather_seen<3, D>), grid, dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((tqk_gather_seen<4, D>), grid, dim3(kThreads), 0, st, a);
 }
 
 struct AttendPlan {
@@ -68,6 +302,15 @@ bool dense_path(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   return !d->input_f32 && t->out_type == 1 && t->q_len > 8;
 }
 
+// Rows that a sequence's queries see at most, in whole tiles.
+int kept_rows(const tqk_attend_desc* t) {
+  const long long tile = kMaxKeys, all = ((long long)t->max_len + tile - 1) / tile * tile;
+  if (t->window == 0 || t->window >= t->max_len) return (int)all;
+  const long long sinks = t->sinks < t->max_len ? t->sinks : t->max_len;
+  const long long rows = (sinks + tile - 1) / tile * tile + ((long long)t->window + t->q_len + tile - 2) / tile * tile + tile;
+  return (int)(rows < all ? rows : all);
+}
+
 tqk_attn_desc dense_desc(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   tqk_attn_desc a{};
   a.batch = t->batch;
@@ -84,7 +327,7 @@ tqk_attn_desc dense_desc(const tqk_cache_desc* d, const tqk_attend_desc* t) {
     a.q_stride[i] = t->q_stride[i];
     a.o_stride[i] = t->o_stride[i];
   }
-  const int64_t row = d->head_dim, head = row * t->max_len;
+  const int64_t row = d->head_dim, head = row * kept_rows(t);
   a.k_stride[0] = a.v_stride[0] = head * d->n_kv_heads;
   a.k_stride[1] = a.v_stride[1] = head;
   a.k_stride[2] = a.v_stride[2] = row;
@@ -179,10 +422,31 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
     uint16_t* v = k + (size_t)t->batch * a.k_stride[0];
     uint16_t* ws = v + (size_t)t->batch * a.k_stride[0];
     if (t->max_len > 0) {
-      const int rd = tqk_dequant_dense(d, p, t->batch, seq_lens, t->max_len, 1, k, v, stream);
-      if (rd != TQK_OK) return rd;
+      GatherArgs g{};
+      g.d = *d;
+      g.p = *p;
+      g.seq_lens = seq_lens;
+      g.q_lens = q_lens;
+      g.k = k;
+      g.v = v;
+      g.q_len = t->q_len;
+      g.max_len = t->max_len;
+      g.window = t->window;
+      g.sinks = t->sinks;
+      g.rows = kept_rows(t);
+      g.steps = g.rows / kGather;
+      const long long units = (long long)t->batch * d->n_kv_heads * g.steps;
+      if (units > INT32_MAX) return TQK_EINVAL;
+      g.units = (int)units;
+      if (d->head_dim == 64)
+        launch_gather<64>(g, st);
+      else if (d->head_dim == 128)
+        launch_gather<128>(g, st);
+      else
+        launch_gather<256>(g, st);
+      if (hipGetLastError() != hipSuccess) return TQK_EHIP;
     }
-    return tqk_attention(&a, q, k, v, seq_lens, q_lens, nullptr, out, ws, tqk_attention_workspace_bytes(&a), stream);
+    return tqk_run_attention(&a, q, k, v, seq_lens, q_lens, nullptr, out, ws, tqk_attention_workspace_bytes(&a), 1, stream);
   }
   const AttendPlan ap = attend_plan(d, t);
   const Plan& pl = ap.pl;

@@ -16,7 +16,7 @@
 // scores come in).  V^T comes from LDS by transposing reads.
 // Bound: the matrix cores and, as closely, LDS reads (16 KiB of K and V for
 // 32 x 64 scores a wave).
-#include "tqk_common.h"
+#include "tqk_attn.h"
 
 namespace {
 
@@ -32,7 +32,6 @@ constexpr int kTileRows = 128; // rows a workgroup
 // keys a tile: at head_dim 256 half as many, which leaves the accumulators their registers
 template <int D>
 constexpr int kTileKeys = D == 256 ? 32 : 64;
-constexpr int kMaxKeys = 64;
 // The running maximum follows the scores only when one exceeds it by this much
 // (log2 units): weights stay at most 2^8, far inside fp16's range, and the
 // accumulators are rescaled a few times a row instead of every tile.
@@ -159,14 +158,6 @@ struct Tiles {
   __device__ __forceinline__ int at(int i) const { return uni(kKeys * (i < n_first ? first + i : second + i - n_first)); }
 };
 
-// Rows of a compact key buffer that are left out before position j: whole tiles
-// between the first visible tokens' and the first of the sequence's window.
-__device__ __forceinline__ int compact_gap(const Seen& s) {
-  const int lo = max(s.low(s.n - s.m), 0) / kMaxKeys * kMaxKeys;
-  const int sink = (s.sink_end + kMaxKeys - 1) / kMaxKeys * kMaxKeys;
-  return max(0, lo - sink);
-}
-
 // blockIdx -> item so that consecutive items, which share keys, go to one XCD
 // (workgroups are dealt to the 8 XCDs, each with its own L2, one after another)
 __device__ __forceinline__ int xcd_item(int x, int n) {
@@ -251,8 +242,8 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
   const long long ks_ = a.d.k_stride[2] * 2, vs_ = a.d.v_stride[2] * 2;
   const char* const kb = static_cast<const char*>(a.k) + 2 * (b * a.d.k_stride[0] + h * a.d.k_stride[1]);
   const char* const vb = static_cast<const char*>(a.v) + 2 * (b * a.d.v_stride[0] + h * a.d.v_stride[1]);
-  const int gap = a.compact ? uni(compact_gap(s)) : 0;
-  const int sink_rows = (s.sink_end + kMaxKeys - 1) / kMaxKeys * kMaxKeys;
+  const KeptRows kept(s.n, s.m, s.start, s.sink_end, s.window);
+  const int gap = a.compact ? uni(kept.gap) : 0, sink_rows = uni(kept.sinks);
   const int my_row = tid / CH, my_ch = tid % CH;
   const uint32_t k_off = (uint32_t)my_row * (uint32_t)ks_ + 16u * (uint32_t)(TG::k_at(my_row, my_ch) / 16 % CH);
   const uint32_t v_off = (uint32_t)my_row * (uint32_t)vs_ + 16u * (uint32_t)(TG::v_at(my_row, my_ch) / 16 % CH);
@@ -572,6 +563,14 @@ size_t tqk_attention_workspace_bytes(const tqk_attn_desc* d) {
 int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const void* v,
                   const int32_t* kv_lens, const int32_t* q_lens, const int32_t* kv_starts, void* out,
                   void* workspace, size_t workspace_bytes, void* stream) {
+  return tqk_run_attention(d, q, k, v, kv_lens, q_lens, kv_starts, out, workspace, workspace_bytes, 0, stream);
+}
+
+}  // extern "C"
+
+int tqk_run_attention(const tqk_attn_desc* d, const void* q, const void* k, const void* v, const int32_t* kv_lens,
+                      const int32_t* q_lens, const int32_t* kv_starts, void* out, void* workspace,
+                      size_t workspace_bytes, int compact, void* stream) {
   const int rc = check_attn(d);
   if (rc != TQK_OK) return rc;
   if (!d->batch || !d->q_len) return TQK_OK;
@@ -592,6 +591,7 @@ int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const vo
   a.row_tiles = pl.row_tiles;
   a.n_splits = pl.n_splits;
   a.rows = pl.rows;
+  a.compact = compact;
   // the accumulators first: 16-byte stores
   a.part_acc = static_cast<float*>(workspace);
   a.part_ml = a.part_acc + (size_t)pl.n_splits * pl.rows * d->head_dim;
@@ -602,5 +602,3 @@ int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const vo
     launch_tiles<__bf16>(a, pl.items, st);
   return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
 }
-
-}  // extern "C"
