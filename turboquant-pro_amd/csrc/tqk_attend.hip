@@ -1,17 +1,19 @@
 // Attention of one or more new queries a sequence over the two-tier cache, with
 // a sliding window and first tokens that stay visible (gfx950).
 //
-// Few queries: every query is an item of its own of the decode kernels (WIN
-// instances of tqk_decode_kernels.h), which read the codes of the groups that
-// it sees and nothing else.  Many queries (fp16 caches): what they see is
-// reconstructed once as dense fp16 keys and values in the workspace, and the
-// kernels of tqk_attention run over it.
+// Few queries: tqk_attend_codes reads the codes of the tokens that they see and
+// nothing else.  Many queries (fp16 caches): what they see is reconstructed once
+// as dense fp16 keys and values in the workspace, and the kernels of
+// tqk_attention run over it.  fp32 caches: every query is an item of its own of
+// the VALU decode (WIN instances of tqk_decode_kernels.h).
+#include "tqk_attend.h"
 #include "tqk_attn.h"
 #include "tqk_decode_kernels.h"
 
 namespace {
 
-constexpr int kMostItems = 4096;  // queries a launch (bounds the partials and the grid)
+constexpr int kMostItems = 4096;  // fp32 caches: queries a launch (bounds the partials and the grid)
+constexpr int kFewMost = 64;      // rows (queries times query heads of a kv head) attended on codes
 
 // Coded groups that one query sees at most, past `max_len` tokens of cache: the
 // first tokens', and the window's less what the hot window holds of it.  A cache
@@ -265,33 +267,12 @@ struct AttendPlan {
   size_t ws_bytes;
 };
 
+// The VALU decode's plan (fp32 caches).
 AttendPlan attend_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   AttendPlan ap{};
   const long long items = (long long)t->batch * t->q_len;
   ap.items = (int)(items < kMostItems ? items : kMostItems);
-  const int n = most_groups(d, t);
-  ap.pl = plan_groups(d, ap.items, n, t->max_len < d->hot_window ? t->max_len : d->hot_window);
-  if (mfma_path(*d) && n > 0) {
-    // A window's few groups in equal shares of blocks: s splits of g groups, each
-    // wave an eighth of a split's blocks (wave_blocks), by the same cost in
-    // groups per wave as plan_groups, with the mid-group starts on top.
-    const int nblk = d->group_tokens / 32, ncu = device_cus();
-    const long long pairs = (long long)ap.items * d->n_kv_heads;
-    double best = 1e30;
-    for (int s = 1; s <= n; ++s) {
-      int g = (n + s - 1) / s;
-      while ((g * nblk) % kMWaves) ++g;
-      if (g > kMaxGPS) continue;
-      const long long rounds = (pairs * ((n + g - 1) / g) + ncu - 1) / ncu;
-      const double cost = (double)rounds * ((double)g / kMWaves + 0.45);
-      if (cost < best - 1e-9) {
-        best = cost;
-        ap.pl.groups_per_split = g;
-        ap.pl.wave_blocks = g * nblk / kMWaves;
-        ap.pl.n_cold_splits = ap.pl.n_hot_splits = (n + g - 1) / g;
-      }
-    }
-  }
+  ap.pl = plan_groups(d, ap.items, most_groups(d, t), t->max_len < d->hot_window ? t->max_len : d->hot_window);
   const size_t ns = (size_t)(ap.pl.n_cold_splits + ap.pl.n_hot_splits);
   ap.ws_bytes = (size_t)ap.items * d->n_q_heads * ns * sizeof(float) * (2 + d->head_dim) + 256;
   return ap;
@@ -299,7 +280,7 @@ AttendPlan attend_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
 
 // Whether the queries go over reconstructed keys and values.
 bool dense_path(const tqk_cache_desc* d, const tqk_attend_desc* t) {
-  return !d->input_f32 && t->out_type == 1 && t->q_len > 8;
+  return !d->input_f32 && t->out_type == 1 && (long long)t->q_len * (d->n_q_heads / d->n_kv_heads) > kFewMost;
 }
 
 // Rows that a sequence's queries see at most, in whole tiles.
@@ -345,18 +326,6 @@ int check_attend(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   return TQK_OK;
 }
 
-template <int GQ, int KB>
-void launch_mfma_kb(const SplitArgs<true>& a, dim3 g1, hipStream_t st) {
-  if (a.d.key_grid == 2)  // PolarQuant keys: value_bits == key_bits
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, KB, KB, true, true>), g1, dim3(kMThreads), 0, st, a);
-  else if (a.d.value_bits == 2)
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 2, KB, false, true>), g1, dim3(kMThreads), 0, st, a);
-  else if (a.d.value_bits == 3)
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 3, KB, false, true>), g1, dim3(kMThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 4, KB, false, true>), g1, dim3(kMThreads), 0, st, a);
-}
-
 template <int GQ, int D>
 void launch_valu(const SplitArgs<true>& a, dim3 grid, hipStream_t st) {
   if (a.d.value_bits == 2)
@@ -369,21 +338,12 @@ void launch_valu(const SplitArgs<true>& a, dim3 grid, hipStream_t st) {
 
 template <int GQ>
 void launch_split(const SplitArgs<true>& a, dim3 grid, hipStream_t st) {
-  if (mfma_path(a.d)) {
-    const dim3 g1(grid.x * grid.y * grid.z);  // over (split, kv head, item)
-    if (a.d.key_bits == 4)
-      launch_mfma_kb<GQ, 4>(a, g1, st);
-    else if (a.d.key_bits == 3)
-      launch_mfma_kb<GQ, 3>(a, g1, st);
-    else
-      launch_mfma_kb<GQ, 2>(a, g1, st);
-  } else if (a.d.head_dim == 64) {
+  if (a.d.head_dim == 64)
     launch_valu<GQ, 64>(a, grid, st);
-  } else if (a.d.head_dim == 128) {
+  else if (a.d.head_dim == 128)
     launch_valu<GQ, 128>(a, grid, st);
-  } else {
+  else
     launch_valu<GQ, 256>(a, grid, st);
-  }
 }
 
 template <int D>
@@ -402,6 +362,7 @@ size_t tqk_attend_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc
     const tqk_attn_desc a = dense_desc(d, t);
     return 4 * (size_t)t->batch * a.k_stride[0] + ((tqk_attention_workspace_bytes(&a) + 255) & ~(size_t)255);
   }
+  if (!d->input_f32) return tqk_few_workspace_bytes(d, t);
   return attend_plan(d, t).ws_bytes;
 }
 
@@ -448,12 +409,10 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
     }
     return tqk_run_attention(&a, q, k, v, seq_lens, q_lens, nullptr, out, ws, tqk_attention_workspace_bytes(&a), 1, stream);
   }
+  if (!d->input_f32) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, stream);
   const AttendPlan ap = attend_plan(d, t);
   const Plan& pl = ap.pl;
   const int gq = d->n_q_heads / d->n_kv_heads;
-  const bool mfma = mfma_path(*d);
-  // one split of 4 or 8 heads: the split kernel ends with the output itself
-  const bool direct = mfma && pl.n_cold_splits == 1 && gq > 2;
   const int n_splits = pl.n_cold_splits + pl.n_hot_splits;
   SplitArgs<true> a{};
   a.d = *d;
@@ -467,10 +426,8 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
   a.n_cold_splits = pl.n_cold_splits;
   a.n_hot_splits = pl.n_hot_splits;
   a.groups_per_split = pl.groups_per_split;
-  a.wave_blocks = pl.wave_blocks;
   a.hot_per_split = pl.hot_per_split;
   a.batch = t->batch;
-  a.out = direct ? static_cast<float*>(out) : nullptr;
   a.w.q_lens = q_lens;
   a.w.q_len = t->q_len;
   a.w.max_len = t->max_len;
@@ -485,7 +442,7 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
   for (long long i0 = 0; i0 < items; i0 += ap.items) {
     const int n = (int)(items - i0 < ap.items ? items - i0 : ap.items);
     a.w.item0 = (int)i0;
-    const dim3 grid(mfma ? pl.n_cold_splits : n_splits, d->n_kv_heads, n);
+    const dim3 grid(n_splits, d->n_kv_heads, n);
     switch (gq) {
       case 1: launch_split<1>(a, grid, st); break;
       case 2: launch_split<2>(a, grid, st); break;
@@ -493,7 +450,6 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
       default: launch_split<8>(a, grid, st); break;
     }
     if (hipGetLastError() != hipSuccess) return TQK_EHIP;
-    if (direct) continue;
     JoinArgs<true> m{};
     m.pm = a.pm;
     m.pl = a.pl;

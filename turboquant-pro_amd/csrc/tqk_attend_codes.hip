@@ -1,0 +1,865 @@
+// Attention of few queries over the codes of an fp16 cache, with a sliding window
+// and first tokens that stay visible (gfx950).
+//
+// A workgroup takes one kv head of one sequence, up to 16 rows (the kv head's
+// query heads, of several queries where they fit) and a share of the blocks of
+// 32 tokens that any of the rows sees; its eight waves take runs of blocks,
+// coded or uncoded, each on its own until the end.
+//
+// A coded block, 16 tokens at a time: a pair of key codes is an entry of a table
+// of fp16 levels, four of them an operand of K Q^T as they are; the group's scale
+// goes into the query (an fp16 pair: 2^-22), its mean into the scores' start.  A
+// side-list entry, whose code is the zero level, adds q (val - mean): the tile's
+// entries stand as fp16 pairs in an otherwise zero LDS tile of the wave, which is
+// a second operand for the same product and is cleared entry by entry.  A lane
+// then holds one row's scores of 8 tokens, which are the operand of V^T P^T as
+// they are.  Value codes become centroids by pairs through a table.  Both
+// codebooks are scaled so that their fp16 roundings nearly vanish (best of 128
+// scales: 2^-12 of a level becomes 2^-14 to 2^-15); weights times norms are
+// rounded to fp16 (2^-12 of each).  The coded part is rotated back once a
+// workgroup, by the matrix cores in fp16 pairs.
+// Bound: few sequences, the chain of dependent loads (lengths, tables, codes);
+// many, the table reads and VALU work of a block beside its codes from HBM.
+#include "tqk_attend.h"
+#include "tqk_wave.h"
+
+namespace {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves, kFewRows = 16;
+constexpr float kFewLazy = 2.0f;  // log2 units: weights stay at most 4, norms at most TQK_MAX_VNORM: fp16
+constexpr int kPairCopies = 4;    // copies of the pair tables, by lane, against bank conflicts
+
+struct FewArgs {
+  tqk_cache_desc d;
+  tqk_cache_ptrs p;
+  const uint16_t* q;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;
+  void* out;
+  float* part_acc;  // [split][row][D]
+  float* part_ml;   // [split][row][2]: running maximum (log2 units) and sum
+  long long rows;   // rows of all sequences, heads and queries
+  long long q_stride[3];
+  long long o_stride[3];
+  int q_len, max_len, window, sinks, out_type;
+  int per_item;     // queries of a workgroup
+  int q_items;      // workgroups a sequence's queries take
+  int n_splits;
+};
+
+// A run of blocks in two pieces, [0, n0) and [from, from + n - n0): the first
+// tokens' and the window's.
+struct BlockRuns {
+  int n0, from, n;
+  __device__ __forceinline__ int at(int i) const { return i < n0 ? i : i - n0 + from; }
+};
+
+// KB: key code bits; PK: PolarQuant keys (KB == VB); TILED: value codes in units
+// of 4 tokens x 8 channels.
+template <int D, int VB, int KB, bool PK, bool TILED>
+__global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes(FewArgs a) {
+  constexpr int CPL = D / 4;          // channels of a lane in a score product: CPL lg + 8 m + e
+  constexpr int NM = D / 32;          // steps of a score product
+  constexpr int KW = CPL * KB / 32 > 0 ? (CPL * KB + 31) / 32 : 1;  // words of a lane's key codes
+  constexpr int NC = D >= 128 ? 8 : 4;          // channels of a lane's value piece
+  constexpr int NS = D == 256 ? 2 : 1;          // value pieces a lane takes (128 channels apart)
+  constexpr int NV = NC * NS;                   // 16-row accumulator tiles
+  constexpr int VROW = D * VB / 8, KROW = D * KB / 8;
+  const tqk_cache_desc& d = a.d;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int ln = lane & 15, lg = lane >> 4;
+  const int G = d.group_tokens, P = d.page_tokens, Hkv = d.n_kv_heads, Hq = d.n_q_heads, gq = Hq / Hkv;
+  int x = blockIdx.x;
+  const int split = x % a.n_splits;
+  x /= a.n_splits;
+  const int h = x % Hkv;
+  x /= Hkv;
+  const int q0 = x % a.q_items * a.per_item, b = x / a.q_items;
+
+  // a wave's side-list tile (hi, then lo: 16 x D fp16 each), later its accumulators
+  __shared__ __align__(16) uint16_t stage_s[kFewWaves][2 * 16 * D];
+  __shared__ __align__(16) float stat_s[kFewWaves][2][D];    // the group's scale and mean
+  __shared__ uint32_t key_s[(1 << (2 * KB)) * kPairCopies];  // a pair of key codes -> two fp16 levels
+  __shared__ uint32_t val_s[(1 << (2 * VB)) * kPairCopies];  // a pair of value codes -> two fp16 centroids
+  __shared__ float lev_s[16], cen_s[16];
+  __shared__ float ml_s[2][kFewWaves][kFewRows];
+
+  const int n = min(a.seq_lens[b], a.max_len);
+  const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+  if (tid < 16) lev_s[tid] = PK ? a.p.vcent[tid & ((1 << VB) - 1)] : key_level(d.key_grid, tid);
+  if (tid < (1 << VB)) cen_s[tid] = a.p.vcent[tid];
+  // the rows: query q0 + row / gq, head h gq + row % gq
+  const int n_rows = min(a.per_item, m - q0) * gq;  // (negative: none)
+  const int row = min(ln, max(n_rows, 1) - 1), t = q0 + row / gq, p = n - m + t;
+  const int p_lo = n - m + q0, p_hi = n - m + min(q0 + a.per_item, m) - 1;
+  const int ng = n_groups_of(n, d.hot_window, G), n_cold = ng * G;
+  auto low = [&](int pos) { return a.window > 0 && a.window <= pos ? pos - a.window + 1 : 0; };
+  const int lo = low(p), lo_first = low(p_lo), lo_last = low(p_hi);
+  const int sinks = min(a.sinks, max(n, 0));
+  auto sees = [&](int tok) { return (tok <= p) & ((tok >= lo) | (tok < sinks)); };
+  auto all_see = [&](int tok, int cnt) { return tok + cnt - 1 <= p_lo && (tok >= lo_last || tok + cnt <= sinks); };
+  // blocks of tokens [from, to) that any row sees, by block(token)
+  auto runs = [&](int from, int to, auto block) {
+    BlockRuns r{0, 0, 0};
+    const int end = min(to, p_hi + 1), s_end = min(min(sinks, end), max(lo_first, from));
+    if (n_rows <= 0 || end <= from) return r;
+    if (s_end > from) r.n0 = block(s_end - 1) + 1;
+    r.from = r.n0;
+    r.n = r.n0;
+    const int w = max(lo_first, from);
+    if (w < end) {
+      r.from = max(block(w), r.n0);
+      r.n += max(block(end - 1) + 1 - r.from, 0);
+    }
+    return r;
+  };
+  const int nblk = (G + 31) / 32;  // blocks of a group
+  const BlockRuns cold = runs(0, n_cold, [&](int tok) { return tok / G * nblk + tok % G / 32; });
+  const BlockRuns hot = runs(n_cold, n, [&](int tok) { return (tok - n_cold) / 32; });
+  // equal runs for the waves of all splits, coded ones first
+  const int n_waves = a.n_splits * kFewWaves;
+  int run = max((cold.n + hot.n + n_waves - 1) / n_waves, 1);
+  while ((cold.n + run - 1) / run + (hot.n + run - 1) / run > n_waves) ++run;
+  const int cold_waves = (cold.n + run - 1) / run;
+  const int gw = split * kFewWaves + wave;
+  const bool is_cold = gw < cold_waves;
+  const int i0 = (is_cold ? gw : gw - cold_waves) * run;
+  const int i1 = min(i0 + run, is_cold ? cold.n : hot.n);
+  __syncthreads();
+
+  // the scale of a codebook: candidate 1 + i / 128 whose entries lose least to
+  // fp16, the first of equals
+  auto best_scale = [&](const float* book, int size) {
+    float err[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float g = 1.0f + (float)(lane + 64 * k) * (1.0f / 128);
+      float e = 0.f;
+      for (int i = 0; i < size; ++i) {
+        const float y = book[i] * g, r = y - (float)(_Float16)y;
+        e = fmaf(r, r, e);
+      }
+      err[k] = e / (g * g);
+    }
+    const float best = -wave_reduce<true>(-fminf(err[0], err[1]));
+    const uint64_t b0 = __builtin_amdgcn_ballot_w64(err[0] == best), b1 = __builtin_amdgcn_ballot_w64(err[1] == best);
+    return 1.0f + (float)(b0 ? __builtin_ctzll(b0) : b1 ? 64 + __builtin_ctzll(b1) : 0) * (1.0f / 128);
+  };
+  const float up = best_scale(cen_s, 1 << VB), k_up = best_scale(lev_s, 1 << KB);
+  for (int i = tid; i < (1 << (2 * VB)) * kPairCopies; i += kFewThreads)
+    val_s[i] = pk_f16(cen_s[i / kPairCopies & ((1 << VB) - 1)] * up, cen_s[i / kPairCopies >> VB] * up);
+  for (int i = tid; i < (1 << (2 * KB)) * kPairCopies; i += kFewThreads)
+    key_s[i] = pk_f16(lev_s[k_code_even(i / kPairCopies, KB)] * k_up, lev_s[k_code_odd(i / kPairCopies, KB)] * k_up);
+  // table reads: the field of `bits` bits at `sh` of w, as an entry of 16 bytes and this lane's copy of it
+  static_assert(kPairCopies == 4, "entries of 16 bytes");
+  const uint32_t copy = 4 * (lane % kPairCopies);
+  auto entry = [&](const uint32_t* table, uint32_t w, int sh, int bits) {
+    const uint32_t mask = ((1u << bits) - 1u) << 4;
+    const uint32_t o = ((sh >= 4 ? w >> (sh - 4) : w << (4 - sh)) & mask) | copy;
+    return *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(table) + o);
+  };
+  // ... of a word array, at any bit
+  auto field = [&](const uint32_t* table, const uint32_t* w, int bit, int bits) {
+    const int wd = bit / 32, sh = bit % 32;
+    return sh + bits > 32 ? entry(table, __builtin_amdgcn_alignbit(w[wd + 1], w[wd], sh), 0, bits)
+                          : entry(table, w[wd], sh, bits);
+  };
+  // (the side-list tile starts at zero)
+#pragma unroll
+  for (int i = 0; i < 4 * D / 64; ++i) reinterpret_cast<u32x4_t*>(stage_s[wave])[64 * i + lane] = u32x4_t{0u, 0u, 0u, 0u};
+
+  // Q: row ln, channels CPL lg + 8 m .. + 7 (rows past the last: a real one's, dropped later)
+  h8_t qf[NM];
+  const uint16_t* const qp = a.q + b * a.q_stride[0] + (h * gq + row % gq) * a.q_stride[1] +
+                             (long long)min(max(t, 0), a.q_len - 1) * a.q_stride[2];
+#pragma unroll
+  for (int mm = 0; mm < NM; ++mm) qf[mm] = *reinterpret_cast<const h8_t*>(qp + CPL * lg + 8 * mm);
+  // the coded keys' weights, an fp16 pair: q * scale / k_up, group by group, or
+  // for rotated keys q @ Pi^T / k_up
+  h8_t wh[NM], wl[NM];
+  if constexpr (PK) {
+    __syncthreads();
+    float* const q_s = reinterpret_cast<float*>(&stage_s[0][0]);  // [16][D]
+    float* const r_s = reinterpret_cast<float*>(&stage_s[1][0]);  // [16][D]
+    if (wave == 0) {
+#pragma unroll
+      for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q_s[ln * D + CPL * lg + 8 * mm + e] = (float)qf[mm][e];
+    }
+    __syncthreads();
+    for (int i = tid; i < kFewRows * D; i += kFewThreads) {
+      const int r = i / D, j = i % D;
+      float y = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < D; ++k) y = fmaf(q_s[r * D + k], a.p.pi_t[k * D + j], y);
+      r_s[i] = y / k_up;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = r_s[ln * D + CPL * lg + 8 * mm + e];
+        wh[mm][e] = (_Float16)y;
+        wl[mm][e] = (_Float16)(y - (float)wh[mm][e]);
+      }
+  }
+  __syncthreads();
+
+  const float c = d.sm_scale * 1.4426950408889634f;
+  float m_run = -INFINITY, l_run = 0.f;
+  f4_t O[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) O[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+
+  // the 8 scores of row ln: tokens 4 lg + i, then 16 + 4 lg + i, of a block at
+  // tok0; tokens from cnt on are none.  Returns the weights.
+  auto weights = [&](const f4_t (&S)[2], int tok0, int cnt, float (&w)[8]) {
+    float sc[8];
+    const bool whole = cnt == 32 && all_see(tok0, 32);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int o = 16 * (i / 4) + 4 * lg + i % 4;
+      sc[i] = S[i / 4][i % 4] * c;
+      if (!whole) sc[i] = o < cnt && sees(tok0 + o) ? sc[i] : -INFINITY;
+      mx = fmaxf(mx, sc[i]);
+    }
+    if (__any(mx > m_run + kFewLazy)) {
+      mx = colgroup_max(mx);
+      const float m_new = fmaxf(m_run, mx);
+      const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) O[i] *= f;
+    }
+    const float at = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(sc[i] - at);
+      l_run += w[i];
+    }
+  };
+
+  if (is_cold && i0 < i1) {
+    uint16_t* const hi_s = stage_s[wave];
+    uint16_t* const lo_s = hi_s + 16 * D;
+    auto at = [](int tok, int ch) { return (tok * (D / 8) + (ch ^ (tok & 7))) * 8; };  // (turned by the row: bank conflicts)
+    const size_t head = (size_t)h * d.n_pages * P;
+    const int32_t* const bt = a.p.block_table + (size_t)b * d.max_pages_per_seq;
+    const int32_t* const gt = a.p.group_table + (size_t)b * d.max_groups_per_seq;
+    const bool listed = !PK && d.outliers_per_channel > 0;
+    // (a valid pointer even without a side-list)
+    const uint32_t* const oent = listed ? a.p.oent : reinterpret_cast<const uint32_t*>(a.p.ocount);
+    const int cap = listed ? d.outlier_cap : 1;
+
+    // Every load of the loop is issued, at an index inside its table, so that the
+    // waits on them stay exact.  Slots and side-list bounds of 64 blocks at a
+    // time, one a lane: their chain of loads is paid once.
+    int meta_slot = 0, meta_lo = 0, meta_hi = 0, meta_i = i0;
+    auto load_meta = [&](int i) {
+      meta_i = i;
+      const int blk = cold.at(min(i + lane, i1 - 1)), g = blk / nblk, k = blk % nblk;
+      meta_slot = gt[g];
+      const int32_t* oc = a.p.ocount + ((size_t)meta_slot * Hkv + h) * TQK_NOB;
+      const int lo_ = oc[max(k - 1, 0)], hi_ = oc[k];
+      meta_lo = listed && k > 0 ? min(lo_, cap) : 0;
+      meta_hi = listed ? min(hi_, cap) : 0;
+    };
+    // the page row of token lane % 32 of block i of the run (past its tokens: the last)
+    auto row_of = [&](int i) {
+      const int blk = cold.at(min(i, i1 - 1)), g = blk / nblk, k = blk % nblk;
+      const int tok = g * G + min(32 * k + (lane & 31), G - 1);
+      return bt[tok / P] * P + tok % P;
+    };
+    constexpr int SPL = D / 64;  // channels a lane brings of the next group's scale and mean
+    uint32_t kw[2][KW], ent[2];
+    float nsc[SPL], nmu[SPL];
+    uint32_t vw[NS][8];
+    float norm = 0.f, kn = 0.f;
+    size_t ob = 0;
+    int e_lo = 0, e_hi = 0;
+    auto load_keys = [&](int i, int rw) {
+      ob = (size_t)__builtin_amdgcn_readlane(meta_slot, i - meta_i) * Hkv + h;
+      e_lo = __builtin_amdgcn_readlane(meta_lo, i - meta_i);
+      e_hi = __builtin_amdgcn_readlane(meta_hi, i - meta_i);
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        const int rr = __shfl(rw, 16 * tile + ln, 64);
+        const uint8_t* src = a.p.kcodes + (head + rr) * KROW + lg * (CPL * KB / 8);
+        if constexpr (CPL * KB % 32 == 0) {
+#pragma unroll
+          for (int e = 0; e < KW; ++e) kw[tile][e] = reinterpret_cast<const uint32_t*>(src)[e];
+        } else {  // six bytes (3-bit keys at head_dim 64)
+          const uint16_t* s2 = reinterpret_cast<const uint16_t*>(src);
+          kw[tile][0] = (uint32_t)s2[0] | (uint32_t)s2[1] << 16;
+          kw[tile][1] = s2[2];
+        }
+      }
+      if constexpr (PK) {
+        kn = a.p.knorm[head + rw];
+      } else {
+#pragma unroll
+        for (int e = 0; e < SPL; ++e) {
+          nsc[e] = a.p.gscale[ob * D + SPL * lane + e];
+          nmu[e] = a.p.gmean[ob * D + SPL * lane + e];
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) ent[s] = oent[ob * cap + min(e_lo + lane + 64 * s, cap - 1)];
+      }
+    };
+    // a group's weights and the start of its scores (q . mean)
+    float bias = 0.f;
+    auto begin_group = [&]() {
+#pragma unroll
+      for (int e = 0; e < SPL; ++e) {
+        stat_s[wave][0][SPL * lane + e] = nsc[e];
+        stat_s[wave][1][SPL * lane + e] = nmu[e];
+      }
+      wave_sync();
+      const float inv = 1.0f / k_up;
+      float y = 0.f;
+#pragma unroll
+      for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const int ch = CPL * lg + 8 * mm + e;
+          const f4_t s4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][0][ch]);
+          const f4_t m4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][1][ch]);
+          float x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float q1 = (float)qf[mm][e + k];
+            y = fmaf(q1, m4[k], y);
+            x[k] = q1 * (s4[k] * inv);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            // (towards zero: two in one instruction, and no infinity up to 2 * 65504)
+            const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x[k], x[k + 1]));
+            const h2_t ll = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hh.x, -1.f, x[k]),
+                                                                                fmaf((float)hh.y, -1.f, x[k + 1])));
+            wh[mm][e + k] = hh.x;
+            wh[mm][e + k + 1] = hh.y;
+            wl[mm][e + k] = ll.x;
+            wl[mm][e + k + 1] = ll.y;
+          }
+        }
+      bias = colgroup_sum(y);
+    };
+    auto load_values = [&](int rw) {
+      norm = a.p.vnorm[head + rw];
+      if constexpr (TILED) {
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+          const int rr = __builtin_amdgcn_readlane(rw, 16 * tile);
+          const uint32_t* src =
+              reinterpret_cast<const uint32_t*>(a.p.vcodes + (head + rr) * VROW + v_unit_offset(lg, ln, VROW));
+#pragma unroll
+          for (int e = 0; e < VB; ++e) vw[0][4 * tile + e] = src[e];
+        }
+      } else {
+        // eight codes of each of the lane's tokens
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int rr = __shfl(rw, 16 * (e / 4) + 4 * lg + e % 4, 64);
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            const uint8_t* src = a.p.vcodes + (head + rr) * VROW + ((D == 64 ? ln / 2 : ln) + 16 * s) * VB;
+            if constexpr (VB == 4)
+              vw[s][e] = *reinterpret_cast<const uint32_t*>(src);
+            else if constexpr (VB == 3)
+              vw[s][e] = (uint32_t)src[0] | (uint32_t)src[1] << 8 | (uint32_t)src[2] << 16;
+            else
+              vw[s][e] = *reinterpret_cast<const uint16_t*>(src);
+          }
+        }
+      }
+    };
+    load_meta(i0);
+    int row_c = row_of(i0), row_n = row_of(i0 + 1);
+    load_keys(i0, row_c);
+    load_values(row_c);
+    for (int i = i0; i < i1; ++i) {
+      const int blk = cold.at(i), g = blk / nblk, k = blk % nblk;
+      const int tok0 = g * G + 32 * k, cnt = min(32, G - 32 * k);
+      const int row_nn = row_of(i + 2);
+      if (!PK && (i == i0 || k == 0 || i == cold.n0)) begin_group();  // (the second run may start inside a group)
+      f4_t S[2];
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        S[tile] = f4_t{bias, bias, bias, bias};
+#pragma unroll
+        for (int mm = 0; mm < NM; ++mm) {
+          union { h8_t h; uint32_t u[4]; } y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y.u[e] = field(key_s, kw[tile], KB * (8 * mm + 2 * e), 2 * KB);
+          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, wl[mm], S[tile], 0, 0, 0);
+          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, wh[mm], S[tile], 0, 0, 0);
+        }
+      }
+      if (!PK && e_hi > e_lo) {
+        // the block's side-list entries, tile by tile
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+          auto put = [&](uint32_t y, bool clear) {
+            const int tok = (int)((y & 0xFFFFu) / D) - 32 * k - 16 * tile, ch = (int)(y & (D - 1));
+            if ((unsigned)tok < 16u) {
+              const int o = at(tok, ch / 8) + ch % 8;
+              const float v = h2f((uint16_t)(y >> 16)) - stat_s[wave][1][ch];
+              const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(v, 0.f));
+              hi_s[o] = clear ? 0 : __builtin_bit_cast(uint16_t, hh.x);
+              lo_s[o] = clear ? 0 : f2h(v - (float)hh.x);
+            }
+          };
+          auto each = [&](bool clear) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              if (e_lo + lane + 64 * s < e_hi) put(ent[s], clear);
+            for (int e = e_lo + 128 + lane; e < e_hi; e += 64) put(oent[ob * cap + e], clear);
+            wave_sync();
+          };
+          each(false);
+#pragma unroll
+          for (int mm = 0; mm < NM; ++mm) {
+            const int o = at(ln, (CPL / 8) * lg + mm);
+            S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8_t*>(lo_s + o), qf[mm], S[tile], 0, 0, 0);
+            S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8_t*>(hi_s + o), qf[mm], S[tile], 0, 0, 0);
+          }
+          wave_sync();
+          each(true);
+        }
+      }
+      if constexpr (PK) {  // score = |k| (q_rot . centroids)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) S[e / 4][e % 4] *= __shfl(kn, 16 * (e / 4) + 4 * lg + e % 4, 64);
+      }
+      const int next = min(i + 1, i1 - 1);
+      if (next >= meta_i + 64) load_meta(next);
+      load_keys(next, row_n);
+      float w[8];
+      weights(S, tok0, cnt, w);
+      h8_t pf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float nv = __shfl(norm, 16 * (e / 4) + 4 * lg + e % 4, 64);
+        pf[e] = (_Float16)(w[e] == 0.f ? 0.f : w[e] * nv);  // (no weight: whatever norm stands there)
+      }
+      // V^T P^T: row ln of the first operand is channel NC ln + j of the piece
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        if constexpr (TILED) {
+          // a channel's token pairs side by side in the unit's bits
+#pragma unroll
+          for (int j = 0; j < NC; ++j) {
+            union { h8_t h; uint32_t u[4]; } y;
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              y.u[f] = field(val_s, vw[0] + 4 * (f / 2), (2 * j + f % 2) * 2 * VB, 2 * VB);
+            }
+            O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, pf, O[j], 0, 0, 0);
+          }
+        } else {
+          // by channel pairs, the tokens of a channel then brought together
+#pragma unroll
+          for (int j = 0; j < NC; j += 2) {
+            uint32_t two[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              two[e] = entry(val_s, D == 64 ? vw[s][e] >> ((ln & 1) * 4 * VB) : vw[s][e], VB * j, 2 * VB);
+            union { h8_t h; uint32_t u[4]; } y0, y1;
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              y0.u[f] = __builtin_amdgcn_perm(two[2 * f + 1], two[2 * f], 0x05040100u);
+              y1.u[f] = __builtin_amdgcn_perm(two[2 * f + 1], two[2 * f], 0x07060302u);
+            }
+            O[NC * s + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y0.h, pf, O[NC * s + j], 0, 0, 0);
+            O[NC * s + j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y1.h, pf, O[NC * s + j + 1], 0, 0, 0);
+          }
+        }
+      }
+      load_values(row_n);
+      row_n = row_nn;
+    }
+  } else if (!is_cold) {
+    // uncoded blocks, straight from the ring
+    const size_t ring = ((size_t)b * Hkv + h) * d.hot_ring;
+    const uint16_t* const hk = static_cast<const uint16_t*>(a.p.hot_k);
+    const uint16_t* const hv = static_cast<const uint16_t*>(a.p.hot_v);
+    for (int i = i0; i < i1; ++i) {
+      const int tok0 = n_cold + 32 * hot.at(i), cnt = min(32, n - tok0), at0 = tok0 % d.hot_ring;
+      // place of token tok0 + o, o < cnt (cnt is at most the ring's size)
+      auto place = [&](int o) { return ring + (at0 + o >= d.hot_ring ? at0 + o - d.hot_ring : at0 + o); };
+      f4_t S[2];
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        const uint16_t* kr = hk + place(min(16 * tile + ln, cnt - 1)) * D + CPL * lg;
+        S[tile] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int mm = 0; mm < NM; ++mm)
+          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8_t*>(kr + 8 * mm), qf[mm], S[tile],
+                                                           0, 0, 0);
+      }
+      // values: token e of this lane, channels NC ln .. + NC - 1 of the piece;
+      // zero where no row sees the token, whatever stands there
+      u32x4_t vv[NS][8];
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int o = 16 * (e / 4) + 4 * lg + e % 4, tok = tok0 + o;
+        const bool any = o < cnt && tok <= p_hi && (tok >= lo_first || tok < sinks);
+        const uint16_t* vr = hv + place(min(o, cnt - 1)) * D + NC * ln;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          if constexpr (NC == 8) {
+            vv[s][e] = *reinterpret_cast<const u32x4_t*>(vr + 128 * s);
+          } else {
+            const u32x2_t y = *reinterpret_cast<const u32x2_t*>(vr);
+            vv[s][e] = u32x4_t{y.x, y.y, 0u, 0u};
+          }
+          if (!any) vv[s][e] = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int f = 0; f < NC / 2; ++f)
+            odd |= (vv[s][e][f] & 0x7C00u) == 0x7C00u || (vv[s][e][f] & 0x7C000000u) == 0x7C000000u;
+        }
+      }
+      float w[8];
+      weights(S, tok0, cnt, w);
+      h8_t pf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pf[e] = (_Float16)w[e];
+      auto products = [&](f4_t (&acc)[NV], const u32x4_t (&val)[NS][8]) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int j = 0; j < NC; ++j) {
+            union { h8_t h; uint32_t u[4]; } y;
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+              y.u[f] = __builtin_amdgcn_perm(val[s][2 * f + 1][j / 2], val[s][2 * f][j / 2],
+                                             (j & 1) ? 0x07060302u : 0x05040100u);
+            acc[NC * s + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, pf, acc[NC * s + j], 0, 0, 0);
+          }
+      };
+      // (an infinity or a NaN that some queries see and others do not: set aside)
+      const bool apart = a.per_item > 1 && __any(odd) && !all_see(tok0, cnt);
+      if (__builtin_expect(apart, 0)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int f = 0; f < NC / 2; ++f) {
+              uint32_t y = vv[s][e][f];
+              y &= (y & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : ~0u;
+              y &= (y & 0x7C000000u) == 0x7C000000u ? 0xFFFFu : ~0u;
+              vv[s][e][f] = y;
+            }
+      }
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          union { h8_t h; uint32_t u[4]; } y;
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            y.u[f] = __builtin_amdgcn_perm(vv[s][2 * f + 1][j / 2], vv[s][2 * f][j / 2],
+                                           (j & 1) ? 0x07060302u : 0x05040100u);
+          O[NC * s + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, pf, O[NC * s + j], 0, 0, 0);
+        }
+      if (__builtin_expect(apart, 0)) {
+        // ... and added to the rows that see it (any positive weight gives the same)
+#pragma unroll 1
+        for (int o = 0; o < cnt; ++o) {
+          const bool vis = sees(tok0 + o);
+          const uint16_t* vr = hv + place(o) * D;
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int j = 0; j < NC; ++j) {
+                const float y = h2f(vr[128 * s + NC * (4 * lg + e) + j]);
+                O[NC * s + j][e] += vis && !(fabsf(y) < INFINITY) ? y : 0.f;
+              }
+        }
+      }
+    }
+  }
+
+  // ---- the waves' states joined: coded ones, rotated back, and uncoded ones
+  const int first_hot = min(max(cold_waves - split * kFewWaves, 0), kFewWaves);  // waves before it are coded
+  // Pi^T's rows e = 16 (wave + 8 nt) + ln, channels 32 mm + 8 lg .. + 7: the
+  // first of them asked for early
+  constexpr int NTR = (D / 16 + kFewWaves - 1) / kFewWaves;
+  f4_t pr[NM][2];
+  auto load_pi = [&](int nt) {
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        pr[mm][e] = *reinterpret_cast<const f4_t*>(
+            a.p.pi_t + (size_t)(16 * ((wave + kFewWaves * nt) % (D / 16)) + ln) * D + 32 * mm + 8 * lg + 4 * e);
+  };
+  if (first_hot > 0) load_pi(0);
+  {
+    const float l = colgroup_sum(l_run);
+    if (lg == 0) {
+      ml_s[0][wave][ln] = m_run;
+      ml_s[1][wave][ln] = l;
+    }
+    float* const o = reinterpret_cast<float*>(stage_s[wave]);  // [16][D]
+    wave_sync();
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[ln * D + 128 * s + NC * (4 * lg + e) + j] = O[NC * s + j][e];
+  }
+  __syncthreads();
+  constexpr int kRowGroups = kFewThreads / D;            // rows side by side
+  constexpr int RPT = (kFewRows + kRowGroups - 1) / kRowGroups;  // rows a thread
+  const int j = tid % D, r0 = tid / D;
+  float cs[RPT], hs[RPT], ls[RPT], ms[RPT];
+#pragma unroll
+  for (int k = 0; k < RPT; ++k) {
+    const int r = r0 + kRowGroups * k;
+    cs[k] = hs[k] = ls[k] = 0.f;
+    ms[k] = -INFINITY;
+    if (r >= n_rows) continue;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) ms[k] = fmaxf(ms[k], ml_s[0][w][r]);
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      const float mw = ml_s[0][w][r], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - ms[k]);
+      const float y = reinterpret_cast<const float*>(stage_s[w])[r * D + j];
+      ls[k] = fmaf(ml_s[1][w][r], f, ls[k]);
+      // (a state without a maximum holds zeros; a NaN among its scores leaves it one)
+      if (w < first_hot) cs[k] += y * f; else hs[k] += y * f;
+    }
+  }
+  if (first_hot > 0) {
+    __syncthreads();
+    // the coded sums over their weights' sum (within fp16's range then) as an
+    // fp16 pair, times Pi's
+    uint16_t* const c_s = &stage_s[0][0];                         // [2][16][D]
+    float* const y_s = reinterpret_cast<float*>(&stage_s[1][0]);  // [16][D]
+#pragma unroll
+    for (int k = 0; k < RPT; ++k) {
+      const int r = r0 + kRowGroups * k;
+      if (r < kFewRows) {
+        const float y = ls[k] != 0.f ? cs[k] / (ls[k] * up) : 0.f;
+        const _Float16 hi = (_Float16)y;
+        c_s[r * D + j] = __builtin_bit_cast(uint16_t, hi);
+        c_s[(kFewRows + r) * D + j] = f2h(y - (float)hi);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NTR; ++nt) {
+      if (wave + kFewWaves * nt < D / 16) {
+        f4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int mm = 0; mm < NM; ++mm) {
+          h8_t ph, pl;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = pr[mm][e / 4][e % 4];
+            ph[e] = (_Float16)y;
+            pl[e] = (_Float16)(y - (float)ph[e]);
+          }
+          const h8_t ch = *reinterpret_cast<const h8_t*>(c_s + ln * D + 32 * mm + 8 * lg);
+          const h8_t cl = *reinterpret_cast<const h8_t*>(c_s + (kFewRows + ln) * D + 32 * mm + 8 * lg);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(cl, ph, acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, pl, acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, ph, acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y_s[(4 * lg + e) * D + 16 * (wave + kFewWaves * nt) + ln] = acc[e];
+        if (nt + 1 < NTR) load_pi(nt + 1);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < RPT; ++k)
+      if (r0 + kRowGroups * k < kFewRows) hs[k] = fmaf(y_s[(r0 + kRowGroups * k) * D + j], ls[k], hs[k]);
+  }
+  // (rows past the queries of the sequence: zero)
+  const int all_rows = min(a.per_item, a.q_len - q0) * gq;
+#pragma unroll
+  for (int k = 0; k < RPT; ++k) {
+    const int r = r0 + kRowGroups * k;
+    if (r >= all_rows) continue;
+    const int tr = q0 + r / gq, hq = h * gq + r % gq;
+    if (a.n_splits == 1) {
+      const long long o = b * a.o_stride[0] + hq * a.o_stride[1] + tr * a.o_stride[2] + j;
+      const float y = r < n_rows && n - m + tr >= 0 ? hs[k] / ls[k] : 0.f;
+      if (a.out_type == 0) static_cast<float*>(a.out)[o] = y;
+      else static_cast<_Float16*>(a.out)[o] = (_Float16)y;
+    } else {
+      const long long o = split * a.rows + ((long long)b * Hq + hq) * a.q_len + tr;
+      a.part_acc[o * D + j] = hs[k];
+      if (j == 0) {
+        a.part_ml[2 * o] = ms[k];
+        a.part_ml[2 * o + 1] = ls[k];
+      }
+    }
+  }
+}
+
+// The splits of a row joined: one wave a row, D / 64 channels a lane.
+template <int D>
+__global__ __launch_bounds__(256) void tqk_attend_join(FewArgs a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const int t = (int)(row % a.q_len);
+  const long long bh = row / a.q_len;
+  const int hq = (int)(bh % a.d.n_q_heads), b = (int)(bh / a.d.n_q_heads);
+  // every split's numbers by a lane of its own, then all accumulators in flight
+  const bool in = lane < a.n_splits;
+  const float ml = in ? a.part_ml[2 * (lane * a.rows + row)] : -INFINITY;
+  const float ll = in ? a.part_ml[2 * (lane * a.rows + row) + 1] : 0.f;
+  const float M = wave_reduce<true>(ml);
+  const float f = ml == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml - M);
+  const float l = wave_reduce<false>(ll * f);
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.n_splits; ++s) {
+    const float g = __shfl(f, s, 64);
+    const float* src = a.part_acc + (s * a.rows + row) * D + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e], g, acc[e]);
+  }
+  const int n = min(a.seq_lens[b], a.max_len);
+  const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+  const bool any = t < m && n - m + t >= 0;
+  const long long o = b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2] + E * lane;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float y = any ? acc[e] / l : 0.f;
+    if (a.out_type == 0) static_cast<float*>(a.out)[o + e] = y;
+    else static_cast<_Float16*>(a.out)[o + e] = (_Float16)y;
+  }
+}
+
+struct FewPlan {
+  int per_item, q_items, n_splits;
+  long long rows, groups;  // rows of all, workgroups
+  size_t ws_bytes;
+};
+
+FewPlan few_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+  FewPlan fp{};
+  const int gq = d->n_q_heads / d->n_kv_heads;
+  fp.per_item = kFewRows / gq < t->q_len ? kFewRows / gq : t->q_len;
+  fp.q_items = (t->q_len + fp.per_item - 1) / fp.per_item;
+  fp.rows = (long long)t->batch * d->n_q_heads * t->q_len;
+  const long long pairs = (long long)t->batch * fp.q_items * d->n_kv_heads;
+  // blocks of 32 tokens that a workgroup's rows see at most
+  long long tokens = t->max_len;
+  if (t->window > 0 && t->window < t->max_len) {
+    const long long w = (long long)t->window + fp.per_item + t->sinks + 64;
+    if (w < tokens) tokens = w;
+  }
+  const long long blocks = (tokens + 31) / 32 + 1;
+  // Splits: rounds of the workgroups that fit (two a CU at head_dim 64)
+  // times a wave's run of blocks and the set-up, joining and rotation of about
+  // three blocks' time; another launch to join them, about two.
+  const long long slots = (d->head_dim == 64 ? 2 : 1) * (long long)device_cus();
+  double best = 1e30;
+  for (int s = 1; s <= 64 && (s == 1 || (long long)kFewWaves * (s - 1) < blocks); ++s) {
+    const long long rounds = (pairs * s + slots - 1) / slots;
+    const long long run = (blocks + (long long)kFewWaves * s - 1) / ((long long)kFewWaves * s);
+    const double cost = (double)rounds * (double)(run + 3) + (s > 1 ? 2.0 : 0.0);
+    if (cost < best - 1e-9) {
+      best = cost;
+      fp.n_splits = s;
+    }
+  }
+  fp.groups = pairs * fp.n_splits;
+  fp.ws_bytes = fp.n_splits > 1 ? (size_t)fp.n_splits * fp.rows * (d->head_dim + 2) * sizeof(float) + 256 : 16;
+  return fp;
+}
+
+template <int D, int VB, bool TILED>
+void launch_keys(const FewArgs& a, dim3 grid, hipStream_t st) {
+  if (a.d.key_grid == 2)
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, VB, true, TILED>), grid, dim3(kFewThreads), 0, st, a);
+  else if (a.d.key_bits == 4)
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 4, false, TILED>), grid, dim3(kFewThreads), 0, st, a);
+  else if (a.d.key_bits == 3)
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 3, false, TILED>), grid, dim3(kFewThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 2, false, TILED>), grid, dim3(kFewThreads), 0, st, a);
+}
+template <int D, bool TILED>
+void launch_values(const FewArgs& a, dim3 grid, hipStream_t st) {
+  if (a.d.value_bits == 2)
+    launch_keys<D, 2, TILED>(a, grid, st);
+  else if (a.d.value_bits == 3)
+    launch_keys<D, 3, TILED>(a, grid, st);
+  else
+    launch_keys<D, 4, TILED>(a, grid, st);
+}
+template <int D>
+void launch_few(const FewArgs& a, dim3 grid, hipStream_t st) {
+  if constexpr (D == TQK_D) {
+    if (v_tiled(a.d.group_tokens, a.d.page_tokens, D, 0))
+      launch_values<D, true>(a, grid, st);
+    else
+      launch_values<D, false>(a, grid, st);
+  } else {
+    launch_values<D, false>(a, grid, st);
+  }
+  if (a.n_splits > 1)
+    hipLaunchKernelGGL(tqk_attend_join<D>, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+}
+
+}  // namespace
+
+size_t tqk_few_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) { return few_plan(d, t).ws_bytes; }
+
+int tqk_run_few(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
+                const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace, void* stream) {
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const FewPlan fp = few_plan(d, t);
+  if (fp.groups > (1LL << 22)) return TQK_EINVAL;  // (512 threads each: fewer than 2^32)
+  FewArgs a{};
+  a.d = *d;
+  a.p = *p;
+  a.q = static_cast<const uint16_t*>(q);
+  a.seq_lens = seq_lens;
+  a.q_lens = q_lens;
+  a.out = out;
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = a.part_acc + (size_t)fp.n_splits * fp.rows * d->head_dim;
+  a.rows = fp.rows;
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = t->q_stride[i];
+    a.o_stride[i] = t->o_stride[i];
+  }
+  a.q_len = t->q_len;
+  a.max_len = t->max_len;
+  a.window = t->window;
+  a.sinks = t->sinks;
+  a.out_type = t->out_type;
+  a.per_item = fp.per_item;
+  a.q_items = fp.q_items;
+  a.n_splits = fp.n_splits;
+  const dim3 grid((unsigned)fp.groups);
+  if (d->head_dim == 64)
+    launch_few<64>(a, grid, st);
+  else if (d->head_dim == 128)
+    launch_few<128>(a, grid, st);
+  else
+    launch_few<256>(a, grid, st);
+  return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+}

@@ -7,13 +7,13 @@ namespace {
 template <int GQ, int KB>
 void launch_mfma_kb(const DecodeArgs& a, dim3 g1, hipStream_t st) {
   if (a.d.key_grid == 2)  // PolarQuant keys: value_bits == key_bits
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, KB, KB, true, false>), g1, dim3(kMThreads), 0, st, SplitArgs<false>{a});
+    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, KB, KB, true>), g1, dim3(kMThreads), 0, st, a);
   else if (a.d.value_bits == 2)
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 2, KB, false, false>), g1, dim3(kMThreads), 0, st, SplitArgs<false>{a});
+    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 2, KB, false>), g1, dim3(kMThreads), 0, st, a);
   else if (a.d.value_bits == 3)
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 3, KB, false, false>), g1, dim3(kMThreads), 0, st, SplitArgs<false>{a});
+    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 3, KB, false>), g1, dim3(kMThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 4, KB, false, false>), g1, dim3(kMThreads), 0, st, SplitArgs<false>{a});
+    hipLaunchKernelGGL((tqk_decode_split_mfma<GQ, 4, KB, false>), g1, dim3(kMThreads), 0, st, a);
 }
 
 template <int GQ, int D>

@@ -1,7 +1,7 @@
 // Fused decode-step attention over the two-tier TurboQuant KV cache (gfx950):
 // the kernels and their launch plan, compiled for whole sequences (one query
 // each) by tqk_decode.hip and, with a window and first tokens that stay visible
-// (WIN), by tqk_attend.hip.
+// (WIN), for fp32 caches by tqk_attend.hip (the VALU kernel and the merge).
 //
 // One workgroup per (split, kv head, sequence).  A split covers a run of coded
 // groups or a slice of the fp16 hot window and produces an unnormalised
@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "tqk_common.h"
+#include "tqk_wave.h"
 
 namespace {
 
@@ -91,8 +92,7 @@ struct SeenTokens {
   }
   __device__ __forceinline__ int group(int v) const { return v + (v >= first ? skip : 0); }
   __device__ __forceinline__ bool sees(int t) const { return (t <= hi) & ((t >= lo) | (t < sinks)); }
-  // n tokens from t: all seen, none seen
-  __device__ __forceinline__ bool all(int t, int n) const { return t + n - 1 <= hi && (t >= lo || t + n <= sinks); }
+  // none of n tokens from t is seen
   __device__ __forceinline__ bool none(int t, int n) const { return t > hi || (t + n <= lo && t >= sinks); }
 };
 // What a split kernel's item is and sees: a whole sequence of L tokens, or with
@@ -106,7 +106,6 @@ struct Item {
   int groups;
   __device__ __forceinline__ int group(int v) const { return v; }
   __device__ __forceinline__ bool sees(int) const { return true; }
-  __device__ __forceinline__ bool all(int, int) const { return true; }
   __device__ __forceinline__ bool none(int, int) const { return false; }
   __device__ __forceinline__ size_t q_at(const SplitArgs<false>& a, int head) const {
     return ((size_t)seq * a.d.n_q_heads + head) * a.d.head_dim;
@@ -170,28 +169,6 @@ constexpr int kVOEnt = 2048;  // VALU decode: side-list entries staged in LDS pe
 
 // workgroups whose LDS a CU holds (160 KiB, given out in pieces of 1280 bytes)
 constexpr int lds_workgroups(size_t bytes) { return (int)(128 / ((bytes + 1279) / 1280)); }
-
-// The wave's sum or maximum in every lane, on the VALU (rotations inside the
-// 16-lane rows, then the two permlane swaps): a butterfly of ds_bpermute is six
-// LDS round trips in a row.
-template <bool IS_MAX>
-__device__ __forceinline__ float wave_reduce(float x) {
-  auto op = [](float a, float b) { return IS_MAX ? fmaxf(a, b) : a + b; };
-  auto ror = [](float v, auto n) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + decltype(n)::value,
-                                                                 0xF, 0xF, true));
-  };
-  x = op(x, ror(x, std::integral_constant<int, 8>{}));
-  x = op(x, ror(x, std::integral_constant<int, 4>{}));
-  x = op(x, ror(x, std::integral_constant<int, 2>{}));
-  x = op(x, ror(x, std::integral_constant<int, 1>{}));
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto r16 = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  x = op(__builtin_bit_cast(float, (uint32_t)r16[0]), __builtin_bit_cast(float, (uint32_t)r16[1]));
-  const uint32_t w = __builtin_bit_cast(uint32_t, x);
-  const auto r32 = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return op(__builtin_bit_cast(float, (uint32_t)r32[0]), __builtin_bit_cast(float, (uint32_t)r32[1]));
-}
 
 template <int GQ, bool IS_MAX>
 __device__ __forceinline__ void block_reduce(float (&v)[GQ], float (*red)[GQ]) {
@@ -828,9 +805,7 @@ __global__ __launch_bounds__(kThreads) void tqk_decode_split_valu(SplitArgs<WIN>
 // current block is computed.
 // ---------------------------------------------------------------------------
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x3_t __attribute__((ext_vector_type(3)));
-typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 // dword 3 of a raw buffer resource on gfx9 (32-bit data, no swizzle)
 constexpr int kBufFlags = 0x00020000;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const void* base, uint32_t bytes) {
@@ -910,31 +885,6 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Orders LDS accesses of one wave across lanes.  A wave's LDS instructions
-// execute in issue order, so program order is enough; this only stops the
-// compiler from moving memory operations across the point (and, unlike a
-// fence, does not wait for the wave's outstanding global loads).
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_wave_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// Cross-lane helpers without LDS traffic.
-__device__ __forceinline__ uint32_t fbits(float x) { return __builtin_bit_cast(uint32_t, x); }
-__device__ __forceinline__ float bitsf(uint32_t x) { return __builtin_bit_cast(float, x); }
-// max / sum over lanes {l, l^16, l^32, l^48}: the four token groups of a column
-__device__ __forceinline__ float colgroup_max(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(fbits(x), fbits(x), false, false);
-  x = fmaxf(bitsf(a[0]), bitsf(a[1]));
-  auto b = __builtin_amdgcn_permlane16_swap(fbits(x), fbits(x), false, false);
-  return fmaxf(bitsf(b[0]), bitsf(b[1]));
-}
-__device__ __forceinline__ float colgroup_sum(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(fbits(x), fbits(x), false, false);
-  x = bitsf(a[0]) + bitsf(a[1]);
-  auto b = __builtin_amdgcn_permlane16_swap(fbits(x), fbits(x), false, false);
-  return bitsf(b[0]) + bitsf(b[1]);
-}
 // value of lane (row-local) column c +/- N within the 16-lane row (DPP row rotate)
 template <int N>
 __device__ __forceinline__ float row_ror(float x) {
@@ -1006,8 +956,7 @@ constexpr float kLazyMax = 2.0f;
 // is rescaled.  (m, l, O) stays consistent for any m, so the softmax is the
 // same.  Accumulator row r = 4lg + i belongs to head r & (GQ - 1), whose
 // correction factor is read from that column with v_readlane.
-// SAFE: scores may be -inf (tokens that are not seen), a state's first ones too.
-template <int GQ, bool SAFE>
+template <int GQ>
 __device__ __forceinline__ void softmax_block(WaveState& st, const float (&s)[8], float (&p)[8],
                                               int lg) {
   float bm = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
@@ -1015,7 +964,7 @@ __device__ __forceinline__ void softmax_block(WaveState& st, const float (&s)[8]
   if (__builtin_amdgcn_ballot_w64(bm > st.mt) != 0) {
     bm = colgroup_max(bm);
     const float mn = fmaxf(st.m, bm);
-    const float corr = SAFE && mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
+    const float corr = __builtin_amdgcn_exp2f(st.m - mn);
     st.m = mn;
     st.mt = mn + kLazyMax;
     st.l *= corr;
@@ -1037,10 +986,9 @@ __device__ __forceinline__ void softmax_block(WaveState& st, const float (&s)[8]
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) st.O[nt] = st.O[nt] * cvec;
   }
-  const float at = SAFE && st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    p[i] = __builtin_amdgcn_exp2f(s[i] - at);
+    p[i] = __builtin_amdgcn_exp2f(s[i] - st.m);
     st.l += p[i];
   }
 }
@@ -1132,13 +1080,7 @@ struct IntC {
   static constexpr int value = K;
 };
 
-// fp16 pair (RNE) of two floats in one dword, and the fp32 value of a half
-__device__ __forceinline__ uint32_t pk_f16(float x, float y) {
-  typedef float float2_t __attribute__((ext_vector_type(2)));
-  typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-  const half2_t hv = __builtin_convertvector((float2_t){x, y}, half2_t);
-  return __builtin_bit_cast(uint32_t, hv);
-}
+// the fp32 values of a dword's halves
 __device__ __forceinline__ float lo_f16(uint32_t pk) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(pk & 0xFFFFu)); }
 __device__ __forceinline__ float hi_f16(uint32_t pk) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(pk >> 16)); }
 
@@ -1184,8 +1126,8 @@ constexpr int kSegTokens = GQ > 4 ? 128 : 256;
 // PK: PolarQuant keys (key_grid 2, KB == VB): the key table holds centroids,
 // the QK^T weights are the rotated query, and every score is scaled by its
 // token's key norm
-template <int GQ, int VB, int KB, bool PK, bool WIN>
-__global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<WIN> a) {
+template <int GQ, int VB, int KB, bool PK>
+__global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(DecodeArgs a) {
   constexpr int D = TQK_D;
   constexpr int VROW = D * VB / 8;
   constexpr int KROW = D * KB / 8;  // key code bytes per token (tqk_common.h layout)
@@ -1210,7 +1152,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
     // (rank, kv head) <-> blockIdx.x is a bijection.  More items than the
     // workgroup has threads keep the plain order.
     const int n_items = a.batch * ncs;
-    if (!WIN && a.reorder && a.batch > 1 && n_items <= kMWaves * 64) {
+    if (a.reorder && a.batch > 1 && n_items <= kMWaves * 64) {
       __shared__ int work_s[kMWaves * 64];
       __shared__ int pick_s;
       const int t = threadIdx.x;
@@ -1240,11 +1182,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, lg = lane >> 4, c = lane & 15;
   const tqk_cache_desc& d = a.d;
   const int Hkv = d.n_kv_heads, Hq = d.n_q_heads, G = d.group_tokens, P = d.page_tokens;
-  Item<WIN> seen(a, b);
-  const int bs = seen.seq;
-  const int L = seen.length(a);
-  // (WIN: which groups the rows below are depends on the length)
-  if constexpr (WIN) seen.look(a, L, G, n_groups_of(L, d.hot_window, G));
+  const int L = a.seq_lens[b];
   // scores in the log2 domain: q * sm_scale * log2(e), softmax with exp2
   const float qscale = d.sm_scale * 1.4426950408889634f;
 
@@ -1322,10 +1260,10 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
   int slot_r[kMetaIt], phys_r[kMetaIt];
 #pragma unroll
   for (int r = 0; r < kMetaIt; ++r) {
-    const int g = min(seen.group(gbeg_m + mrow(r)), mg - 1);
+    const int g = min(gbeg_m + mrow(r), mg - 1);
     const int t = g * G + 16 * (mf & 15);
-    const uint32_t gi = tables ? (uint32_t)bs * (uint32_t)mg + (uint32_t)g : 0u;
-    const uint32_t bi = tables ? (uint32_t)bs * (uint32_t)mp + (uint32_t)min(t / P, mp - 1) : 0u;
+    const uint32_t gi = tables ? (uint32_t)b * (uint32_t)mg + (uint32_t)g : 0u;
+    const uint32_t bi = tables ? (uint32_t)b * (uint32_t)mp + (uint32_t)min(t / P, mp - 1) : 0u;
     slot_r[r] = (int)__builtin_amdgcn_raw_buffer_load_b32(r < n_it ? rg : rnone, (int)(4u * gi), 0, 0);
     phys_r[r] = (int)__builtin_amdgcn_raw_buffer_load_b32(r < n_it ? rb : rnone, (int)(4u * bi), 0, 0);
   }
@@ -1338,11 +1276,10 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
   for (int r = 0; r < kQIt; ++r) {
     const int i = min(tid + r * kMThreads, GQ * D - 1);
     const int hi = min(i / D, gq - 1);
-    const uint32_t x = static_cast<const uint16_t*>(a.q)[seen.q_at(a, h * gq + hi) + i % D];
+    const uint32_t x = static_cast<const uint16_t*>(a.q)[((size_t)b * Hq + h * gq + hi) * D + i % D];
     qraw[r] = i / D < gq ? x : 0u;
   }
   const int ng = n_groups_of(L, d.hot_window, G);
-  if constexpr (!WIN) seen.look(a, L, G, ng);
   // the levels go through the wave's own stats slot (free until the stream
   // starts): a wave-local exchange, no workgroup barrier in front of the fill
   if (lane < 32) gsm_s[w][lane] = lvl;
@@ -1384,7 +1321,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
   }
   {
     // the outlier bounds of the split's groups by slot, then the rows
-    const int gcnt = max(0, min(seen.groups, gbeg_m + a.groups_per_split) - gbeg_m);
+    const int gcnt = max(0, min(ng, gbeg_m + a.groups_per_split) - gbeg_m);
     int oc_r[kMetaIt];
 #pragma unroll
     for (int r = 0; r < kMetaIt; ++r) {
@@ -1400,7 +1337,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
     for (int r = 0; r < kMetaIt; ++r) {
       if (r >= n_it) continue;
       const int jg = mrow(r);
-      const int g = min(seen.group(gbeg_m + jg), mg - 1);
+      const int g = min(gbeg_m + jg, mg - 1);
       const int t = g * G + 16 * (mf & 15);
       const uint32_t obase = (uint32_t)slot_r[r] * (uint32_t)Hkv + (uint32_t)h;
       int v = 0;
@@ -1472,7 +1409,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
     // at block kb0 of its first group.
     const int wu = __builtin_amdgcn_readfirstlane(w);
     const int gbeg = split * a.groups_per_split;
-    const int gcnt = max(0, min(seen.groups, gbeg + a.groups_per_split) - gbeg);
+    const int gcnt = max(0, min(ng, gbeg + a.groups_per_split) - gbeg);
     const int nblk = G / 32;
     int g0, gstep, kb0, nw, T;
     if (a.wave_blocks > 0) {
@@ -1954,8 +1891,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
       };
       // blk1: block index of block i + 1 inside its group (whose weights and
       // corrections are built before the step when it starts a segment)
-      // (tb: first token of block i, WIN only)
-      auto process = [&](const ColdBlock<VB>& cur, const ColdBlock<VB>& nx1, int blk1, int tb) {
+      auto process = [&](const ColdBlock<VB>& cur, const ColdBlock<VB>& nx1, int blk1) {
         const floatx4_t CA = CAn, CB = CBn;
         float sc[8];
 #pragma unroll
@@ -1975,24 +1911,14 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
           sc[7] *= row_bcast<7>(cur.kn);
         }
         float p[8];
-        const bool part = WIN && !seen.all(tb, 32);  // (the same for every lane)
-        if (part) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sc[i] = seen.sees(tb + 16 * (i / 4) + 4 * lg + i % 4) ? sc[i] : -INFINITY;
-        }
-        softmax_block<GQ, WIN>(st, sc, p, lg);
+        softmax_block<GQ>(st, sc, p, lg);
         // A operand of PV: weight times value norm of the lane's 8 tokens
         // (tile A 4lg..4lg+3, tile B 4lg..4lg+3) for head hq, fp16 hi in rows
         // c < 8, the fp16 residual in rows c >= 8
-        float pn[8] = {p[0] * row_bcast<0>(cur.nv), p[1] * row_bcast<1>(cur.nv),
-                       p[2] * row_bcast<2>(cur.nv), p[3] * row_bcast<3>(cur.nv),
-                       p[4] * row_bcast<4>(cur.nv), p[5] * row_bcast<5>(cur.nv),
-                       p[6] * row_bcast<6>(cur.nv), p[7] * row_bcast<7>(cur.nv)};
-        if (part) {  // (no weight, whatever norm stands at a token that is not seen)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pn[i] = seen.sees(tb + 16 * (i / 4) + 4 * lg + i % 4) ? pn[i] : 0.f;
-        }
-        const H8 pw = split8(pn[0], pn[1], pn[2], pn[3], pn[4], pn[5], pn[6], pn[7], lo_sel);
+        const H8 pw = split8(p[0] * row_bcast<0>(cur.nv), p[1] * row_bcast<1>(cur.nv),
+                             p[2] * row_bcast<2>(cur.nv), p[3] * row_bcast<3>(cur.nv),
+                             p[4] * row_bcast<4>(cur.nv), p[5] * row_bcast<5>(cur.nv),
+                             p[6] * row_bcast<6>(cur.nv), p[7] * row_bcast<7>(cur.nv), lo_sel);
         H8 vv[8], xa[8], xb[8];
         // (no scheduling fences between the phases: the compiler's own
         // interleaving measured faster and needs fewer registers)
@@ -2035,7 +1961,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
       wave_sync();
       load_block_entries();
       load_next(nxt);
-      process(cur, nx1, kb1, WIN ? seen.group(gbeg + g0 + gstep * jp) * G + 32 * kbp : 0);
+      process(cur, nx1, kb1);
       if (++kbp == nblk) {
         kbp = 0;
         ++jp;
@@ -2112,7 +2038,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
   reset_state(st);
   {
     const int n_cold = ng * G, R = d.hot_ring;
-    const size_t hbase = ((size_t)bs * Hkv + h) * R;
+    const size_t hbase = ((size_t)b * Hkv + h) * R;
     const int nhb = (L - n_cold + 31) / 32;
     // B operand of QK^T: q (fp16, exact) of head c for channels 32ks + 8lg + e
     H8 Bq[4];
@@ -2124,8 +2050,6 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
       // are consecutive and inside the ring, so every row is loaded (keys and
       // values together) and rows at or past L are masked afterwards
       const int t0 = n_cold + 32 * hb;
-      if (seen.none(t0, 32)) continue;
-      auto sees = [&](int t) { return t < L && seen.sees(t); };
       const uint16_t* kr = static_cast<const uint16_t*>(a.p.hot_k) + (hbase + (t0 % R)) * D;
       const uint16_t* vr = static_cast<const uint16_t*>(a.p.hot_v) + (hbase + (t0 % R)) * D;
       H8 ka[4], kb[4];
@@ -2150,11 +2074,11 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
       float s[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[i] = sees(t0 + 4 * lg + i) ? CA[i] * qscale : -INFINITY;
-        s[4 + i] = sees(t0 + 16 + 4 * lg + i) ? CB[i] * qscale : -INFINITY;
+        s[i] = (t0 + 4 * lg + i < L) ? CA[i] * qscale : -INFINITY;
+        s[4 + i] = (t0 + 16 + 4 * lg + i < L) ? CB[i] * qscale : -INFINITY;
       }
       float p[8];
-      softmax_block<GQ, WIN>(st, s, p, lg);
+      softmax_block<GQ>(st, s, p, lg);
       H8 pa;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -2165,7 +2089,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int tt = (e < 4) ? 4 * lg + e : 16 + 4 * lg + (e - 4);
-        if (!sees(t0 + tt)) vv[e] = make_uint4(0u, 0u, 0u, 0u);
+        if (t0 + tt >= L) vv[e] = make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
@@ -2401,10 +2325,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(SplitArgs<
         float o = hr[r];
 #pragma unroll 8
         for (int k = 0; k < D; ++k) o += q_h_s[qi][k] * pi_s[k * D + j];
-        if constexpr (WIN)
-          put_seen(a.w, a.out, bs, seen.query, h * gq + qi, j, seen.hi >= 0, o / den[r]);
-        else
-          a.out[((size_t)b * Hq + h * gq + qi) * D + j] = o / den[r];
+        a.out[((size_t)b * Hq + h * gq + qi) * D + j] = o / den[r];
       }
     }
   }

@@ -31,6 +31,7 @@ PER_UNIT = {
     "tqk_block.hip": ["-ffp-contract=off"],
     "tqk_decode.hip": [],
     "tqk_attend.hip": [],
+    "tqk_attend_codes.hip": [],
     "tqk_rope.hip": [],
     "tqk_attn.hip": [],
 }
