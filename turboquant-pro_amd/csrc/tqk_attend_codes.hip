@@ -7,17 +7,20 @@
 // coded or uncoded, each on its own until the end.
 //
 // A coded block, 16 tokens at a time: a pair of key codes is an entry of a table
-// of fp16 levels, four of them an operand of K Q^T as they are; the group's scale
-// goes into the query (an fp16 pair: 2^-22), its mean into the scores' start.  A
+// of levels as fp16 pairs (hi + lo: 2^-22), four of them an operand of K Q^T as
+// they are; the group's scale goes into the query, a pair too, its mean into the
+// scores' start.  A
 // side-list entry, whose code is the zero level, adds q (val - mean): the tile's
 // entries stand as fp16 pairs in an otherwise zero LDS tile of the wave, which is
 // a second operand for the same product and is cleared entry by entry.  A lane
 // then holds one row's scores of 8 tokens, which are the operand of V^T P^T as
-// they are.  Value codes become centroids by pairs through a table.  Both
-// codebooks are scaled so that their fp16 roundings nearly vanish (best of 128
-// scales: 2^-12 of a level becomes 2^-14 to 2^-15); weights times norms are
-// rounded to fp16 (2^-12 of each).  The coded part is rotated back once a
-// workgroup, by the matrix cores in fp16 pairs.
+// they are.  Value codes become centroids by pairs through a table, the codebook
+// scaled so that its fp16 roundings nearly vanish (best of 128 scales: 2^-12 of a
+// centroid becomes 2^-14 to 2^-15); weights times norms are rounded to fp16 (2^-12
+// of each).  The coded part is rotated back once a workgroup, by the matrix cores
+// in fp16 pairs.  Up to head_dim 128 a table entry has a row of 256 bytes of
+// copies, by lane: a lookup's bank is its lane's own, and its address one byte
+// permutation; at head_dim 256 the waves' tiles leave room for four copies.
 // Bound: few sequences, the chain of dependent loads (lengths, tables, codes);
 // many, the table reads and VALU work of a block beside its codes from HBM.
 #include "tqk_attend.h"
@@ -28,7 +31,6 @@ namespace {
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves, kFewRows = 16;
 constexpr float kFewLazy = 2.0f;  // log2 units: weights stay at most 4, norms at most TQK_MAX_VNORM: fp16
-constexpr int kPairCopies = 4;    // copies of the pair tables, by lane, against bank conflicts
 
 struct FewArgs {
   tqk_cache_desc d;
@@ -58,7 +60,7 @@ struct BlockRuns {
 // KB: key code bits; PK: PolarQuant keys (KB == VB); TILED: value codes in units
 // of 4 tokens x 8 channels.
 template <int D, int VB, int KB, bool PK, bool TILED>
-__global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes(FewArgs a) {
+__global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
   constexpr int CPL = D / 4;          // channels of a lane in a score product: CPL lg + 8 m + e
   constexpr int NM = D / 32;          // steps of a score product
   constexpr int KW = CPL * KB / 32 > 0 ? (CPL * KB + 31) / 32 : 1;  // words of a lane's key codes
@@ -80,9 +82,17 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
   // a wave's side-list tile (hi, then lo: 16 x D fp16 each), later its accumulators
   __shared__ __align__(16) uint16_t stage_s[kFewWaves][2 * 16 * D];
   __shared__ __align__(16) float stat_s[kFewWaves][2][D];    // the group's scale and mean
-  __shared__ uint32_t key_s[(1 << (2 * KB)) * kPairCopies];  // a pair of key codes -> two fp16 levels
-  __shared__ uint32_t val_s[(1 << (2 * VB)) * kPairCopies];  // a pair of value codes -> two fp16 centroids
-  __shared__ float lev_s[16], cen_s[16];
+  // a pair of key codes -> its levels, {hi, hi} and {lo, lo}; a pair of value codes
+  // -> its centroids; with 4-bit keys and values one row for both
+  constexpr bool kRow = D <= 128, kShared = kRow && KB == 4 && VB == 4;
+  constexpr int kKeyLog = kRow ? 8 : 5, kValLog = kRow ? 8 : 4;  // log2 of an entry's bytes
+  constexpr int kKeyCopies = kShared ? 16 : (1 << kKeyLog) / 8, kValCopies = kShared ? 32 : (1 << kValLog) / 4;
+  constexpr int kKeyEntries = 1 << (2 * KB), kValEntries = 1 << (2 * VB);
+  __shared__ __align__(256) uint8_t key_s[kKeyEntries << kKeyLog];
+  __shared__ __align__(256) uint8_t val_own[kShared ? 4 : kValEntries << kValLog];
+  uint8_t* const val_s = kShared ? key_s : val_own;
+  constexpr uint32_t kValOff = kShared ? 128 : 0;
+  __shared__ __align__(16) float lev_s[16], cen_s[16];
   __shared__ float ml_s[2][kFewWaves][kFewRows];
 
   const int n = min(a.seq_lens[b], a.max_len);
@@ -126,48 +136,6 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
   const bool is_cold = gw < cold_waves;
   const int i0 = (is_cold ? gw : gw - cold_waves) * run;
   const int i1 = min(i0 + run, is_cold ? cold.n : hot.n);
-  __syncthreads();
-
-  // the scale of a codebook: candidate 1 + i / 128 whose entries lose least to
-  // fp16, the first of equals
-  auto best_scale = [&](const float* book, int size) {
-    float err[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float g = 1.0f + (float)(lane + 64 * k) * (1.0f / 128);
-      float e = 0.f;
-      for (int i = 0; i < size; ++i) {
-        const float y = book[i] * g, r = y - (float)(_Float16)y;
-        e = fmaf(r, r, e);
-      }
-      err[k] = e / (g * g);
-    }
-    const float best = -wave_reduce<true>(-fminf(err[0], err[1]));
-    const uint64_t b0 = __builtin_amdgcn_ballot_w64(err[0] == best), b1 = __builtin_amdgcn_ballot_w64(err[1] == best);
-    return 1.0f + (float)(b0 ? __builtin_ctzll(b0) : b1 ? 64 + __builtin_ctzll(b1) : 0) * (1.0f / 128);
-  };
-  const float up = best_scale(cen_s, 1 << VB), k_up = best_scale(lev_s, 1 << KB);
-  for (int i = tid; i < (1 << (2 * VB)) * kPairCopies; i += kFewThreads)
-    val_s[i] = pk_f16(cen_s[i / kPairCopies & ((1 << VB) - 1)] * up, cen_s[i / kPairCopies >> VB] * up);
-  for (int i = tid; i < (1 << (2 * KB)) * kPairCopies; i += kFewThreads)
-    key_s[i] = pk_f16(lev_s[k_code_even(i / kPairCopies, KB)] * k_up, lev_s[k_code_odd(i / kPairCopies, KB)] * k_up);
-  // table reads: the field of `bits` bits at `sh` of w, as an entry of 16 bytes and this lane's copy of it
-  static_assert(kPairCopies == 4, "entries of 16 bytes");
-  const uint32_t copy = 4 * (lane % kPairCopies);
-  auto entry = [&](const uint32_t* table, uint32_t w, int sh, int bits) {
-    const uint32_t mask = ((1u << bits) - 1u) << 4;
-    const uint32_t o = ((sh >= 4 ? w >> (sh - 4) : w << (4 - sh)) & mask) | copy;
-    return *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(table) + o);
-  };
-  // ... of a word array, at any bit
-  auto field = [&](const uint32_t* table, const uint32_t* w, int bit, int bits) {
-    const int wd = bit / 32, sh = bit % 32;
-    return sh + bits > 32 ? entry(table, __builtin_amdgcn_alignbit(w[wd + 1], w[wd], sh), 0, bits)
-                          : entry(table, w[wd], sh, bits);
-  };
-  // (the side-list tile starts at zero)
-#pragma unroll
-  for (int i = 0; i < 4 * D / 64; ++i) reinterpret_cast<u32x4_t*>(stage_s[wave])[64 * i + lane] = u32x4_t{0u, 0u, 0u, 0u};
 
   // Q: row ln, channels CPL lg + 8 m .. + 7 (rows past the last: a real one's, dropped later)
   h8_t qf[NM];
@@ -175,9 +143,228 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
                              (long long)min(max(t, 0), a.q_len - 1) * a.q_stride[2];
 #pragma unroll
   for (int mm = 0; mm < NM; ++mm) qf[mm] = *reinterpret_cast<const h8_t*>(qp + CPL * lg + 8 * mm);
-  // the coded keys' weights, an fp16 pair: q * scale / k_up, group by group, or
-  // for rotated keys q @ Pi^T / k_up
+  // the coded keys' weights, an fp16 pair: q * scale group by group, or for
+  // rotated keys q @ Pi^T
   h8_t wh[NM], wl[NM];
+
+  // ---- the coded blocks of this wave: state and loads
+  uint16_t* const hi_s = stage_s[wave];
+  uint16_t* const lo_s = hi_s + 16 * D;
+  auto at = [](int tok, int ch) { return (tok * (D / 8) + (ch ^ (tok & 7))) * 8; };  // (turned by the row: bank conflicts)
+  const size_t head = (size_t)h * d.n_pages * P;
+  const int32_t* const bt = a.p.block_table + (size_t)b * d.max_pages_per_seq;
+  const int32_t* const gt = a.p.group_table + (size_t)b * d.max_groups_per_seq;
+  const bool listed = !PK && d.outliers_per_channel > 0;
+  // (a valid pointer even without a side-list)
+  const uint32_t* const oent = listed ? a.p.oent : reinterpret_cast<const uint32_t*>(a.p.ocount);
+  const int cap = listed ? d.outlier_cap : 1;
+
+  // Every load of the loop is issued, at an index inside its table, so that the
+  // waits on them stay exact.  Slots and side-list bounds of 64 blocks at a
+  // time, one a lane: their chain of loads is paid once.
+  int meta_slot = 0, meta_lo = 0, meta_hi = 0, meta_i = i0;
+  auto load_meta = [&](int i) {
+    meta_i = i;
+    const int blk = cold.at(min(i + lane, i1 - 1)), g = blk / nblk, k = blk % nblk;
+    meta_slot = gt[g];
+    const int32_t* oc = a.p.ocount + ((size_t)meta_slot * Hkv + h) * TQK_NOB;
+    const int lo_ = oc[max(k - 1, 0)], hi_ = oc[k];
+    meta_lo = listed && k > 0 ? min(lo_, cap) : 0;
+    meta_hi = listed ? min(hi_, cap) : 0;
+  };
+  // a block of the run: its group and place in it, walked without divisions
+  struct Place {
+    int g, k;
+  };
+  auto place_of = [&](int i) {
+    const int blk = cold.at(i);
+    return Place{blk / nblk, blk % nblk};
+  };
+  auto after = [&](Place x, int i) {  // the block after x, which is block i of the run (the last: itself)
+    if (i + 1 >= i1) return x;
+    if (i + 1 == cold.n0) return place_of(i + 1);
+    return x.k + 1 == nblk ? Place{x.g + 1, 0} : Place{x.g, x.k + 1};
+  };
+  // the page row of token lane % 32 of a block (past its tokens: the last); pages
+  // inside a group by a product (fewer than 256 tokens: exact)
+  const float per_page = 1.0f / (float)P;
+  const int group_pages = G / P;
+  auto row_of = [&](Place x) {
+    const int o = min(32 * x.k + (lane & 31), G - 1), pg = (int)(((float)o + 0.5f) * per_page);
+    return bt[x.g * group_pages + pg] * P + o - pg * P;
+  };
+  constexpr int SPL = D / 64;  // channels a lane brings of the next group's scale and mean
+  uint32_t kw[2][KW], ent[2];
+  float nsc[SPL], nmu[SPL];
+  uint32_t vw[NS][8];
+  float norm = 0.f, kn = 0.f;
+  size_t ob = 0;
+  int e_lo = 0, e_hi = 0;
+  auto load_keys = [&](int i, int rw) {
+    ob = (size_t)__builtin_amdgcn_readlane(meta_slot, i - meta_i) * Hkv + h;
+    e_lo = __builtin_amdgcn_readlane(meta_lo, i - meta_i);
+    e_hi = __builtin_amdgcn_readlane(meta_hi, i - meta_i);
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      const int rr = __shfl(rw, 16 * tile + ln, 64);
+      const uint8_t* src = a.p.kcodes + (head + rr) * KROW + lg * (CPL * KB / 8);
+      if constexpr (CPL * KB % 32 == 0) {
+#pragma unroll
+        for (int e = 0; e < KW; ++e) kw[tile][e] = reinterpret_cast<const uint32_t*>(src)[e];
+      } else {  // six bytes (3-bit keys at head_dim 64)
+        const uint16_t* s2 = reinterpret_cast<const uint16_t*>(src);
+        kw[tile][0] = (uint32_t)s2[0] | (uint32_t)s2[1] << 16;
+        kw[tile][1] = s2[2];
+      }
+    }
+    if constexpr (PK) {
+      kn = a.p.knorm[head + rw];
+    } else {
+#pragma unroll
+      for (int e = 0; e < SPL; ++e) {
+        nsc[e] = a.p.gscale[ob * D + SPL * lane + e];
+        nmu[e] = a.p.gmean[ob * D + SPL * lane + e];
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) ent[s] = oent[ob * cap + min(e_lo + lane + 64 * s, cap - 1)];
+    }
+  };
+  // a group's weights and the start of its scores (q . mean)
+  float bias = 0.f;
+  auto begin_group = [&]() {
+#pragma unroll
+    for (int e = 0; e < SPL; ++e) {
+      stat_s[wave][0][SPL * lane + e] = nsc[e];
+      stat_s[wave][1][SPL * lane + e] = nmu[e];
+    }
+    wave_sync();
+    float y = 0.f;
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const int ch = CPL * lg + 8 * mm + e;
+        const f4_t s4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][0][ch]);
+        const f4_t m4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][1][ch]);
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float q1 = (float)qf[mm][e + k];
+          y = fmaf(q1, m4[k], y);
+          x[k] = q1 * s4[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          // (towards zero: two in one instruction, and no infinity up to 2 * 65504)
+          const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x[k], x[k + 1]));
+          const h2_t ll = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hh.x, -1.f, x[k]),
+                                                                              fmaf((float)hh.y, -1.f, x[k + 1])));
+          wh[mm][e + k] = hh.x;
+          wh[mm][e + k + 1] = hh.y;
+          wl[mm][e + k] = ll.x;
+          wl[mm][e + k + 1] = ll.y;
+        }
+      }
+    bias = colgroup_sum(y);
+  };
+  auto load_values = [&](int rw) {
+    norm = a.p.vnorm[head + rw];
+    if constexpr (TILED) {
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        const int rr = __builtin_amdgcn_readlane(rw, 16 * tile);
+        const uint32_t* src =
+            reinterpret_cast<const uint32_t*>(a.p.vcodes + (head + rr) * VROW + v_unit_offset(lg, ln, VROW));
+#pragma unroll
+        for (int e = 0; e < VB; ++e) vw[0][4 * tile + e] = src[e];
+      }
+    } else {
+      // eight codes of each of the lane's tokens
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int rr = __shfl(rw, 16 * (e / 4) + 4 * lg + e % 4, 64);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const uint8_t* src = a.p.vcodes + (head + rr) * VROW + ((D == 64 ? ln / 2 : ln) + 16 * s) * VB;
+          if constexpr (VB == 4)
+            vw[s][e] = *reinterpret_cast<const uint32_t*>(src);
+          else if constexpr (VB == 3)
+            vw[s][e] = (uint32_t)src[0] | (uint32_t)src[1] << 8 | (uint32_t)src[2] << 16;
+          else
+            vw[s][e] = *reinterpret_cast<const uint16_t*>(src);
+        }
+      }
+    }
+  };
+  Place at_0{0, 0}, at_1{0, 0}, at_2{0, 0};  // blocks i, i + 1, i + 2
+  int row_n = 0;
+  const bool has_codes = is_cold && i0 < i1;
+  if (has_codes) {
+    at_0 = place_of(i0);
+    at_1 = after(at_0, i0);
+    at_2 = after(at_1, i0 + 1);
+    load_meta(i0);
+    const int row_c = row_of(at_0);
+    row_n = row_of(at_1);
+    load_keys(i0, row_c);
+    load_values(row_c);
+  }
+
+  lds_barrier();
+
+  // the scale of the value codebook: candidate 1 + i / 128 whose centroids lose
+  // least to fp16, the first of equals
+  float up;
+  {
+    float err[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float g = 1.0f + (float)(lane + 64 * k) * (1.0f / 128);
+      float e = 0.f;
+#pragma unroll
+      for (int i = 0; i < (1 << VB); ++i) {
+        const float y = cen_s[i] * g, r = y - (float)(_Float16)y;
+        e = fmaf(r, r, e);
+      }
+      err[k] = e / (g * g);
+    }
+    const float best = -wave_reduce<true>(-fminf(err[0], err[1]));
+    const uint64_t b0 = __builtin_amdgcn_ballot_w64(err[0] == best), b1 = __builtin_amdgcn_ballot_w64(err[1] == best);
+    up = 1.0f + (float)(b0 ? __builtin_ctzll(b0) : b1 ? 64 + __builtin_ctzll(b1) : 0) * (1.0f / 128);
+  }
+  for (int i = tid; i < kKeyEntries * kKeyCopies; i += kFewThreads) {
+    const int e = i / kKeyCopies;
+    *reinterpret_cast<uint2*>(key_s + (e << kKeyLog) + 8 * (i % kKeyCopies)) =
+        split_pair(lev_s[k_code_even(e, KB)], lev_s[k_code_odd(e, KB)]);
+  }
+  for (int i = tid; i < kValEntries * kValCopies; i += kFewThreads) {
+    const int e = i / kValCopies;
+    *reinterpret_cast<uint32_t*>(val_s + (e << kValLog) + kValOff + 4 * (i % kValCopies)) =
+        pk_f16(cen_s[e & ((1 << VB) - 1)] * up, cen_s[e >> VB] * up);
+  }
+  // a table read: the field of `bits` bits at bit `bit` of the word array w, as an
+  // entry of 2^lg bytes and this lane's copy in it
+  const uint32_t k_copy = 8 * (lane % kKeyCopies), v_copy = kValOff + 4 * (lane % kValCopies);
+  auto place_in = [](const uint32_t* w, int bit, int bits, int lg, uint32_t copy) -> uint32_t {
+    const int wd = bit / 32, sh = bit % 32;
+    if (bits == 8 && lg == 8)  // byte sh / 8 above the copy's byte
+      return __builtin_amdgcn_perm(w[wd], copy, 0x0C0C0000u | (4u + sh / 8) << 8);
+    const uint32_t mask = ((1u << bits) - 1u) << lg;
+    const uint32_t x = sh + bits > 32 ? __builtin_amdgcn_alignbit(w[wd + 1], w[wd], sh) << lg
+                       : sh >= lg     ? w[wd] >> (sh - lg)
+                                      : w[wd] << (lg - sh);
+    return (x & mask) | copy;
+  };
+  auto levels = [&](const uint32_t* w, int bit) {
+    return *reinterpret_cast<const uint2*>(key_s + place_in(w, bit, 2 * KB, kKeyLog, k_copy));
+  };
+  auto centroids = [&](const uint32_t* w, int bit) {
+    return *reinterpret_cast<const uint32_t*>(val_s + place_in(w, bit, 2 * VB, kValLog, v_copy));
+  };
+  // (the side-list tile starts at zero)
+#pragma unroll
+  for (int i = 0; i < 4 * D / 64; ++i) reinterpret_cast<u32x4_t*>(stage_s[wave])[64 * i + lane] = u32x4_t{0u, 0u, 0u, 0u};
+
   if constexpr (PK) {
     __syncthreads();
     float* const q_s = reinterpret_cast<float*>(&stage_s[0][0]);  // [16][D]
@@ -194,7 +381,7 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
       float y = 0.f;
 #pragma unroll 8
       for (int k = 0; k < D; ++k) y = fmaf(q_s[r * D + k], a.p.pi_t[k * D + j], y);
-      r_s[i] = y / k_up;
+      r_s[i] = y;
     }
     __syncthreads();
 #pragma unroll
@@ -206,7 +393,7 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
         wl[mm][e] = (_Float16)(y - (float)wh[mm][e]);
       }
   }
-  __syncthreads();
+  lds_barrier();
 
   const float c = d.sm_scale * 1.4426950408889634f;
   float m_run = -INFINITY, l_run = 0.f;
@@ -244,149 +431,10 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
     }
   };
 
-  if (is_cold && i0 < i1) {
-    uint16_t* const hi_s = stage_s[wave];
-    uint16_t* const lo_s = hi_s + 16 * D;
-    auto at = [](int tok, int ch) { return (tok * (D / 8) + (ch ^ (tok & 7))) * 8; };  // (turned by the row: bank conflicts)
-    const size_t head = (size_t)h * d.n_pages * P;
-    const int32_t* const bt = a.p.block_table + (size_t)b * d.max_pages_per_seq;
-    const int32_t* const gt = a.p.group_table + (size_t)b * d.max_groups_per_seq;
-    const bool listed = !PK && d.outliers_per_channel > 0;
-    // (a valid pointer even without a side-list)
-    const uint32_t* const oent = listed ? a.p.oent : reinterpret_cast<const uint32_t*>(a.p.ocount);
-    const int cap = listed ? d.outlier_cap : 1;
-
-    // Every load of the loop is issued, at an index inside its table, so that the
-    // waits on them stay exact.  Slots and side-list bounds of 64 blocks at a
-    // time, one a lane: their chain of loads is paid once.
-    int meta_slot = 0, meta_lo = 0, meta_hi = 0, meta_i = i0;
-    auto load_meta = [&](int i) {
-      meta_i = i;
-      const int blk = cold.at(min(i + lane, i1 - 1)), g = blk / nblk, k = blk % nblk;
-      meta_slot = gt[g];
-      const int32_t* oc = a.p.ocount + ((size_t)meta_slot * Hkv + h) * TQK_NOB;
-      const int lo_ = oc[max(k - 1, 0)], hi_ = oc[k];
-      meta_lo = listed && k > 0 ? min(lo_, cap) : 0;
-      meta_hi = listed ? min(hi_, cap) : 0;
-    };
-    // the page row of token lane % 32 of block i of the run (past its tokens: the last)
-    auto row_of = [&](int i) {
-      const int blk = cold.at(min(i, i1 - 1)), g = blk / nblk, k = blk % nblk;
-      const int tok = g * G + min(32 * k + (lane & 31), G - 1);
-      return bt[tok / P] * P + tok % P;
-    };
-    constexpr int SPL = D / 64;  // channels a lane brings of the next group's scale and mean
-    uint32_t kw[2][KW], ent[2];
-    float nsc[SPL], nmu[SPL];
-    uint32_t vw[NS][8];
-    float norm = 0.f, kn = 0.f;
-    size_t ob = 0;
-    int e_lo = 0, e_hi = 0;
-    auto load_keys = [&](int i, int rw) {
-      ob = (size_t)__builtin_amdgcn_readlane(meta_slot, i - meta_i) * Hkv + h;
-      e_lo = __builtin_amdgcn_readlane(meta_lo, i - meta_i);
-      e_hi = __builtin_amdgcn_readlane(meta_hi, i - meta_i);
-#pragma unroll
-      for (int tile = 0; tile < 2; ++tile) {
-        const int rr = __shfl(rw, 16 * tile + ln, 64);
-        const uint8_t* src = a.p.kcodes + (head + rr) * KROW + lg * (CPL * KB / 8);
-        if constexpr (CPL * KB % 32 == 0) {
-#pragma unroll
-          for (int e = 0; e < KW; ++e) kw[tile][e] = reinterpret_cast<const uint32_t*>(src)[e];
-        } else {  // six bytes (3-bit keys at head_dim 64)
-          const uint16_t* s2 = reinterpret_cast<const uint16_t*>(src);
-          kw[tile][0] = (uint32_t)s2[0] | (uint32_t)s2[1] << 16;
-          kw[tile][1] = s2[2];
-        }
-      }
-      if constexpr (PK) {
-        kn = a.p.knorm[head + rw];
-      } else {
-#pragma unroll
-        for (int e = 0; e < SPL; ++e) {
-          nsc[e] = a.p.gscale[ob * D + SPL * lane + e];
-          nmu[e] = a.p.gmean[ob * D + SPL * lane + e];
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) ent[s] = oent[ob * cap + min(e_lo + lane + 64 * s, cap - 1)];
-      }
-    };
-    // a group's weights and the start of its scores (q . mean)
-    float bias = 0.f;
-    auto begin_group = [&]() {
-#pragma unroll
-      for (int e = 0; e < SPL; ++e) {
-        stat_s[wave][0][SPL * lane + e] = nsc[e];
-        stat_s[wave][1][SPL * lane + e] = nmu[e];
-      }
-      wave_sync();
-      const float inv = 1.0f / k_up;
-      float y = 0.f;
-#pragma unroll
-      for (int mm = 0; mm < NM; ++mm)
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const int ch = CPL * lg + 8 * mm + e;
-          const f4_t s4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][0][ch]);
-          const f4_t m4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][1][ch]);
-          float x[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float q1 = (float)qf[mm][e + k];
-            y = fmaf(q1, m4[k], y);
-            x[k] = q1 * (s4[k] * inv);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            // (towards zero: two in one instruction, and no infinity up to 2 * 65504)
-            const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x[k], x[k + 1]));
-            const h2_t ll = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hh.x, -1.f, x[k]),
-                                                                                fmaf((float)hh.y, -1.f, x[k + 1])));
-            wh[mm][e + k] = hh.x;
-            wh[mm][e + k + 1] = hh.y;
-            wl[mm][e + k] = ll.x;
-            wl[mm][e + k + 1] = ll.y;
-          }
-        }
-      bias = colgroup_sum(y);
-    };
-    auto load_values = [&](int rw) {
-      norm = a.p.vnorm[head + rw];
-      if constexpr (TILED) {
-#pragma unroll
-        for (int tile = 0; tile < 2; ++tile) {
-          const int rr = __builtin_amdgcn_readlane(rw, 16 * tile);
-          const uint32_t* src =
-              reinterpret_cast<const uint32_t*>(a.p.vcodes + (head + rr) * VROW + v_unit_offset(lg, ln, VROW));
-#pragma unroll
-          for (int e = 0; e < VB; ++e) vw[0][4 * tile + e] = src[e];
-        }
-      } else {
-        // eight codes of each of the lane's tokens
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int rr = __shfl(rw, 16 * (e / 4) + 4 * lg + e % 4, 64);
-#pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            const uint8_t* src = a.p.vcodes + (head + rr) * VROW + ((D == 64 ? ln / 2 : ln) + 16 * s) * VB;
-            if constexpr (VB == 4)
-              vw[s][e] = *reinterpret_cast<const uint32_t*>(src);
-            else if constexpr (VB == 3)
-              vw[s][e] = (uint32_t)src[0] | (uint32_t)src[1] << 8 | (uint32_t)src[2] << 16;
-            else
-              vw[s][e] = *reinterpret_cast<const uint16_t*>(src);
-          }
-        }
-      }
-    };
-    load_meta(i0);
-    int row_c = row_of(i0), row_n = row_of(i0 + 1);
-    load_keys(i0, row_c);
-    load_values(row_c);
+  if (has_codes) {
     for (int i = i0; i < i1; ++i) {
-      const int blk = cold.at(i), g = blk / nblk, k = blk % nblk;
-      const int tok0 = g * G + 32 * k, cnt = min(32, G - 32 * k);
-      const int row_nn = row_of(i + 2);
+      const int k = at_0.k, tok0 = at_0.g * G + 32 * k, cnt = min(32, G - 32 * k);
+      const int row_nn = row_of(at_2);
       if (!PK && (i == i0 || k == 0 || i == cold.n0)) begin_group();  // (the second run may start inside a group)
       f4_t S[2];
 #pragma unroll
@@ -394,32 +442,45 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
         S[tile] = f4_t{bias, bias, bias, bias};
 #pragma unroll
         for (int mm = 0; mm < NM; ++mm) {
-          union { h8_t h; uint32_t u[4]; } y;
+          union { h8_t h; uint32_t u[4]; } hi, lo16;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y.u[e] = field(key_s, kw[tile], KB * (8 * mm + 2 * e), 2 * KB);
-          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, wl[mm], S[tile], 0, 0, 0);
-          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, wh[mm], S[tile], 0, 0, 0);
+          for (int e = 0; e < 4; ++e) {
+            const uint2 y = levels(kw[tile], KB * (8 * mm + 2 * e));
+            hi.u[e] = y.x;
+            lo16.u[e] = y.y;
+          }
+          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16.h, wh[mm], S[tile], 0, 0, 0);
+          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.h, wl[mm], S[tile], 0, 0, 0);
+          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.h, wh[mm], S[tile], 0, 0, 0);
         }
       }
       if (!PK && e_hi > e_lo) {
-        // the block's side-list entries, tile by tile
+        // the block's side-list entries, tile by tile: an entry's place in the
+        // sparse tile and its value over the mean, as a pair
+        struct Spot {
+          int tile, o;
+          uint32_t hi, lo;
+        };
+        auto spot = [&](uint32_t y, bool real) {
+          const int tok = (int)((y & 0xFFFFu) / D) - 32 * k, ch = (int)(y & (D - 1));
+          const float v = h2f((uint16_t)(y >> 16)) - stat_s[wave][1][ch];
+          const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(v, 0.f));
+          return Spot{real && (unsigned)tok < 32u ? tok >> 4 : 2, at(tok & 15, ch / 8) + ch % 8,
+                      __builtin_bit_cast(uint16_t, hh.x), f2h(v - (float)hh.x)};
+        };
+        auto put = [&](const Spot& x, int tile, bool clear) {
+          if (x.tile == tile) {
+            hi_s[x.o] = clear ? 0 : (uint16_t)x.hi;
+            lo_s[x.o] = clear ? 0 : (uint16_t)x.lo;
+          }
+        };
+        const Spot e0 = spot(ent[0], e_lo + lane < e_hi), e1 = spot(ent[1], e_lo + 64 + lane < e_hi);
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
-          auto put = [&](uint32_t y, bool clear) {
-            const int tok = (int)((y & 0xFFFFu) / D) - 32 * k - 16 * tile, ch = (int)(y & (D - 1));
-            if ((unsigned)tok < 16u) {
-              const int o = at(tok, ch / 8) + ch % 8;
-              const float v = h2f((uint16_t)(y >> 16)) - stat_s[wave][1][ch];
-              const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(v, 0.f));
-              hi_s[o] = clear ? 0 : __builtin_bit_cast(uint16_t, hh.x);
-              lo_s[o] = clear ? 0 : f2h(v - (float)hh.x);
-            }
-          };
           auto each = [&](bool clear) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-              if (e_lo + lane + 64 * s < e_hi) put(ent[s], clear);
-            for (int e = e_lo + 128 + lane; e < e_hi; e += 64) put(oent[ob * cap + e], clear);
+            put(e0, tile, clear);
+            put(e1, tile, clear);
+            for (int e = e_lo + 128 + lane; e < e_hi; e += 64) put(spot(oent[ob * cap + e], true), tile, clear);
             wave_sync();
           };
           each(false);
@@ -458,7 +519,7 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
             union { h8_t h; uint32_t u[4]; } y;
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
-              y.u[f] = field(val_s, vw[0] + 4 * (f / 2), (2 * j + f % 2) * 2 * VB, 2 * VB);
+              y.u[f] = centroids(vw[0] + 4 * (f / 2), (2 * j + f % 2) * 2 * VB);
             }
             O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, pf, O[j], 0, 0, 0);
           }
@@ -468,8 +529,10 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
           for (int j = 0; j < NC; j += 2) {
             uint32_t two[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              two[e] = entry(val_s, D == 64 ? vw[s][e] >> ((ln & 1) * 4 * VB) : vw[s][e], VB * j, 2 * VB);
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t y = D == 64 ? vw[s][e] >> ((ln & 1) * 4 * VB) : vw[s][e];
+              two[e] = centroids(&y, VB * j);
+            }
             union { h8_t h; uint32_t u[4]; } y0, y1;
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
@@ -483,6 +546,9 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
       }
       load_values(row_n);
       row_n = row_nn;
+      at_0 = at_1;
+      at_1 = at_2;
+      at_2 = after(at_2, i + 2);
     }
   } else if (!is_cold) {
     // uncoded blocks, straight from the ring
@@ -506,7 +572,8 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
       // values: token e of this lane, channels NC ln .. + NC - 1 of the piece;
       // zero where no row sees the token, whatever stands there
       u32x4_t vv[NS][8];
-      bool odd = false;
+      typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
+      us2_t top = {0, 0};  // the largest exponent fields
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int o = 16 * (e / 4) + 4 * lg + e % 4, tok = tok0 + o;
@@ -523,7 +590,7 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
           if (!any) vv[s][e] = u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
           for (int f = 0; f < NC / 2; ++f)
-            odd |= (vv[s][e][f] & 0x7C00u) == 0x7C00u || (vv[s][e][f] & 0x7C000000u) == 0x7C000000u;
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(us2_t, vv[s][e][f] & 0x7C007C00u));
         }
       }
       float w[8];
@@ -531,21 +598,8 @@ __global__ __launch_bounds__(kFewThreads, D <= 64 ? 4 : 2) void tqk_attend_codes
       h8_t pf;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pf[e] = (_Float16)w[e];
-      auto products = [&](f4_t (&acc)[NV], const u32x4_t (&val)[NS][8]) {
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-          for (int j = 0; j < NC; ++j) {
-            union { h8_t h; uint32_t u[4]; } y;
-#pragma unroll
-            for (int f = 0; f < 4; ++f)
-              y.u[f] = __builtin_amdgcn_perm(val[s][2 * f + 1][j / 2], val[s][2 * f][j / 2],
-                                             (j & 1) ? 0x07060302u : 0x05040100u);
-            acc[NC * s + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, pf, acc[NC * s + j], 0, 0, 0);
-          }
-      };
       // (an infinity or a NaN that some queries see and others do not: set aside)
-      const bool apart = a.per_item > 1 && __any(odd) && !all_see(tok0, cnt);
+      const bool apart = a.per_item > 1 && __any(top.x == 0x7C00 || top.y == 0x7C00) && !all_see(tok0, cnt);
       if (__builtin_expect(apart, 0)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -770,10 +824,9 @@ FewPlan few_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
     if (w < tokens) tokens = w;
   }
   const long long blocks = (tokens + 31) / 32 + 1;
-  // Splits: rounds of the workgroups that fit (two a CU at head_dim 64)
-  // times a wave's run of blocks and the set-up, joining and rotation of about
+  // Splits: rounds of the workgroups that fit (one a CU) times a wave's run of blocks and the set-up, joining and rotation of about
   // three blocks' time; another launch to join them, about two.
-  const long long slots = (d->head_dim == 64 ? 2 : 1) * (long long)device_cus();
+  const long long slots = device_cus();
   double best = 1e30;
   for (int s = 1; s <= 64 && (s == 1 || (long long)kFewWaves * (s - 1) < blocks); ++s) {
     const long long rounds = (pairs * s + slots - 1) / slots;

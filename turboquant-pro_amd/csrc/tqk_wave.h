@@ -29,6 +29,26 @@ __device__ __forceinline__ float wave_reduce(float x) {
   return op(__builtin_bit_cast(float, (uint32_t)r32[0]), __builtin_bit_cast(float, (uint32_t)r32[1]));
 }
 
+// two floats as fp16 pairs: {hi, hi}, {lo, lo}
+__device__ __forceinline__ uint2 split_pair(float x0, float x1) {
+  const _Float16 h0 = (_Float16)x0, h1 = (_Float16)x1;
+  const _Float16 l0 = (_Float16)(x0 - (float)h0), l1 = (_Float16)(x1 - (float)h1);
+  return make_uint2((uint32_t)__builtin_bit_cast(uint16_t, h0) |
+                        ((uint32_t)__builtin_bit_cast(uint16_t, h1) << 16),
+                    (uint32_t)__builtin_bit_cast(uint16_t, l0) |
+                        ((uint32_t)__builtin_bit_cast(uint16_t, l1) << 16));
+}
+
+// Workgroup barrier for LDS data only: this wave's LDS operations complete
+// (lgkmcnt 0), then s_barrier.  Unlike __syncthreads it leaves the wave's
+// global loads in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // vmcnt 63, expcnt 7, lgkmcnt 0
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Orders LDS accesses of one wave across lanes.  A wave's LDS instructions
 // execute in issue order, so program order is enough; this only stops the
 // compiler from moving memory operations across the point (and, unlike a
