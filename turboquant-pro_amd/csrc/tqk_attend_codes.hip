@@ -6,23 +6,27 @@
 // 32 tokens that any of the rows sees; its eight waves take runs of blocks,
 // coded or uncoded, each on its own until the end.
 //
-// A coded block, 16 tokens at a time: a pair of key codes is an entry of a table
-// of levels as fp16 pairs (hi + lo: 2^-22), four of them an operand of K Q^T as
-// they are; the group's scale goes into the query, a pair too, its mean into the
-// scores' start.  A
-// side-list entry, whose code is the zero level, adds q (val - mean): the tile's
-// entries stand as fp16 pairs in an otherwise zero LDS tile of the wave, which is
-// a second operand for the same product and is cleared entry by entry.  A lane
-// then holds one row's scores of 8 tokens, which are the operand of V^T P^T as
-// they are.  Value codes become centroids by pairs through a table, the codebook
-// scaled so that its fp16 roundings nearly vanish (best of 128 scales: 2^-12 of a
-// centroid becomes 2^-14 to 2^-15); weights times norms are rounded to fp16 (2^-12
-// of each).  The coded part is rotated back once a workgroup, by the matrix cores
-// in fp16 pairs.  Up to head_dim 128 a table entry has a row of 256 bytes of
-// copies, by lane: a lookup's bank is its lane's own, and its address one byte
-// permutation; at head_dim 256 the waves' tiles leave room for four copies.
-// Bound: few sequences, the chain of dependent loads (lengths, tables, codes);
-// many, the table reads and VALU work of a block beside its codes from HBM.
+// A coded block: a pair of key codes is an entry of a table of levels as fp16 pairs
+// (hi + lo: 2^-22; scaled single ones were 1 us of 33 faster, and the result's error
+// a third larger), four of them an operand of K Q^T as they are; the group's scale
+// goes into the query, a pair too, its mean into the scores' start.  A side-list
+// entry, whose code is the zero level, adds q (val - mean): the block's entries
+// stand in an otherwise zero LDS tile of the wave, the first halves of their fp16
+// pairs, then the second ones, each a second operand of the same product, and are
+// cleared one by one.  They go there before the block's lookups, whose time hides
+// the trip.  A lane then holds one row's scores of 8 tokens, which are the operand
+// of V^T P^T as they are.  Value codes become centroids by pairs through a table,
+// the codebook scaled so that its fp16 roundings nearly vanish (best of 128 scales:
+// 2^-12 of a centroid becomes about 2^-14 to 2^-15); weights times norms are rounded
+// to fp16 (2^-12 of each).  The coded part is rotated back once a workgroup, by the
+// matrix cores in fp16 pairs.  Up to head_dim 128 a table entry has a row of 256
+// bytes of copies, by lane: a lookup's bank is its lane's own, and its address one
+// byte permutation; at head_dim 256 the waves' tiles leave room for four copies.
+// Bound: few sequences, the chain of dependent loads (lengths, tables, codes) and
+// the set-up; many, a wave's chain of LDS trips and products beside its codes from
+// HBM: 16 sequences of 8192 tokens, 8 kv heads of 128, 35 us with a window of 4096,
+// of which a one-block window takes 8; with every page and group the same one, in
+// cache, no more than 3% less.
 #include "tqk_attend.h"
 #include "tqk_wave.h"
 
@@ -79,8 +83,8 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
   x /= Hkv;
   const int q0 = x % a.q_items * a.per_item, b = x / a.q_items;
 
-  // a wave's side-list tile (hi, then lo: 16 x D fp16 each), later its accumulators
-  __shared__ __align__(16) uint16_t stage_s[kFewWaves][2 * 16 * D];
+  // a wave's side-list tile (32 x D fp16), later its accumulators
+  __shared__ __align__(16) uint16_t stage_s[kFewWaves][2 * 16 * D + 8];
   __shared__ __align__(16) float stat_s[kFewWaves][2][D];    // the group's scale and mean
   // a pair of key codes -> its levels, {hi, hi} and {lo, lo}; a pair of value codes
   // -> its centroids; with 4-bit keys and values one row for both
@@ -93,6 +97,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
   uint8_t* const val_s = kShared ? key_s : val_own;
   constexpr uint32_t kValOff = kShared ? 128 : 0;
   __shared__ __align__(16) float lev_s[16], cen_s[16];
+  __shared__ float up_s[2][2];  // the best of the scales of a half: its loss, itself
   __shared__ float ml_s[2][kFewWaves][kFewRows];
 
   const int n = min(a.seq_lens[b], a.max_len);
@@ -148,8 +153,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
   h8_t wh[NM], wl[NM];
 
   // ---- the coded blocks of this wave: state and loads
-  uint16_t* const hi_s = stage_s[wave];
-  uint16_t* const lo_s = hi_s + 16 * D;
+  uint16_t* const list_s = stage_s[wave];
   auto at = [](int tok, int ch) { return (tok * (D / 8) + (ch ^ (tok & 7))) * 8; };  // (turned by the row: bank conflicts)
   const size_t head = (size_t)h * d.n_pages * P;
   const int32_t* const bt = a.p.block_table + (size_t)b * d.max_pages_per_seq;
@@ -160,54 +164,75 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
   const int cap = listed ? d.outlier_cap : 1;
 
   // Every load of the loop is issued, at an index inside its table, so that the
-  // waits on them stay exact.  Slots and side-list bounds of 64 blocks at a
+  // waits on them stay exact.  What the tables say of 64 blocks of the run at a
   // time, one a lane: their chain of loads is paid once.
-  int meta_slot = 0, meta_lo = 0, meta_hi = 0, meta_i = i0;
-  auto load_meta = [&](int i) {
-    meta_i = i;
-    const int blk = cold.at(min(i + lane, i1 - 1)), g = blk / nblk, k = blk % nblk;
-    meta_slot = gt[g];
-    const int32_t* oc = a.p.ocount + ((size_t)meta_slot * Hkv + h) * TQK_NOB;
-    const int lo_ = oc[max(k - 1, 0)], hi_ = oc[k];
-    meta_lo = listed && k > 0 ? min(lo_, cap) : 0;
-    meta_hi = listed ? min(hi_, cap) : 0;
-  };
-  // a block of the run: its group and place in it, walked without divisions
-  struct Place {
-    int g, k;
-  };
-  auto place_of = [&](int i) {
-    const int blk = cold.at(i);
-    return Place{blk / nblk, blk % nblk};
-  };
-  auto after = [&](Place x, int i) {  // the block after x, which is block i of the run (the last: itself)
-    if (i + 1 >= i1) return x;
-    if (i + 1 == cold.n0) return place_of(i + 1);
-    return x.k + 1 == nblk ? Place{x.g + 1, 0} : Place{x.g, x.k + 1};
-  };
-  // the page row of token lane % 32 of a block (past its tokens: the last); pages
-  // inside a group by a product (fewer than 256 tokens: exact)
   const float per_page = 1.0f / (float)P;
   const int group_pages = G / P;
-  auto row_of = [&](Place x) {
-    const int o = min(32 * x.k + (lane & 31), G - 1), pg = (int)(((float)o + 0.5f) * per_page);
-    return bt[x.g * group_pages + pg] * P + o - pg * P;
+  // the page row of token o of group g (pages inside a group by a product: fewer
+  // than 256 tokens, exact)
+  auto page_row = [&](int g, int o) {
+    const int pg = (int)(((float)o + 0.5f) * per_page);
+    return bt[g * group_pages + pg] * P + o - pg * P;
+  };
+  int meta_i = i0, meta_g = 0, meta_k = 0, meta_ob = 0, meta_lo = 0, meta_hi = 0, meta_row[2] = {0, 0};
+  auto load_meta = [&](int i) {
+    meta_i = i;
+    const int blk = cold.at(min(i + lane, i1 - 1));
+    meta_g = blk / nblk;
+    meta_k = blk % nblk;
+    meta_ob = gt[meta_g] * Hkv + h;
+    if constexpr (TILED) {  // (16 tokens lie in one page)
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) meta_row[tile] = page_row(meta_g, 32 * meta_k + 16 * tile);
+    }
+    const int32_t* oc = a.p.ocount + (size_t)meta_ob * TQK_NOB;
+    const int lo_ = oc[max(meta_k - 1, 0)], hi_ = oc[meta_k];
+    meta_lo = listed && meta_k > 0 ? min(lo_, cap) : 0;
+    meta_hi = listed ? min(hi_, cap) : 0;
+  };
+  auto of = [&](int x, int i) { return __builtin_amdgcn_readlane(x, i - meta_i); };  // block i's
+  // rows of block i (past the run: of its last): TILED, of its tiles' first
+  // tokens; else of token lane % 32 (past the block's: of the last)
+  struct Rows {
+    int r[2];
+  };
+  auto rows_of = [&](int i) {
+    i = min(i, i1 - 1);
+    if constexpr (TILED) return Rows{of(meta_row[0], i), of(meta_row[1], i)};
+    else return Rows{page_row(of(meta_g, i), min(32 * of(meta_k, i) + (lane & 31), G - 1)), 0};
   };
   constexpr int SPL = D / 64;  // channels a lane brings of the next group's scale and mean
   uint32_t kw[2][KW], ent[2];
   float nsc[SPL], nmu[SPL];
   uint32_t vw[NS][8];
-  float norm = 0.f, kn = 0.f;
+  float norm[8], kn[8];
   size_t ob = 0;
   int e_lo = 0, e_hi = 0;
-  auto load_keys = [&](int i, int rw) {
-    ob = (size_t)__builtin_amdgcn_readlane(meta_slot, i - meta_i) * Hkv + h;
-    e_lo = __builtin_amdgcn_readlane(meta_lo, i - meta_i);
-    e_hi = __builtin_amdgcn_readlane(meta_hi, i - meta_i);
+  // the norms of a lane's 8 tokens of a block: 4 lg .. + 3 and 16 + 4 lg .. + 3
+  auto load_norms = [&](float (&x)[8], const float* from, const Rows& rw) {
+    if constexpr (TILED) {
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        const f4_t y = *reinterpret_cast<const f4_t*>(from + (head + rw.r[tile]) + (uint32_t)(4 * lg));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * tile + e] = y[e];
+      }
+    } else {
+      x[0] = from[head + rw.r[0]];  // (token lane % 32's: handed out when needed)
+    }
+  };
+  auto norm_of = [&](const float (&x)[8], int e) {
+    return TILED ? x[e] : __shfl(x[0], 16 * (e / 4) + 4 * lg + e % 4, 64);
+  };
+  auto load_keys = [&](int i, const Rows& rw) {
+    ob = of(meta_ob, i);
+    e_lo = of(meta_lo, i);
+    e_hi = of(meta_hi, i);
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
-      const int rr = __shfl(rw, 16 * tile + ln, 64);
-      const uint8_t* src = a.p.kcodes + (head + rr) * KROW + lg * (CPL * KB / 8);
+      const uint8_t* src;
+      if constexpr (TILED) src = a.p.kcodes + (head + rw.r[tile]) * KROW + (uint32_t)(ln * KROW + lg * (CPL * KB / 8));
+      else src = a.p.kcodes + (head + __shfl(rw.r[0], 16 * tile + ln, 64)) * KROW + lg * (CPL * KB / 8);
       if constexpr (CPL * KB % 32 == 0) {
 #pragma unroll
         for (int e = 0; e < KW; ++e) kw[tile][e] = reinterpret_cast<const uint32_t*>(src)[e];
@@ -218,7 +243,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       }
     }
     if constexpr (PK) {
-      kn = a.p.knorm[head + rw];
+      load_norms(kn, a.p.knorm, rw);
     } else {
 #pragma unroll
       for (int e = 0; e < SPL; ++e) {
@@ -267,14 +292,13 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       }
     bias = colgroup_sum(y);
   };
-  auto load_values = [&](int rw) {
-    norm = a.p.vnorm[head + rw];
+  auto load_values = [&](const Rows& rw) {
+    load_norms(norm, a.p.vnorm, rw);
     if constexpr (TILED) {
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
-        const int rr = __builtin_amdgcn_readlane(rw, 16 * tile);
-        const uint32_t* src =
-            reinterpret_cast<const uint32_t*>(a.p.vcodes + (head + rr) * VROW + v_unit_offset(lg, ln, VROW));
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(a.p.vcodes + (head + rw.r[tile]) * VROW +
+                                                                (uint32_t)v_unit_offset(lg, ln, VROW));
 #pragma unroll
         for (int e = 0; e < VB; ++e) vw[0][4 * tile + e] = src[e];
       }
@@ -282,7 +306,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       // eight codes of each of the lane's tokens
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int rr = __shfl(rw, 16 * (e / 4) + 4 * lg + e % 4, 64);
+        const int rr = __shfl(rw.r[0], 16 * (e / 4) + 4 * lg + e % 4, 64);
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
           const uint8_t* src = a.p.vcodes + (head + rr) * VROW + ((D == 64 ? ln / 2 : ln) + 16 * s) * VB;
@@ -296,51 +320,47 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       }
     }
   };
-  Place at_0{0, 0}, at_1{0, 0}, at_2{0, 0};  // blocks i, i + 1, i + 2
-  int row_n = 0;
+  Rows next_rows{0, 0};
   const bool has_codes = is_cold && i0 < i1;
   if (has_codes) {
-    at_0 = place_of(i0);
-    at_1 = after(at_0, i0);
-    at_2 = after(at_1, i0 + 1);
     load_meta(i0);
-    const int row_c = row_of(at_0);
-    row_n = row_of(at_1);
-    load_keys(i0, row_c);
-    load_values(row_c);
+    const Rows first = rows_of(i0);
+    next_rows = rows_of(i0 + 1);
+    load_keys(i0, first);
+    load_values(first);
   }
 
   lds_barrier();
 
   // the scale of the value codebook: candidate 1 + i / 128 whose centroids lose
-  // least to fp16, the first of equals
-  float up;
+  // least to fp16, the first of equals; half of them by even waves, half by odd ones
   {
-    float err[2];
+    const float g = 1.0f + (float)(2 * lane + wave % 2) * (1.0f / 128);
+    float err = 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float g = 1.0f + (float)(lane + 64 * k) * (1.0f / 128);
-      float e = 0.f;
-#pragma unroll
-      for (int i = 0; i < (1 << VB); ++i) {
-        const float y = cen_s[i] * g, r = y - (float)(_Float16)y;
-        e = fmaf(r, r, e);
-      }
-      err[k] = e / (g * g);
+    for (int i = 0; i < (1 << VB); ++i) {
+      const float y = cen_s[i] * g, r = y - (float)(_Float16)y;
+      err = fmaf(r, r, err);
     }
-    const float best = -wave_reduce<true>(-fminf(err[0], err[1]));
-    const uint64_t b0 = __builtin_amdgcn_ballot_w64(err[0] == best), b1 = __builtin_amdgcn_ballot_w64(err[1] == best);
-    up = 1.0f + (float)(b0 ? __builtin_ctzll(b0) : b1 ? 64 + __builtin_ctzll(b1) : 0) * (1.0f / 128);
+    err *= __builtin_amdgcn_rcpf(g * g);
+    const float best = -wave_reduce<true>(-err);
+    const uint64_t first = __builtin_amdgcn_ballot_w64(err == best);
+    if (wave < 2 && lane == 0) {
+      up_s[wave][0] = best;
+      up_s[wave][1] = 1.0f + (float)(first ? 2 * __builtin_ctzll(first) + wave : 0) * (1.0f / 128);
+    }
   }
-  for (int i = tid; i < kKeyEntries * kKeyCopies; i += kFewThreads) {
-    const int e = i / kKeyCopies;
-    *reinterpret_cast<uint2*>(key_s + (e << kKeyLog) + 8 * (i % kKeyCopies)) =
-        split_pair(lev_s[k_code_even(e, KB)], lev_s[k_code_odd(e, KB)]);
+  for (int i = tid; i < kKeyEntries * kKeyCopies / 2; i += kFewThreads) {
+    const int e = i / (kKeyCopies / 2);
+    const uint2 y = split_pair(lev_s[k_code_even(e, KB)], lev_s[k_code_odd(e, KB)]);
+    *reinterpret_cast<u32x4_t*>(key_s + (e << kKeyLog) + 16 * (i % (kKeyCopies / 2))) = u32x4_t{y.x, y.y, y.x, y.y};
   }
-  for (int i = tid; i < kValEntries * kValCopies; i += kFewThreads) {
-    const int e = i / kValCopies;
-    *reinterpret_cast<uint32_t*>(val_s + (e << kValLog) + kValOff + 4 * (i % kValCopies)) =
-        pk_f16(cen_s[e & ((1 << VB) - 1)] * up, cen_s[e >> VB] * up);
+  lds_barrier();
+  const float up = up_s[up_s[1][0] < up_s[0][0]][1];
+  for (int i = tid; i < kValEntries * kValCopies / 4; i += kFewThreads) {
+    const int e = i / (kValCopies / 4);
+    const uint32_t y = pk_f16(cen_s[e & ((1 << VB) - 1)] * up, cen_s[e >> VB] * up);
+    *reinterpret_cast<u32x4_t*>(val_s + (e << kValLog) + kValOff + 16 * (i % (kValCopies / 4))) = u32x4_t{y, y, y, y};
   }
   // a table read: the field of `bits` bits at bit `bit` of the word array w, as an
   // entry of 2^lg bytes and this lane's copy in it
@@ -403,17 +423,20 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
 
   // the 8 scores of row ln: tokens 4 lg + i, then 16 + 4 lg + i, of a block at
   // tok0; tokens from cnt on are none.  Returns the weights.
-  auto weights = [&](const f4_t (&S)[2], int tok0, int cnt, float (&w)[8]) {
-    float sc[8];
-    const bool whole = cnt == 32 && all_see(tok0, 32);
+  auto weights = [&](f4_t (&S)[2], int tok0, int cnt, bool whole, float (&w)[8]) {
+    S[0] *= c;
+    S[1] *= c;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int o = 16 * (i / 4) + 4 * lg + i % 4;
+        S[i / 4][i % 4] = (o < cnt) & sees(tok0 + o) ? S[i / 4][i % 4] : -INFINITY;
+      }
+      asm volatile("");  // (one branch for the eight)
+    }
     float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int o = 16 * (i / 4) + 4 * lg + i % 4;
-      sc[i] = S[i / 4][i % 4] * c;
-      if (!whole) sc[i] = o < cnt && sees(tok0 + o) ? sc[i] : -INFINITY;
-      mx = fmaxf(mx, sc[i]);
-    }
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, S[i / 4][i % 4]);
     if (__any(mx > m_run + kFewLazy)) {
       mx = colgroup_max(mx);
       const float m_new = fmaxf(m_run, mx);
@@ -426,16 +449,43 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
     const float at = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      w[i] = __builtin_amdgcn_exp2f(sc[i] - at);
+      w[i] = __builtin_amdgcn_exp2f(S[i / 4][i % 4] - at);
       l_run += w[i];
     }
   };
 
   if (has_codes) {
     for (int i = i0; i < i1; ++i) {
-      const int k = at_0.k, tok0 = at_0.g * G + 32 * k, cnt = min(32, G - 32 * k);
-      const int row_nn = row_of(at_2);
+      const int k = of(meta_k, i), tok0 = of(meta_g, i) * G + 32 * k, cnt = min(32, G - 32 * k);
+      if (i + 2 >= meta_i + 64 && i + 1 < i1) load_meta(i);
+      const Rows after = rows_of(i + 2);
       if (!PK && (i == i0 || k == 0 || i == cold.n0)) begin_group();  // (the second run may start inside a group)
+      // the block's side-list entries, 128 at a time: an entry's place in the sparse
+      // tile (none: behind it) and its value over the mean, as a pair: its first
+      // half there, then its second
+      struct Spot {
+        int o;
+        uint16_t half[2];
+      };
+      auto spot_of = [&](uint32_t y, bool real) {
+        const int tok = (int)((y & 0xFFFFu) / D) - 32 * k, ch = (int)(y & (D - 1));
+        const float v = h2f((uint16_t)(y >> 16)) - stat_s[wave][1][ch];
+        const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(v, 0.f));
+        return Spot{real & ((unsigned)tok < 32u) ? at(tok, ch / 8) + ch % 8 : 32 * D,
+                    {__builtin_bit_cast(uint16_t, hh.x), f2h(v - (float)hh.x)}};
+      };
+      Spot spot[2];
+      auto put = [&](int half) {  // (2: cleared)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) list_s[spot[s].o] = half == 2 ? 0 : spot[s].half[half];
+        wave_sync();
+      };
+      const bool lists = !PK && e_hi > e_lo;
+      if (lists) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) spot[s] = spot_of(ent[s], e_lo + lane + 64 * s < e_hi);
+        put(0);
+      }
       f4_t S[2];
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
@@ -454,59 +504,38 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
           S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.h, wh[mm], S[tile], 0, 0, 0);
         }
       }
-      if (!PK && e_hi > e_lo) {
-        // the block's side-list entries, tile by tile: an entry's place in the
-        // sparse tile and its value over the mean, as a pair
-        struct Spot {
-          int tile, o;
-          uint32_t hi, lo;
-        };
-        auto spot = [&](uint32_t y, bool real) {
-          const int tok = (int)((y & 0xFFFFu) / D) - 32 * k, ch = (int)(y & (D - 1));
-          const float v = h2f((uint16_t)(y >> 16)) - stat_s[wave][1][ch];
-          const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(v, 0.f));
-          return Spot{real && (unsigned)tok < 32u ? tok >> 4 : 2, at(tok & 15, ch / 8) + ch % 8,
-                      __builtin_bit_cast(uint16_t, hh.x), f2h(v - (float)hh.x)};
-        };
-        auto put = [&](const Spot& x, int tile, bool clear) {
-          if (x.tile == tile) {
-            hi_s[x.o] = clear ? 0 : (uint16_t)x.hi;
-            lo_s[x.o] = clear ? 0 : (uint16_t)x.lo;
-          }
-        };
-        const Spot e0 = spot(ent[0], e_lo + lane < e_hi), e1 = spot(ent[1], e_lo + 64 + lane < e_hi);
+      if (lists) {
+        for (int e = e_lo;;) {
 #pragma unroll
-        for (int tile = 0; tile < 2; ++tile) {
-          auto each = [&](bool clear) {
-            put(e0, tile, clear);
-            put(e1, tile, clear);
-            for (int e = e_lo + 128 + lane; e < e_hi; e += 64) put(spot(oent[ob * cap + e], true), tile, clear);
+          for (int half = 0; half < 2; ++half) {
+            if (half) put(1);
+#pragma unroll
+            for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+              for (int tile = 0; tile < 2; ++tile)
+                S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    *reinterpret_cast<const h8_t*>(list_s + at(16 * tile + ln, (CPL / 8) * lg + mm)), qf[mm], S[tile], 0, 0, 0);
             wave_sync();
-          };
-          each(false);
-#pragma unroll
-          for (int mm = 0; mm < NM; ++mm) {
-            const int o = at(ln, (CPL / 8) * lg + mm);
-            S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8_t*>(lo_s + o), qf[mm], S[tile], 0, 0, 0);
-            S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8_t*>(hi_s + o), qf[mm], S[tile], 0, 0, 0);
           }
-          wave_sync();
-          each(true);
+          put(2);
+          if ((e += 128) >= e_hi) break;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) spot[s] = spot_of(oent[ob * cap + min(e + lane + 64 * s, cap - 1)], e + lane + 64 * s < e_hi);
+          put(0);
         }
       }
       if constexpr (PK) {  // score = |k| (q_rot . centroids)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) S[e / 4][e % 4] *= __shfl(kn, 16 * (e / 4) + 4 * lg + e % 4, 64);
+        for (int e = 0; e < 8; ++e) S[e / 4][e % 4] *= norm_of(kn, e);
       }
-      const int next = min(i + 1, i1 - 1);
-      if (next >= meta_i + 64) load_meta(next);
-      load_keys(next, row_n);
+      load_keys(min(i + 1, i1 - 1), next_rows);
       float w[8];
-      weights(S, tok0, cnt, w);
+      const bool whole = cnt == 32 && all_see(tok0, 32);
+      weights(S, tok0, cnt, whole, w);
       h8_t pf;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float nv = __shfl(norm, 16 * (e / 4) + 4 * lg + e % 4, 64);
+        const float nv = norm_of(norm, e);
         pf[e] = (_Float16)(w[e] == 0.f ? 0.f : w[e] * nv);  // (no weight: whatever norm stands there)
       }
       // V^T P^T: row ln of the first operand is channel NC ln + j of the piece
@@ -544,33 +573,57 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
           }
         }
       }
-      load_values(row_n);
-      row_n = row_nn;
-      at_0 = at_1;
-      at_1 = at_2;
-      at_2 = after(at_2, i + 2);
+      load_values(next_rows);
+      next_rows = after;
     }
   } else if (!is_cold) {
     // uncoded blocks, straight from the ring
     const size_t ring = ((size_t)b * Hkv + h) * d.hot_ring;
     const uint16_t* const hk = static_cast<const uint16_t*>(a.p.hot_k);
     const uint16_t* const hv = static_cast<const uint16_t*>(a.p.hot_v);
-    for (int i = i0; i < i1; ++i) {
+    // a block's place in the ring: token tok0 + o, o < cnt (cnt is at most the
+    // ring's size)
+    auto place = [&](int at0, int o) { return ring + (at0 + o >= d.hot_ring ? at0 + o - d.hot_ring : at0 + o); };
+    // up to head_dim 128 the next block's rows are on their way meanwhile
+    constexpr bool kAhead = D <= 128;
+    h8_t kf[2][NM];
+    u32x4_t vn[NS][8];
+    auto load = [&](int i) {
       const int tok0 = n_cold + 32 * hot.at(i), cnt = min(32, n - tok0), at0 = tok0 % d.hot_ring;
-      // place of token tok0 + o, o < cnt (cnt is at most the ring's size)
-      auto place = [&](int o) { return ring + (at0 + o >= d.hot_ring ? at0 + o - d.hot_ring : at0 + o); };
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        const uint16_t* kr = hk + place(at0, min(16 * tile + ln, cnt - 1)) * D + CPL * lg;
+#pragma unroll
+        for (int mm = 0; mm < NM; ++mm) kf[tile][mm] = *reinterpret_cast<const h8_t*>(kr + 8 * mm);
+      }
+      // values: token e of this lane, channels NC ln .. + NC - 1 of the piece
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t* vr = hv + place(at0, min(16 * (e / 4) + 4 * lg + e % 4, cnt - 1)) * D + NC * ln;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          if constexpr (NC == 8) {
+            vn[s][e] = *reinterpret_cast<const u32x4_t*>(vr + 128 * s);
+          } else {
+            const u32x2_t y = *reinterpret_cast<const u32x2_t*>(vr);
+            vn[s][e] = u32x4_t{y.x, y.y, 0u, 0u};
+          }
+        }
+      }
+    };
+    if (kAhead && i0 < i1) load(i0);
+    for (int i = i0; i < i1; ++i) {
+      if constexpr (!kAhead) load(i);
+      const int tok0 = n_cold + 32 * hot.at(i), cnt = min(32, n - tok0), at0 = tok0 % d.hot_ring;
       f4_t S[2];
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
-        const uint16_t* kr = hk + place(min(16 * tile + ln, cnt - 1)) * D + CPL * lg;
         S[tile] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int mm = 0; mm < NM; ++mm)
-          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8_t*>(kr + 8 * mm), qf[mm], S[tile],
-                                                           0, 0, 0);
+          S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tile][mm], qf[mm], S[tile], 0, 0, 0);
       }
-      // values: token e of this lane, channels NC ln .. + NC - 1 of the piece;
-      // zero where no row sees the token, whatever stands there
+      // values of tokens that no row sees: zero, whatever stands there
       u32x4_t vv[NS][8];
       typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
       us2_t top = {0, 0};  // the largest exponent fields
@@ -578,23 +631,17 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       for (int e = 0; e < 8; ++e) {
         const int o = 16 * (e / 4) + 4 * lg + e % 4, tok = tok0 + o;
         const bool any = o < cnt && tok <= p_hi && (tok >= lo_first || tok < sinks);
-        const uint16_t* vr = hv + place(min(o, cnt - 1)) * D + NC * ln;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          if constexpr (NC == 8) {
-            vv[s][e] = *reinterpret_cast<const u32x4_t*>(vr + 128 * s);
-          } else {
-            const u32x2_t y = *reinterpret_cast<const u32x2_t*>(vr);
-            vv[s][e] = u32x4_t{y.x, y.y, 0u, 0u};
-          }
-          if (!any) vv[s][e] = u32x4_t{0u, 0u, 0u, 0u};
+          vv[s][e] = any ? vn[s][e] : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
           for (int f = 0; f < NC / 2; ++f)
             top = __builtin_elementwise_max(top, __builtin_bit_cast(us2_t, vv[s][e][f] & 0x7C007C00u));
         }
       }
+      if (kAhead && i + 1 < i1) load(i + 1);
       float w[8];
-      weights(S, tok0, cnt, w);
+      weights(S, tok0, cnt, cnt == 32 && all_see(tok0, 32), w);
       h8_t pf;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pf[e] = (_Float16)w[e];
@@ -629,7 +676,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
 #pragma unroll 1
         for (int o = 0; o < cnt; ++o) {
           const bool vis = sees(tok0 + o);
-          const uint16_t* vr = hv + place(o) * D;
+          const uint16_t* vr = hv + place(at0, o) * D;
 #pragma unroll
           for (int s = 0; s < NS; ++s)
 #pragma unroll
