@@ -425,19 +425,21 @@ int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const vo
  * - m + t and sees the tokens j of [0, p] with j > p - window or j < sinks.
  * Only the coded groups that a query sees are read.  Queries with p < 0 and
  * rows t >= m get zeros.
- *   q        [batch][n_q_heads][q_len][head_dim] by strides, fp16 (fp32 when input_f32)
+ *   q        [batch][n_q_heads][q_len][head_dim] by strides, fp16 (fp32 when input_f32),
+ *            16-byte aligned, as out
  *   seq_lens [batch] i32 (device), clamped to max_len
  *   q_lens   [batch] i32 (device) or null (q_len); clamped to [0, q_len]
  *   out      like q by strides, fp32 or fp16
  * The windowed form of tqk_decode, for one query (a decode step), a few (a
  * verification step) or a prompt's chunk.  Few queries are attended in code
- * space; more than 8 fp16 ones with an fp16 output over keys and values
- * reconstructed in the workspace (weights and keys rounded to fp16).
+ * space; more (over 128 rows: queries times query heads of a kv head) of an fp16
+ * cache with an fp16 output over keys and values reconstructed in the workspace
+ * (weights, keys and values rounded to fp16).
  */
 typedef struct tqk_attend_desc {
   int32_t batch;        /* at most n_pages of the cache */
   int32_t q_len;        /* query rows of every sequence */
-  int32_t max_len;      /* the longest sequence */
+  int32_t max_len;      /* the longest sequence; the tables reach that far */
   int32_t window;       /* tokens a query sees back from itself, itself included; 0: all */
   int32_t sinks;        /* first tokens that stay visible */
   int32_t out_type;     /* 0 fp32, 1 fp16 */

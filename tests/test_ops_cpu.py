@@ -139,3 +139,44 @@ def test_attention_abi_status_codes():
     assert rc(kv_len=1 << 20, window=0) == N.TQK_EWORKSPACE
     assert rc(kv_len=1 << 20, window=0, ws=at, n=need - 1) == N.TQK_EWORKSPACE
     assert lib.tqk_attention_workspace_bytes(ctypes.byref(desc(q_len=1 << 29))) == 0
+
+
+def test_attend_abi_status_codes():
+    N, lib = _lib()
+    buf = ctypes.create_string_buffer(512)
+    at = (ctypes.addressof(buf) + 15) & ~15
+    cache = dict(head_dim=128, key_bits=4, value_bits=4, n_kv_heads=2, n_q_heads=8, hot_window=512, group_tokens=256,
+                 page_tokens=64, hot_ring=512, max_groups_per_seq=6, max_pages_per_seq=24, n_pages=24, outlier_cap=64,
+                 outliers_per_channel=2, sm_scale=0.1)
+
+    def desc(**kw):
+        base = dict(batch=1, q_len=4, max_len=2000, window=300, sinks=1, out_type=1)
+        base.update(kw)
+        stride = base.pop("stride", 1024)
+        t = N.AttendDesc(**base)
+        t.q_stride[:] = t.o_stride[:] = [stride] * 3
+        return t
+
+    def rc(q=at, out=at, ws=at, n=0, c=(), **kw):
+        d = N.CacheDesc(**{**cache, **dict(c)})
+        return lib.tqk_attend(ctypes.byref(d), ctypes.byref(N.CachePtrs()), ctypes.byref(desc(**kw)), q, at, None, out,
+                              ws, n, None)
+
+    d = N.CacheDesc(**cache)
+    assert lib.tqk_attend(None, None, ctypes.byref(desc()), at, at, None, at, at, 0, None) == N.TQK_EINVAL
+    assert lib.tqk_attend(ctypes.byref(d), None, None, at, at, None, at, at, 0, None) == N.TQK_EINVAL
+    assert rc(c=dict(head_dim=96)) == N.TQK_EUNSUPPORTED
+    assert rc(c=dict(n_q_heads=32)) == N.TQK_EUNSUPPORTED  # 16 query heads a kv head
+    assert rc(out_type=2) == N.TQK_EUNSUPPORTED
+    for bad in (dict(batch=-1), dict(q_len=-1), dict(max_len=-1), dict(window=-1), dict(sinks=-1), dict(stride=4),
+                dict(q=at + 8), dict(out=at + 2), dict(q=None), dict(out=None), dict(q_len=1 << 29),
+                dict(batch=25), dict(max_len=1 << 16), dict(c=dict(max_pages_per_seq=20)), dict(c=dict(sm_scale=0.0)),
+                dict(c=dict(sm_scale=float("nan"))), dict(c=dict(key_grid=2, outliers_per_channel=0))):
+        assert rc(**bad) == N.TQK_EINVAL, bad
+    assert rc(batch=0, q=None) == N.TQK_OK and rc(q_len=0, q=None) == N.TQK_OK
+    for q_len in (4, 64):  # over the codes; over reconstructed keys and values
+        need = lib.tqk_attend_workspace_bytes(ctypes.byref(d), ctypes.byref(desc(q_len=q_len)))
+        assert need > 0
+        for ws, n in ((at, need - 1), (at + 8, need), (None, need)):
+            assert rc(q_len=q_len, ws=ws, n=n) == N.TQK_EWORKSPACE
+    assert lib.tqk_attend_workspace_bytes(ctypes.byref(d), ctypes.byref(desc(window=-1))) == 0

@@ -13,7 +13,13 @@
 namespace {
 
 constexpr int kMostItems = 4096;  // fp32 caches: queries a launch (bounds the partials and the grid)
-constexpr int kFewMost = 64;      // rows (queries times query heads of a kv head) attended on codes
+// Rows (queries times query heads of a kv head) attended on codes.  A workgroup of
+// that kernel takes 16 rows and reads the codes again for the next 16; dense keys
+// and values are made once, however few the queries.  8 sequences of 8192 tokens, 8
+// kv heads of 128, window 4096, codes and dense: 32 rows 38 and 105 us, 64 rows 52
+// and 108, 128 rows 100 and 117; one sequence of 16384: 128 rows 29 and 53; head_dim
+// 256, 4 sequences: 128 rows 121 and 148, 64: 256 rows 46 and 48.
+constexpr int kFewMost = 128;
 
 // Coded groups that one query sees at most, past `max_len` tokens of cache: the
 // first tokens', and the window's less what the hot window holds of it.  A cache
@@ -323,6 +329,12 @@ int check_attend(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   if (t->q_len > (1 << 28) || t->max_len > (1 << 30) || t->batch > counter_seqs(*d)) return TQK_EINVAL;
   if ((long long)t->batch * t->q_len > (1LL << 30)) return TQK_EINVAL;
   if (!(d->sm_scale > 0.f)) return TQK_EINVAL;
+  // (the tables reach as far as the longest sequence may)
+  const int groups = n_groups_of(t->max_len, d->hot_window, d->group_tokens);
+  if (groups > d->max_groups_per_seq || (long long)groups * (d->group_tokens / d->page_tokens) > d->max_pages_per_seq)
+    return TQK_EINVAL;
+  for (int i = 0; i < 3; ++i)
+    if (t->q_stride[i] % 8 || t->o_stride[i] % 8) return TQK_EINVAL;
   return TQK_OK;
 }
 
@@ -372,12 +384,14 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
   const int rc = check_attend(d, t);
   if (rc != TQK_OK) return rc;
   if (!t->batch || !t->q_len) return TQK_OK;
-  if (!p || !q || !seq_lens || !out) return TQK_EINVAL;
+  if (!p || !q || !seq_lens || !out || (((uintptr_t)q | (uintptr_t)out) & 15)) return TQK_EINVAL;
   if (d->key_grid == 2 && !p->knorm) return TQK_EINVAL;
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < tqk_attend_workspace_bytes(d, t))
-    return TQK_EWORKSPACE;
+  if (!workspace || ((uintptr_t)workspace & 15)) return TQK_EWORKSPACE;
+  const bool dense = dense_path(d, t);
+  if (!dense && !d->input_f32) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, workspace_bytes, stream);
+  if (workspace_bytes < tqk_attend_workspace_bytes(d, t)) return TQK_EWORKSPACE;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dense_path(d, t)) {
+  if (dense) {
     const tqk_attn_desc a = dense_desc(d, t);
     uint16_t* k = static_cast<uint16_t*>(workspace);
     uint16_t* v = k + (size_t)t->batch * a.k_stride[0];
@@ -409,7 +423,6 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
     }
     return tqk_run_attention(&a, q, k, v, seq_lens, q_lens, nullptr, out, ws, tqk_attention_workspace_bytes(&a), 1, stream);
   }
-  if (!d->input_f32) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, stream);
   const AttendPlan ap = attend_plan(d, t);
   const Plan& pl = ap.pl;
   const int gq = d->n_q_heads / d->n_kv_heads;

@@ -645,8 +645,9 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       h8_t pf;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pf[e] = (_Float16)w[e];
-      // (an infinity or a NaN that some queries see and others do not: set aside)
-      const bool apart = a.per_item > 1 && __any(top.x == 0x7C00 || top.y == 0x7C00) && !all_see(tok0, cnt);
+      // (infinities and NaN set aside: a row may not see them, and a weight that
+      // fp16 rounds to zero would make a NaN of an infinity)
+      const bool apart = __any(top.x == 0x7C00 || top.y == 0x7C00);
       if (__builtin_expect(apart, 0)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -871,17 +872,18 @@ FewPlan few_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
     if (w < tokens) tokens = w;
   }
   const long long blocks = (tokens + 31) / 32 + 1;
-  // Splits: rounds of the workgroups that fit (one a CU) times a wave's run of blocks and the set-up, joining and rotation of about
-  // three blocks' time; another launch to join them, about two.
-  const long long slots = device_cus();
+  // Splits: rounds of the workgroups that fit (one a CU) times a wave's run of
+  // blocks and the set-up, joining and rotation of about three blocks' time;
+  // another launch to join them, about two.
+  const uint32_t slots = (uint32_t)device_cus(), most = pairs < (1 << 20) ? 64 : 1;
   double best = 1e30;
-  for (int s = 1; s <= 64 && (s == 1 || (long long)kFewWaves * (s - 1) < blocks); ++s) {
-    const long long rounds = (pairs * s + slots - 1) / slots;
-    const long long run = (blocks + (long long)kFewWaves * s - 1) / ((long long)kFewWaves * s);
+  for (uint32_t s = 1; s <= most && (s == 1 || kFewWaves * (s - 1) < (uint64_t)blocks); ++s) {
+    const uint32_t rounds = most > 1 ? ((uint32_t)pairs * s + slots - 1) / slots : 1;
+    const uint32_t run = ((uint32_t)blocks + kFewWaves * s - 1) / (kFewWaves * s);
     const double cost = (double)rounds * (double)(run + 3) + (s > 1 ? 2.0 : 0.0);
     if (cost < best - 1e-9) {
       best = cost;
-      fp.n_splits = s;
+      fp.n_splits = (int)s;
     }
   }
   fp.groups = pairs * fp.n_splits;
@@ -928,9 +930,11 @@ void launch_few(const FewArgs& a, dim3 grid, hipStream_t st) {
 size_t tqk_few_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) { return few_plan(d, t).ws_bytes; }
 
 int tqk_run_few(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
-                const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace, void* stream) {
+                const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace, size_t workspace_bytes,
+                void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const FewPlan fp = few_plan(d, t);
+  if (workspace_bytes < fp.ws_bytes) return TQK_EWORKSPACE;
   if (fp.groups > (1LL << 22)) return TQK_EINVAL;  // (512 threads each: fewer than 2^32)
   FewArgs a{};
   a.d = *d;

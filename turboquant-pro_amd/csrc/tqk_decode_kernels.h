@@ -771,7 +771,8 @@ __global__ __launch_bounds__(kThreads) void tqk_decode_split_valu(SplitArgs<WIN>
     if (tid == i && i < gq) {
       const size_t o = ((size_t)b * Hq + h * gq + i) * ns + split;
       a.pm[o] = m_run[i];
-      a.pl[o] = l_run[i];
+      // (a NaN among the scores: the join passes over sums that are not above zero)
+      a.pl[o] = WIN && !(l_run[i] == l_run[i]) ? INFINITY : l_run[i];
     }
   }
 }

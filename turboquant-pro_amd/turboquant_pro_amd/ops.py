@@ -10,6 +10,7 @@ and ``TQKVPool.attend`` are their counterparts on a coded cache.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 from . import _native as N
@@ -21,6 +22,7 @@ def _torch():
     return torch
 
 
+@functools.lru_cache(None)
 def _types():
     torch = _torch()
     return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -54,12 +56,16 @@ class on_device:
 
 
 def stream_of(dev):
-    return ctypes.c_void_p(_torch().cuda.current_stream(dev).cuda_stream)
+    """The current stream of ``dev`` as the C ABI takes it (the handle alone: the
+    stream object of ``torch.cuda.current_stream`` costs a small call 2 us)."""
+    return _torch()._C._cuda_getCurrentRawStream(dev.index)
 
 
 def aligned(x):
     """``x`` with its last dimension contiguous, 16-byte rows and a 16-byte
     start: itself, or a copy."""
+    if x.is_contiguous() and x.shape[-1] % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x  # (the usual case, without a walk over the strides)
     el = x.element_size()
     if (x.stride(-1) == 1 or x.shape[-1] == 1) and x.data_ptr() % 16 == 0 and all(
             s % 8 == 0 and s * el % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
@@ -154,6 +160,12 @@ def window_args(window, sinks):
     return 0 if window is None or int(window) > top else int(window), min(int(sinks), top)
 
 
+def strides_of(x):
+    """Batch, head and token strides for the C ABI (of a size of one: 0)."""
+    (b, h, t, _), (sb, sh, st, _) = x.shape, x.stride()
+    return sb if b > 1 else 0, sh if h > 1 else 0, st if t > 1 else 0
+
+
 def lengths_arg(x, B, name):
     torch = _torch()
     if x is None:
@@ -213,8 +225,7 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
         return out
     d = N.AttnDesc(batch=B, n_q_heads=Hq, n_kv_heads=Hkv, head_dim=D, q_len=T, kv_len=L, window=window, sinks=sinks,
                    type=types[q.dtype], sm_scale=scale)
-    for dst, x in ((d.q_stride, q), (d.k_stride, k), (d.v_stride, v), (d.o_stride, out)):
-        dst[:] = [s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape[:3])]
+    d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = map(strides_of, (q, k, v, out))
     lib = N.lib()
     with on_device(dev):
         need = lib.tqk_attention_workspace_bytes(ctypes.byref(d))

@@ -27,7 +27,7 @@ from . import _native as N
 from .formats import (NF4_ZERO_CODE, codes_from_key_rows, key_rows_from_codes, nf4_codes,
                       pack_key_codes, pack_values, tile_value_rows, uniform_codes, unpack_key_codes,
                       unpack_values, untile_value_rows)
-from .ops import aligned, lengths_arg, norm_rope, on_device, stream_of, window_args
+from .ops import aligned, lengths_arg, norm_rope, on_device, stream_of, strides_of, window_args
 from .codebooks import (HEAD_DIMS, dc_channel_mask, dc_mask_words, group_tokens_for, n_groups_for,
                         outliers_per_channel, random_rotation, rope_averaged_bias, value_codebook)
 
@@ -454,10 +454,7 @@ class TQKVPool:
             out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device).transpose(1, 2)
         if B * T == 0:
             return out
-        t = N.AttendDesc(batch=B, q_len=T, max_len=max(self.lengths), window=window, sinks=sinks,
-                         out_type=0 if self.f32 else 1)
-        for dst, x in ((t.q_stride, q), (t.o_stride, out)):
-            dst[:] = [s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape[:3])]
+        t = N.AttendDesc(B, T, max(self.lengths), window, sinks, 0 if self.f32 else 1, strides_of(q), strides_of(out))
         lib = N.lib()
         with on_device(q.device):
             need = lib.tqk_attend_workspace_bytes(ctypes.byref(self.desc), ctypes.byref(t))
