@@ -180,3 +180,17 @@ def test_attend_abi_status_codes():
         for ws, n in ((at, need - 1), (at + 8, need), (None, need)):
             assert rc(q_len=q_len, ws=ws, n=n) == N.TQK_EWORKSPACE
     assert lib.tqk_attend_workspace_bytes(ctypes.byref(d), ctypes.byref(desc(window=-1))) == 0
+
+
+def test_gradients_are_refused():
+    x = torch.zeros(2, 3, 12 * 128, dtype=torch.float16, requires_grad=True)
+    q = torch.zeros(2, 8, 3, 128, dtype=torch.float16, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="backward"):
+        _call_rope(qkv=x)
+    with pytest.raises(NotImplementedError, match="backward"):
+        _call_window(q=q)
+    with torch.no_grad():  # no gradient asked: refused for the CPU tensors only
+        with pytest.raises(RuntimeError, match="GPU"):
+            _call_rope(qkv=x)
+        with pytest.raises(RuntimeError, match="GPU"):
+            _call_window(q=q)

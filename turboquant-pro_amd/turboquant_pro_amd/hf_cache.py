@@ -12,7 +12,10 @@ GPU (quantize-on-append in the encode kernel) and:
   is ``"tqk_gfx950"`` (``enable_turboquant_cache`` sets it) runs the fused
   decode-on-codes kernel: ``update`` hands the attention function the layer
   instead of dense K/V, and nothing is dequantized;
-* prefill, masked (padded) batches, and models on another attention
+* with a sliding window (the module's ``sliding_window`` and a mask that is
+  that window's) a decode step attends on the codes of the window's tokens
+  (``TQKVPool.attend``), and a prefill or chunk runs ``window_attention``;
+* other prefill, masked (padded) batches, and models on another attention
   implementation get dense K/V -- the cold groups dequantized by the GPU
   dequant kernel, bit-exact to the reference's decompress -- as in the
   reference.
@@ -32,6 +35,9 @@ does (hf_cache.py:247-299).
 from __future__ import annotations
 
 from functools import partial
+
+from .codebooks import HEAD_DIMS
+from .ops import needs_grad, window_attention
 
 try:
     import torch
@@ -154,6 +160,16 @@ class TurboQuantLayer(CacheLayerMixin):
         pool.desc.sm_scale = float(scaling)
         return pool.decode(query[:, :, 0].to(pool.dtype).contiguous())
 
+    def attend(self, query, scaling: float, window: int):
+        """The last query tokens ``(B, Hq, T, D)`` over the cache with a sliding
+        window: ``(B, Hq, T, D)`` in the pool's input type."""
+        pool = self.pool
+        if query.shape[1] != pool.n_q_heads:
+            raise ValueError(f"the layer's pool serves {pool.n_q_heads} query heads, "
+                             f"got {query.shape[1]} (pass the model config)")
+        pool.desc.sm_scale = float(scaling)
+        return pool.attend(query.to(pool.dtype), window=window)
+
     # ------------------------------------------------------------ contract
     def get_seq_length(self) -> int:
         return self.pool.lengths[0] if self.is_initialized else 0
@@ -229,20 +245,46 @@ def _mask_is_trivial(mask, kv_len: int) -> bool:
     return bool((m == 0).all())
 
 
+def _mask_is_window(mask, kv_len: int, window: int) -> bool:
+    """True when ``mask`` ``(B or 1, 1, T, kv_len)`` lets each of the last T
+    queries attend its own and the ``window - 1`` tokens before it, in every
+    sequence (a padded batch's does not)."""
+    if mask is None or mask.dim() != 4 or mask.shape[3] != kv_len or mask.shape[1] != 1:
+        return False
+    T = int(mask.shape[2])
+    seen = mask if mask.dtype == torch.bool else mask == 0
+    at = torch.arange(kv_len, device=mask.device)
+    p = torch.arange(kv_len - T, kv_len, device=mask.device)[:, None]
+    return bool((seen == ((at <= p) & (at > p - window))).all())
+
+
 def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.0,
                   scaling: float | None = None, **kwargs):
     """Attention function registered as ``"tqk_gfx950"``: a decode step on a
-    :class:`TurboQuantLayer` runs the fused kernel; anything else (prefill,
-    padded batches, dropout, dense K/V) runs PyTorch SDPA on dense K/V."""
+    :class:`TurboQuantLayer` runs the fused kernel; so does, with the module's
+    sliding window, one whose mask is that window's, and a prefill or chunk with
+    such a mask (fp16 or bf16 on the GPU) runs
+    :func:`~turboquant_pro_amd.ops.window_attention`.  Anything else (prefill
+    without a window, padded batches, dropout, soft-capped scores) runs PyTorch
+    SDPA on dense K/V."""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     layer = getattr(key, "_tq_layer", None)
+    window = kwargs.get("sliding_window")
+    windowed = (window and attention_mask is not None and dropout == 0.0 and query.is_cuda
+                and not needs_grad(query, key, value) and not any(kwargs.get(x) is not None for x in ("softcap", "s_aux", "position_bias")))
     if layer is not None:
         sc = float(scaling) if scaling is not None else layer.head_dim ** -0.5
         if (query.shape[2] == 1 and dropout == 0.0
                 and _mask_is_trivial(attention_mask, layer.get_seq_length())):
             out = layer.decode(query, sc)                       # (B, Hq, D) fp32
             return out.to(query.dtype)[:, None], None            # (B, 1, Hq, D)
+        if windowed and _mask_is_window(attention_mask, layer.get_seq_length(), window):
+            return layer.attend(query, sc, window).to(query.dtype).transpose(1, 2), None
         key, value = layer.dense()
+    elif (windowed and query.dtype in (torch.float16, torch.bfloat16) and query.dtype == key.dtype == value.dtype
+          and query.shape[3] in HEAD_DIMS and _mask_is_window(attention_mask, key.shape[2], window)):
+        out = window_attention(query, key, value, window=window, scale=scaling)
+        return out.transpose(1, 2), None                         # (B, T, Hq, D)
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
                                   scaling=scaling, **kwargs)
 

@@ -3,7 +3,7 @@ rotation (:func:`norm_rope`) and attention over dense keys and values with a
 sliding window and first tokens that stay visible (:func:`window_attention`).
 
 Both run hand-written gfx950 kernels behind ``include/tqk.h`` on the current
-stream of their tensors' device and have no CPU form.  ``TQKVPool.append_qkv``
+stream of their tensors' device; they have no CPU form and no backward pass.  ``TQKVPool.append_qkv``
 and ``TQKVPool.attend`` are their counterparts on a coded cache.
 """
 
@@ -37,6 +37,11 @@ def _on_gpu(what, *tensors):
         if t is not None and t.device != dev:
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
     return dev
+
+
+def needs_grad(*tensors):
+    """Whether a gradient is asked of any of the tensors (None: none)."""
+    return _torch().is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 class on_device:
@@ -124,6 +129,8 @@ def norm_rope(qkv, n_q_heads: int, n_kv_heads: int, inv_freq, positions, *, q_we
     ``TQKVPool.append`` and ``TQKVPool.attend`` take."""
     torch = _torch()
     B, T, D, dtype = _check_rope(qkv, n_q_heads, n_kv_heads, inv_freq, positions, q_weight, k_weight, dtype)
+    if needs_grad(qkv, q_weight, k_weight):
+        raise NotImplementedError("norm_rope has no backward pass: call it under torch.no_grad()")
     dev = _on_gpu("norm_rope", qkv, inv_freq, positions, q_weight, k_weight)
     types = _types()
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
@@ -215,6 +222,8 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
                                                               (kv_starts, "kv_starts")))
     if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype):
         raise ValueError(f"out is {tuple(q.shape)} {q.dtype}, not {tuple(out.shape)} {out.dtype}")
+    if needs_grad(q, k, v):
+        raise NotImplementedError("window_attention has no backward pass: call it under torch.no_grad()")
     dev = _on_gpu("window_attention", q, k, v, kv_lens, q_lens, kv_starts, out)
     q, k, v = aligned(q), aligned(k), aligned(v)
     if out is None:
