@@ -17,6 +17,7 @@
 // Bound: the matrix cores and, as closely, LDS reads (16 KiB of K and V for
 // 32 x 64 scores a wave).
 #include "tqk_attn.h"
+#include "tqk_wave.h"
 
 namespace {
 
@@ -444,22 +445,22 @@ __global__ __launch_bounds__(256) void tqk_attn_join(AttnArgs a) {
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= a.rows) return;
-  float M = -INFINITY;
-  for (int s = 0; s < a.n_splits; ++s) {
-    const long long at = s * a.rows + row;
-    if (a.part_ml[2 * at + 1] != 0.f) M = fmaxf(M, a.part_ml[2 * at]);
-  }
-  float l = 0.f, acc[E];
+  // every split's numbers by a lane of its own, then all accumulators in flight
+  const bool in = lane < a.n_splits;
+  const float2 ml = in ? *reinterpret_cast<const float2*>(&a.part_ml[2 * (lane * a.rows + row)]) : make_float2(0.f, 0.f);
+  const float m = ml.y != 0.f ? ml.x : -INFINITY, M = wave_reduce<true>(m);
+  const float f = ml.y != 0.f ? __builtin_amdgcn_exp2f(m - M) : 0.f;
+  const float l = wave_reduce<false>(ml.y * f);
+  const uint64_t live = __builtin_amdgcn_ballot_w64(ml.y != 0.f);
+  float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
   for (int s = 0; s < a.n_splits; ++s) {
-    const long long at = s * a.rows + row;
-    const float ls = a.part_ml[2 * at + 1];
-    if (ls == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - M);
-    l = fmaf(ls, f, l);
+    const float g = __shfl(f, s, 64);
+    const float* src = a.part_acc + (s * a.rows + row) * D + E * lane;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(a.part_acc[at * D + E * lane + e], f, acc[e]);
+    for (int e = 0; e < E; ++e) acc[e] = live >> s & 1 ? fmaf(src[e], g, acc[e]) : acc[e];
   }
   const int t = (int)(row % a.d.q_len);
   const long long bh = row / a.d.q_len;
