@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_attend import check, make_pool, queries  # noqa: E402
+from test_gpu_attend import cached, check, make_pool, queries  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +161,24 @@ def test_a_captured_step_between_other_calls():
         torch.cuda.synchronize()
         assert torch.equal(out, want), i
         out.zero_()
+
+
+@pytest.mark.parametrize("D,Hq,H,T", [(64, 8, 1, 50), (128, 8, 2, 100), (256, 4, 1, 90)])
+def test_chunks_keep_what_rounding_keys_leaves(D, Hq, H, T):
+    """A chunk's reconstructed keys are fp16 pairs: with keys of large scores the
+    result is as close as on the codes, 2^-10 together (the weights', values' and
+    output's roundings, each at most 2^-11 and rarely near it)."""
+    from test_gpu_attend import attention, visible
+    print(f"[attend] pairs D={D} T={T}", flush=True)
+    pool = make_pool(29, [2300, 1200], Hq, H, D, value_bits=4)
+    q = (3.0 * queries(29, pool, T)).half()
+    out = pool.attend(q, window=900, sinks=4)
+    check(pool, out, q, 900, 4, what="pairs")
+    off = tot = 0.0
+    for b in range(2):
+        k, v = cached(pool, b)
+        sees = visible(pool.lengths[b], T, T, 0, 900, 4, "cuda")
+        want = attention(q[b], k, v, sees, D ** -0.5)[0]
+        off += float((out[b].double() - want).square().sum())
+        tot += float(want.square().sum())
+    assert (off / tot) ** 0.5 <= 2.0 ** -10

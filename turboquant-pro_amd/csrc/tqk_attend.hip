@@ -37,12 +37,15 @@ int most_groups(const tqk_cache_desc* d, const tqk_attend_desc* t) {
 // ---- reconstruction of what a chunk's queries see ---------------------------
 // Rows [0, kept.sinks) and from the window on, moved down by kept.gap
 // (tqk_attn.h), 64 tokens of a kv head a step: keys as grid value with the
-// side-list's over it, values as (cent[code] @ Pi) * norm, hot tokens as they
-// are, all in fp16.  Pi in fp16 and the centroids times a power of two near
-// sqrt(D) in fp16 (2^-12 of a value each, as the result's own rounding), summed
-// in fp32 by the matrix cores: the rotation costs a wave 16 products a step where
-// the ordered sums of tqk_dequant_dense took 2 D VALU operations a value.
-// Bound: writing the rows (4 D bytes a token and kv head).
+// side-list's over it, an fp16 pair (a single fp16 moves a score of 60 by 0.01: the
+// result was three times as far off, and 30 us of 172 faster), values as
+// (cent[code] @ Pi) * norm and hot tokens as they are, in fp16.  PolarQuant keys are
+// rotated as the values and single.  Pi is an fp16 pair up to head_dim 128 (fp16 at
+// 256) and the centroids are scaled against their roundings, summed in fp32 by the
+// matrix cores: the rotation costs a wave 32 products a step where the ordered sums
+// of tqk_dequant_dense took 2 D VALU operations a value.
+// Bound: writing the rows (6 D bytes a token and kv head): 41 us for two windows of
+// 4096 and 8 kv heads of 128, of a chunk's 172.
 constexpr int kGather = 64;  // tokens a step
 static_assert(kGather == kMaxKeys, "a step lies on one side of the gap");
 
@@ -52,6 +55,7 @@ struct GatherArgs {
   const int32_t* seq_lens;
   const int32_t* q_lens;
   uint16_t* k;
+  uint16_t* k_lo;  // what the keys' rounding left (not for PolarQuant keys)
   uint16_t* v;
   int q_len, max_len, window, sinks;
   int rows;   // rows of a sequence and kv head
@@ -68,25 +72,44 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, ln = lane & 15, lg = lane >> 4;
   const int G = d.group_tokens, P = d.page_tokens, Hkv = d.n_kv_heads, kb = d.key_bits;
   const bool polar = d.key_grid == 2;
-  __shared__ __align__(16) uint16_t k_s[kGather][D];
+  __shared__ __align__(16) uint16_t k_s[kGather][D], kl_s[kGather][D];
   __shared__ __align__(16) uint16_t c_s[kGather * D];  // centroids, then rotated values
   __shared__ int row_s[kGather];   // row in the head's pages; -1: a hot token
   __shared__ int slot_s[kGather];
   __shared__ float norm_s[2][kGather];  // value norms, key norms (PolarQuant keys)
   __shared__ float lev_s[16], cen_s[16];
-  // centroids near 1: a power of two, exact
-  const float up = D == 64 ? 8.f : 16.f, down = 1.f / up;
   if (tid < 16) lev_s[tid] = key_level(d.key_grid == 1, tid);
+  // centroids near 1, at the scale of 64 over a power of two whose fp16 roundings
+  // lose least (the first of equals): 2^-12 of a centroid becomes about 2^-14
+  float up;
+  {
+    const float g = (D == 64 ? 8.f : 16.f) * (1.0f + (float)lane * (1.0f / 64));
+    float err = 0.f;
+#pragma unroll
+    for (int i = 0; i < (1 << VB); ++i) {
+      const float y = a.p.vcent[i] * g, r = y - (float)(_Float16)y;
+      err = fmaf(r, r, err);
+    }
+    err *= __builtin_amdgcn_rcpf(g * g);
+    const float best = -wave_reduce<true>(-err);
+    const uint64_t first = __builtin_amdgcn_ballot_w64(err == best);
+    up = (D == 64 ? 8.f : 16.f) * (1.0f + (float)(first ? __builtin_ctzll(first) : 0) * (1.0f / 64));
+  }
+  const float down = 1.f / up;
   if (tid < (1 << VB)) cen_s[tid] = a.p.vcent[tid] * up;
-  // Pi: columns e = 16 (NT wave + nt) + ln, rows 32 ks + 8 lg .. + 7 (a row of Pi^T)
-  h8_t pf[NT][NK];
+  // Pi, up to head_dim 128 as fp16 pairs (there are no registers for more): columns e = 16 (NT wave + nt) + ln, rows 32 ks + 8 lg .. + 7 (a row of Pi^T)
+  constexpr bool kPairs = D <= 128;
+  h8_t pf[NT][NK], pl[kPairs ? NT : 1][kPairs ? NK : 1];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) {
       const float* r = a.p.pi_t + (size_t)(16 * (NT * wave + nt) + ln) * D + 32 * ks + 8 * lg;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pf[nt][ks][e] = (_Float16)r[e];
+      for (int e = 0; e < 8; ++e) {
+        pf[nt][ks][e] = (_Float16)r[e];
+        if constexpr (kPairs) pl[nt][ks][e] = (_Float16)(r[e] - (float)pf[nt][ks][e]);
+      }
     }
   // place of a row's 16-byte piece: turned by the row, against bank conflicts
   auto at = [](int t, int c) { return (t * CH + (c ^ (t & 7))) * 8; };
@@ -117,6 +140,7 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
     }
     __syncthreads();
     uint16_t* const ko = a.k + ((size_t)bh * a.rows + r0) * D;
+    uint16_t* const klo = a.k_lo + ((size_t)bh * a.rows + r0) * D;
     uint16_t* const vo = a.v + ((size_t)bh * a.rows + r0) * D;
 
     // eight codes of a row from channel 8 c on, 4-bit keys' nibbles in order
@@ -154,8 +178,11 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
         for (int ks = 0; ks < NK; ++ks) {
           const h8_t x = *reinterpret_cast<const h8_t*>(c_s + at(16 * tt + ln, 4 * ks + lg));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)  // transposed: a lane gets four channels of one token
+          for (int nt = 0; nt < NT; ++nt) {  // transposed: a lane gets four channels of one token
+            if constexpr (kPairs)
+              acc[nt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[nt][ks], x, acc[nt][tt], 0, 0, 0);
             acc[nt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf[nt][ks], x, acc[nt][tt], 0, 0, 0);
+          }
         }
       }
       __syncthreads();
@@ -192,21 +219,27 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
         if (row_s[t] < 0) {
           *reinterpret_cast<uint4*>(&k_s[t][8 * c]) =
               *reinterpret_cast<const uint4*>(hot_k + (ring + (t0 + t) % d.hot_ring) * D + 8 * c);
+          *reinterpret_cast<uint4*>(&kl_s[t][8 * c]) = make_uint4(0u, 0u, 0u, 0u);
           continue;
         }
         const uint32_t w = codes8(a.p.kcodes + (head + row_s[t]) * k_row_bytes(kb, D), kb, c, true);
         const size_t mb = ((size_t)slot_s[t] * Hkv + h) * D + 8 * c;
-        h8_t x;
+        h8_t x, y;
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
           const float4 sc = *reinterpret_cast<const float4*>(a.p.gscale + mb + e);
           const float4 mu = *reinterpret_cast<const float4*>(a.p.gmean + mb + e);
           const float scv[4] = {sc.x, sc.y, sc.z, sc.w}, muv[4] = {mu.x, mu.y, mu.z, mu.w};
 #pragma unroll
-          for (int f = 0; f < 4; ++f)
-            x[e + f] = (_Float16)fmaf(scv[f], lev_s[(w >> (kb * (e + f))) & ((1u << kb) - 1u)], muv[f]);
+          for (int f = 0; f < 4; ++f) {
+            const float k = fmaf(scv[f], lev_s[(w >> (kb * (e + f))) & ((1u << kb) - 1u)], muv[f]);
+            x[e + f] = (_Float16)k;
+            const float left = k - (float)x[e + f];
+            y[e + f] = (_Float16)(fabsf(left) < INFINITY ? left : 0.f);
+          }
         }
         *reinterpret_cast<h8_t*>(&k_s[t][8 * c]) = x;
+        *reinterpret_cast<h8_t*>(&kl_s[t][8 * c]) = y;
       }
     }
     if (D == TQK_D && v_tiled(G, P, D, 0)) {
@@ -244,13 +277,18 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
           for (int e = lo + tid; e < hi; e += kThreads) {
             const uint32_t ent = a.p.oent[ob * d.outlier_cap + e], pos = ent & 0xFFFFu;
             const int t = g * G + (int)(pos / D);
-            if (t >= lo_t && t < hi_t) k_s[t - t0][pos % D] = (uint16_t)(ent >> 16);
+            if (t >= lo_t && t < hi_t) {
+              k_s[t - t0][pos % D] = (uint16_t)(ent >> 16);
+              kl_s[t - t0][pos % D] = 0;
+            }
           }
         }
         __syncthreads();
       }
-      for (int i = tid; i < nt_ * CH; i += kThreads)
+      for (int i = tid; i < nt_ * CH; i += kThreads) {
         reinterpret_cast<uint4*>(ko)[i] = reinterpret_cast<const uint4*>(&k_s[0][0])[i];
+        reinterpret_cast<uint4*>(klo)[i] = reinterpret_cast<const uint4*>(&kl_s[0][0])[i];
+      }
     }
     rotate_out(vo, norm_s[0], static_cast<const uint16_t*>(a.p.hot_v));
   }
@@ -372,7 +410,7 @@ size_t tqk_attend_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc
   if (!t->batch || !t->q_len) return 0;
   if (dense_path(d, t)) {
     const tqk_attn_desc a = dense_desc(d, t);
-    return 4 * (size_t)t->batch * a.k_stride[0] + ((tqk_attention_workspace_bytes(&a) + 255) & ~(size_t)255);
+    return 6 * (size_t)t->batch * a.k_stride[0] + ((tqk_attention_workspace_bytes(&a) + 255) & ~(size_t)255);
   }
   if (!d->input_f32) return tqk_few_workspace_bytes(d, t);
   return attend_plan(d, t).ws_bytes;
@@ -394,7 +432,8 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
   if (dense) {
     const tqk_attn_desc a = dense_desc(d, t);
     uint16_t* k = static_cast<uint16_t*>(workspace);
-    uint16_t* v = k + (size_t)t->batch * a.k_stride[0];
+    uint16_t* k_lo = k + (size_t)t->batch * a.k_stride[0];
+    uint16_t* v = k_lo + (size_t)t->batch * a.k_stride[0];
     uint16_t* ws = v + (size_t)t->batch * a.k_stride[0];
     if (t->max_len > 0) {
       GatherArgs g{};
@@ -403,6 +442,7 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
       g.seq_lens = seq_lens;
       g.q_lens = q_lens;
       g.k = k;
+      g.k_lo = k_lo;
       g.v = v;
       g.q_len = t->q_len;
       g.max_len = t->max_len;
@@ -421,7 +461,8 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
         launch_gather<256>(g, st);
       if (hipGetLastError() != hipSuccess) return TQK_EHIP;
     }
-    return tqk_run_attention(&a, q, k, v, seq_lens, q_lens, nullptr, out, ws, tqk_attention_workspace_bytes(&a), 1, stream);
+    return tqk_run_attention(&a, q, k, v, seq_lens, q_lens, nullptr, out, ws, tqk_attention_workspace_bytes(&a), 1,
+                             d->key_grid == 2 ? nullptr : k_lo, stream);
   }
   const AttendPlan ap = attend_plan(d, t);
   const Plan& pl = ap.pl;

@@ -23,7 +23,8 @@ struct KeptRows {
   __host__ __device__ int row(int pos) const { return pos - (pos >= sinks ? gap : 0); }
 };
 
-// tqk_attention; compact: keys and values hold the kept rows only.
+// tqk_attention; compact: keys and values hold the kept rows only.  k_lo, where
+// given (fp16): what the keys' rounding left, laid out as they are.
 int tqk_run_attention(const tqk_attn_desc* d, const void* q, const void* k, const void* v, const int32_t* kv_lens,
                       const int32_t* q_lens, const int32_t* kv_starts, void* out, void* workspace,
-                      size_t workspace_bytes, int compact, void* stream);
+                      size_t workspace_bytes, int compact, const void* k_lo, void* stream);

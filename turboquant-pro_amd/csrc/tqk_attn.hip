@@ -15,7 +15,10 @@
 // order of the keys inside a product is free: both operands take the order the
 // scores come in).  V^T comes from LDS by transposing reads.
 // Bound: the matrix cores and, as closely, LDS reads (16 KiB of K and V for
-// 32 x 64 scores a wave).
+// 32 x 64 scores a wave).  A prompt of 8192 tokens, 32 heads of 128, window 4096:
+// 460 us, 900 TFLOP/s (a large library product: 1200); head_dim 256, 16 heads,
+// 4096 tokens: 282 us, 490 TFLOP/s, at one wave a SIMD, which leaves the softmax
+// nothing to hide behind (two waves spill: 442 us).  Few rows: HBM and the join.
 #include "tqk_attn.h"
 #include "tqk_wave.h"
 
@@ -30,9 +33,12 @@ typedef short s8_t __attribute__((ext_vector_type(8)));
 constexpr int kTileThreads = 256;
 constexpr int kRows = 32;      // rows a wave
 constexpr int kTileRows = 128; // rows a workgroup
-// keys a tile: at head_dim 256 half as many, which leaves the accumulators their registers
-template <int D>
-constexpr int kTileKeys = D == 256 ? 32 : 64;
+// keys a tile: at head_dim 256 half as many, which leaves the accumulators their
+// registers; so at head_dim 128 with keys in pairs, which leaves LDS to two
+// workgroups (a chunk of 512 over a window of 4096, 4 sequences: 300 us, with 64
+// keys 407; at head_dim 64 178, with 64 keys 163)
+template <int D, bool PAIR = false>
+constexpr int kTileKeys = D == 256 || (D == 128 && PAIR) ? 32 : 64;
 // The running maximum follows the scores only when one exceeds it by this much
 // (log2 units): weights stay at most 2^8, far inside fp16's range, and the
 // accumulators are rescaled a few times a row instead of every tile.
@@ -43,6 +49,7 @@ struct AttnArgs {
   const void* q;
   const void* k;
   const void* v;
+  const void* k_lo;  // PAIR: what the keys' rounding left
   const int32_t* kv_lens;
   const int32_t* q_lens;
   const int32_t* kv_starts;
@@ -176,15 +183,16 @@ struct TileGeom {
   static __device__ __forceinline__ int v_at(int row, int c) { return (row * CH + (c ^ ((row & 3) << 1))) * 16; }
 };
 
-template <int D, typename T>
+// PAIR: keys as the sum of two fp16, a product each.
+template <int D, typename T, bool PAIR>
 __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles(AttnArgs a) {
   typedef typename Mma<T>::v8 v8;
-  constexpr int kKeys = kTileKeys<D>, NU = kKeys / 32;
+  constexpr int kKeys = kTileKeys<D, PAIR>, NU = kKeys / 32, NP = PAIR ? 2 : 1;
   constexpr int CH = D / 8, NST = kKeys * CH / kTileThreads;  // 16-byte chunks a thread stages of K, and of V
   constexpr int ND = D / 32, NK = D / 16;
   constexpr int kBytes = kKeys * D * 2;
   using TG = TileGeom<D>;
-  __shared__ __align__(16) uint8_t k0_s[kBytes], v0_s[kBytes], k1_s[kBytes], v1_s[kBytes];
+  __shared__ __align__(16) uint8_t k0_s[NP * kBytes], v0_s[kBytes], k1_s[NP * kBytes], v1_s[kBytes];
   __shared__ int odd_s;  // an infinity or a NaN among the values that only some rows see
 
   const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, ln = lane & 31, lh = lane >> 5;
@@ -242,6 +250,7 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
   // the last key: rows past it are not read.
   const long long ks_ = a.d.k_stride[2] * 2, vs_ = a.d.v_stride[2] * 2;
   const char* const kb = static_cast<const char*>(a.k) + 2 * (b * a.d.k_stride[0] + h * a.d.k_stride[1]);
+  const char* const lb = PAIR ? static_cast<const char*>(a.k_lo) + 2 * (b * a.d.k_stride[0] + h * a.d.k_stride[1]) : kb;
   const char* const vb = static_cast<const char*>(a.v) + 2 * (b * a.d.v_stride[0] + h * a.d.v_stride[1]);
   const KeptRows kept(s.n, s.m, s.start, s.sink_end, s.window);
   const int gap = a.compact ? uni(kept.gap) : 0, sink_rows = uni(kept.sinks);
@@ -256,12 +265,16 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
     const long long r0 = k0 - (k0 >= sink_rows ? gap : 0);
     const long long rows = min(kKeys, s.n - k0);
     const __amdgpu_buffer_rsrc_t rk = tile_rsrc(kb + r0 * ks_, (rows - 1) * ks_ + 2 * D);
+    const __amdgpu_buffer_rsrc_t rl = tile_rsrc(lb + r0 * ks_, (rows - 1) * ks_ + 2 * D);
     const __amdgpu_buffer_rsrc_t rv = tile_rsrc(vb + r0 * vs_, (rows - 1) * vs_ + 2 * D);
 #pragma unroll
     for (int i = 0; i < NST; ++i) {
       typedef __attribute__((address_space(3))) void* lds;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds)(kd + 1024 * wave + 16 * kTileThreads * i), 16, (int)k_off,
                                                (int)(i * (kTileThreads / CH) * ks_), 0, 0);
+      if constexpr (PAIR)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, (lds)(kd + kBytes + 1024 * wave + 16 * kTileThreads * i), 16,
+                                                 (int)k_off, (int)(i * (kTileThreads / CH) * ks_), 0, 0);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds)(vd + 1024 * wave + 16 * kTileThreads * i), 16, (int)v_off,
                                                (int)(i * (kTileThreads / CH) * vs_), 0, 0);
     }
@@ -291,14 +304,16 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
     f16v_t S[NU];
     // (the reads run a few products ahead: a read's latency is several products)
     constexpr int kAhead = 4;
-    v8 kf[NU * NK];
+    v8 kf[NU * NK * NP];
 #pragma unroll
-    for (int i = 0; i < NU * NK + kAhead; ++i) {
-      if (i < NU * NK)
-        kf[i] = *reinterpret_cast<const v8*>(k_t + TG::k_at(32 * (i / NK) + ln, 2 * (i % NK) + lh));
+    for (int i = 0; i < NU * NK * NP + kAhead; ++i) {
+      if (i < NU * NK * NP) {  // (the second halves first)
+        const int x = i / NP, half = NP - 1 - i % NP;
+        kf[i] = *reinterpret_cast<const v8*>(k_t + half * kBytes + TG::k_at(32 * (x / NK) + ln, 2 * (x % NK) + lh));
+      }
       if (i >= kAhead) {
-        const int u = (i - kAhead) / NK, ks = (i - kAhead) % NK;
-        if (ks == 0) S[u] = Mma<T>::m32(kf[i - kAhead], qf[ks], f16v_t{});
+        const int x = (i - kAhead) / NP, u = x / NK, ks = x % NK;
+        if (ks == 0 && (i - kAhead) % NP == 0) S[u] = Mma<T>::m32(kf[i - kAhead], qf[ks], f16v_t{});
         else S[u] = Mma<T>::m32(kf[i - kAhead], qf[ks], S[u]);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -537,7 +552,12 @@ int check_attn(const tqk_attn_desc* d) {
 
 template <int D, typename T>
 void launch_tiles(const AttnArgs& a, long long items, hipStream_t st) {
-  hipLaunchKernelGGL((tqk_attn_tiles<D, T>), dim3((unsigned)items), dim3(kTileThreads), 0, st, a);
+  if constexpr (__is_same(T, _Float16)) {
+    if (a.k_lo) hipLaunchKernelGGL((tqk_attn_tiles<D, T, true>), dim3((unsigned)items), dim3(kTileThreads), 0, st, a);
+    else hipLaunchKernelGGL((tqk_attn_tiles<D, T, false>), dim3((unsigned)items), dim3(kTileThreads), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((tqk_attn_tiles<D, T, false>), dim3((unsigned)items), dim3(kTileThreads), 0, st, a);
+  }
   if (a.n_splits > 1)
     hipLaunchKernelGGL((tqk_attn_join<D, T>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
 }
@@ -564,14 +584,14 @@ size_t tqk_attention_workspace_bytes(const tqk_attn_desc* d) {
 int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const void* v,
                   const int32_t* kv_lens, const int32_t* q_lens, const int32_t* kv_starts, void* out,
                   void* workspace, size_t workspace_bytes, void* stream) {
-  return tqk_run_attention(d, q, k, v, kv_lens, q_lens, kv_starts, out, workspace, workspace_bytes, 0, stream);
+  return tqk_run_attention(d, q, k, v, kv_lens, q_lens, kv_starts, out, workspace, workspace_bytes, 0, nullptr, stream);
 }
 
 }  // extern "C"
 
 int tqk_run_attention(const tqk_attn_desc* d, const void* q, const void* k, const void* v, const int32_t* kv_lens,
                       const int32_t* q_lens, const int32_t* kv_starts, void* out, void* workspace,
-                      size_t workspace_bytes, int compact, void* stream) {
+                      size_t workspace_bytes, int compact, const void* k_lo, void* stream) {
   const int rc = check_attn(d);
   if (rc != TQK_OK) return rc;
   if (!d->batch || !d->q_len) return TQK_OK;
@@ -585,6 +605,7 @@ int tqk_run_attention(const tqk_attn_desc* d, const void* q, const void* k, cons
   a.q = q;
   a.k = k;
   a.v = v;
+  a.k_lo = k_lo;
   a.kv_lens = kv_lens;
   a.q_lens = q_lens;
   a.kv_starts = kv_starts;
