@@ -157,10 +157,10 @@ def test_attend_abi_status_codes():
         t.q_stride[:] = t.o_stride[:] = [stride] * 3
         return t
 
-    def rc(q=at, out=at, ws=at, n=0, c=(), **kw):
+    def rc(q=at, out=at, ws=at, n=0, c=(), none=None, **kw):
         d = N.CacheDesc(**{**cache, **dict(c)})
-        return lib.tqk_attend(ctypes.byref(d), ctypes.byref(N.CachePtrs()), ctypes.byref(desc(**kw)), q, at, None, out,
-                              ws, n, None)
+        p = N.CachePtrs(**{name: at for name, _ in N.CachePtrs._fields_ if name != none})
+        return lib.tqk_attend(ctypes.byref(d), ctypes.byref(p), ctypes.byref(desc(**kw)), q, at, None, out, ws, n, None)
 
     d = N.CacheDesc(**cache)
     assert lib.tqk_attend(None, None, ctypes.byref(desc()), at, at, None, at, at, 0, None) == N.TQK_EINVAL
@@ -171,7 +171,9 @@ def test_attend_abi_status_codes():
     for bad in (dict(batch=-1), dict(q_len=-1), dict(max_len=-1), dict(window=-1), dict(sinks=-1), dict(stride=4),
                 dict(q=at + 8), dict(out=at + 2), dict(q=None), dict(out=None), dict(q_len=1 << 29),
                 dict(batch=25), dict(max_len=1 << 16), dict(c=dict(max_pages_per_seq=20)), dict(c=dict(sm_scale=0.0)),
-                dict(c=dict(sm_scale=float("nan"))), dict(c=dict(key_grid=2, outliers_per_channel=0))):
+                dict(c=dict(sm_scale=float("nan"))), dict(none="knorm", c=dict(key_grid=2, outliers_per_channel=0)),
+                *(dict(none=x) for x in ("kcodes", "gscale", "gmean", "ocount", "oent", "vcodes", "vnorm", "hot_k",
+                                         "hot_v", "block_table", "group_table", "vcent", "pi", "pi_t"))):
         assert rc(**bad) == N.TQK_EINVAL, bad
     assert rc(batch=0, q=None) == N.TQK_OK and rc(q_len=0, q=None) == N.TQK_OK
     for q_len in (4, 64):  # over the codes; over reconstructed keys and values

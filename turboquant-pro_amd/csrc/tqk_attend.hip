@@ -376,6 +376,13 @@ int check_attend(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   return TQK_OK;
 }
 
+// Every buffer that a cache of this form has.
+bool have_buffers(const tqk_cache_desc& d, const tqk_cache_ptrs& p) {
+  const bool keys = d.key_grid == 2 ? p.knorm != nullptr : p.gscale && p.gmean;
+  return keys && p.kcodes && p.vcodes && p.vnorm && p.ocount && (d.outliers_per_channel == 0 || p.oent) && p.hot_k &&
+         p.hot_v && p.block_table && p.group_table && p.vcent && p.pi && p.pi_t;
+}
+
 template <int GQ, int D>
 void launch_valu(const SplitArgs<true>& a, dim3 grid, hipStream_t st) {
   if (a.d.value_bits == 2)
@@ -422,8 +429,7 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
   const int rc = check_attend(d, t);
   if (rc != TQK_OK) return rc;
   if (!t->batch || !t->q_len) return TQK_OK;
-  if (!p || !q || !seq_lens || !out || (((uintptr_t)q | (uintptr_t)out) & 15)) return TQK_EINVAL;
-  if (d->key_grid == 2 && !p->knorm) return TQK_EINVAL;
+  if (!p || !q || !seq_lens || !out || (((uintptr_t)q | (uintptr_t)out) & 15) || !have_buffers(*d, *p)) return TQK_EINVAL;
   if (!workspace || ((uintptr_t)workspace & 15)) return TQK_EWORKSPACE;
   const bool dense = dense_path(d, t);
   if (!dense && !d->input_f32) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, workspace_bytes, stream);
