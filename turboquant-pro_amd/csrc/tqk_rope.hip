@@ -12,7 +12,9 @@
 // Bound: HBM, every element is read once and written once.  A wave takes one
 // token (or, with few tokens, a part of its heads): its lanes compute the
 // token's R/2 rotations once, one or two each, and hand them round through the
-// wave's own LDS; then 64 lanes take 512 channels at a time, 8 a lane.
+// wave's own LDS; then 64 lanes take 512 channels at a time, 8 a lane.  Four prompts
+// of 8192 tokens, 32 query and 8 kv heads of 128, bf16 to fp16: 157 us, 5.1 TB/s (a
+// large copy: 4.9); 16 single tokens: 4.2 us of a call's 15 on the host.
 #include "tqk_common.h"
 
 namespace {

@@ -41,7 +41,10 @@ def _on_gpu(what, *tensors):
 
 def needs_grad(*tensors):
     """Whether a gradient is asked of any of the tensors (None: none)."""
-    return _torch().is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return _torch().is_grad_enabled()
+    return False
 
 
 class on_device:
@@ -143,12 +146,10 @@ def norm_rope(qkv, n_q_heads: int, n_kv_heads: int, inv_freq, positions, *, q_we
     k = torch.empty((B, n_kv_heads, T, D), dtype=dtype, device=dev)
     v = torch.empty_like(k)
     if B * T:
-        d = N.RopeDesc(batch=B, tokens=T, n_q_heads=n_q_heads, n_kv_heads=n_kv_heads, head_dim=D,
-                       rotary_dim=2 * inv_freq.shape[0], interleaved=int(bool(interleaved)), in_type=types[qkv.dtype],
-                       out_type=types[dtype], weight_type=0 if w is None else types[w.dtype],
-                       pos_i64=int(positions.dtype == torch.int64), pos_per_token=int(positions.dim() == 2),
-                       batch_stride=qkv.stride(0) if B > 1 else 0, token_stride=qkv.stride(1) if T > 1 else 0,
-                       eps=eps, weight_offset=weight_offset, rope_scale=rope_scale)
+        d = N.RopeDesc(B, T, n_q_heads, n_kv_heads, D, 2 * inv_freq.shape[0], bool(interleaved), types[qkv.dtype],
+                       types[dtype], 0 if w is None else types[w.dtype], positions.dtype == torch.int64,
+                       positions.dim() == 2, qkv.stride(0) if B > 1 else 0, qkv.stride(1) if T > 1 else 0,
+                       eps, weight_offset, rope_scale)
         with on_device(dev):
             N.check(N.lib().tqk_norm_rope(ctypes.byref(d), qkv.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
                                           None if q_weight is None else q_weight.data_ptr(),
@@ -174,9 +175,9 @@ def strides_of(x):
 
 
 def lengths_arg(x, B, name):
-    torch = _torch()
     if x is None:
         return None
+    torch = _torch()
     if tuple(x.shape) != (B,) or x.dtype != torch.int32:
         raise ValueError(f"{name} is ({B},) int32, not {tuple(x.shape)} {x.dtype}")
     return x.contiguous()
@@ -204,8 +205,8 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"window_attention expects q (B, Hq, T, D) and k, v (B, Hkv, L, D), got {tuple(q.shape)}, "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
-    B, Hq, T, D = (int(x) for x in q.shape)
-    Hkv, L = int(k.shape[1]), int(k.shape[2])
+    B, Hq, T, D = q.shape
+    _, Hkv, L, _ = k.shape
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads are no multiple of {Hkv} kv heads")
     if D not in HEAD_DIMS:
@@ -218,8 +219,8 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not scale > 0.0 or not math.isfinite(scale):
         raise ValueError(f"scale is positive and finite, not {scale}")
-    kv_lens, q_lens, kv_starts = (lengths_arg(x, B, n) for x, n in ((kv_lens, "kv_lens"), (q_lens, "q_lens"),
-                                                              (kv_starts, "kv_starts")))
+    kv_lens, q_lens, kv_starts = (lengths_arg(kv_lens, B, "kv_lens"), lengths_arg(q_lens, B, "q_lens"),
+                                  lengths_arg(kv_starts, B, "kv_starts"))
     if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype):
         raise ValueError(f"out is {tuple(q.shape)} {q.dtype}, not {tuple(out.shape)} {out.dtype}")
     if needs_grad(q, k, v):
@@ -232,8 +233,7 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
         raise ValueError("out needs channels side by side, rows of whole 16 bytes and a 16-byte start")
     if B * T == 0:
         return out
-    d = N.AttnDesc(batch=B, n_q_heads=Hq, n_kv_heads=Hkv, head_dim=D, q_len=T, kv_len=L, window=window, sinks=sinks,
-                   type=types[q.dtype], sm_scale=scale)
+    d = N.AttnDesc(B, Hq, Hkv, D, T, L, window, sinks, types[q.dtype], scale)
     d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = map(strides_of, (q, k, v, out))
     lib = N.lib()
     with on_device(dev):

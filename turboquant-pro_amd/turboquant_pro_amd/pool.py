@@ -454,7 +454,8 @@ class TQKVPool:
             out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device).transpose(1, 2)
         if B * T == 0:
             return out
-        t = N.AttendDesc(B, T, max(self.lengths), window, sinks, 0 if self.f32 else 1, strides_of(q), strides_of(out))
+        t = N.AttendDesc(B, T, max(self.lengths), window, sinks, 0 if self.f32 else 1)
+        t.q_stride[:], t.o_stride[:] = strides_of(q), strides_of(out)
         lib = N.lib()
         with on_device(q.device):
             need = lib.tqk_attend_workspace_bytes(ctypes.byref(self.desc), ctypes.byref(t))
