@@ -270,13 +270,13 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
 #pragma unroll
     for (int i = 0; i < NST; ++i) {
       typedef __attribute__((address_space(3))) void* lds;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds)(kd + 1024 * wave + 16 * kTileThreads * i), 16, (int)k_off,
-                                               (int)(i * (kTileThreads / CH) * ks_), 0, 0);
-      if constexpr (PAIR)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, (lds)(kd + kBytes + 1024 * wave + 16 * kTileThreads * i), 16,
-                                                 (int)k_off, (int)(i * (kTileThreads / CH) * ks_), 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds)(vd + 1024 * wave + 16 * kTileThreads * i), 16, (int)v_off,
-                                               (int)(i * (kTileThreads / CH) * vs_), 0, 0);
+      // (the whole offset in the operand that is held against the resource's end: the
+      // scalar one is not, and a last tile of few rows ends before most steps)
+      const int step = i * (kTileThreads / CH), at = 16 * kTileThreads * i + 1024 * wave;
+      const int ko = (int)(k_off + (uint32_t)step * (uint32_t)ks_), vo = (int)(v_off + (uint32_t)step * (uint32_t)vs_);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds)(kd + at), 16, ko, 0, 0, 0);
+      if constexpr (PAIR) __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, (lds)(kd + kBytes + at), 16, ko, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds)(vd + at), 16, vo, 0, 0, 0);
     }
   };
   // The tile has arrived (every wave waits for its own loads).  Values that no
