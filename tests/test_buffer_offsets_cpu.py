@@ -40,3 +40,15 @@ def test_loads_into_lds_are_checked_whole(path):
 def test_the_tiles_load_that_way():
     text = open(os.path.join(CSRC, "tqk_attn.hip")).read()
     assert len(list(calls(text, "__builtin_amdgcn_raw_ptr_buffer_load_lds"))) == 3
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=os.path.basename)
+def test_loads_from_registers_steps_are_checked(path):
+    """A constant step of a register load, as through a side-list that ends inside
+    it, is no scalar offset either."""
+    with open(path) as f:
+        text = f.read()
+    for bits in ("b32", "b64", "b96", "b128"):
+        for args in calls(text, "__builtin_amdgcn_raw_buffer_load_" + bits):
+            assert len(args) == 4, args
+            assert args[2] == "0" or not args[2].isdigit(), f"{os.path.basename(path)}: scalar offset {args[2]}"

@@ -1577,8 +1577,8 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(DecodeArgs
                                                  real ? 4u * (uint32_t)cap : 0u);
       const int off = 4 * (lo + lane * E);
       const u32x4_t x0 = __builtin_amdgcn_raw_buffer_load_b128(ro, off, 0, 0);
-      const u32x4_t x1 = __builtin_amdgcn_raw_buffer_load_b128(ro, off, 16, 0);
-      const u32x4_t x2 = __builtin_amdgcn_raw_buffer_load_b128(ro, off, 32, 0);
+      const u32x4_t x1 = __builtin_amdgcn_raw_buffer_load_b128(ro, off + 16, 0, 0);
+      const u32x4_t x2 = __builtin_amdgcn_raw_buffer_load_b128(ro, off + 32, 0, 0);
       gent[0] = x0.x; gent[1] = x0.y; gent[2] = x0.z; gent[3] = x0.w;
       gent[4] = x1.x; gent[5] = x1.y; gent[6] = x1.z; gent[7] = x1.w;
       gent[8] = x2.x; gent[9] = x2.y; gent[10] = x2.z; gent[11] = x2.w;
