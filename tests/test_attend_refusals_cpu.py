@@ -1,0 +1,34 @@
+"""What tqk_attend and TQKVPool.attend refuse before any GPU work (no GPU needed)."""
+
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_ops_cpu import _lib  # noqa: E402
+
+CACHE = dict(head_dim=128, key_bits=4, value_bits=4, n_kv_heads=2, n_q_heads=8, hot_window=512, group_tokens=256,
+             page_tokens=64, hot_ring=512, max_groups_per_seq=6, max_pages_per_seq=24, n_pages=24, outlier_cap=64,
+             outliers_per_channel=2, sm_scale=0.1)
+
+
+def attend_desc(N, **kw):
+    t = N.AttendDesc(**{**dict(batch=1, q_len=4, max_len=2000, window=300, sinks=1, out_type=1), **kw})
+    t.q_stride[:] = t.o_stride[:] = [1024] * 3
+    return t
+
+
+@pytest.mark.parametrize("q_len", [1, 64])
+def test_a_side_list_without_room_is_refused(q_len):
+    """Outliers but a capacity of none: a load of an entry would have no place to go."""
+    N, lib = _lib()
+    buf = ctypes.create_string_buffer(512)
+    at = (ctypes.addressof(buf) + 15) & ~15
+    p = N.CachePtrs(**{name: at for name, _ in N.CachePtrs._fields_})
+    for cap, outliers, want in ((0, 2, N.TQK_EINVAL), (0, 0, N.TQK_EWORKSPACE), (1, 2, N.TQK_EWORKSPACE)):
+        d = N.CacheDesc(**{**CACHE, "outlier_cap": cap, "outliers_per_channel": outliers})
+        t = attend_desc(N, q_len=q_len)
+        assert lib.tqk_attend(ctypes.byref(d), ctypes.byref(p), ctypes.byref(t), at, at, None, at, at, 0, None) == want
+        need = lib.tqk_attend_workspace_bytes(ctypes.byref(d), ctypes.byref(t))
+        assert (need == 0) == (want == N.TQK_EINVAL)
