@@ -32,3 +32,18 @@ def test_a_side_list_without_room_is_refused(q_len):
         assert lib.tqk_attend(ctypes.byref(d), ctypes.byref(p), ctypes.byref(t), at, at, None, at, at, 0, None) == want
         need = lib.tqk_attend_workspace_bytes(ctypes.byref(d), ctypes.byref(t))
         assert (need == 0) == (want == N.TQK_EINVAL)
+
+
+@pytest.mark.parametrize("batch,heads,D,max_len,window", [(16, 8, 128, 131072, 0), (16, 8, 128, 131072, 131000),
+                                                          (1, 8, 256, 1 << 19, 0), (1, 2, 128, 1 << 21, 0),
+                                                          (64, 8, 64, 32768, 20000), (5, 8, 128, 70000, 0)])
+@pytest.mark.parametrize("q_len", [33, 129, 512])
+def test_a_chunk_s_workspace_is_bounded(batch, heads, D, max_len, window, q_len):
+    """Keys and values reconstructed at a time stay within a GiB (and the splits of the
+    attention over them within 512 workgroups' rows and numbers), whatever the batch."""
+    N, lib = _lib()
+    d = N.CacheDesc(**{**CACHE, "head_dim": D, "n_kv_heads": heads, "n_q_heads": 4 * heads, "max_groups_per_seq": 1 << 14,
+                       "max_pages_per_seq": 1 << 16, "n_pages": 1 << 22})
+    need = lib.tqk_attend_workspace_bytes(ctypes.byref(d), ctypes.byref(attend_desc(
+        N, batch=batch, q_len=q_len, max_len=max_len, window=window)))
+    assert 0 < need <= (1 << 30) + 512 * 128 * (D + 2) * 4 + 512

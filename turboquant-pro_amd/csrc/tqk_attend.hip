@@ -20,6 +20,12 @@ constexpr int kMostItems = 4096;  // fp32 caches: queries a launch (bounds the p
 // and 108, 128 rows 100 and 117; one sequence of 16384: 128 rows 29 and 53; head_dim
 // 256, 4 sequences: 128 rows 121 and 148, 64: 256 rows 46 and 48.
 constexpr int kFewMost = 128;
+// Bytes of keys and values reconstructed at a time: sequences, or kv heads of one,
+// go one slice after another through the same workspace.  A slice of this size alone
+// fills the chip (1 GiB is 170 us of writes), and a workspace of every sequence would
+// be six times the codes' own size.  Where one kv head of one sequence needs more
+// (1.4 million tokens at head_dim 128), the codes are attended, however many rows.
+constexpr size_t kMostDense = (size_t)1 << 30;
 
 // Coded groups that one query sees at most, past `max_len` tokens of cache: the
 // first tokens', and the window's less what the hot window holds of it.  A cache
@@ -60,7 +66,8 @@ struct GatherArgs {
   int q_len, max_len, window, sinks;
   int rows;   // rows of a sequence and kv head
   int steps;  // of kGather rows
-  int units;  // batch * n_kv_heads * steps
+  int units;  // seqs * heads * steps
+  int b0, h0, heads;  // the slice's first sequence and kv head, and its kv heads
 };
 
 template <int VB, int D>
@@ -115,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
   auto at = [](int t, int c) { return (t * CH + (c ^ (t & 7))) * 8; };
 
   for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-    const int step = unit % a.steps, bh = unit / a.steps, h = bh % Hkv, b = bh / Hkv;
+    const int step = unit % a.steps, bh = unit / a.steps, h = a.h0 + bh % a.heads, b = a.b0 + bh / a.heads;
     const int n = min(a.seq_lens[b], a.max_len);
     const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
     const KeptRows kept(n, m, 0, min(a.sinks, n), a.window);
@@ -322,11 +329,6 @@ AttendPlan attend_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   return ap;
 }
 
-// Whether the queries go over reconstructed keys and values.
-bool dense_path(const tqk_cache_desc* d, const tqk_attend_desc* t) {
-  return !d->input_f32 && t->out_type == 1 && (long long)t->q_len * (d->n_q_heads / d->n_kv_heads) > kFewMost;
-}
-
 // Rows that a sequence's queries see at most, in whole tiles.
 int kept_rows(const tqk_attend_desc* t) {
   const long long tile = kMaxKeys, all = ((long long)t->max_len + tile - 1) / tile * tile;
@@ -336,11 +338,37 @@ int kept_rows(const tqk_attend_desc* t) {
   return (int)(rows < all ? rows : all);
 }
 
-tqk_attn_desc dense_desc(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+// Bytes of the reconstructed keys (pairs) and values of a sequence and kv head.
+size_t dense_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) { return (size_t)6 * kept_rows(t) * d->head_dim; }
+
+// Whether the queries go over reconstructed keys and values.
+bool dense_path(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+  return !d->input_f32 && t->out_type == 1 && (long long)t->q_len * (d->n_q_heads / d->n_kv_heads) > kFewMost &&
+         dense_bytes(d, t) <= kMostDense;
+}
+
+// Sequences and kv heads reconstructed at a time: as many sequences as fit, or of
+// one sequence as many kv heads, in slices of about one size.
+struct Slice {
+  int seqs, heads;
+  Slice(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+    auto even = [](int n, size_t most) {
+      if (most >= (size_t)n) return n;
+      const int count = (n + (int)most - 1) / (int)most;
+      return (n + count - 1) / count;
+    };
+    const size_t one = dense_bytes(d, t), fit = one ? kMostDense / one : (size_t)INT32_MAX;
+    heads = even(d->n_kv_heads, fit);
+    seqs = heads < d->n_kv_heads ? 1 : even(t->batch, fit / d->n_kv_heads);
+  }
+};
+
+// Attention over the reconstruction of some sequences' kv heads.
+tqk_attn_desc dense_desc(const tqk_cache_desc* d, const tqk_attend_desc* t, int seqs, int heads) {
   tqk_attn_desc a{};
-  a.batch = t->batch;
-  a.n_q_heads = d->n_q_heads;
-  a.n_kv_heads = d->n_kv_heads;
+  a.batch = seqs;
+  a.n_q_heads = heads * (d->n_q_heads / d->n_kv_heads);
+  a.n_kv_heads = heads;
   a.head_dim = d->head_dim;
   a.q_len = t->q_len;
   a.kv_len = t->max_len;
@@ -353,10 +381,22 @@ tqk_attn_desc dense_desc(const tqk_cache_desc* d, const tqk_attend_desc* t) {
     a.o_stride[i] = t->o_stride[i];
   }
   const int64_t row = d->head_dim, head = row * kept_rows(t);
-  a.k_stride[0] = a.v_stride[0] = head * d->n_kv_heads;
+  a.k_stride[0] = a.v_stride[0] = head * heads;
   a.k_stride[1] = a.v_stride[1] = head;
   a.k_stride[2] = a.v_stride[2] = row;
   return a;
+}
+
+// Workspace of the attention over a slice, the last ones (which are smaller) too.
+size_t slice_attention_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const Slice& sl) {
+  size_t most = 0;
+  for (int seqs : {sl.seqs, t->batch % sl.seqs})
+    for (int heads : {sl.heads, d->n_kv_heads % sl.heads}) {
+      const tqk_attn_desc a = dense_desc(d, t, seqs, heads);
+      const size_t need = seqs && heads ? tqk_attention_workspace_bytes(&a) : 0;
+      if (need > most) most = need;
+    }
+  return most;
 }
 
 int check_attend(const tqk_cache_desc* d, const tqk_attend_desc* t) {
@@ -418,8 +458,8 @@ size_t tqk_attend_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc
   if (check_attend(d, t) != TQK_OK) return 0;
   if (!t->batch || !t->q_len) return 0;
   if (dense_path(d, t)) {
-    const tqk_attn_desc a = dense_desc(d, t);
-    return 6 * (size_t)t->batch * a.k_stride[0] + ((tqk_attention_workspace_bytes(&a) + 255) & ~(size_t)255);
+    const Slice sl(d, t);
+    return (size_t)sl.seqs * sl.heads * dense_bytes(d, t) + ((slice_attention_bytes(d, t, sl) + 255) & ~(size_t)255);
   }
   if (!d->input_f32) return tqk_few_workspace_bytes(d, t);
   return attend_plan(d, t).ws_bytes;
@@ -438,39 +478,47 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
   if (workspace_bytes < tqk_attend_workspace_bytes(d, t)) return TQK_EWORKSPACE;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dense) {
-    const tqk_attn_desc a = dense_desc(d, t);
-    uint16_t* k = static_cast<uint16_t*>(workspace);
-    uint16_t* k_lo = k + (size_t)t->batch * a.k_stride[0];
-    uint16_t* v = k_lo + (size_t)t->batch * a.k_stride[0];
-    uint16_t* ws = v + (size_t)t->batch * a.k_stride[0];
-    if (t->max_len > 0) {
-      GatherArgs g{};
-      g.d = *d;
-      g.p = *p;
-      g.seq_lens = seq_lens;
-      g.q_lens = q_lens;
-      g.k = k;
-      g.k_lo = k_lo;
-      g.v = v;
-      g.q_len = t->q_len;
-      g.max_len = t->max_len;
-      g.window = t->window;
-      g.sinks = t->sinks;
-      g.rows = kept_rows(t);
-      g.steps = g.rows / kGather;
-      const long long units = (long long)t->batch * d->n_kv_heads * g.steps;
-      if (units > INT32_MAX) return TQK_EINVAL;
-      g.units = (int)units;
-      if (d->head_dim == 64)
-        launch_gather<64>(g, st);
-      else if (d->head_dim == 128)
-        launch_gather<128>(g, st);
-      else
-        launch_gather<256>(g, st);
-      if (hipGetLastError() != hipSuccess) return TQK_EHIP;
-    }
-    return tqk_run_attention(&a, q, k, v, seq_lens, q_lens, nullptr, out, ws, tqk_attention_workspace_bytes(&a), 1,
-                             d->key_grid == 2 ? nullptr : k_lo, stream);
+    const Slice sl(d, t);
+    const int gq = d->n_q_heads / d->n_kv_heads;
+    const size_t attn_bytes = slice_attention_bytes(d, t, sl);
+    GatherArgs g{};
+    g.d = *d;
+    g.p = *p;
+    g.seq_lens = seq_lens;
+    g.q_lens = q_lens;
+    g.k = static_cast<uint16_t*>(workspace);
+    g.q_len = t->q_len;
+    g.max_len = t->max_len;
+    g.window = t->window;
+    g.sinks = t->sinks;
+    g.rows = kept_rows(t);
+    g.steps = g.rows / kGather;
+    for (g.b0 = 0; g.b0 < t->batch; g.b0 += sl.seqs)
+      for (g.h0 = 0; g.h0 < d->n_kv_heads; g.h0 += sl.heads) {
+        const int seqs = t->batch - g.b0 < sl.seqs ? t->batch - g.b0 : sl.seqs;
+        g.heads = d->n_kv_heads - g.h0 < sl.heads ? d->n_kv_heads - g.h0 : sl.heads;
+        const tqk_attn_desc a = dense_desc(d, t, seqs, g.heads);
+        const size_t rows = (size_t)seqs * a.k_stride[0];
+        g.k_lo = g.k + rows;
+        g.v = g.k_lo + rows;
+        if (t->max_len > 0) {
+          g.units = seqs * g.heads * g.steps;
+          if (d->head_dim == 64)
+            launch_gather<64>(g, st);
+          else if (d->head_dim == 128)
+            launch_gather<128>(g, st);
+          else
+            launch_gather<256>(g, st);
+          if (hipGetLastError() != hipSuccess) return TQK_EHIP;
+        }
+        const long long at_q = g.b0 * t->q_stride[0] + (long long)g.h0 * gq * t->q_stride[1];
+        const long long at_o = g.b0 * t->o_stride[0] + (long long)g.h0 * gq * t->o_stride[1];
+        const int arc = tqk_run_attention(&a, static_cast<const uint16_t*>(q) + at_q, g.k, g.v, seq_lens + g.b0,
+                                          q_lens ? q_lens + g.b0 : nullptr, nullptr, static_cast<uint16_t*>(out) + at_o,
+                                          g.v + rows, attn_bytes, 1, d->key_grid == 2 ? nullptr : g.k_lo, stream);
+        if (arc != TQK_OK) return arc;
+      }
+    return TQK_OK;
   }
   const AttendPlan ap = attend_plan(d, t);
   const Plan& pl = ap.pl;
