@@ -9,7 +9,8 @@
 // A coded block: a pair of key codes is an entry of a table of levels as fp16 pairs
 // (hi + lo: 2^-22; scaled single ones were 1 us of 33 faster, and the result's error
 // a third larger), four of them an operand of K Q^T as they are; the group's scale
-// goes into the query, a pair too, its mean into the scores' start.  A side-list
+// goes into the query, a pair too (over a power of two where a product passes fp16),
+// its mean into the scores afterwards.  A side-list
 // entry, whose code is the zero level, adds q (val - mean): the block's entries
 // stand in an otherwise zero LDS tile of the wave, the first halves of their fp16
 // pairs, then the second ones, each a second operand of the same product, and are
@@ -149,8 +150,23 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
 #pragma unroll
   for (int mm = 0; mm < NM; ++mm) qf[mm] = *reinterpret_cast<const h8_t*>(qp + CPL * lg + 8 * mm);
   // the coded keys' weights, an fp16 pair: q * scale group by group, or for
-  // rotated keys q @ Pi^T
+  // rotated keys q @ Pi^T; over a power of two, w_up, where they pass fp16
   h8_t wh[NM], wl[NM];
+  float w_up = 1.f;
+  // the wave's largest |q| (what is not finite: as the largest of fp16; its rows
+  // are lost whatever the power)
+  float q_top = 0.f;
+  if constexpr (!PK) {
+    typedef uint16_t us8_t __attribute__((ext_vector_type(8)));
+    us8_t top = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(us8_t, qf[mm]) & (uint16_t)0x7FFF);
+    uint16_t one = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one = top[e] > one ? top[e] : one;
+    q_top = wave_reduce<true>(h2f(one < 0x7C00 ? one : (uint16_t)0x7BFF));
+  }
 
   // ---- the coded blocks of this wave: state and loads
   uint16_t* const list_s = stage_s[wave];
@@ -254,9 +270,22 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       for (int s = 0; s < 2; ++s) ent[s] = oent[ob * cap + min(e_lo + lane + 64 * s, cap - 1)];
     }
   };
-  // a group's weights and the start of its scores (q . mean)
+  // a group's weights and the rest of its scores (q . mean)
   float bias = 0.f;
   auto begin_group = [&]() {
+    // q * scale within fp16: a scale of keys near 65504 times a large query is not
+    float s_top = 0.f;
+#pragma unroll
+    for (int e = 0; e < SPL; ++e) s_top = fmaxf(s_top, fabsf(nsc[e]));
+    w_up = 1.f;
+    if (__builtin_expect(__any(s_top * q_top > 65504.f), 0)) {
+      s_top = wave_reduce<true>(s_top);
+      // (s_top q_top < 2^e; an infinite scale's group is lost whatever the power)
+      const int e = min(__builtin_amdgcn_frexp_expf(s_top) + __builtin_amdgcn_frexp_expf(q_top), 126);
+      w_up = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ldexpf(1.f, e - 15))));
+#pragma unroll
+      for (int i = 0; i < SPL; ++i) nsc[i] *= ldexpf(1.f, 15 - e);
+    }
 #pragma unroll
     for (int e = 0; e < SPL; ++e) {
       stat_s[wave][0][SPL * lane + e] = nsc[e];
@@ -280,7 +309,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
         }
 #pragma unroll
         for (int k = 0; k < 4; k += 2) {
-          // (towards zero: two in one instruction, and no infinity up to 2 * 65504)
+          // (towards zero: two in one instruction)
           const h2_t hh = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x[k], x[k + 1]));
           const h2_t ll = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hh.x, -1.f, x[k]),
                                                                               fmaf((float)hh.y, -1.f, x[k + 1])));
@@ -489,7 +518,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       f4_t S[2];
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
-        S[tile] = f4_t{bias, bias, bias, bias};
+        S[tile] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int mm = 0; mm < NM; ++mm) {
           union { h8_t h; uint32_t u[4]; } hi, lo16;
@@ -502,6 +531,10 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
           S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16.h, wh[mm], S[tile], 0, 0, 0);
           S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.h, wl[mm], S[tile], 0, 0, 0);
           S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.h, wh[mm], S[tile], 0, 0, 0);
+        }
+        if constexpr (!PK) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[tile][e] = fmaf(S[tile][e], w_up, bias);
         }
       }
       if (lists) {
