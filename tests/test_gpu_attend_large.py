@@ -94,3 +94,21 @@ def test_queries_times_group_scales_past_fp16(D, Hq, H, form, T):
         pool.desc.sm_scale = scale
         for window, sinks in ((None, 0), (700, 5)):
             check(pool, pool.attend(q, window=window, sinks=sinks), q, window, sinks, scale, what=f"{scale} {window}")
+
+
+@pytest.mark.parametrize("D,bits", [(64, 4), (128, 3), (256, 2), (256, 4)])
+@pytest.mark.parametrize("T", [1, None])
+def test_rotated_queries_past_fp16(D, bits, T):
+    """PolarQuant keys: a query that one row of the rotation gathers to 10^6."""
+    T = 65 if T is None else T
+    print(f"[attend] large rotated queries D={D} T={T}", flush=True)
+    k, v = (2.0 * randn(5, 1, 2, 900, D)).half(), randn(6, 1, 2, 900, D).half()
+    pool = pool_of(k, v, 4, key_grid="polar", key_bits=bits, value_bits=bits, hot_window=128)
+    q = (3000.0 * queries(7, pool, T)).half()
+    q[:, 1] = (60000.0 * torch.sign(pool.pi_t[:, 3])).half()
+    q[:, 2] = (60000.0 * torch.sign(pool.pi_t[:, D - 1])).half()
+    assert float((q[0, 1].float() @ pool.pi_t).abs().max()) > 131008
+    scale = 2.0 ** -18
+    pool.desc.sm_scale = scale
+    for window, sinks in ((None, 0), (300, 5)):
+        check(pool, pool.attend(q, window=window, sinks=sinks), q, window, sinks, scale, what=f"{window}")

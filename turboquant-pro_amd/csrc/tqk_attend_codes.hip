@@ -433,11 +433,25 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       r_s[i] = y;
     }
     __syncthreads();
+    // (the rotation may gather a row's channels in one, sqrt(D) times as large: over a
+    // power of two then, of every row here, so that every wave has the same)
+    float y_top = 0.f;
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y_top = fmaxf(y_top, fabsf(r_s[ln * D + CPL * lg + 8 * mm + e]));
+    y_top = fminf(wave_reduce<true>(y_top), 16.f * 65504.f);  // (more: not of finite queries)
+    float down = 1.f;
+    if (y_top > 65504.f) {
+      const int e = __builtin_amdgcn_frexp_expf(y_top);  // y_top < 2^e
+      down = ldexpf(1.f, 15 - e);
+      w_up = ldexpf(1.f, e - 15);
+    }
 #pragma unroll
     for (int mm = 0; mm < NM; ++mm)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = r_s[ln * D + CPL * lg + 8 * mm + e];
+        const float y = r_s[ln * D + CPL * lg + 8 * mm + e] * down;
         wh[mm][e] = (_Float16)y;
         wl[mm][e] = (_Float16)(y - (float)wh[mm][e]);
       }
@@ -559,7 +573,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
       }
       if constexpr (PK) {  // score = |k| (q_rot . centroids)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) S[e / 4][e % 4] *= norm_of(kn, e);
+        for (int e = 0; e < 8; ++e) S[e / 4][e % 4] *= norm_of(kn, e) * w_up;
       }
       load_keys(min(i + 1, i1 - 1), next_rows);
       float w[8];
