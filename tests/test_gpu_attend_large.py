@@ -112,3 +112,26 @@ def test_rotated_queries_past_fp16(D, bits, T):
     pool.desc.sm_scale = scale
     for window, sinks in ((None, 0), (300, 5)):
         check(pool, pool.attend(q, window=window, sinks=sinks), q, window, sinks, scale, what=f"{window}")
+
+
+@pytest.mark.parametrize("D,Hq,H,form", [(64, 4, 2, dict()), (128, 4, 2, dict(outlier_frac=0.0)), (256, 2, 1, dict())])
+@pytest.mark.parametrize("T", [1, None])
+def test_keys_reconstructed_past_fp16(D, Hq, H, form, T):
+    """Keys near 65504 whose code stands for more (an NF4 level above them, or a rotated
+    centroid; a uniform grid ends at the group's largest key): the formula's result, of
+    few queries and of a chunk."""
+    T = 128 * H // Hq + 1 if T is None else T
+    print(f"[attend] large keys D={D} T={T} {form}", flush=True)
+    L = 1100
+    u = torch.rand((1, H, L, D), generator=torch.Generator(device="cuda").manual_seed(8), device="cuda")
+    share = torch.linspace(0.3, 0.95, D, device="cuda")
+    up = torch.rand((1, H, L, D), generator=torch.Generator(device="cuda").manual_seed(9), device="cuda") < share
+    k = torch.where(up, 52000 + 13504 * u, -62000 + 14000 * u).half()
+    assert bool(torch.isfinite(k).all())
+    pool = pool_of(k, randn(10, 1, H, L, D).half(), Hq, hot_window=128, **form)
+    assert float(cached(pool, 0)[0].abs().max()) > 65520
+    q = queries(11, pool, T)
+    scale = 2.0 ** -18
+    pool.desc.sm_scale = scale
+    for window, sinks in ((None, 0), (300, 5)):
+        check(pool, pool.attend(q, window=window, sinks=sinks), q, window, sinks, scale, what=f"{window}")

@@ -240,9 +240,10 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
             const float k = fmaf(scv[f], lev_s[(w >> (kb * (e + f))) & ((1u << kb) - 1u)], muv[f]);
-            x[e + f] = (_Float16)k;
-            const float left = k - (float)x[e + f];
-            y[e + f] = (_Float16)(fabsf(left) < INFINITY ? left : 0.f);
+            // (a code near 65504 may stand for more: the rest goes into the second half,
+            // and so does an infinity or a NaN)
+            x[e + f] = (_Float16)fminf(fmaxf(k, -65504.f), 65504.f);
+            y[e + f] = (_Float16)(k - (float)x[e + f]);
           }
         }
         *reinterpret_cast<h8_t*>(&k_s[t][8 * c]) = x;
