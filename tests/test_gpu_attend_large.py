@@ -114,7 +114,10 @@ def test_rotated_queries_past_fp16(D, bits, T):
         check(pool, pool.attend(q, window=window, sinks=sinks), q, window, sinks, scale, what=f"{window}")
 
 
-@pytest.mark.parametrize("D,Hq,H,form", [(64, 4, 2, dict()), (128, 4, 2, dict(outlier_frac=0.0)), (256, 2, 1, dict())])
+@pytest.mark.parametrize("D,Hq,H,form", [(64, 4, 2, dict()), (128, 4, 2, dict(outlier_frac=0.0)), (256, 2, 1, dict()),
+                                         (128, 4, 2, dict(key_grid="polar", key_bits=3, value_bits=3)),
+                                         (64, 4, 2, dict(key_grid="polar", key_bits=2, value_bits=2)),
+                                         (256, 4, 2, dict(key_grid="polar", key_bits=4, value_bits=4))])
 @pytest.mark.parametrize("T", [1, None])
 def test_keys_reconstructed_past_fp16(D, Hq, H, form, T):
     """Keys near 65504 whose code stands for more (an NF4 level above them, or a rotated

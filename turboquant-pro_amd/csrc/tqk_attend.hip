@@ -46,7 +46,7 @@ int most_groups(const tqk_cache_desc* d, const tqk_attend_desc* t) {
 // side-list's over it, an fp16 pair (a single fp16 moves a score of 60 by 0.01: the
 // result was three times as far off, and 30 us of 172 faster), values as
 // (cent[code] @ Pi) * norm and hot tokens as they are, in fp16.  PolarQuant keys are
-// rotated as the values and single.  Pi is an fp16 pair up to head_dim 128 (fp16 at
+// rotated as the values, and pairs.  Pi is an fp16 pair up to head_dim 128 (fp16 at
 // 256) and the centroids are scaled against their roundings, summed in fp32 by the
 // matrix cores: the rotation costs a wave 32 products a step where the ordered sums
 // of tqk_dequant_dense took 2 D VALU operations a value.
@@ -61,7 +61,7 @@ struct GatherArgs {
   const int32_t* seq_lens;
   const int32_t* q_lens;
   uint16_t* k;
-  uint16_t* k_lo;  // what the keys' rounding left (not for PolarQuant keys)
+  uint16_t* k_lo;  // what the keys' rounding left
   uint16_t* v;
   int q_len, max_len, window, sinks;
   int rows;   // rows of a sequence and kv head
@@ -173,8 +173,11 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
         *reinterpret_cast<h8_t*>(c_s + at(t, c)) = x;
       }
     };
-    // c_s @ Pi times the norms, back into c_s, then out (hot rows from the ring)
-    auto rotate_out = [&](uint16_t* out, const float* norm, const uint16_t* hot) {
+    // c_s @ Pi times the norms, back into c_s, then out (hot rows from the ring);
+    // keys as pairs, the second halves by way of kl_s
+    uint16_t* const cl_s = &kl_s[0][0];
+    auto rotate_out = [&](auto pair, uint16_t* out, uint16_t* out_lo, const float* norm, const uint16_t* hot) {
+      constexpr bool kPair = decltype(pair)::value;
       __syncthreads();
       f4_t acc[NT][4];
 #pragma unroll
@@ -199,11 +202,16 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-          h4_t y;
+          h4_t y, z;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = (_Float16)(acc[nt][tt][e] * f);
+          for (int e = 0; e < 4; ++e) {
+            const float x = acc[nt][tt][e] * f;
+            y[e] = (_Float16)(kPair ? fminf(fmaxf(x, -65504.f), 65504.f) : x);
+            z[e] = (_Float16)(x - (float)y[e]);
+          }
           const int ch = 16 * (NT * wave + nt) + 4 * lg;
           *reinterpret_cast<h4_t*>(c_s + at(16 * tt + ln, ch / 8) + ch % 8) = y;
+          if constexpr (kPair) *reinterpret_cast<h4_t*>(cl_s + at(16 * tt + ln, ch / 8) + ch % 8) = z;
         }
       }
       __syncthreads();
@@ -212,13 +220,16 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
         const uint4* src = row_s[t] < 0 ? reinterpret_cast<const uint4*>(hot + (ring + (t0 + t) % d.hot_ring) * D + 8 * c)
                                         : reinterpret_cast<const uint4*>(c_s + at(t, c));
         *reinterpret_cast<uint4*>(out + (size_t)t * D + 8 * c) = *src;
+        if constexpr (kPair)
+          *reinterpret_cast<uint4*>(out_lo + (size_t)t * D + 8 * c) =
+              row_s[t] < 0 ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4*>(cl_s + at(t, c));
       }
     };
 
     const uint16_t* const hot_k = static_cast<const uint16_t*>(a.p.hot_k);
     if (polar) {
       put_centroids(a.p.kcodes, VB, k_row_bytes(VB, D), true);
-      rotate_out(ko, norm_s[1], hot_k);
+      rotate_out(std::true_type{}, ko, klo, norm_s[1], hot_k);
       __syncthreads();
     } else {
       for (int i = tid; i < nt_ * CH; i += kThreads) {
@@ -298,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void tqk_gather_seen(GatherArgs a) {
         reinterpret_cast<uint4*>(klo)[i] = reinterpret_cast<const uint4*>(&kl_s[0][0])[i];
       }
     }
-    rotate_out(vo, norm_s[0], static_cast<const uint16_t*>(a.p.hot_v));
+    rotate_out(std::false_type{}, vo, nullptr, norm_s[0], static_cast<const uint16_t*>(a.p.hot_v));
   }
 }
 
@@ -516,7 +527,7 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
         const long long at_o = g.b0 * t->o_stride[0] + (long long)g.h0 * gq * t->o_stride[1];
         const int arc = tqk_run_attention(&a, static_cast<const uint16_t*>(q) + at_q, g.k, g.v, seq_lens + g.b0,
                                           q_lens ? q_lens + g.b0 : nullptr, nullptr, static_cast<uint16_t*>(out) + at_o,
-                                          g.v + rows, attn_bytes, 1, d->key_grid == 2 ? nullptr : g.k_lo, stream);
+                                          g.v + rows, attn_bytes, 1, g.k_lo, stream);
         if (arc != TQK_OK) return arc;
       }
     return TQK_OK;
