@@ -1,0 +1,50 @@
+"""Calls of the operators around the cache that would be answered without what was
+asked for: gradients, forward-mode tangents (no GPU needed)."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_ops_cpu import _call_rope, _call_window  # noqa: E402
+
+
+def pool_without_a_gpu():
+    """A pool's numbers alone: what attend checks before any GPU work."""
+    from turboquant_pro_amd import TQKVPool
+    pool = object.__new__(TQKVPool)
+    pool.max_batch, pool.n_q_heads, pool.n_kv_heads, pool.head_dim = 2, 8, 2, 128
+    pool.dtype, pool.input_dtype, pool.f32 = torch.float16, "float16", False
+    pool.kcodes = torch.empty(1, dtype=torch.uint8, device="meta")
+    return pool
+
+
+def query(T=3):
+    return torch.zeros(2, 8, T, 128, dtype=torch.float16)
+
+
+def test_attend_refuses_gradients():
+    pool = pool_without_a_gpu()
+    with pytest.raises(NotImplementedError, match="backward"):
+        pool.attend(query().requires_grad_())
+    with pytest.raises(NotImplementedError, match="backward"):
+        pool.attend(query(), out=query().requires_grad_())
+    with torch.no_grad(), pytest.raises(ValueError, match="is on cpu"):  # no gradient asked: refused for its place
+        pool.attend(query().requires_grad_())
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    rows = torch.zeros(2, 3, 12 * 128, dtype=torch.float16)
+    kv = torch.zeros(2, 2, 9, 128, dtype=torch.float16)
+    with fwd.dual_level():
+        for call in (lambda: _call_rope(qkv=fwd.make_dual(rows, rows)),
+                     lambda: _call_rope(q_weight=fwd.make_dual(torch.ones(128), torch.ones(128))),
+                     lambda: _call_window(q=fwd.make_dual(query(), query())),
+                     lambda: _call_window(v=fwd.make_dual(kv, kv)),
+                     lambda: pool_without_a_gpu().attend(fwd.make_dual(query(), query()))):
+            with pytest.raises(NotImplementedError, match="backward"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="backward"):
+                call()
+        with pytest.raises(RuntimeError, match="GPU"):  # none carried: refused for the CPU tensors only
+            _call_window()

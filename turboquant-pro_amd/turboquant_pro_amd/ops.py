@@ -40,10 +40,15 @@ def _on_gpu(what, *tensors):
 
 
 def needs_grad(*tensors):
-    """Whether a gradient is asked of any of the tensors (None: none)."""
+    """Whether a gradient or a forward-mode tangent is asked of any of the tensors
+    (None: none)."""
+    torch = _torch()
+    fwd = torch.autograd.forward_ad
+    dual = getattr(fwd, "_current_level", 0) >= 0  # (inside a dual level: rare, and dear to ask every tensor)
     for t in tensors:
-        if t is not None and t.requires_grad:
-            return _torch().is_grad_enabled()
+        if t is not None and ((t.requires_grad and torch.is_grad_enabled())
+                              or (dual and fwd.unpack_dual(t).tangent is not None)):
+            return True
     return False
 
 
@@ -223,7 +228,7 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
                                   lengths_arg(kv_starts, B, "kv_starts"))
     if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype):
         raise ValueError(f"out is {tuple(q.shape)} {q.dtype}, not {tuple(out.shape)} {out.dtype}")
-    if needs_grad(q, k, v):
+    if needs_grad(q, k, v, out):
         raise NotImplementedError("window_attention has no backward pass: call it under torch.no_grad()")
     dev = _on_gpu("window_attention", q, k, v, kv_lens, q_lens, kv_starts, out)
     q, k, v = aligned(q), aligned(k), aligned(v)

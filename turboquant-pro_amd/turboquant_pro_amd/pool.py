@@ -27,7 +27,7 @@ from . import _native as N
 from .formats import (NF4_ZERO_CODE, codes_from_key_rows, key_rows_from_codes, nf4_codes,
                       pack_key_codes, pack_values, tile_value_rows, uniform_codes, unpack_key_codes,
                       unpack_values, untile_value_rows)
-from .ops import aligned, lengths_arg, norm_rope, on_device, stream_of, strides_of, window_args
+from .ops import aligned, lengths_arg, needs_grad, norm_rope, on_device, stream_of, strides_of, window_args
 from .codebooks import (HEAD_DIMS, dc_channel_mask, dc_mask_words, group_tokens_for, n_groups_for,
                         outliers_per_channel, random_rotation, rope_averaged_bias, value_codebook)
 
@@ -440,6 +440,8 @@ class TQKVPool:
             raise ValueError(f"attend expects {self.input_dtype} q of shape ({B}, {Hq}, T, {D}), got {q.dtype} "
                              f"{tuple(q.shape)}")
         T = int(q.shape[2])
+        if needs_grad(q, out):
+            raise NotImplementedError("attend has no backward pass: call it under torch.no_grad()")
         window, sinks = window_args(window, sinks)
         q_lens = lengths_arg(q_lens, B, "q_lens")
         if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or aligned(out) is not out):
