@@ -1,5 +1,5 @@
 """Calls of the operators around the cache that would be answered without what was
-asked for: gradients, forward-mode tangents (no GPU needed)."""
+asked for: gradients, forward-mode tangents, outputs that share places (no GPU needed)."""
 
 import pytest
 
@@ -48,3 +48,32 @@ def test_tangents_are_refused():
                 call()
         with pytest.raises(RuntimeError, match="GPU"):  # none carried: refused for the CPU tensors only
             _call_window()
+
+
+def outputs():
+    """Outputs that write one place twice, then ones that do not."""
+    e = lambda *s: torch.empty(s, dtype=torch.float16)  # noqa: E731
+    bad = [e(1, 8, 3, 128).expand(2, -1, -1, -1), e(2, 1, 3, 128).expand(-1, 8, -1, -1), e(2, 8, 1, 128).expand(-1, -1, 3, -1),
+           e(8 * 3 * 2 * 128).as_strided((2, 8, 3, 128), (8 * 2 * 128, 2 * 128, 64, 1)),
+           e(4 * 8 * 3 * 128).as_strided((2, 8, 3, 128), (1024, 384, 128, 1))]
+    good = [e(2, 8, 3, 128), e(2, 3, 8, 128).transpose(1, 2), e(3, 2, 8, 136)[..., :128].permute(1, 2, 0, 3),
+            e(2, 12, 5, 128)[:, 2:10, 1:4]]
+    return bad, good
+
+
+def test_outputs_that_overlap_themselves():
+    bad, good = outputs()
+    for out in bad:
+        with pytest.raises(ValueError, match="share memory"):
+            _call_window(out=out)
+        with pytest.raises(ValueError, match="share memory"):
+            pool_without_a_gpu().attend(query(), out=out)
+    for out in good:
+        with pytest.raises(RuntimeError, match="GPU"):
+            _call_window(out=out)
+        with pytest.raises(ValueError, match="is on cpu"):
+            pool_without_a_gpu().attend(query(), out=out)
+    one = torch.empty((1, 8, 1, 128), dtype=torch.float16)  # dimensions of one: any stride
+    with pytest.raises(RuntimeError, match="GPU"):
+        _call_window(q=query()[:1, :, :1], k=torch.zeros(1, 2, 9, 128, dtype=torch.float16),
+                     v=torch.zeros(1, 2, 9, 128, dtype=torch.float16), out=one.as_strided((1, 8, 1, 128), (0, 128, 0, 1)))

@@ -74,16 +74,36 @@ def stream_of(dev):
     return _torch()._C._cuda_getCurrentRawStream(dev.index)
 
 
+def _is_aligned(x):
+    if x.is_contiguous() and x.shape[-1] % 8 == 0 and x.data_ptr() % 16 == 0:
+        return True  # (the usual case, without a walk over the strides)
+    el = x.element_size()
+    return (x.stride(-1) == 1 or x.shape[-1] == 1) and x.data_ptr() % 16 == 0 and all(
+        s % 8 == 0 and s * el % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1)
+
+
 def aligned(x):
     """``x`` with its last dimension contiguous, 16-byte rows and a 16-byte
     start: itself, or a copy."""
-    if x.is_contiguous() and x.shape[-1] % 8 == 0 and x.data_ptr() % 16 == 0:
-        return x  # (the usual case, without a walk over the strides)
-    el = x.element_size()
-    if (x.stride(-1) == 1 or x.shape[-1] == 1) and x.data_ptr() % 16 == 0 and all(
-            s % 8 == 0 and s * el % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
+    if _is_aligned(x):
         return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
+
+
+def check_out(out, like):
+    """A given output: of the queries' shape and type, channels side by side,
+    rows of whole 16 bytes and a 16-byte start, no two rows in one place."""
+    if tuple(out.shape) != tuple(like.shape) or out.dtype != like.dtype:
+        raise ValueError(f"out is {tuple(like.shape)} {like.dtype}, not {tuple(out.shape)} {out.dtype}")
+    if not _is_aligned(out):
+        raise ValueError("out needs channels side by side, rows of whole 16 bytes and a 16-byte start")
+    if out.is_contiguous():
+        return
+    extent = out.shape[-1]
+    for s, n in sorted((s, n) for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1):
+        if s < extent:  # (a dimension lies inside the next one's step)
+            raise ValueError(f"out: rows share memory (strides {tuple(out.stride())})")
+        extent += s * (n - 1)
 
 
 def _check_rope(qkv, n_q_heads, n_kv_heads, inv_freq, positions, q_weight, k_weight, dtype):
@@ -202,7 +222,8 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
     ``j < start + sinks``.  Lengths are int32 ``(B,)`` tensors on the device.
 
     Returns ``(B, Hq, T, D)`` in the inputs' type, ``out`` where given (any
-    strides of whole 16 bytes), else laid out ``(B, T, Hq, D)`` as the output
+    strides of whole 16 bytes that keep its rows apart; it shares no memory
+    with ``k`` and ``v``), else laid out ``(B, T, Hq, D)`` as the output
     projection reads it.  A query that sees nothing and rows ``t >= m`` get
     zeros.  ``scale``: ``1/sqrt(D)`` by default, positive."""
     torch = _torch()
@@ -226,16 +247,14 @@ def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0, scal
         raise ValueError(f"scale is positive and finite, not {scale}")
     kv_lens, q_lens, kv_starts = (lengths_arg(kv_lens, B, "kv_lens"), lengths_arg(q_lens, B, "q_lens"),
                                   lengths_arg(kv_starts, B, "kv_starts"))
-    if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype):
-        raise ValueError(f"out is {tuple(q.shape)} {q.dtype}, not {tuple(out.shape)} {out.dtype}")
+    if out is not None:
+        check_out(out, q)
     if needs_grad(q, k, v, out):
         raise NotImplementedError("window_attention has no backward pass: call it under torch.no_grad()")
     dev = _on_gpu("window_attention", q, k, v, kv_lens, q_lens, kv_starts, out)
     q, k, v = aligned(q), aligned(k), aligned(v)
     if out is None:
         out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev).transpose(1, 2)
-    elif aligned(out) is not out:
-        raise ValueError("out needs channels side by side, rows of whole 16 bytes and a 16-byte start")
     if B * T == 0:
         return out
     d = N.AttnDesc(B, Hq, Hkv, D, T, L, window, sinks, types[q.dtype], scale)

@@ -27,7 +27,7 @@ from . import _native as N
 from .formats import (NF4_ZERO_CODE, codes_from_key_rows, key_rows_from_codes, nf4_codes,
                       pack_key_codes, pack_values, tile_value_rows, uniform_codes, unpack_key_codes,
                       unpack_values, untile_value_rows)
-from .ops import aligned, lengths_arg, needs_grad, norm_rope, on_device, stream_of, strides_of, window_args
+from .ops import aligned, check_out, lengths_arg, needs_grad, norm_rope, on_device, stream_of, strides_of, window_args
 from .codebooks import (HEAD_DIMS, dc_channel_mask, dc_mask_words, group_tokens_for, n_groups_for,
                         outliers_per_channel, random_rotation, rope_averaged_bias, value_codebook)
 
@@ -432,7 +432,7 @@ class TQKVPool:
         Only the coded groups that a query sees are read.
 
         Returns ``(B, Hq, T, D)`` in the queries' type (``out`` where given,
-        else laid out ``(B, T, Hq, D)``); rows ``t >= m`` and queries before
+        its rows apart, else laid out ``(B, T, Hq, D)``); rows ``t >= m`` and queries before
         the first token get zeros."""
         torch = _torch()
         B, Hq, D = self.max_batch, self.n_q_heads, self.head_dim
@@ -444,9 +444,8 @@ class TQKVPool:
             raise NotImplementedError("attend has no backward pass: call it under torch.no_grad()")
         window, sinks = window_args(window, sinks)
         q_lens = lengths_arg(q_lens, B, "q_lens")
-        if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or aligned(out) is not out):
-            raise ValueError(f"out is {tuple(q.shape)} {q.dtype} with channels side by side, rows of whole 16 bytes "
-                             "and a 16-byte start")
+        if out is not None:
+            check_out(out, q)
         for name, x in (("q", q), ("q_lens", q_lens), ("out", out)):
             if x is not None and x.device != self.kcodes.device:
                 raise ValueError(f"attend: {name} is on {x.device}, the pool on {self.kcodes.device}")
