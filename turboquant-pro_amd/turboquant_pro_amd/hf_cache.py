@@ -248,14 +248,21 @@ def _mask_is_trivial(mask, kv_len: int) -> bool:
 def _mask_is_window(mask, kv_len: int, window: int) -> bool:
     """True when ``mask`` ``(B or 1, 1, T, kv_len)`` lets each of the last T
     queries attend its own and the ``window - 1`` tokens before it, in every
-    sequence (a padded batch's does not)."""
+    sequence (a padded batch's does not), and none of the others: an additive
+    mask holds minus infinity there, or the lowest value of its type (a smaller
+    bias still lets a key count)."""
     if mask is None or mask.dim() != 4 or mask.shape[3] != kv_len or mask.shape[1] != 1:
         return False
+    if mask.dtype != torch.bool and not mask.dtype.is_floating_point:
+        return False
     T = int(mask.shape[2])
-    seen = mask if mask.dtype == torch.bool else mask == 0
     at = torch.arange(kv_len, device=mask.device)
     p = torch.arange(kv_len - T, kv_len, device=mask.device)[:, None]
-    return bool((seen == ((at <= p) & (at > p - window))).all())
+    window_sees = (at <= p) & (at > p - window)
+    if mask.dtype == torch.bool:
+        return bool((mask == window_sees).all())
+    lowest = torch.finfo(torch.float16 if mask.dtype == torch.float16 else torch.bfloat16).min
+    return bool(torch.where(window_sees, mask == 0, mask <= lowest).all())
 
 
 def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.0,
