@@ -1,0 +1,64 @@
+"""Calls of the HuggingFace attention function with a window's mask that the kernels do
+not take: they run SDPA, as without a window."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytest.importorskip("transformers")
+
+from test_gpu_hf_window import counted, rows  # noqa: E402
+from test_hf_window_cpu import window_mask  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm GPU visible")
+
+
+def module(groups=1):
+    m = torch.nn.Module()
+    m.num_key_value_groups = groups
+    return m
+
+
+def sdpa(q, k, v, mask, scale):
+    g = q.shape[1] // k.shape[1]
+    return torch.nn.functional.scaled_dot_product_attention(
+        q, k.repeat_interleave(g, 1), v.repeat_interleave(g, 1), attn_mask=mask, scale=scale).transpose(1, 2)
+
+
+@pytest.mark.parametrize("scaling,dv", [(0.0, 64), (-0.125, 64), (0.125, 128)])
+@torch.no_grad()
+def test_scales_and_value_widths_stay_with_sdpa(scaling, dv, monkeypatch):
+    """A scale that is not positive, values of another width than the keys'."""
+    from turboquant_pro_amd.hf_cache import tqk_attention
+    print(f"[hf window] scaling={scaling} dv={dv}", flush=True)
+    calls = counted(monkeypatch)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = rows(gen, 2, 4, 900, 64), rows(gen, 2, 2, 900, 64), rows(gen, 2, 2, 900, dv)
+    mask = window_mask(900, 900, 90, 2).cuda()
+    out, _ = tqk_attention(module(2), q, k, v, mask, scaling=scaling, sliding_window=90)
+    assert calls["window"] == 0 and calls["attend"] == 0
+    # (two calls of one library: the same up to the order of its sums)
+    assert float((out - sdpa(q, k, v, mask, scaling)).abs().max()) <= 2.0 ** -9
+
+
+@pytest.mark.parametrize("scaling", [0.0, -0.125])
+@torch.no_grad()
+def test_scales_of_a_coded_layer_stay_with_sdpa(scaling, monkeypatch):
+    from turboquant_pro_amd.hf_cache import TurboQuantLayer, tqk_attention
+    print(f"[hf window] layer scaling={scaling}", flush=True)
+    calls = counted(monkeypatch)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    layer = TurboQuantLayer(hot_window=64, value_bits=4, n_q_heads=4, max_cache_len=512, fused_decode=True)
+    layer.update(rows(gen, 2, 2, 200, 64), rows(gen, 2, 2, 200, 64))
+    q = rows(gen, 2, 4, 1, 64)
+    kk, vv = layer.update(rows(gen, 2, 2, 1, 64), rows(gen, 2, 2, 1, 64))
+    mask = window_mask(1, 201, 50, 2).cuda()
+    out, _ = tqk_attention(module(2), q, kk, vv, mask, scaling=scaling, sliding_window=50)
+    assert calls["attend"] == 0
+    k, v = layer.dense()
+    assert float((out - sdpa(q, k, v, mask, scaling)).abs().max()) <= 2.0 ** -9

@@ -34,6 +34,7 @@ does (hf_cache.py:247-299).
 
 from __future__ import annotations
 
+import math
 from functools import partial
 
 from .codebooks import HEAD_DIMS
@@ -278,6 +279,7 @@ def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.
     layer = getattr(key, "_tq_layer", None)
     window = kwargs.get("sliding_window")
     windowed = (window and attention_mask is not None and dropout == 0.0 and query.is_cuda
+                and (scaling is None or 0.0 < scaling < math.inf)
                 and not needs_grad(query, key, value) and not any(kwargs.get(x) is not None for x in ("softcap", "s_aux", "position_bias")))
     if layer is not None:
         sc = float(scaling) if scaling is not None else layer.head_dim ** -0.5
@@ -289,7 +291,8 @@ def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.
             return layer.attend(query, sc, window).to(query.dtype).transpose(1, 2), None
         key, value = layer.dense()
     elif (windowed and query.dtype in (torch.float16, torch.bfloat16) and query.dtype == key.dtype == value.dtype
-          and query.shape[3] in HEAD_DIMS and _mask_is_window(attention_mask, key.shape[2], window)):
+          and query.shape[3] in HEAD_DIMS and key.shape == value.shape and query.shape[0] == key.shape[0]
+          and query.shape[1] % key.shape[1] == 0 and _mask_is_window(attention_mask, key.shape[2], window)):
         out = window_attention(query, key, value, window=window, scale=scaling)
         return out.transpose(1, 2), None                         # (B, T, Hq, D)
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
