@@ -62,3 +62,28 @@ def test_scales_of_a_coded_layer_stay_with_sdpa(scaling, monkeypatch):
     assert calls["attend"] == 0
     k, v = layer.dense()
     assert float((out - sdpa(q, k, v, mask, scaling)).abs().max()) <= 2.0 ** -9
+
+
+@torch.no_grad()
+def test_a_captured_prefill_stays_with_sdpa(monkeypatch):
+    """The mask is read on the host, which a capture cannot wait for."""
+    from turboquant_pro_amd.hf_cache import tqk_attention
+    print("[hf window] capture", flush=True)
+    calls = counted(monkeypatch)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (rows(gen, 1, 2, 900, 64) for _ in range(3))
+    mask = window_mask(900, 900, 90).cuda()
+    want, _ = tqk_attention(module(), q, k, v, mask, scaling=0.125, sliding_window=90)
+    assert calls["window"] == 1
+    sdpa(q, k, v, mask, 0.125)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = tqk_attention(module(), q, k, v, mask, scaling=0.125, sliding_window=90)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        # (both round a value of at most 4 to fp16, weights and sums before it)
+        assert float((out - want).abs().max()) <= 2.0 ** -8
+    assert calls["window"] == 1

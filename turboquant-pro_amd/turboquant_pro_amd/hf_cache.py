@@ -280,6 +280,8 @@ def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.
     window = kwargs.get("sliding_window")
     windowed = (window and attention_mask is not None and dropout == 0.0 and query.is_cuda
                 and (scaling is None or 0.0 < scaling < math.inf)
+                # (the mask is read on the host: not while a graph is captured or traced)
+                and not torch.cuda.is_current_stream_capturing() and not torch.compiler.is_compiling()
                 and not needs_grad(query, key, value) and not any(kwargs.get(x) is not None for x in ("softcap", "s_aux", "position_bias")))
     if layer is not None:
         sc = float(scaling) if scaling is not None else layer.head_dim ** -0.5
