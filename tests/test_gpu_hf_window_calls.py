@@ -87,3 +87,21 @@ def test_a_captured_prefill_stays_with_sdpa(monkeypatch):
         # (both round a value of at most 4 to fp16, weights and sums before it)
         assert float((out - want).abs().max()) <= 2.0 ** -8
     assert calls["window"] == 1
+
+
+@pytest.mark.parametrize("B,Hq,T,L,kernel", [(1, 8, 64, 64, False), (1, 32, 256, 256, False), (1, 8, 1, 1024, False),
+                                             (1, 8, 2, 1024, True), (1, 8, 1, 1500, True), (8, 32, 300, 300, True)])
+@torch.no_grad()
+def test_short_calls_stay_with_sdpa(B, Hq, T, L, kernel, monkeypatch):
+    """Where reading the mask costs more than the kernel gains, SDPA's time is kept;
+    the result is the same either way."""
+    from turboquant_pro_amd.hf_cache import tqk_attention
+    print(f"[hf window] B={B} Hq={Hq} T={T} L={L}", flush=True)
+    calls = counted(monkeypatch)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    q, k, v = rows(gen, B, Hq, T, 128), rows(gen, B, Hq // 4, L, 128), rows(gen, B, Hq // 4, L, 128)
+    mask = window_mask(T, L, L // 3, B).cuda()
+    out, _ = tqk_attention(module(4), q, k, v, mask, scaling=128 ** -0.5, sliding_window=L // 3)
+    assert calls["window"] == kernel
+    # (values of at most 5: their weights' and the output's roundings to fp16)
+    assert float((out - sdpa(q, k, v, mask, 128 ** -0.5)).abs().max()) <= 2 * 5 * 2.0 ** -11 * 2

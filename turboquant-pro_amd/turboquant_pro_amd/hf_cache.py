@@ -266,15 +266,26 @@ def _mask_is_window(mask, kv_len: int, window: int) -> bool:
     return bool(torch.where(window_sees, mask == 0, mask <= lowest).all())
 
 
+def _window_pays(B: int, Hq: int, T: int, L: int, D: int) -> bool:
+    """Whether a windowed call over dense keys is faster through the kernel, reading
+    its mask on the host included, than through SDPA on that mask.  Microseconds of
+    SDPA and of the kernel, 1 sequence, 8 to 32 heads, head_dim 64 to 256: 64 keys
+    43-48 and 69-77, 512 50-80 and 85-95, 768 51-130 and 78-93, 1024 84-160 and
+    79-106, 2048 106-254 and 81-103; one query: 1024 61-115 and 78-79, 2048 102-195
+    and 78-81.  Batches fill the chip earlier: 8 sequences of 256 keys and queries
+    69-160 and 78-104."""
+    return L >= (896 if T > 1 else 1280) or B * Hq * L * (D + T / 4) >= 12 << 20
+
+
 def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.0,
                   scaling: float | None = None, **kwargs):
     """Attention function registered as ``"tqk_gfx950"``: a decode step on a
     :class:`TurboQuantLayer` runs the fused kernel; so does, with the module's
     sliding window, one whose mask is that window's, and a prefill or chunk with
-    such a mask (fp16 or bf16 on the GPU) runs
+    such a mask (fp16 or bf16 on the GPU, from some 900 keys on) runs
     :func:`~turboquant_pro_amd.ops.window_attention`.  Anything else (prefill
-    without a window, padded batches, dropout, soft-capped scores) runs PyTorch
-    SDPA on dense K/V."""
+    without a window, short ones, padded batches, dropout, soft-capped scores)
+    runs PyTorch SDPA on dense K/V."""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     layer = getattr(key, "_tq_layer", None)
     window = kwargs.get("sliding_window")
@@ -294,7 +305,8 @@ def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.
         key, value = layer.dense()
     elif (windowed and query.dtype in (torch.float16, torch.bfloat16) and query.dtype == key.dtype == value.dtype
           and query.shape[3] in HEAD_DIMS and key.shape == value.shape and query.shape[0] == key.shape[0]
-          and query.shape[1] % key.shape[1] == 0 and _mask_is_window(attention_mask, key.shape[2], window)):
+          and query.shape[1] % key.shape[1] == 0 and _window_pays(*query.shape[:3], *key.shape[2:])
+          and _mask_is_window(attention_mask, key.shape[2], window)):
         out = window_attention(query, key, value, window=window, scale=scaling)
         return out.transpose(1, 2), None                         # (B, T, Hq, D)
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
