@@ -425,7 +425,8 @@ int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const vo
  * - m + t and sees the tokens j of [0, p] with j > p - window or j < sinks.
  * Only the coded groups that a query sees are read.  Queries with p < 0 and
  * rows t >= m get zeros.  A cache with outliers_per_channel > 0 has an
- * outlier_cap of 1 or more (else TQK_EINVAL).
+ * outlier_cap of 1 or more (else TQK_EINVAL), an fp16 one n_pages * page_tokens
+ * below 2^31 (else TQK_EUNSUPPORTED).
  *   q        [batch][n_q_heads][q_len][head_dim] by strides, fp16 (fp32 when input_f32),
  *            16-byte aligned, as out
  *   seq_lens [batch] i32 (device), clamped to max_len

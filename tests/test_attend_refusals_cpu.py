@@ -47,3 +47,17 @@ def test_a_chunk_s_workspace_is_bounded(batch, heads, D, max_len, window, q_len)
     need = lib.tqk_attend_workspace_bytes(ctypes.byref(d), ctypes.byref(attend_desc(
         N, batch=batch, q_len=q_len, max_len=max_len, window=window)))
     assert 0 < need <= (1 << 30) + 512 * 128 * (D + 2) * 4 + 512
+
+
+@pytest.mark.parametrize("q_len", [1, 64])
+def test_page_pools_past_32_bits_are_refused(q_len):
+    """A head's rows are held in 32 bits by the fp16 caches' kernels."""
+    N, lib = _lib()
+    buf = ctypes.create_string_buffer(512)
+    at = (ctypes.addressof(buf) + 15) & ~15
+    p = N.CachePtrs(**{name: at for name, _ in N.CachePtrs._fields_})
+    for pages, f32, want in ((1 << 25, 0, N.TQK_EUNSUPPORTED), ((1 << 25) - 1, 0, N.TQK_EWORKSPACE),
+                             (1 << 25, 1, N.TQK_EWORKSPACE)):
+        d = N.CacheDesc(**{**CACHE, "n_pages": pages, "input_f32": f32})
+        t = attend_desc(N, q_len=q_len)
+        assert lib.tqk_attend(ctypes.byref(d), ctypes.byref(p), ctypes.byref(t), at, at, None, at, at, 0, None) == want

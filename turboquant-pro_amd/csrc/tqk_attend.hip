@@ -419,6 +419,8 @@ int check_attend(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   if (t->q_len > (1 << 28) || t->max_len > (1 << 30) || t->batch > counter_seqs(*d)) return TQK_EINVAL;
   if ((long long)t->batch * t->q_len > (1LL << 30)) return TQK_EINVAL;
   if (!(d->sm_scale > 0.f)) return TQK_EINVAL;
+  // (the fp16 caches' kernels hold a head's rows in 32 bits)
+  if (!d->input_f32 && (long long)d->n_pages * d->page_tokens > INT32_MAX) return TQK_EUNSUPPORTED;
   // (a side-list without room for one entry: its loads have no place to go)
   if (d->outliers_per_channel > 0 && d->outlier_cap < 1) return TQK_EINVAL;
   // (the tables reach as far as the longest sequence may)
