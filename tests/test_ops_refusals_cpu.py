@@ -77,3 +77,12 @@ def test_outputs_that_overlap_themselves():
     with pytest.raises(RuntimeError, match="GPU"):
         _call_window(q=query()[:1, :, :1], k=torch.zeros(1, 2, 9, 128, dtype=torch.float16),
                      v=torch.zeros(1, 2, 9, 128, dtype=torch.float16), out=one.as_strided((1, 8, 1, 128), (0, 128, 0, 1)))
+
+
+def test_append_qkv_refuses_rows_of_another_device():
+    """Rows, and positions beside them, that are not on the pool's device."""
+    pool = pool_without_a_gpu()
+    pool.seq_lens, pool.device = torch.zeros(2, dtype=torch.int32), torch.device("meta")
+    rows = torch.zeros(2, 3, 12 * 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="the pool on"):
+        pool.append_qkv(rows, torch.ones(64), positions=torch.zeros(2, dtype=torch.int32))

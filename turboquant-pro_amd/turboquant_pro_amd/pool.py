@@ -479,6 +479,8 @@ class TQKVPool:
                 int(qkv.shape[2]) != (self.n_q_heads + 2 * self.n_kv_heads) * self.head_dim:
             raise ValueError(f"append_qkv expects ({self.max_batch}, T, {self.n_q_heads + 2 * self.n_kv_heads} * "
                              f"{self.head_dim}) rows, got {tuple(qkv.shape)}")
+        if qkv.device != self.kcodes.device:
+            raise ValueError(f"append_qkv: rows are on {qkv.device}, the pool on {self.kcodes.device}")
         q, k, v = norm_rope(qkv, self.n_q_heads, self.n_kv_heads, inv_freq,
                             self.seq_lens if positions is None else positions, q_weight=q_weight, k_weight=k_weight,
                             eps=eps, weight_offset=weight_offset, interleaved=interleaved, rope_scale=rope_scale,
