@@ -2,9 +2,9 @@
 // a sliding window and first tokens that stay visible (gfx950).
 //
 // Few queries: tqk_attend_codes reads the codes of the tokens that they see and
-// nothing else.  Many queries (fp16 caches): what they see is reconstructed once
-// as dense fp16 keys and values in the workspace, and the kernels of
-// tqk_attention run over it.  fp32 caches: every query is an item of its own of
+// nothing else.  Many queries (fp16 caches): what they see is reconstructed as
+// dense keys (fp16 pairs) and fp16 values in the workspace, a GiB at a time, and the
+// kernels of tqk_attention run over it.  fp32 caches: every query is an item of its own of
 // the VALU decode (WIN instances of tqk_decode_kernels.h).
 #include "tqk_attend.h"
 #include "tqk_attn.h"
@@ -44,14 +44,18 @@ int most_groups(const tqk_cache_desc* d, const tqk_attend_desc* t) {
 // Rows [0, kept.sinks) and from the window on, moved down by kept.gap
 // (tqk_attn.h), 64 tokens of a kv head a step: keys as grid value with the
 // side-list's over it, an fp16 pair (a single fp16 moves a score of 60 by 0.01: the
-// result was three times as far off, and 30 us of 172 faster), values as
-// (cent[code] @ Pi) * norm and hot tokens as they are, in fp16.  PolarQuant keys are
-// rotated as the values, and pairs.  Pi is an fp16 pair up to head_dim 128 (fp16 at
+// result was three times as far off, and a chunk a fifth faster), values as
+// (cent[code] @ Pi) * norm and hot tokens as they are, in fp16 (half a step of a value
+// in the result, as its own rounding; a pair would be a third product of tiles).
+// PolarQuant keys are rotated as the values, and pairs (single: 141 us of 184 at
+// head_dim 128, 378 of 432 at 256, and infinities past 65504).  Pi is an fp16 pair up to head_dim 128 (fp16 at
 // 256) and the centroids are scaled against their roundings, summed in fp32 by the
 // matrix cores: the rotation costs a wave 32 products a step where the ordered sums
 // of tqk_dequant_dense took 2 D VALU operations a value.
-// Bound: writing the rows (6 D bytes a token and kv head): 41 us for two windows of
-// 4096 and 8 kv heads of 128, of a chunk's 172.
+// Bound: the chain of a step's loads and barriers, and each workgroup's set-up (64 KiB
+// of Pi split into pairs, the codebook's scale), beside the rows' writes (6 D bytes a
+// token and kv head): two windows of 4096 and 8 kv heads of 128, a step a workgroup,
+// 40 us of a chunk's 184 (1.4 TB/s); two whole caches of 16384, 100 to 114 us (2).
 constexpr int kGather = 64;  // tokens a step
 static_assert(kGather == kMaxKeys, "a step lies on one side of the gap");
 

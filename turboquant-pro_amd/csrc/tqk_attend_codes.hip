@@ -18,14 +18,16 @@
 // the trip.  A lane then holds one row's scores of 8 tokens, which are the operand
 // of V^T P^T as they are.  Value codes become centroids by pairs through a table,
 // the codebook scaled so that its fp16 roundings nearly vanish (best of 128 scales:
-// 2^-12 of a centroid becomes about 2^-14 to 2^-15); weights times norms are rounded
-// to fp16 (2^-12 of each).  The coded part is rotated back once a workgroup, by the
-// matrix cores in fp16 pairs.  Up to head_dim 128 a table entry has a row of 256
+// 2^-12 of a centroid becomes about 2^-14 to 2^-15).  Weights times norms, and an
+// uncoded block's weights, are rounded to fp16 as the matrix cores take them (at most
+// 2^-11 of each; pairs would double the lookups' and values' products): 2.8e-4 to
+// 3.0e-4 off 64 bits, where the output's rounding alone is 2.1e-4 off.  The coded part
+// is rotated back once a workgroup, by the matrix cores in fp16 pairs.  Up to head_dim 128 a table entry has a row of 256
 // bytes of copies, by lane: a lookup's bank is its lane's own, and its address one
 // byte permutation; at head_dim 256 the waves' tiles leave room for four copies.
 // Bound: few sequences, the chain of dependent loads (lengths, tables, codes) and
 // the set-up; many, a wave's chain of LDS trips and products beside its codes from
-// HBM: 16 sequences of 8192 tokens, 8 kv heads of 128, 35 us with a window of 4096,
+// HBM: 16 sequences of 32768 tokens, 8 kv heads of 128, 37.6 us with a window of 4096,
 // of which a one-block window takes 8; with every page and group the same one, in
 // cache, no more than 3% less.
 #include "tqk_attend.h"
