@@ -401,15 +401,32 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
     __syncthreads();
   }
 
-  if (__builtin_expect(odd_s != 0, 0)) {
-    // the infinities and NaN set aside, into the rows that see them (any
-    // positive weight gives the same)
+  const float l = sum_half(l_run);
+  // a result that is not finite beside a sum that is: an infinity or a NaN among the
+  // values of a whole tile, which a weight that rounds to zero may have turned into a NaN
+  float zero = 0.f;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) zero = fmaf(O[i][r], 0.f, zero);
+  const bool lost = __any(real && zero != 0.f && l == l);
+  if (__builtin_expect(odd_s != 0 || lost, 0)) {
+    // the infinities and NaN that a row sees are its result in their channels,
+    // whatever their positive weights
+    f16v_t odd[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) odd[i] = f16v_t{};
     for (int it = i0; it < i1; ++it) {
-      const int k0 = tiles.at(it);
-      if (whole(k0)) continue;
-      for (int j = k0; j < min(k0 + kKeys, s.n); ++j) {
-        const bool vis = s.sees(p, lo, j);
-        const T* vr = reinterpret_cast<const T*>(vb + (j - (k0 >= sink_rows ? gap : 0)) * vs_) + 4 * lh;
+      const int k0 = tiles.at(it), rows = min(kKeys, s.n - k0);
+      if (!lost && whole(k0)) continue;
+      const char* const vt = vb + (k0 - (k0 >= sink_rows ? gap : 0)) * vs_;
+      bool has = false;
+      for (int x = lane; x < rows * CH; x += 64)
+        has |= not_finite<T>(*reinterpret_cast<const u4_t*>(vt + x / CH * vs_ + 16 * (x % CH)));
+      if (!__any(has)) continue;
+      for (int j = 0; j < rows; ++j) {
+        const bool vis = s.sees(p, lo, k0 + j);
+        const T* vr = reinterpret_cast<const T*>(vt + j * vs_) + 4 * lh;
 #pragma unroll
         for (int i = 0; i < ND; ++i)
 #pragma unroll
@@ -419,14 +436,17 @@ __global__ __launch_bounds__(kTileThreads, D <= 128 ? 2 : 1) void tqk_attn_tiles
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float y = (float)x[e];
-              O[i][r + e] += vis && !(fabsf(y) < INFINITY) ? y : 0.f;
+              odd[i][r + e] += vis && !(fabsf(y) < INFINITY) ? y : 0.f;
             }
           }
       }
     }
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) O[i][r] = odd[i][r] == 0.f ? O[i][r] : odd[i][r];
   }
 
-  const float l = sum_half(l_run);
   if (!inside) return;
   if (a.n_splits == 1) {
     // rows that see nothing, and those past the sequence's queries: zero
@@ -481,7 +501,8 @@ __global__ __launch_bounds__(256) void tqk_attn_join(AttnArgs a) {
     const float g = __shfl(f, s, 64);
     const float* src = a.part_acc + (s * a.rows + row) * D + E * lane;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = live >> s & 1 ? fmaf(src[e], g, acc[e]) : acc[e];
+    for (int e = 0; e < E; ++e)  // (an infinity stays one, however far behind its split's weights are)
+      acc[e] = live >> s & 1 ? (fabsf(src[e]) < INFINITY ? fmaf(src[e], g, acc[e]) : acc[e] + src[e]) : acc[e];
   }
   const int t = (int)(row % a.d.q_len);
   const long long bh = row / a.d.q_len;
