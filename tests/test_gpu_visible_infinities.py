@@ -80,3 +80,12 @@ def attend(D, Hq, H, dtype, T, spread):
 def test_attend_chunks(D, Hq, H, spread):
     """Uncoded values of a chunk over reconstructed keys and values."""
     attend(D, Hq, H, "float16", 128 * H // Hq + 1, spread)
+
+
+@pytest.mark.parametrize("D,Hq,H", [(64, 4, 2), (128, 8, 2), (256, 4, 2)])
+@pytest.mark.parametrize("T", [1, 7])
+@pytest.mark.parametrize("spread", [1.0, 5.0, 40.0])
+def test_attend_few(D, Hq, H, T, spread):
+    """Over the codes: weights that another wave's, split's or later block's scores
+    leave behind by more than fp32 holds."""
+    attend(D, Hq, H, "float16", T, spread)

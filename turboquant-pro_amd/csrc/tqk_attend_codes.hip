@@ -485,7 +485,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
     if (__any(mx > m_run + kFewLazy)) {
       mx = colgroup_max(mx);
       const float m_new = fmaxf(m_run, mx);
-      const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      const float f = m_new == -INFINITY ? 1.f : above_zero(__builtin_amdgcn_exp2f(m_run - m_new));
       m_run = m_new;
       l_run *= f;
 #pragma unroll
@@ -786,7 +786,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_codes(FewArgs a) {
     for (int w = 0; w < kFewWaves; ++w) ms[k] = fmaxf(ms[k], ml_s[0][w][r]);
 #pragma unroll
     for (int w = 0; w < kFewWaves; ++w) {
-      const float mw = ml_s[0][w][r], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - ms[k]);
+      const float mw = ml_s[0][w][r], f = mw == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(mw - ms[k]));
       const float y = reinterpret_cast<const float*>(stage_s[w])[r * D + j];
       ls[k] = fmaf(ml_s[1][w][r], f, ls[k]);
       // (a state without a maximum holds zeros; a NaN among its scores leaves it one)
@@ -877,7 +877,7 @@ __global__ __launch_bounds__(256) void tqk_attend_join(FewArgs a) {
   const float ml = in ? a.part_ml[2 * (lane * a.rows + row)] : -INFINITY;
   const float ll = in ? a.part_ml[2 * (lane * a.rows + row) + 1] : 0.f;
   const float M = wave_reduce<true>(ml);
-  const float f = ml == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml - M);
+  const float f = ml == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(ml - M));
   const float l = wave_reduce<false>(ll * f);
   float acc[E];
 #pragma unroll

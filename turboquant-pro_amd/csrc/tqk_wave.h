@@ -29,6 +29,10 @@ __device__ __forceinline__ float wave_reduce(float x) {
   return op(__builtin_bit_cast(float, (uint32_t)r32[0]), __builtin_bit_cast(float, (uint32_t)r32[1]));
 }
 
+// A positive weight that fp32 holds as zero, as its smallest normal number: what an
+// infinity needs to stay one, and nothing to a finite value.
+__device__ __forceinline__ float above_zero(float w) { return w < 0x1p-126f ? 0x1p-126f : w; }
+
 // two floats as fp16 pairs: {hi, hi}, {lo, lo}
 __device__ __forceinline__ uint2 split_pair(float x0, float x1) {
   const _Float16 h0 = (_Float16)x0, h1 = (_Float16)x1;
