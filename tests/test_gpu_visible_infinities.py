@@ -89,3 +89,10 @@ def test_attend_few(D, Hq, H, T, spread):
     """Over the codes: weights that another wave's, split's or later block's scores
     leave behind by more than fp32 holds."""
     attend(D, Hq, H, "float16", T, spread)
+
+
+@pytest.mark.parametrize("D,Hq,H", [(64, 4, 2), (128, 4, 2), (256, 2, 1)])
+@pytest.mark.parametrize("T", [1, 7])
+@pytest.mark.parametrize("spread", [1.0, 5.0, 40.0])
+def test_attend_fp32_caches(D, Hq, H, T, spread):
+    attend(D, Hq, H, "float32", T, spread)

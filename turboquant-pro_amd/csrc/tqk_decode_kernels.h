@@ -188,7 +188,8 @@ __device__ __forceinline__ void block_reduce(float (&v)[GQ], float (*red)[GQ]) {
 
 // Online-softmax update over the n scores in sc[i][0..n) (already scaled).
 // On return sc[i][t] holds p_t (times the value norm when norms != nullptr).
-// SAFE: a whole block's scores may be -inf (tokens that are not seen).
+// SAFE: a whole block's scores may be -inf (tokens that are not seen), and the weights
+// of those that are stay above zero.
 template <int GQ, bool SAFE>
 __device__ __forceinline__ void softmax_update(float (*sc)[kThreads], int n, float (&m_run)[GQ],
                                                float (&l_run)[GQ], float (&acc0)[GQ],
@@ -204,12 +205,14 @@ __device__ __forceinline__ void softmax_update(float (*sc)[kThreads], int n, flo
   for (int i = 0; i < GQ; ++i) {
     const float mn = fmaxf(m_run[i], mx[i]);
     const float at = SAFE && mn == -INFINITY ? 0.f : mn;
-    const float corr = __expf(m_run[i] - at);
+    const float corr = SAFE ? above_zero(__expf(m_run[i] - at)) : __expf(m_run[i] - at);
     m_run[i] = mn;
     l_run[i] *= corr;
     acc0[i] *= corr;
     acc1[i] *= corr;
     p[i] = (t < n) ? __expf(sc[i][t] - at) : 0.0f;
+    if constexpr (SAFE)
+      if (t < n && sc[i][t] != -INFINITY) p[i] = above_zero(p[i]);
     ps[i] = p[i];
   }
   block_reduce<GQ, false>(ps, red);
@@ -994,7 +997,7 @@ __device__ __forceinline__ float ld_agent(const float* p) {
 // n_live are known to be empty (l = 0, which the pass skips anyway): they are
 // not loaded.  Both merges (tqk_merge and the in-kernel one) use it, so they
 // agree bit for bit whatever n_live they pass.
-template <int D, class Load>
+template <int D, bool WIN, class Load>
 __device__ __forceinline__ void merge_chunked(Load ld, const float* pl, const float* pm,
                                               const float* pacc, size_t base, int ns, int n_live,
                                               int n_cold, int j, float& M, float& dn, float& cr,
@@ -1023,7 +1026,7 @@ __device__ __forceinline__ void merge_chunked(Load ld, const float* pl, const fl
     for (int k = 0; k < C; ++k)
       if (vl[k] > 0.f) Mc = fmaxf(Mc, vm[k]);
     if (Mc > M) {
-      const float f = __expf(M - Mc);  // 0 on the first round (the sums are 0)
+      const float f = WIN ? above_zero(__expf(M - Mc)) : __expf(M - Mc);  // 0 on the first round (the sums are 0)
       dn *= f;
       cr *= f;
       hh *= f;
@@ -1032,7 +1035,7 @@ __device__ __forceinline__ void merge_chunked(Load ld, const float* pl, const fl
 #pragma unroll
     for (int k = 0; k < C; ++k) {
       if (vl[k] > 0.f) {
-        const float wt = __expf(vm[k] - M);
+        const float wt = WIN ? above_zero(__expf(vm[k] - M)) : __expf(vm[k] - M);
         dn += vl[k] * wt;
         const float x = va[k] * wt;
         if (s0 + k < n_cold) cr += x; else hh += x;
@@ -2291,7 +2294,7 @@ __global__ __launch_bounds__(kMThreads, 1) void tqk_decode_split_mfma(DecodeArgs
         if (qi < gq) {
           const size_t base = ((size_t)b * Hq + h * gq + qi) * ns;
           float M, dn, cr, hh;
-          merge_chunked<D>([](const float* p) { return ld_agent(p); }, a.pl, a.pm, a.pacc, base, ns,
+          merge_chunked<D, false>([](const float* p) { return ld_agent(p); }, a.pl, a.pm, a.pacc, base, ns,
                            a.n_cold_splits + hot_live, a.n_cold_splits, j, M, dn, cr, hh);
           q_h_s[qi][j] = cr;
           hr[r] = hh;
@@ -2374,7 +2377,7 @@ __global__ __launch_bounds__(2 * D) void tqk_merge(JoinArgs<WIN> a) {
     float dn = 0.f, cr = 0.f, hh = 0.f;
     for (int s = 0; s < ns; ++s) {
       if (vl[s] > 0.f) {
-        const float wt = __expf(vm[s] - M);
+        const float wt = WIN ? above_zero(__expf(vm[s] - M)) : __expf(vm[s] - M);
         dn += vl[s] * wt;
         const float v = va[s] * wt;
         if (s < a.n_cold_splits) cr += v; else hh += v;
@@ -2403,7 +2406,7 @@ __global__ __launch_bounds__(2 * D) void tqk_merge(JoinArgs<WIN> a) {
       if (qi < GQ) {
         const size_t base = ((size_t)b * a.n_q_heads + h * GQ + qi) * a.n_splits;
         float M, dn, cr, hh;
-        merge_chunked<D>([](const float* p) { return *p; }, a.pl, a.pm, a.pacc, base, a.n_splits,
+        merge_chunked<D, WIN>([](const float* p) { return *p; }, a.pl, a.pm, a.pacc, base, a.n_splits,
                          a.n_splits, a.n_cold_splits, j, M, dn, cr, hh);
         crot_s[qi][j] = cr;
         hr[u] = hh;
