@@ -436,8 +436,9 @@ int tqk_attention(const tqk_attn_desc* d, const void* q, const void* k, const vo
  * verification step) or a prompt's chunk.  Few queries are attended in code
  * space; more (over 128 rows: queries times query heads of a kv head) of an fp16
  * cache with an fp16 output over keys and values reconstructed in the workspace
- * (weights and values rounded to fp16, keys in fp16 pairs), at most 1 GiB of them at
- * a time, whatever the batch and the lengths.
+ * (weights and values rounded to fp16, keys in fp16 pairs; PolarQuant keys from
+ * centroids, and at head_dim 256 a rotation, of fp16), at most 1 GiB of them at a time,
+ * whatever the batch and the lengths.
  */
 typedef struct tqk_attend_desc {
   int32_t batch;        /* at most n_pages of the cache */

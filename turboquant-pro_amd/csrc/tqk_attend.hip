@@ -48,10 +48,12 @@ int most_groups(const tqk_cache_desc* d, const tqk_attend_desc* t) {
 // (cent[code] @ Pi) * norm and hot tokens as they are, in fp16 (half a step of a value
 // in the result, as its own rounding; a pair would be a third product of tiles).
 // PolarQuant keys are rotated as the values, and pairs (single: 141 us of 184 at
-// head_dim 128, 378 of 432 at 256, and infinities past 65504).  Pi is an fp16 pair up to head_dim 128 (fp16 at
-// 256) and the centroids are scaled against their roundings, summed in fp32 by the
-// matrix cores: the rotation costs a wave 32 products a step where the ordered sums
-// of tqk_dequant_dense took 2 D VALU operations a value.
+// head_dim 128, 378 of 432 at 256, and infinities past 65504); their centroids'
+// roundings stay, and at 256 Pi's: up to 1.7e-3 of the result where a score of 60
+// decides.  Pi is an fp16 pair up to head_dim 128 (fp16 at 256) and the centroids are
+// scaled against their roundings, summed in fp32 by the matrix cores: the rotation
+// costs a wave 32 products a step where the ordered sums of tqk_dequant_dense took 2 D
+// VALU operations a value.
 // Bound: the chain of a step's loads and barriers, and each workgroup's set-up (64 KiB
 // of Pi split into pairs, the codebook's scale), beside the rows' writes (6 D bytes a
 // token and kv head): two windows of 4096 and 8 kv heads of 128, a step a workgroup,

@@ -16,8 +16,8 @@
 // scores come in).  V^T comes from LDS by transposing reads.
 // Bound: the matrix cores and, as closely, LDS reads (16 KiB of K and V for
 // 32 x 64 scores a wave).  A prompt of 8192 tokens, 32 heads of 128, window 4096:
-// 470 us, 880 TFLOP/s (a large library product: 1200); head_dim 256, 16 heads,
-// 4096 tokens: 282 us, 490 TFLOP/s, at one wave a SIMD, which leaves the softmax
+// 464 to 480 us, 860 to 890 TFLOP/s (a large library product: 1200); head_dim 256, 16
+// heads, 4096 tokens: 284 us, 485 TFLOP/s, at one wave a SIMD, which leaves the softmax
 // nothing to hide behind (two waves spill: 442 us).  Few rows: HBM and the join.
 //
 // The weights are rounded to the inputs' type, as the matrix cores take them (pairs
