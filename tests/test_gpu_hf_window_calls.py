@@ -105,3 +105,19 @@ def test_short_calls_stay_with_sdpa(B, Hq, T, L, kernel, monkeypatch):
     assert calls["window"] == kernel
     # (values of at most 5: their weights' and the output's roundings to fp16)
     assert float((out - sdpa(q, k, v, mask, 128 ** -0.5)).abs().max()) <= 2 * 5 * 2.0 ** -11 * 2
+
+
+@torch.no_grad()
+def test_one_mask_row_for_every_query_stays_with_sdpa(monkeypatch):
+    """A mask row that is broadcast over the queries is no window of each of them, though
+    it is the last one's."""
+    from turboquant_pro_amd.hf_cache import tqk_attention
+    print("[hf window] one mask row", flush=True)
+    calls = counted(monkeypatch)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    q, k, v = rows(gen, 2, 4, 70, 64), rows(gen, 2, 2, 1000, 64), rows(gen, 2, 2, 1000, 64)
+    mask = window_mask(1, 1000, 90, 2).cuda()
+    out, _ = tqk_attention(module(2), q, k, v, mask, scaling=0.125, sliding_window=90)
+    assert calls["window"] == 0
+    # (two calls of one library: the same up to the order of its sums)
+    assert float((out - sdpa(q, k, v, mask, 0.125)).abs().max()) <= 2.0 ** -9

@@ -290,6 +290,9 @@ def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.
     layer = getattr(key, "_tq_layer", None)
     window = kwargs.get("sliding_window")
     windowed = (window and attention_mask is not None and dropout == 0.0 and query.is_cuda
+                # (a row of the mask for every query: one that is broadcast is not each one's window)
+                and attention_mask.dim() == 4 and attention_mask.shape[2] == query.shape[2]
+                and attention_mask.shape[0] in (1, query.shape[0])
                 and (scaling is None or 0.0 < scaling < math.inf)
                 # (the mask is read on the host: not while a graph is captured or traced)
                 and not torch.cuda.is_current_stream_capturing() and not torch.compiler.is_compiling()
