@@ -121,3 +121,23 @@ def test_one_mask_row_for_every_query_stays_with_sdpa(monkeypatch):
     assert calls["window"] == 0
     # (two calls of one library: the same up to the order of its sums)
     assert float((out - sdpa(q, k, v, mask, 0.125)).abs().max()) <= 2.0 ** -9
+
+
+@torch.no_grad()
+def test_a_layer_without_the_query_heads_stays_with_sdpa(monkeypatch):
+    """A cache made without the model's config: its windowed steps run on dense keys and
+    values, as they did."""
+    from turboquant_pro_amd.hf_cache import TurboQuantLayer, tqk_attention
+    print("[hf window] no config", flush=True)
+    calls = counted(monkeypatch)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    layer = TurboQuantLayer(hot_window=64, value_bits=4, max_cache_len=512, fused_decode=True)
+    layer.update(rows(gen, 2, 2, 200, 64), rows(gen, 2, 2, 200, 64))
+    q = rows(gen, 2, 8, 1, 64)
+    kk, vv = layer.update(rows(gen, 2, 2, 1, 64), rows(gen, 2, 2, 1, 64))
+    mask = window_mask(1, 201, 50, 2).cuda()
+    out, _ = tqk_attention(module(4), q, kk, vv, mask, scaling=0.125, sliding_window=50)
+    assert calls["attend"] == 0
+    k, v = layer.dense()
+    # (two calls of one library: the same up to the order of its sums)
+    assert float((out - sdpa(q, k, v, mask, 0.125)).abs().max()) <= 2.0 ** -9

@@ -303,7 +303,8 @@ def tqk_attention(module, query, key, value, attention_mask, dropout: float = 0.
                 and _mask_is_trivial(attention_mask, layer.get_seq_length())):
             out = layer.decode(query, sc)                       # (B, Hq, D) fp32
             return out.to(query.dtype)[:, None], None            # (B, 1, Hq, D)
-        if windowed and _mask_is_window(attention_mask, layer.get_seq_length(), window):
+        if (windowed and query.shape[1] == layer.pool.n_q_heads  # (not without the model's config)
+                and _mask_is_window(attention_mask, layer.get_seq_length(), window)):
             return layer.attend(query, sc, window).to(query.dtype).transpose(1, 2), None
         key, value = layer.dense()
     elif (windowed and query.dtype in (torch.float16, torch.bfloat16) and query.dtype == key.dtype == value.dtype
