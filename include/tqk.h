@@ -460,6 +460,104 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
                const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace,
                size_t workspace_bytes, void* stream);
 
+/*
+ * tqk_attend over listed groups: query t sees the tokens j <= p of the coded groups
+ * in its list and the uncoded ones (t->window and t->sinks are 0).  Entries outside
+ * [0, groups of the sequence) are none; a group listed twice counts twice.
+ *   groups [batch][n_kv_heads][q_len][n] i32 by the list's strides, entries side by
+ *   side; a query stride of 0: one list for all queries of a (sequence, kv head)
+ * fp16 caches, over the codes however many queries.  No counterpart in the reference,
+ * whose decode reads every group (turboquant_pro/kv_kernel.py:319-381).
+ */
+typedef struct tqk_group_list {
+  int32_t n;          /* entries of a list */
+  int64_t stride[3];  /* entries between sequences, kv heads and queries */
+} tqk_group_list;
+
+size_t tqk_attend_groups_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l);
+
+int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t,
+                      const tqk_group_list* l, const void* q, const int32_t* seq_lens,
+                      const int32_t* q_lens, const int32_t* groups, void* out, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * tqk_attend that keeps account of the groups' weight: weights[b][h][g] += the softmax
+ * weights of group g's tokens, summed over the sequence's queries and kv head h's query
+ * heads.
+ *   weights [batch][n_kv_heads][max_groups_per_seq] fp32 (batch * n_kv_heads at most 65535)
+ * fp16 caches, over the codes however many queries; 256 MiB of blocks' sums at a time
+ * beside the partial results.
+ */
+size_t tqk_attend_weights_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t);
+
+int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
+                       const int32_t* seq_lens, const int32_t* q_lens, void* out, float* weights,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * tqk_attend (t->window and t->sinks are 0) of sequences whose first `groups` coded
+ * groups are the same pages and slots in every sequence's tables: they are read
+ * through the first sequence's, once for all.  Every query sees them whole (p is at
+ * least groups * group_tokens - 1).  fp16 caches.
+ */
+size_t tqk_attend_shared_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups);
+
+int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, int32_t groups,
+                      const void* q, const int32_t* seq_lens, const int32_t* q_lens, void* out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The coded groups that every query attends, by a score of their scales and zero
+ * points (no code is read).  Query t stands at p = n - m + t, as in tqk_attend, and has
+ * for candidates the c groups with a token j <= p.  All of them where c <= top; else
+ * the first `first` and last `last` ones and those of the largest
+ *   score = max over the kv head's query heads of sum_i q_i mid_i + spread |q_i| half_i
+ * where mid +- half are the ends of channel i's key levels in the group (a side-list's
+ * values may lie outside): at spread 1 a bound on the products with its keys, at 0 the
+ * product with the levels' centre.  In 64 bits; a score that is no number ranks above
+ * all, equal ones by the lower index.
+ *   groups [batch][n_kv_heads][q_len][top] i32, ascending, then -1
+ * fp16 caches with per-channel keys (key_grid 0 or 1).  No counterpart in the reference.
+ */
+typedef struct tqk_select_desc {
+  int32_t batch;
+  int32_t q_len;
+  int32_t max_len;
+  int32_t top;    /* at least 1 */
+  int32_t first;  /* first + last <= top */
+  int32_t last;
+  float spread;
+  int64_t q_stride[3];
+} tqk_select_desc;
+
+size_t tqk_select_groups_workspace_bytes(const tqk_cache_desc* d, const tqk_select_desc* s);
+
+int tqk_select_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_select_desc* s, const void* q,
+                      const int32_t* seq_lens, const int32_t* q_lens, int32_t* groups, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * Coded groups leave the cache: of every sequence with more than `keep`, the first
+ * `first`, the last `last` and those of the largest weight stay (the sum of weights[b][h][g]
+ * over h in 64 bits; a sum that is no number ranks above all, equal ones by the lower
+ * index).  No code moves: the sequence's table rows are reordered (what stays, what
+ * leaves, entries without a group as they were), its length shortened by the groups
+ * that left, its hot ring turned to the shorter length and its weights moved along
+ * (the rest of them zero).  The keys keep the rotation of the positions that they had.
+ *   block_table, group_table  the cache's own (p->block_table, p->group_table), rewritten
+ *   seq_lens [batch] i32, rewritten;  weights [batch][n_kv_heads][max_groups_per_seq] fp32, rewritten
+ *   kept [batch][keep] i32: the former index of every group that stays, ascending, then -1
+ * zero_point 0 and 1 (the "bias" zero points of later groups belong to their positions:
+ * TQK_EUNSUPPORTED); hot_ring * 16 bytes within 64 KiB.
+ */
+size_t tqk_evict_groups_workspace_bytes(const tqk_cache_desc* d, int32_t batch);
+
+int tqk_evict_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, int32_t batch, int32_t keep, int32_t first,
+                     int32_t last, float* weights, int32_t* seq_lens, int32_t* block_table,
+                     int32_t* group_table, int32_t* kept, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

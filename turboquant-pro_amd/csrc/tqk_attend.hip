@@ -417,34 +417,6 @@ size_t slice_attention_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, 
   return most;
 }
 
-int check_attend(const tqk_cache_desc* d, const tqk_attend_desc* t) {
-  const int rc = tqk_check_desc(d);
-  if (rc != TQK_OK) return rc;
-  if (!t || t->batch < 0 || t->q_len < 0 || t->max_len < 0 || t->window < 0 || t->sinks < 0) return TQK_EINVAL;
-  if (t->out_type != 0 && t->out_type != 1) return TQK_EUNSUPPORTED;
-  if (t->q_len > (1 << 28) || t->max_len > (1 << 30) || t->batch > counter_seqs(*d)) return TQK_EINVAL;
-  if ((long long)t->batch * t->q_len > (1LL << 30)) return TQK_EINVAL;
-  if (!(d->sm_scale > 0.f)) return TQK_EINVAL;
-  // (the fp16 caches' kernels hold a head's rows in 32 bits)
-  if (!d->input_f32 && (long long)d->n_pages * d->page_tokens > INT32_MAX) return TQK_EUNSUPPORTED;
-  // (a side-list without room for one entry: its loads have no place to go)
-  if (d->outliers_per_channel > 0 && d->outlier_cap < 1) return TQK_EINVAL;
-  // (the tables reach as far as the longest sequence may)
-  const int groups = n_groups_of(t->max_len, d->hot_window, d->group_tokens);
-  if (groups > d->max_groups_per_seq || (long long)groups * (d->group_tokens / d->page_tokens) > d->max_pages_per_seq)
-    return TQK_EINVAL;
-  for (int i = 0; i < 3; ++i)
-    if (t->q_stride[i] % 8 || t->o_stride[i] % 8) return TQK_EINVAL;
-  return TQK_OK;
-}
-
-// Every buffer that a cache of this form has.
-bool have_buffers(const tqk_cache_desc& d, const tqk_cache_ptrs& p) {
-  const bool keys = d.key_grid == 2 ? p.knorm != nullptr : p.gscale && p.gmean;
-  return keys && p.kcodes && p.vcodes && p.vnorm && p.ocount && (d.outliers_per_channel == 0 || p.oent) && p.hot_k &&
-         p.hot_v && p.block_table && p.group_table && p.vcent && p.pi && p.pi_t;
-}
-
 template <int GQ, int D>
 void launch_valu(const SplitArgs<true>& a, dim3 grid, hipStream_t st) {
   if (a.d.value_bits == 2)
@@ -472,10 +444,38 @@ void launch_join(const JoinArgs<true>& m, dim3 grid, hipStream_t st) {
 
 }  // namespace
 
+int tqk_check_attend(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+  const int rc = tqk_check_desc(d);
+  if (rc != TQK_OK) return rc;
+  if (!t || t->batch < 0 || t->q_len < 0 || t->max_len < 0 || t->window < 0 || t->sinks < 0) return TQK_EINVAL;
+  if (t->out_type != 0 && t->out_type != 1) return TQK_EUNSUPPORTED;
+  if (t->q_len > (1 << 28) || t->max_len > (1 << 30) || t->batch > counter_seqs(*d)) return TQK_EINVAL;
+  if ((long long)t->batch * t->q_len > (1LL << 30)) return TQK_EINVAL;
+  if (!(d->sm_scale > 0.f)) return TQK_EINVAL;
+  // (the fp16 caches' kernels hold a head's rows in 32 bits)
+  if (!d->input_f32 && (long long)d->n_pages * d->page_tokens > INT32_MAX) return TQK_EUNSUPPORTED;
+  // (a side-list without room for one entry: its loads have no place to go)
+  if (d->outliers_per_channel > 0 && d->outlier_cap < 1) return TQK_EINVAL;
+  // (the tables reach as far as the longest sequence may)
+  const int groups = n_groups_of(t->max_len, d->hot_window, d->group_tokens);
+  if (groups > d->max_groups_per_seq || (long long)groups * (d->group_tokens / d->page_tokens) > d->max_pages_per_seq)
+    return TQK_EINVAL;
+  for (int i = 0; i < 3; ++i)
+    if (t->q_stride[i] % 8 || t->o_stride[i] % 8) return TQK_EINVAL;
+  return TQK_OK;
+}
+
+// Every buffer that a cache of this form has.
+bool tqk_have_buffers(const tqk_cache_desc& d, const tqk_cache_ptrs& p) {
+  const bool keys = d.key_grid == 2 ? p.knorm != nullptr : p.gscale && p.gmean;
+  return keys && p.kcodes && p.vcodes && p.vnorm && p.ocount && (d.outliers_per_channel == 0 || p.oent) && p.hot_k &&
+         p.hot_v && p.block_table && p.group_table && p.vcent && p.pi && p.pi_t;
+}
+
 extern "C" {
 
 size_t tqk_attend_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) {
-  if (check_attend(d, t) != TQK_OK) return 0;
+  if (tqk_check_attend(d, t) != TQK_OK) return 0;
   if (!t->batch || !t->q_len) return 0;
   if (dense_path(d, t)) {
     const Slice sl(d, t);
@@ -488,10 +488,10 @@ size_t tqk_attend_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc
 int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
                const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace,
                size_t workspace_bytes, void* stream) {
-  const int rc = check_attend(d, t);
+  const int rc = tqk_check_attend(d, t);
   if (rc != TQK_OK) return rc;
   if (!t->batch || !t->q_len) return TQK_OK;
-  if (!p || !q || !seq_lens || !out || (((uintptr_t)q | (uintptr_t)out) & 15) || !have_buffers(*d, *p)) return TQK_EINVAL;
+  if (!p || !q || !seq_lens || !out || (((uintptr_t)q | (uintptr_t)out) & 15) || !tqk_have_buffers(*d, *p)) return TQK_EINVAL;
   if (!workspace || ((uintptr_t)workspace & 15)) return TQK_EWORKSPACE;
   const bool dense = dense_path(d, t);
   if (!dense && !d->input_f32) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, workspace_bytes, stream);

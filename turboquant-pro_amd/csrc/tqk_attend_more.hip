@@ -1,0 +1,455 @@
+// Attention over the codes of an fp16 cache of more kinds than a window's (gfx950):
+// over listed groups, with the weight that every coded group received, and over a
+// prefix that all sequences share (tqk_attend_codes_kernels.h has the kernel).
+//
+// Listed groups: a workgroup's blocks are those of its list, nothing else is read.
+//
+// Weights: softmax_j = 2^(s_j - M) / L with a row's maximum M and sum L, which are
+// known when its splits are joined.  A wave writes each block's own maximum and sum
+// beside its partial results (8 bytes a row and block of 32 tokens), the join writes M
+// and L, and tqk_group_weights adds 2^(m - M) l / L over a kv head's rows and a
+// group's blocks, in one order and 64 bits: no atomics.
+//
+// A shared prefix: rows of all sequences are attended 16 at a time over one copy of
+// its codes, then each sequence's rows over its other tokens; the join takes both.
+#include "tqk_attend_codes_kernels.h"
+
+namespace {
+
+// Bytes of blocks' maxima and sums at a time: more queries go in slices.
+constexpr long long kMostBlockBytes = (long long)256 << 20;
+
+struct JoinMoreArgs {
+  const float* part_acc;  // [split][row][D]
+  const float* part_ml;   // [split][row][2]
+  const int32_t* seq_lens;
+  const int32_t* q_lens;
+  void* out;
+  float* row_ml;  // [row][2]: maximum and sum over all splits, or null
+  long long rows;
+  long long o_stride[3];
+  int n_splits, n_q_heads, q_len, max_len, out_type, t0, t_len;
+};
+
+// The partial results of a row joined: one wave a row, D / 64 channels a lane.
+template <int D>
+__global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const int t = a.t0 + (int)(row % a.t_len);
+  const long long bh = row / a.t_len;
+  const int hq = (int)(bh % a.n_q_heads), b = (int)(bh / a.n_q_heads);
+  float M = -INFINITY;
+  for (int s = lane; s < a.n_splits; s += 64) M = fmaxf(M, a.part_ml[2 * (s * a.rows + row)]);
+  M = wave_reduce<true>(M);
+  float acc[E], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s0 = 0; s0 < a.n_splits; s0 += 64) {
+    const bool in = s0 + lane < a.n_splits;
+    const long long at = 2 * ((s0 + lane) * a.rows + row);
+    const float ml = in ? a.part_ml[at] : -INFINITY;
+    const float f = ml == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(ml - M));
+    l += in ? a.part_ml[at + 1] * f : 0.f;
+    const int n = min(64, a.n_splits - s0);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float g = __shfl(f, s, 64);
+      const float* src = a.part_acc + ((s0 + s) * a.rows + row) * D + E * lane;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e], g, acc[e]);
+    }
+  }
+  l = wave_reduce<false>(l);
+  const int n = min(a.seq_lens[b], a.max_len);
+  const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+  const bool any = t < m && n - m + t >= 0 && l != 0.f;  // (listed groups may leave a query nothing)
+  const long long o = b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2] + E * lane;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float y = any ? acc[e] / l : 0.f;
+    if (a.out_type == 0) static_cast<float*>(a.out)[o + e] = y;
+    else static_cast<_Float16*>(a.out)[o + e] = (_Float16)y;
+  }
+  if (a.row_ml && lane == 0) {
+    a.row_ml[2 * row] = M;
+    a.row_ml[2 * row + 1] = l;
+  }
+}
+
+struct WeightArgs {
+  tqk_cache_desc d;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;
+  const float* block_ml;  // [row][blocks][2]
+  const float* row_ml;    // [row][2]
+  float* weights;         // [sequence][kv head][max_groups_per_seq]
+  int q_len, max_len, window, sinks, t0, t_len, blocks, nblk;
+};
+
+// weights += what the launch's queries gave every group.  A thread a block of 32
+// tokens (blockIdx.x: whole groups of them), rows one after another.
+__global__ __launch_bounds__(256) void tqk_group_weights(WeightArgs a) {
+  const tqk_cache_desc& d = a.d;
+  const int G = d.group_tokens, Hkv = d.n_kv_heads, gq = d.n_q_heads / Hkv;
+  const int h = blockIdx.y % Hkv, b = blockIdx.y / Hkv, tid = threadIdx.x;
+  const int per = 256 / a.nblk;  // groups of a workgroup
+  const int n = min(a.seq_lens[b], a.max_len), ng = n_groups_of(n, d.hot_window, G);
+  const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+  const int g = blockIdx.x * per + tid / a.nblk, k = tid % a.nblk;
+  const int first = g * G + 32 * k, last = first + min(32, G - 32 * k) - 1;
+  const bool mine = tid < per * a.nblk && g < ng;
+  const int t_end = min(m, a.t0 + a.t_len), sinks = min(a.sinks, max(n, 0));
+  double sum = 0.0;
+  for (int i = 0; i < gq; ++i) {
+    const long long row0 = ((long long)b * d.n_q_heads + h * gq + i) * a.t_len - a.t0;
+    for (int t = max(a.t0, m - n); t < t_end; ++t) {
+      const int p = n - m + t, lo = a.window > 0 && a.window <= p ? p - a.window + 1 : 0;
+      // (only blocks that this row sees were visited)
+      if (mine && first <= p && (min(last, p) >= lo || first < sinks)) {
+        const float* x = a.block_ml + ((row0 + t) * a.blocks + g * a.nblk + k) * 2;
+        const float* r = a.row_ml + 2 * (row0 + t);
+        const float l = x[1];
+        if (l != 0.f) sum += (double)(__builtin_amdgcn_exp2f(x[0] - r[0]) * l / r[1]);
+      }
+    }
+  }
+  __shared__ double sum_s[256];
+  sum_s[tid] = sum;
+  __syncthreads();
+  if (mine && k == 0) {
+    double y = 0.0;
+    for (int i = 0; i < a.nblk; ++i) y += sum_s[tid + i];
+    float* const w = a.weights + ((long long)b * Hkv + h) * d.max_groups_per_seq + g;
+    *w = (float)((double)*w + y);
+  }
+}
+
+template <int D, int VB, bool TILED>
+void launch_keys(const MoreArgs& a, dim3 grid, hipStream_t st) {
+  if (a.d.key_grid == 2)
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, VB, true, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
+  else if (a.d.key_bits == 4)
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 4, false, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
+  else if (a.d.key_bits == 3)
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 3, false, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 2, false, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
+}
+template <int D, bool TILED>
+void launch_values(const MoreArgs& a, dim3 grid, hipStream_t st) {
+  if (a.d.value_bits == 2)
+    launch_keys<D, 2, TILED>(a, grid, st);
+  else if (a.d.value_bits == 3)
+    launch_keys<D, 3, TILED>(a, grid, st);
+  else
+    launch_keys<D, 4, TILED>(a, grid, st);
+}
+void launch_more(const MoreArgs& a, long long groups, hipStream_t st) {
+  const dim3 grid((unsigned)groups);
+  if (a.d.head_dim == 64)
+    launch_values<64, false>(a, grid, st);
+  else if (a.d.head_dim == 256)
+    launch_values<256, false>(a, grid, st);
+  else if (v_tiled(a.d.group_tokens, a.d.page_tokens, TQK_D, 0))
+    launch_values<TQK_D, true>(a, grid, st);
+  else
+    launch_values<TQK_D, false>(a, grid, st);
+}
+
+void launch_join(const JoinMoreArgs& a, int D, hipStream_t st) {
+  const dim3 grid((unsigned)((a.rows + 3) / 4));
+  if (D == 64)
+    hipLaunchKernelGGL(tqk_join_more<64>, grid, dim3(256), 0, st, a);
+  else if (D == TQK_D)
+    hipLaunchKernelGGL(tqk_join_more<TQK_D>, grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(tqk_join_more<256>, grid, dim3(256), 0, st, a);
+}
+
+size_t partial_bytes(long long rows, int splits, int D) { return (size_t)splits * rows * (D + 2) * sizeof(float) + 256; }
+
+// Queries, kv heads and sequences of a launch, and its splits.
+struct MorePlan {
+  int per_item, q_items, n_splits;
+  long long pairs;  // workgroups of a split
+};
+MorePlan more_plan(const tqk_cache_desc* d, long long batch, int queries, int most_per_item, long long tokens, double join) {
+  MorePlan mp{};
+  const int gq = d->n_q_heads / d->n_kv_heads;
+  mp.per_item = kFewRows / gq < queries ? kFewRows / gq : queries;
+  if (mp.per_item > most_per_item) mp.per_item = most_per_item;
+  mp.q_items = (queries + mp.per_item - 1) / mp.per_item;
+  mp.pairs = batch * mp.q_items * d->n_kv_heads;
+  mp.n_splits = few_splits(mp.pairs, (tokens + 31) / 32 + 1, join);
+  return mp;
+}
+
+// Tokens that one workgroup's rows see at most of a window.
+long long window_tokens(const tqk_attend_desc* t, int per_item) {
+  if (t->window > 0 && t->window < t->max_len) {
+    const long long w = (long long)t->window + per_item + t->sinks + 64;
+    if (w < t->max_len) return w;
+  }
+  return t->max_len;
+}
+
+MoreArgs more_args(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
+                   const int32_t* seq_lens, const int32_t* q_lens, void* out) {
+  MoreArgs a{};
+  a.d = *d;
+  a.p = *p;
+  a.q = static_cast<const uint16_t*>(q);
+  a.seq_lens = seq_lens;
+  a.q_lens = q_lens;
+  a.out = out;
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = t->q_stride[i];
+    a.o_stride[i] = t->o_stride[i];
+  }
+  a.q_len = t->q_len;
+  a.max_len = t->max_len;
+  a.window = t->window;
+  a.sinks = t->sinks;
+  a.out_type = t->out_type;
+  a.batch = t->batch;
+  a.t_len = t->q_len;
+  return a;
+}
+
+JoinMoreArgs join_args(const MoreArgs& a, int splits, float* row_ml) {
+  JoinMoreArgs j{};
+  j.part_acc = a.part_acc;
+  j.part_ml = a.part_ml;
+  j.seq_lens = a.seq_lens;
+  j.q_lens = a.q_lens;
+  j.out = a.out;
+  j.row_ml = row_ml;
+  j.rows = a.rows;
+  for (int i = 0; i < 3; ++i) j.o_stride[i] = a.o_stride[i];
+  j.n_splits = splits;
+  j.n_q_heads = a.d.n_q_heads;
+  j.q_len = a.q_len;
+  j.max_len = a.max_len;
+  j.out_type = a.out_type;
+  j.t0 = a.t0;
+  j.t_len = a.t_len;
+  return j;
+}
+
+int checked(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
+            const int32_t* seq_lens, const void* out, const void* workspace) {
+  if (!p || !q || !seq_lens || !out || (((uintptr_t)q | (uintptr_t)out) & 15) || !tqk_have_buffers(*d, *p)) return TQK_EINVAL;
+  if (!workspace || ((uintptr_t)workspace & 15)) return TQK_EWORKSPACE;
+  return TQK_OK;
+}
+int check_more(const tqk_cache_desc* d, const tqk_attend_desc* t, bool windowed) {
+  const int rc = tqk_check_attend(d, t);
+  if (rc != TQK_OK) return rc;
+  if (d->input_f32) return TQK_EUNSUPPORTED;
+  if (!windowed && (t->window || t->sinks)) return TQK_EINVAL;
+  if ((long long)t->batch * d->n_q_heads * t->q_len > INT32_MAX / 2) return TQK_EINVAL;
+  return TQK_OK;
+}
+constexpr long long kMostGroups = 1LL << 22;  // (512 threads each: fewer than 2^32)
+
+// ---- listed groups ----------------------------------------------------------
+int check_list(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
+  const int rc = check_more(d, t, false);
+  if (rc != TQK_OK) return rc;
+  if (!l || l->n < 0 || l->n > (1 << 24)) return TQK_EINVAL;
+  return TQK_OK;
+}
+MorePlan list_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
+  const int G = d->group_tokens, nblk = (G + 31) / 32;
+  const long long groups = n_groups_of(t->max_len, d->hot_window, G);
+  const long long listed = l->n < groups ? l->n : groups;  // (more: of one twice)
+  const long long hot = t->max_len < d->hot_window ? t->max_len : d->hot_window;
+  return more_plan(d, t->batch, t->q_len, l->stride[2] ? 1 : INT32_MAX, 32 * listed * nblk + hot, 2.0);
+}
+
+// ---- weights ----------------------------------------------------------------
+struct WeightPlan {
+  int t_len;   // queries of a slice
+  int blocks;  // blocks of a row
+  MorePlan mp;
+};
+WeightPlan weight_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+  WeightPlan w{};
+  const int G = d->group_tokens, nblk = (G + 31) / 32, ng = n_groups_of(t->max_len, d->hot_window, G);
+  w.blocks = ng * nblk;
+  const long long one = (long long)t->batch * d->n_q_heads * w.blocks * 8;  // bytes of a query
+  long long fit = one ? kMostBlockBytes / one : t->q_len;
+  fit = fit < 1 ? 1 : fit;
+  w.t_len = fit < t->q_len ? (int)fit : t->q_len;
+  // (whole workgroups where a slice ends)
+  const int gq = d->n_q_heads / d->n_kv_heads, per = kFewRows / gq;
+  if (w.t_len < t->q_len && w.t_len > per) w.t_len = w.t_len / per * per;
+  w.mp = more_plan(d, t->batch, w.t_len, INT32_MAX, window_tokens(t, per), 0.0);
+  return w;
+}
+size_t weight_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const WeightPlan& w) {
+  const long long rows = (long long)t->batch * d->n_q_heads * w.t_len;
+  return partial_bytes(rows, w.mp.n_splits, d->head_dim) + (size_t)rows * 8 + (size_t)rows * w.blocks * 8;
+}
+
+// ---- a shared prefix ---------------------------------------------------------
+struct SharedPlan {
+  MorePlan pre, rest;
+};
+SharedPlan shared_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, int groups) {
+  SharedPlan s{};
+  const int gq = d->n_q_heads / d->n_kv_heads, tokens = groups * d->group_tokens;
+  s.pre.per_item = 1;
+  s.pre.q_items = (int)(((long long)t->batch * t->q_len * gq + kFewRows - 1) / kFewRows);
+  s.pre.pairs = (long long)s.pre.q_items * d->n_kv_heads;
+  s.pre.n_splits = few_splits(s.pre.pairs, (long long)groups * ((d->group_tokens + 31) / 32), 0.0);
+  s.rest = more_plan(d, t->batch, t->q_len, INT32_MAX, t->max_len - tokens, 0.0);
+  return s;
+}
+int check_shared(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
+  const int rc = check_more(d, t, false);
+  if (rc != TQK_OK) return rc;
+  if (groups < 1 || groups > n_groups_of(t->max_len, d->hot_window, d->group_tokens)) return TQK_EINVAL;
+  return TQK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tqk_attend_groups_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
+  if (check_list(d, t, l) != TQK_OK || !t->batch || !t->q_len) return 0;
+  const MorePlan mp = list_plan(d, t, l);
+  return mp.n_splits > 1 ? partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, mp.n_splits, d->head_dim) : 16;
+}
+
+int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t,
+                      const tqk_group_list* l, const void* q, const int32_t* seq_lens, const int32_t* q_lens,
+                      const int32_t* groups, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_list(d, t, l);
+  if (rc != TQK_OK) return rc;
+  if (!t->batch || !t->q_len) return TQK_OK;
+  rc = checked(d, p, t, q, seq_lens, out, workspace);
+  if (rc != TQK_OK) return rc;
+  if (l->n > 0 && !groups) return TQK_EINVAL;
+  if (workspace_bytes < tqk_attend_groups_workspace_bytes(d, t, l)) return TQK_EWORKSPACE;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const MorePlan mp = list_plan(d, t, l);
+  if (mp.pairs * mp.n_splits > kMostGroups) return TQK_EINVAL;
+  MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
+  // (a list of none: any pointer, which is not read)
+  a.groups = groups ? groups : reinterpret_cast<const int32_t*>(seq_lens);
+  for (int i = 0; i < 3; ++i) a.g_stride[i] = l->stride[i];
+  a.n_list = l->n;
+  a.per_item = mp.per_item;
+  a.q_items = mp.q_items;
+  a.n_splits = mp.n_splits;
+  a.direct = mp.n_splits == 1;
+  a.rows = (long long)t->batch * d->n_q_heads * t->q_len;
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = a.part_acc + (size_t)mp.n_splits * a.rows * d->head_dim;
+  launch_more(a, mp.pairs * mp.n_splits, st);
+  if (!a.direct) launch_join(join_args(a, mp.n_splits, nullptr), d->head_dim, st);
+  return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+}
+
+size_t tqk_attend_weights_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+  if (check_more(d, t, true) != TQK_OK || !t->batch || !t->q_len) return 0;
+  return weight_bytes(d, t, weight_plan(d, t));
+}
+
+int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
+                       const int32_t* seq_lens, const int32_t* q_lens, void* out, float* weights, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  int rc = check_more(d, t, true);
+  if (rc != TQK_OK) return rc;
+  if (!t->batch || !t->q_len) return TQK_OK;
+  rc = checked(d, p, t, q, seq_lens, out, workspace);
+  if (rc != TQK_OK) return rc;
+  if (!weights || (long long)t->batch * d->n_kv_heads > 65535) return TQK_EINVAL;
+  const WeightPlan w = weight_plan(d, t);
+  if (workspace_bytes < weight_bytes(d, t, w)) return TQK_EWORKSPACE;
+  if (w.mp.pairs * w.mp.n_splits > kMostGroups) return TQK_EINVAL;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int nblk = (d->group_tokens + 31) / 32, per = 256 / nblk, ng = w.blocks / nblk;
+  MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
+  a.per_item = w.mp.per_item;
+  a.n_splits = w.mp.n_splits;
+  a.blocks = w.blocks;
+  a.part_acc = static_cast<float*>(workspace);
+  for (a.t0 = 0; a.t0 < t->q_len; a.t0 += w.t_len) {
+    a.t_len = t->q_len - a.t0 < w.t_len ? t->q_len - a.t0 : w.t_len;
+    a.q_items = (a.t_len + a.per_item - 1) / a.per_item;
+    a.rows = (long long)t->batch * d->n_q_heads * a.t_len;
+    a.part_ml = a.part_acc + (size_t)a.n_splits * a.rows * d->head_dim;
+    float* const row_ml = a.part_ml + (size_t)a.n_splits * a.rows * 2;
+    a.block_ml = row_ml + (size_t)a.rows * 2;
+    launch_more(a, (long long)t->batch * a.q_items * d->n_kv_heads * a.n_splits, st);
+    launch_join(join_args(a, a.n_splits, row_ml), d->head_dim, st);
+    if (ng > 0) {
+      WeightArgs g{};
+      g.d = *d;
+      g.seq_lens = seq_lens;
+      g.q_lens = q_lens;
+      g.block_ml = a.block_ml;
+      g.row_ml = row_ml;
+      g.weights = weights;
+      g.q_len = t->q_len;
+      g.max_len = t->max_len;
+      g.window = t->window;
+      g.sinks = t->sinks;
+      g.t0 = a.t0;
+      g.t_len = a.t_len;
+      g.blocks = w.blocks;
+      g.nblk = nblk;
+      hipLaunchKernelGGL(tqk_group_weights, dim3((unsigned)((ng + per - 1) / per), (unsigned)(t->batch * d->n_kv_heads)),
+                         dim3(256), 0, st, g);
+    }
+    if (hipGetLastError() != hipSuccess) return TQK_EHIP;
+  }
+  return TQK_OK;
+}
+
+size_t tqk_attend_shared_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
+  if (check_shared(d, t, groups) != TQK_OK || !t->batch || !t->q_len) return 0;
+  const SharedPlan s = shared_plan(d, t, groups);
+  return partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, s.pre.n_splits + s.rest.n_splits, d->head_dim);
+}
+
+int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, int32_t groups,
+                      const void* q, const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  int rc = check_shared(d, t, groups);
+  if (rc != TQK_OK) return rc;
+  if (!t->batch || !t->q_len) return TQK_OK;
+  rc = checked(d, p, t, q, seq_lens, out, workspace);
+  if (rc != TQK_OK) return rc;
+  if (workspace_bytes < tqk_attend_shared_workspace_bytes(d, t, groups)) return TQK_EWORKSPACE;
+  const SharedPlan s = shared_plan(d, t, groups);
+  if (s.pre.pairs * s.pre.n_splits > kMostGroups || s.rest.pairs * s.rest.n_splits > kMostGroups) return TQK_EINVAL;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int splits = s.pre.n_splits + s.rest.n_splits;
+  MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
+  a.rows = (long long)t->batch * d->n_q_heads * t->q_len;
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = a.part_acc + (size_t)splits * a.rows * d->head_dim;
+  a.per_item = 1;
+  a.q_items = s.pre.q_items;
+  a.n_splits = s.pre.n_splits;
+  a.shared = groups * d->group_tokens;
+  launch_more(a, s.pre.pairs * s.pre.n_splits, st);
+  a.skip = a.shared;
+  a.shared = 0;
+  a.split0 = s.pre.n_splits;
+  a.per_item = s.rest.per_item;
+  a.q_items = s.rest.q_items;
+  a.n_splits = s.rest.n_splits;
+  launch_more(a, s.rest.pairs * s.rest.n_splits, st);
+  launch_join(join_args(a, splits, nullptr), d->head_dim, st);
+  return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+}
+
+}  // extern "C"

@@ -32,6 +32,8 @@ PER_UNIT = {
     "tqk_decode.hip": [],
     "tqk_attend.hip": [],
     "tqk_attend_codes.hip": [],
+    "tqk_attend_more.hip": [],
+    "tqk_groups.hip": [],
     "tqk_rope.hip": [],
     "tqk_attn.hip": [],
 }

@@ -30,7 +30,10 @@ EXPORTS = (
     "tqk_decode_noalloc", "tqk_decode_partials", "tqk_decode_splits", "tqk_decode_merge", "tqk_encode_groups",
     "tqk_append_hot", "tqk_append_tokens", "tqk_dequant_groups", "tqk_dequant_dense", "tqk_encode_key_block", "tqk_encode_value_block",
     "tqk_dequant_key_block", "tqk_dequant_value_block", "tqk_norm_rope", "tqk_attention_workspace_bytes",
-    "tqk_attention", "tqk_attend_workspace_bytes", "tqk_attend",
+    "tqk_attention", "tqk_attend_workspace_bytes", "tqk_attend", "tqk_attend_groups_workspace_bytes",
+    "tqk_attend_groups", "tqk_attend_weights_workspace_bytes", "tqk_attend_weights",
+    "tqk_attend_shared_workspace_bytes", "tqk_attend_shared", "tqk_select_groups_workspace_bytes",
+    "tqk_select_groups", "tqk_evict_groups_workspace_bytes", "tqk_evict_groups",
 )
 
 
@@ -80,6 +83,17 @@ class AttendDesc(ctypes.Structure):
         (n, ctypes.c_int64 * 3) for n in ("q_stride", "o_stride")]
 
 
+class GroupList(ctypes.Structure):
+    """``tqk_group_list``: the coded groups that every query sees."""
+    _fields_ = [("n", ctypes.c_int32), ("stride", ctypes.c_int64 * 3)]
+
+
+class SelectDesc(ctypes.Structure):
+    """``tqk_select_desc``: the choice of groups by their scales and zero points."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "q_len", "max_len", "top", "first", "last")] + [
+        ("spread", ctypes.c_float), ("q_stride", ctypes.c_int64 * 3)]
+
+
 _lib = None
 
 
@@ -90,6 +104,7 @@ def load(path: str) -> ctypes.CDLL:
     vp, i32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
     pd, pp, pb = ctypes.POINTER(CacheDesc), ctypes.POINTER(CachePtrs), ctypes.POINTER(BlockDesc)
     pr, pa, pt = ctypes.POINTER(RopeDesc), ctypes.POINTER(AttnDesc), ctypes.POINTER(AttendDesc)
+    pl, ps = ctypes.POINTER(GroupList), ctypes.POINTER(SelectDesc)
     sig = {
         "tqk_version": ([], ctypes.c_int),
         "tqk_check_desc": ([pd], ctypes.c_int),
@@ -113,6 +128,16 @@ def load(path: str) -> ctypes.CDLL:
         "tqk_attend_workspace_bytes": ([pd, pt], sz),
         "tqk_attend": ([pd, pp, pt, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
         "tqk_attention": ([pa, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
+        "tqk_attend_groups_workspace_bytes": ([pd, pt, pl], sz),
+        "tqk_attend_groups": ([pd, pp, pt, pl, vp, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
+        "tqk_attend_weights_workspace_bytes": ([pd, pt], sz),
+        "tqk_attend_weights": ([pd, pp, pt, vp, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
+        "tqk_attend_shared_workspace_bytes": ([pd, pt, i32], sz),
+        "tqk_attend_shared": ([pd, pp, pt, i32, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
+        "tqk_select_groups_workspace_bytes": ([pd, ps], sz),
+        "tqk_select_groups": ([pd, pp, ps, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
+        "tqk_evict_groups_workspace_bytes": ([pd, i32], sz),
+        "tqk_evict_groups": ([pd, pp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(l_, name)

@@ -39,6 +39,11 @@ ZERO_POINTS = {"calibrated": 0, "sparse": 1, "bias": 2, "symmetric": 1}
 KEY_GRIDS = {"nf4_asym": 0, "uniform": 1, "polar": 2}
 
 
+# rows of a sequence (queries times query heads of a kv head) up to which a step reads
+# a shared prefix once for all
+SHARED_ROWS = 128
+
+
 def _torch():
     import torch
     return torch
@@ -186,6 +191,12 @@ class TQKVPool:
         # call that reads the cache raises it, not only the first
         self._error = None
         self._ws = None
+        # coded groups that all sequences share (share_prefix); tokens that left
+        # every sequence (evict), and on the device; the tables as they were made
+        self._shared = 0
+        self._evicted = [0] * max_batch
+        self._evicted_dev = None
+        self._made_tables = None
 
     # ------------------------------------------------------------------ #
     @staticmethod
@@ -220,6 +231,12 @@ class TQKVPool:
         self._error = None
         self.lengths = [0] * self.max_batch
         self.seq_lens.zero_()
+        self._shared = 0
+        self._evicted, self._evicted_dev = [0] * self.max_batch, None
+        if self._made_tables is not None:
+            self.block_table.copy_(self._made_tables[0])
+            self.group_table.copy_(self._made_tables[1])
+            self._made_tables = None
 
     def check(self, wait: bool = True) -> None:
         """Raise the first error an earlier append's encode flagged (a value
@@ -289,6 +306,7 @@ class TQKVPool:
         new.hot_k.copy_(self.hot_k)
         new.hot_v.copy_(self.hot_v)
         new.lengths = list(self.lengths)
+        new._evicted = list(self._evicted)
         new.seq_lens.copy_(self.seq_lens)
         torch.cuda.synchronize(dev)
         return new
@@ -419,7 +437,8 @@ class TQKVPool:
                 "tqk_decode_partials")
         return m, l_, acc
 
-    def attend(self, q, *, window: int | None = None, sinks: int = 0, q_lens=None, out=None):
+    def attend(self, q, *, window: int | None = None, sinks: int = 0, q_lens=None, out=None, groups=None,
+               weights=None):
         """Attention of every sequence's last queries over its cache, with a
         sliding window and first tokens that stay visible.
 
@@ -431,6 +450,20 @@ class TQKVPool:
         j <= p with ``j > p - window`` (every one with None) or ``j < sinks``.
         Only the coded groups that a query sees are read.
 
+        ``groups`` (int32 ``(B, Hkv, T, K)`` on the device, or ``(B, Hkv, 1, K)``:
+        one list for all queries; :meth:`select_groups` makes them) instead of a
+        window: query t sees the tokens j <= p of the listed coded groups and the
+        uncoded ones.  Entries that are no group of the sequence (-1) are none; a group
+        listed twice counts twice.
+
+        ``weights`` (fp32 ``(B, Hkv, max_groups)``, contiguous) is added to: the
+        softmax weights of every coded group's tokens, summed over the queries and
+        the kv head's query heads (what :meth:`evict` goes by).  Both of them fp16
+        pools, over the codes however many queries.
+
+        After :meth:`share_prefix`, steps of few queries without a window read the
+        shared groups once for all sequences.
+
         Returns ``(B, Hq, T, D)`` in the queries' type (``out`` where given,
         its rows apart, else laid out ``(B, T, Hq, D)``); rows ``t >= m`` and queries before
         the first token get zeros."""
@@ -440,13 +473,15 @@ class TQKVPool:
             raise ValueError(f"attend expects {self.input_dtype} q of shape ({B}, {Hq}, T, {D}), got {q.dtype} "
                              f"{tuple(q.shape)}")
         T = int(q.shape[2])
-        if needs_grad(q, out):
+        if needs_grad(q, out, weights):
             raise NotImplementedError("attend has no backward pass: call it under torch.no_grad()")
         window, sinks = window_args(window, sinks)
         q_lens = lengths_arg(q_lens, B, "q_lens")
         if out is not None:
             check_out(out, q)
-        for name, x in (("q", q), ("q_lens", q_lens), ("out", out)):
+        if groups is not None or weights is not None:
+            groups = self._check_more(q, T, window, sinks, groups, weights)
+        for name, x in (("q", q), ("q_lens", q_lens), ("out", out), ("groups", groups), ("weights", weights)):
             if x is not None and x.device != self.kcodes.device:
                 raise ValueError(f"attend: {name} is on {x.device}, the pool on {self.kcodes.device}")
         self.check()
@@ -458,14 +493,189 @@ class TQKVPool:
         t = N.AttendDesc(B, T, max(self.lengths), window, sinks, 0 if self.f32 else 1)
         t.q_stride[:], t.o_stride[:] = strides_of(q), strides_of(out)
         lib = N.lib()
+        d, p, td = ctypes.byref(self.desc), ctypes.byref(self.ptrs), ctypes.byref(t)
+        args = (q.data_ptr(), self.seq_lens.data_ptr(), None if q_lens is None else q_lens.data_ptr())
+        if groups is not None:
+            lists = N.GroupList(groups.shape[3])
+            lists.stride[:] = [s if n > 1 else 0 for n, s in zip(groups.shape[:3], groups.stride()[:3])]
+            what, extra, args = "tqk_attend_groups", (ctypes.byref(lists),), args + (groups.data_ptr(), out.data_ptr())
+        elif weights is not None:
+            what, extra, args = "tqk_attend_weights", (), args + (out.data_ptr(), weights.data_ptr())
+        elif self._shared_step(T, t.window, t.max_len):
+            what, extra, args = "tqk_attend_shared", (self._shared,), args + (out.data_ptr(),)
+            t.window = t.sinks = 0
+        else:
+            what, extra, args = "tqk_attend", (), args + (out.data_ptr(),)
         with on_device(q.device):
-            need = lib.tqk_attend_workspace_bytes(ctypes.byref(self.desc), ctypes.byref(t))
+            need = getattr(lib, what + "_workspace_bytes")(d, td, *extra)
             # (a call's own: calls on several streams and captured graphs share nothing)
             ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=q.device)
-            N.check(lib.tqk_attend(ctypes.byref(self.desc), ctypes.byref(self.ptrs), ctypes.byref(t), q.data_ptr(),
-                                   self.seq_lens.data_ptr(), None if q_lens is None else q_lens.data_ptr(),
-                                   out.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(q.device)), "tqk_attend")
+            N.check(getattr(lib, what)(d, p, td, *extra, *args, ws.data_ptr(), ws.numel(), stream_of(q.device)), what)
         return out
+
+    def _check_more(self, q, T, window, sinks, groups, weights):
+        """``attend`` with groups or weights: the groups with entries side by side."""
+        torch = _torch()
+        B, H = self.max_batch, self.n_kv_heads
+        if self.f32:
+            raise NotImplementedError("attend: groups and weights take fp16 pools")
+        if groups is not None:
+            if weights is not None or window or sinks:
+                raise ValueError("attend: groups go without a window, sinks and weights")
+            if groups.dim() != 4 or tuple(groups.shape[:2]) != (B, H) or groups.shape[2] not in (1, T) or \
+                    groups.dtype != torch.int32:
+                raise ValueError(f"groups are int32 ({B}, {H}, {T}, K) or ({B}, {H}, 1, K), not {groups.dtype} "
+                                 f"{tuple(groups.shape)}")
+            if groups.shape[3] > 1 and groups.stride(3) != 1:
+                groups = groups.contiguous()
+        elif tuple(weights.shape) != (B, H, self.max_groups) or weights.dtype != torch.float32 or \
+                not weights.is_contiguous():
+            raise ValueError(f"weights are contiguous fp32 ({B}, {H}, {self.max_groups}), not {weights.dtype} "
+                             f"{tuple(weights.shape)}")
+        return groups
+
+    def _shared_step(self, T, window, max_len):
+        """Whether a step of T queries reads a shared prefix once for all sequences:
+        every query stands behind it and sees it whole, and the rows are as few as
+        go over the codes."""
+        return (self._shared > 0 and not self.f32 and (window == 0 or window >= max_len)
+                and T * (self.n_q_heads // self.n_kv_heads) <= SHARED_ROWS
+                and min(self.lengths) - T >= self._shared * self.group_tokens - 1)
+
+    def select_groups(self, q, top: int, *, first: int = 1, last: int = 1, spread: float = 1.0, q_lens=None):
+        """The coded groups that every query attends, for ``attend(groups=...)``:
+        int32 ``(B, Hkv, T, top)``, ascending, then -1.
+
+        ``q`` and ``q_lens`` as for :meth:`attend`.  Of the groups that begin at or
+        before a query the ``first`` and ``last`` ones are always chosen, and those with
+        the largest ``max over the kv head's query heads of sum_i q_i mid_i + spread
+        |q_i| half_i``, ``mid +- half`` the ends of channel i's key levels in the group
+        (a side-list's values may lie outside).  ``spread=1``: a bound on the products
+        with its keys; 0: the product with the levels' centre.  Only the groups' scales
+        and zero points are read; 64 bits, equal scores by the lower index, a score
+        that is no number above all.  fp16 pools with per-channel keys."""
+        torch = _torch()
+        B, Hq, D = self.max_batch, self.n_q_heads, self.head_dim
+        if self.f32 or self.key_grid == "polar":
+            raise NotImplementedError("select_groups takes fp16 pools with per-channel keys")
+        if q.dim() != 4 or tuple(q.shape[:2]) != (B, Hq) or q.shape[3] != D or q.dtype != self.dtype:
+            raise ValueError(f"select_groups expects {self.input_dtype} q of shape ({B}, {Hq}, T, {D}), got {q.dtype} "
+                             f"{tuple(q.shape)}")
+        top, first, last, spread = int(top), int(first), int(last), float(spread)
+        if top < 1 or first < 0 or last < 0 or first + last > top or top > 2 ** 24:
+            raise ValueError(f"select_groups chooses at least one group, the first and last ones among them: top {top}, "
+                             f"first {first}, last {last}")
+        if not 0.0 <= spread < math.inf:
+            raise ValueError(f"spread is not negative and finite, not {spread}")
+        q_lens = lengths_arg(q_lens, B, "q_lens")
+        for name, x in (("q", q), ("q_lens", q_lens)):
+            if x is not None and x.device != self.kcodes.device:
+                raise ValueError(f"select_groups: {name} is on {x.device}, the pool on {self.kcodes.device}")
+        self.check()
+        q, T = aligned(q.detach()), int(q.shape[2])
+        got = torch.empty((B, self.n_kv_heads, T, top), dtype=torch.int32, device=q.device)
+        if B * T == 0:
+            return got
+        s = N.SelectDesc(B, T, max(self.lengths), top, first, last, spread)
+        s.q_stride[:] = strides_of(q)
+        lib = N.lib()
+        with on_device(q.device):
+            need = lib.tqk_select_groups_workspace_bytes(ctypes.byref(self.desc), ctypes.byref(s))
+            ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=q.device)
+            N.check(lib.tqk_select_groups(ctypes.byref(self.desc), ctypes.byref(self.ptrs), ctypes.byref(s),
+                                          q.data_ptr(), self.seq_lens.data_ptr(),
+                                          None if q_lens is None else q_lens.data_ptr(), got.data_ptr(),
+                                          ws.data_ptr(), ws.numel(), stream_of(q.device)), "tqk_select_groups")
+        return got
+
+    def _keep_tables(self, what):
+        """The tables as they were made, for ``reset``, before a call that changes them."""
+        if _torch().cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} changes the pool's lengths on the host: it is not captured in a HIP graph")
+        if self._made_tables is None:
+            self._made_tables = (self.block_table.clone(), self.group_table.clone())
+
+    def evict(self, weights, keep: int, *, first: int = 1, last: int = 1):
+        """Coded groups leave the cache: of every sequence with more than ``keep`` of
+        them the ``first``, the ``last`` and those of the largest weight stay.
+
+        ``weights`` (fp32 ``(B, Hkv, max_groups)``, as ``attend(weights=...)`` adds it
+        up): a group's is its sum over the heads, in 64 bits; equal ones by the lower
+        index, a sum that is no number above all.  The weights move along with their
+        groups, the rest become zero.  No code moves: the sequences' table rows are
+        reordered, their lengths shortened and their rings turned; the freed pages take
+        the sequence's next groups.  A shared prefix stays whole.
+
+        Keys keep the rotation of the positions that they had; :meth:`append_qkv` goes
+        on counting from there, other callers add ``evicted_tokens``.  Returns the former
+        indices of the groups that stay, int32 ``(B, keep)``, ascending, then -1."""
+        torch = _torch()
+        B, keep, first, last = self.max_batch, int(keep), int(first), int(last)
+        if self.zero_point == "bias":
+            raise NotImplementedError('evict: the zero points of zero_point="bias" belong to the groups\' positions')
+        if first < 0 or last < 0:
+            raise ValueError("evict: first and last are not negative")
+        first = max(first, self._shared)
+        if keep < first + last:
+            raise ValueError(f"evict keeps the first {first} and the last {last} groups: keep is at least that, not {keep}")
+        if tuple(weights.shape) != (B, self.n_kv_heads, self.max_groups) or weights.dtype != torch.float32 or \
+                not weights.is_contiguous():
+            raise ValueError(f"weights are contiguous fp32 ({B}, {self.n_kv_heads}, {self.max_groups}), not "
+                             f"{weights.dtype} {tuple(weights.shape)}")
+        if weights.device != self.kcodes.device:
+            raise ValueError(f"evict: weights are on {weights.device}, the pool on {self.kcodes.device}")
+        if needs_grad(weights):
+            raise NotImplementedError("evict has no backward pass: call it under torch.no_grad()")
+        self.check()
+        self._keep_tables("evict")
+        kept = torch.empty((B, keep), dtype=torch.int32, device=weights.device)
+        gone = [max(0, self.n_groups(b) - keep) * self.group_tokens for b in range(B)]
+        lib = N.lib()
+        with on_device(weights.device):
+            need = lib.tqk_evict_groups_workspace_bytes(ctypes.byref(self.desc), B)
+            ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=weights.device)
+            N.check(lib.tqk_evict_groups(ctypes.byref(self.desc), ctypes.byref(self.ptrs), B, keep, first, last,
+                                         weights.data_ptr(), self.seq_lens.data_ptr(), self.block_table.data_ptr(),
+                                         self.group_table.data_ptr(), kept.data_ptr(), ws.data_ptr(), ws.numel(),
+                                         stream_of(weights.device)), "tqk_evict_groups")
+        if any(gone):
+            self.lengths = [n - x for n, x in zip(self.lengths, gone)]
+            self._evicted = [n + x for n, x in zip(self._evicted, gone)]
+            self._evicted_dev = None
+        return kept
+
+    @property
+    def evicted_tokens(self) -> list:
+        """Tokens that :meth:`evict` took from every sequence: the next token's position
+        is ``lengths[b] + evicted_tokens[b]``."""
+        return list(self._evicted)
+
+    def share_prefix(self, source: int = 0) -> None:
+        """Every other sequence (all of them empty) gets the tokens of ``source``: its
+        coded groups by reference, its uncoded tokens copied.  ``attend`` reads the
+        shared groups once for all sequences; what is appended later is each
+        sequence's own.  They stay shared until :meth:`reset`."""
+        torch = _torch()
+        B, source = self.max_batch, int(source)
+        if not 0 <= source < B:
+            raise ValueError(f"share_prefix: sequence {source} of {B}")
+        if self.lengths[source] <= 0:
+            raise ValueError(f"share_prefix: sequence {source} is empty")
+        if any(n for b, n in enumerate(self.lengths) if b != source):
+            raise ValueError("share_prefix: the other sequences are not empty")
+        self.check()
+        self._keep_tables("share_prefix")
+        groups = self.n_groups(source)
+        pages = groups * self.group_tokens // self.page_tokens
+        with torch.no_grad():
+            self.block_table[:, :pages] = self.block_table[source, :pages].clone()
+            self.group_table[:, :groups] = self.group_table[source, :groups].clone()
+            self.hot_k.copy_(self.hot_k[source].clone())
+            self.hot_v.copy_(self.hot_v[source].clone())
+            self.seq_lens.copy_(self.seq_lens[source].clone())
+        self.lengths = [self.lengths[source]] * B
+        self._evicted, self._evicted_dev = [self._evicted[source]] * B, None
+        self._shared = groups if B > 1 else 0
 
     def append_qkv(self, qkv, inv_freq, *, q_weight=None, k_weight=None, eps: float = 1e-6,
                    weight_offset: float = 0.0, interleaved: bool = False, rope_scale: float = 1.0, positions=None,
@@ -481,8 +691,13 @@ class TQKVPool:
                              f"{self.head_dim}) rows, got {tuple(qkv.shape)}")
         if qkv.device != self.kcodes.device:
             raise ValueError(f"append_qkv: rows are on {qkv.device}, the pool on {self.kcodes.device}")
-        q, k, v = norm_rope(qkv, self.n_q_heads, self.n_kv_heads, inv_freq,
-                            self.seq_lens if positions is None else positions, q_weight=q_weight, k_weight=k_weight,
+        if positions is None:
+            positions = self.seq_lens
+            if any(self._evicted):  # (positions count what left the cache)
+                if self._evicted_dev is None:
+                    self._evicted_dev = _torch().tensor(self._evicted, dtype=_torch().int32).to(self.kcodes.device)
+                positions = positions + self._evicted_dev
+        q, k, v = norm_rope(qkv, self.n_q_heads, self.n_kv_heads, inv_freq, positions, q_weight=q_weight, k_weight=k_weight,
                             eps=eps, weight_offset=weight_offset, interleaved=interleaved, rope_scale=rope_scale,
                             dtype=self.dtype)
         self.append(k, v, n_new=n_new)
@@ -618,6 +833,8 @@ class TQKVPool:
         tiled pool stores them in its MFMA-tiled order."""
         torch = _torch()
         H, G, D = self.n_kv_heads, self.group_tokens, self.head_dim
+        if g < self._shared:
+            raise ValueError(f"group {g} is shared by all sequences (share_prefix)")
         phys, off = self._rows(b, g)
         slot = int(self.group_table[b, g])
         if keys is not None and self.key_grid == "polar":
