@@ -35,13 +35,6 @@
 #include "tqk_attend.h"
 #include "tqk_wave.h"
 
-namespace {
-
-typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves, kFewRows = 16;
-constexpr int kNoToken = 1 << 30;  // past every token (max_len is at most that)
-constexpr float kFewLazy = 2.0f;  // log2 units: weights stay at most 4, norms at most TQK_MAX_VNORM: fp16
-
 struct FewArgs {
   tqk_cache_desc d;
   tqk_cache_ptrs p;
@@ -77,6 +70,13 @@ struct MoreArgs : FewArgs {
   float* block_ml;   // [row][blocks][2]: maximum and sum of a coded block, or null
   int blocks;        // blocks of a row there
 };
+
+namespace {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves, kFewRows = 16;
+constexpr int kNoToken = 1 << 30;  // past every token (max_len is at most that)
+constexpr float kFewLazy = 2.0f;  // log2 units: weights stay at most 4, norms at most TQK_MAX_VNORM: fp16
 
 // A run of blocks in two pieces, [0, n0) and [from, from + n - n0): the first
 // tokens' and the window's.

@@ -14,6 +14,11 @@
 // its codes, then each sequence's rows over its other tokens; the join takes both.
 #include "tqk_attend_codes_kernels.h"
 
+// up to eight rows of a (sequence, kv head) a workgroup (tqk_attend_rows.h)
+void tqk_launch_rows_64(const MoreArgs& a, unsigned groups, hipStream_t st);
+void tqk_launch_rows_128(const MoreArgs& a, unsigned groups, hipStream_t st);
+void tqk_launch_rows_256(const MoreArgs& a, unsigned groups, hipStream_t st);
+
 namespace {
 
 // Bytes of blocks' maxima and sums at a time: more queries go in slices.
@@ -31,38 +36,77 @@ struct JoinMoreArgs {
   int n_splits, n_q_heads, q_len, max_len, out_type, t0, t_len;
 };
 
-// The partial results of a row joined: one wave a row, D / 64 channels a lane.
-template <int D>
+// The partial results of a row joined: NW waves a row, wave w the splits w, w + NW, ..,
+// eight of them on their way at a time (one after another they are a chain of loads:
+// 23 splits 8.7 us, where four waves take 4), D / 64 channels a lane.
+template <int D, int NW>
 __global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
+  constexpr int E = D / 64, kAhead = 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % NW;
+  const long long row = (long long)blockIdx.x * (4 / NW) + wave / NW;
+  __shared__ float acc_s[4][D], ml_s[4][2];
+  const bool real = row < a.rows;
+  const long long from = real ? row : 0;
+  float M = -INFINITY, l = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s0 = w; s0 < a.n_splits; s0 += NW * kAhead) {
+    float x[kAhead][E], m_[kAhead], l_[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const long long o = min(s0 + u * NW, a.n_splits - 1) * a.rows + from;
+      m_[u] = a.part_ml[2 * o];
+      l_[u] = a.part_ml[2 * o + 1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[u][e] = a.part_acc[o * D + E * lane + e];
+    }
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) top = fmaxf(top, m_[u]);  // (a repeated last split: none below)
+    const float f0 = M == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(M - top));
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= f0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s0 + u * NW < a.n_splits) {
+        const float f = m_[u] == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(m_[u] - top));
+        l = fmaf(l_[u], f, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(x[u][e], f, acc[e]);
+      }
+    }
+    M = top;
+  }
+  if constexpr (NW > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc_s[wave][E * lane + e] = acc[e];
+    if (lane == 0) {
+      ml_s[wave][0] = M;
+      ml_s[wave][1] = l;
+    }
+    __syncthreads();
+    if (w != 0) return;
+    float top = M;
+#pragma unroll
+    for (int u = 1; u < NW; ++u) top = fmaxf(top, ml_s[wave + u][0]);
+    const float f0 = M == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(M - top));
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= f0;
+#pragma unroll
+    for (int u = 1; u < NW; ++u) {
+      const float mu = ml_s[wave + u][0], f = mu == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(mu - top));
+      l = fmaf(ml_s[wave + u][1], f, l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(acc_s[wave + u][E * lane + e], f, acc[e]);
+    }
+    M = top;
+  }
+  if (!real) return;
   const int t = a.t0 + (int)(row % a.t_len);
   const long long bh = row / a.t_len;
   const int hq = (int)(bh % a.n_q_heads), b = (int)(bh / a.n_q_heads);
-  float M = -INFINITY;
-  for (int s = lane; s < a.n_splits; s += 64) M = fmaxf(M, a.part_ml[2 * (s * a.rows + row)]);
-  M = wave_reduce<true>(M);
-  float acc[E], l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s0 = 0; s0 < a.n_splits; s0 += 64) {
-    const bool in = s0 + lane < a.n_splits;
-    const long long at = 2 * ((s0 + lane) * a.rows + row);
-    const float ml = in ? a.part_ml[at] : -INFINITY;
-    const float f = ml == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(ml - M));
-    l += in ? a.part_ml[at + 1] * f : 0.f;
-    const int n = min(64, a.n_splits - s0);
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float g = __shfl(f, s, 64);
-      const float* src = a.part_acc + ((s0 + s) * a.rows + row) * D + E * lane;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e], g, acc[e]);
-    }
-  }
-  l = wave_reduce<false>(l);
   const int n = min(a.seq_lens[b], a.max_len);
   const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
   const bool any = t < m && n - m + t >= 0 && l != 0.f;  // (listed groups may leave a query nothing)
@@ -159,14 +203,30 @@ void launch_more(const MoreArgs& a, long long groups, hipStream_t st) {
     launch_values<TQK_D, false>(a, grid, st);
 }
 
-void launch_join(const JoinMoreArgs& a, int D, hipStream_t st) {
-  const dim3 grid((unsigned)((a.rows + 3) / 4));
-  if (D == 64)
-    hipLaunchKernelGGL(tqk_join_more<64>, grid, dim3(256), 0, st, a);
-  else if (D == TQK_D)
-    hipLaunchKernelGGL(tqk_join_more<TQK_D>, grid, dim3(256), 0, st, a);
+template <int D>
+void launch_join_rows(const JoinMoreArgs& a, hipStream_t st) {
+  // (few rows: a workgroup each; many, whose waves hide each other's loads, four)
+  if (a.n_splits > 4 && a.rows <= 4096)
+    hipLaunchKernelGGL((tqk_join_more<D, 4>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL(tqk_join_more<256>, grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((tqk_join_more<D, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+}
+void launch_join(const JoinMoreArgs& a, int D, hipStream_t st) {
+  if (D == 64)
+    launch_join_rows<64>(a, st);
+  else if (D == TQK_D)
+    launch_join_rows<TQK_D>(a, st);
+  else
+    launch_join_rows<256>(a, st);
+}
+
+void launch_rows(const MoreArgs& a, long long groups, hipStream_t st) {
+  if (a.d.head_dim == 64)
+    tqk_launch_rows_64(a, (unsigned)groups, st);
+  else if (a.d.head_dim == TQK_D)
+    tqk_launch_rows_128(a, (unsigned)groups, st);
+  else
+    tqk_launch_rows_256(a, (unsigned)groups, st);
 }
 
 size_t partial_bytes(long long rows, int splits, int D) { return (size_t)splits * rows * (D + 2) * sizeof(float) + 256; }
@@ -179,7 +239,7 @@ struct MorePlan {
 MorePlan more_plan(const tqk_cache_desc* d, long long batch, int queries, int most_per_item, long long tokens, double join) {
   MorePlan mp{};
   const int gq = d->n_q_heads / d->n_kv_heads;
-  mp.per_item = kFewRows / gq < queries ? kFewRows / gq : queries;
+  mp.per_item = 8 / gq < queries ? 8 / gq : queries;
   if (mp.per_item > most_per_item) mp.per_item = most_per_item;
   mp.q_items = (queries + mp.per_item - 1) / mp.per_item;
   mp.pairs = batch * mp.q_items * d->n_kv_heads;
@@ -285,7 +345,7 @@ WeightPlan weight_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   fit = fit < 1 ? 1 : fit;
   w.t_len = fit < t->q_len ? (int)fit : t->q_len;
   // (whole workgroups where a slice ends)
-  const int gq = d->n_q_heads / d->n_kv_heads, per = kFewRows / gq;
+  const int gq = d->n_q_heads / d->n_kv_heads, per = 8 / gq;
   if (w.t_len < t->q_len && w.t_len > per) w.t_len = w.t_len / per * per;
   w.mp = more_plan(d, t->batch, w.t_len, INT32_MAX, window_tokens(t, per), 0.0);
   return w;
@@ -351,7 +411,7 @@ int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   a.rows = (long long)t->batch * d->n_q_heads * t->q_len;
   a.part_acc = static_cast<float*>(workspace);
   a.part_ml = a.part_acc + (size_t)mp.n_splits * a.rows * d->head_dim;
-  launch_more(a, mp.pairs * mp.n_splits, st);
+  launch_rows(a, mp.pairs * mp.n_splits, st);
   if (!a.direct) launch_join(join_args(a, mp.n_splits, nullptr), d->head_dim, st);
   return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
 }
@@ -387,7 +447,7 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
     a.part_ml = a.part_acc + (size_t)a.n_splits * a.rows * d->head_dim;
     float* const row_ml = a.part_ml + (size_t)a.n_splits * a.rows * 2;
     a.block_ml = row_ml + (size_t)a.rows * 2;
-    launch_more(a, (long long)t->batch * a.q_items * d->n_kv_heads * a.n_splits, st);
+    launch_rows(a, (long long)t->batch * a.q_items * d->n_kv_heads * a.n_splits, st);
     launch_join(join_args(a, a.n_splits, row_ml), d->head_dim, st);
     if (ng > 0) {
       WeightArgs g{};
@@ -447,7 +507,7 @@ int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   a.per_item = s.rest.per_item;
   a.q_items = s.rest.q_items;
   a.n_splits = s.rest.n_splits;
-  launch_more(a, s.rest.pairs * s.rest.n_splits, st);
+  launch_rows(a, s.rest.pairs * s.rest.n_splits, st);
   launch_join(join_args(a, splits, nullptr), d->head_dim, st);
   return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
 }

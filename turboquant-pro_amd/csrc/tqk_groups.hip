@@ -129,9 +129,11 @@ __device__ void pick(int c, int top, int first, int last, int tid, int (&count_s
   uint64_t keys[KPL > 0 ? KPL : 1];
   if constexpr (KPL > 0) {
 #pragma unroll
+    for (int j = 0; j < KPL; ++j) keys[j] = load(min(j * NT + tid, max(c - 1, 0)));  // (all on their way at once)
+#pragma unroll
     for (int j = 0; j < KPL; ++j) {
       const int i = j * NT + tid;
-      keys[j] = !all && i < c && !always(i) ? load(i) : 0ull;
+      keys[j] = !all && i < c && !always(i) ? keys[j] : 0ull;
     }
   }
   auto key = [&](int j) -> uint64_t {

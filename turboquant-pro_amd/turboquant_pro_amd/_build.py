@@ -33,6 +33,9 @@ PER_UNIT = {
     "tqk_attend.hip": [],
     "tqk_attend_codes.hip": [],
     "tqk_attend_more.hip": [],
+    "tqk_attend_rows_64.hip": [],
+    "tqk_attend_rows_128.hip": [],
+    "tqk_attend_rows_256.hip": [],
     "tqk_groups.hip": [],
     "tqk_rope.hip": [],
     "tqk_attn.hip": [],
