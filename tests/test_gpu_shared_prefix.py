@@ -36,12 +36,25 @@ def shared_pool(seed, prefix, more, Hq, H, D=128, source=0, room=0, **kw):
     return pool
 
 
-def check(pool, out, q, q_lens=None, what=""):
+def read_once(pool, T):
+    """Whether a step of T queries reads the prefix once (its workspace tells)."""
+    import ctypes
+    from turboquant_pro_amd import _native as N
+    if not pool._shared_step(T, 0, max(pool.lengths)):
+        return False
+    t = N.AttendDesc(pool.max_batch, T, max(pool.lengths), 0, 0, 1)
+    t.q_stride[:] = t.o_stride[:] = [8, 8, 8]
+    d, lib = ctypes.byref(pool.desc), N.lib()
+    return (lib.tqk_attend_shared_workspace_bytes(d, ctypes.byref(t), pool._shared)
+            != lib.tqk_attend_workspace_bytes(d, ctypes.byref(t)))
+
+
+def check(pool, out, q, q_lens=None, what="", only=None):
     B, Hq, T, D = q.shape
     H = pool.n_kv_heads
     gq = Hq // H
     off = tot = 0.0
-    for b in range(B):
+    for b in range(B) if only is None else only:
         n, m = pool.lengths[b], T if q_lens is None else q_lens[b]
         k, v = cached(pool, b)
         sees = visible(n, m, T, 0, None, 0, "cuda")
@@ -74,13 +87,52 @@ def test_attention_over_a_shared_prefix(prefix, more, Hq, H, D, form):
     assert pool._shared > 0
     for T in (1, 3, 16):
         q = queries(T, pool, T)
-        assert pool._shared_step(T, 0, max(pool.lengths)) == (T * Hq // H <= 128)
+        assert pool._shared_step(T, 0, max(pool.lengths)) == (T * Hq // H <= 128 and pool.key_grid != "polar")
         out = pool.attend(q)
         check(pool, out, q, what=f"T={T}")
         assert torch.equal(out, pool.attend(q))
         assert torch.equal(out, pool.attend(q, window=10 ** 6))
         ql = [(b + T) % (T + 1) for b in range(len(more))]
         check(pool, pool.attend(q, q_lens=torch.tensor(ql, dtype=torch.int32, device="cuda")), q, ql, f"ragged T={T}")
+
+
+ONCE = [
+    # prefix, sequences, Hq, H, D, form: batches that read the prefix once
+    (2600, 64, 32, 8, 128, dict()),
+    (2600, 64, 8, 8, 128, dict(value_bits=4, outlier_frac=0.1)),
+    (2600, 90, 56, 8, 128, dict(value_bits=2, hot_window=64)),
+    (1400, 90, 16, 8, 128, dict(key_grid="uniform", key_bits=3, hot_window=47, page_tokens=12)),
+    (1400, 90, 16, 8, 128, dict(value_bits=2, hot_window=48, page_tokens=8)),
+    (1400, 90, 16, 8, 128, dict(value_bits=4, hot_window=15, page_tokens=4, outlier_frac=0.5)),
+    (2600, 90, 32, 8, 64, dict(value_bits=4)),
+    (2600, 90, 16, 8, 64, dict(value_bits=3, hot_window=64)),
+    (2600, 90, 16, 8, 64, dict(value_bits=2, key_grid="uniform", key_bits=4, outlier_frac=0.0)),
+    (2600, 40, 16, 8, 256, dict(value_bits=3)),
+    (2600, 40, 8, 8, 256, dict(value_bits=4, outlier_frac=0.1)),
+    (2600, 40, 32, 8, 256, dict(value_bits=2, key_grid="uniform", key_bits=2, hot_window=100, page_tokens=10)),
+]
+
+
+@pytest.mark.parametrize("prefix,B,Hq,H,D,form", ONCE)
+def test_a_prefix_read_once(prefix, B, Hq, H, D, form):
+    """One and several queries, rows past a workgroup's, tiles and blocks that end short."""
+    print(f"[shared] once {prefix} x {B} {Hq}/{H} D={D} {form}", flush=True)
+    more = [(37 * b) % 130 + 3 for b in range(B)]
+    pool = shared_pool(3, prefix, more, Hq, H, D, **form)
+    only = [0, 1, 31, B - 1]
+    for T in (1, 3):
+        q = queries(T, pool, T)
+        assert read_once(pool, T) or (T > 1 and Hq // H < 7)  # (few rows a sequence: 16 go together for each)
+        out = pool.attend(q)
+        check(pool, out, q, what=f"T={T}", only=only)
+        assert torch.equal(out, pool.attend(q))
+        ql = [(b + T) % (T + 1) for b in range(B)]
+        check(pool, pool.attend(q, q_lens=torch.tensor(ql, dtype=torch.int32, device="cuda")), q, ql, f"ragged T={T}", only)
+    # as each sequence for itself, but for the roundings of weights and centroids
+    q = queries(5, pool, 1)
+    got, pool._shared = pool.attend(q).float(), 0
+    want = pool.attend(q).float()
+    assert float((got - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max())
 
 
 def test_a_shared_pool_holds_what_separate_ones_do():

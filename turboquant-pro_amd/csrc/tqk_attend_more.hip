@@ -12,12 +12,7 @@
 //
 // A shared prefix: rows of all sequences are attended 16 at a time over one copy of
 // its codes, then each sequence's rows over its other tokens; the join takes both.
-#include "tqk_attend_codes_kernels.h"
-
-// up to eight rows of a (sequence, kv head) a workgroup (tqk_attend_rows.h)
-void tqk_launch_rows_64(const MoreArgs& a, unsigned groups, hipStream_t st);
-void tqk_launch_rows_128(const MoreArgs& a, unsigned groups, hipStream_t st);
-void tqk_launch_rows_256(const MoreArgs& a, unsigned groups, hipStream_t st);
+#include "tqk_attend_few.h"
 
 namespace {
 
@@ -123,6 +118,144 @@ __global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
   }
 }
 
+// The same where the first `pre` splits hold sums of centroids (of a shared prefix): four
+// rows a workgroup, four waves each (a wave a row was a chain of loads: 16 us for 33
+// splits of 1024 rows); the centroids' sums over all of the row's weights as an fp16
+// pair, times Pi's, by the matrix cores.
+template <int D>
+__global__ __launch_bounds__(1024) void tqk_join_shared(JoinMoreArgs a, const float* pi_t, int pre) {
+  constexpr int E = D / 64, NM = D / 32, kAhead = 8, NW = 4, NR = 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, lg = lane >> 4;
+  const int w = wave % NW, r = wave / NW;
+  __shared__ __align__(16) uint16_t c_s[2 * NR][D + 8];  // first halves, then second ones
+  __shared__ __align__(16) float y_s[NR][D + 4], acc_s[NR][NW][2][D];
+  __shared__ float ml_s[NR][NW][2];
+  const long long row = (long long)blockIdx.x * NR + r;
+  const long long from = row < a.rows ? row : a.rows - 1;
+  float M = -INFINITY, l = 0.f, acc[2][E];  // [0] centroids' sums, [1] values'
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[0][e] = acc[1][e] = 0.f;
+  auto add = [&](auto kind, int s_from, int s_to) {
+    constexpr int k = decltype(kind)::value;
+    for (int s0 = s_from + w; s0 < s_to; s0 += NW * kAhead) {
+      float x[kAhead][E], m_[kAhead], l_[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const long long o = min(s0 + u * NW, s_to - 1) * a.rows + from;
+        m_[u] = a.part_ml[2 * o];
+        l_[u] = a.part_ml[2 * o + 1];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = a.part_acc[o * D + E * lane + e];
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) top = fmaxf(top, s0 + u * NW < s_to ? m_[u] : -INFINITY);
+      const float f0 = M == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(M - top));
+      l *= f0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        acc[0][e] *= f0;
+        acc[1][e] *= f0;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s0 + u * NW < s_to) {
+          const float f = m_[u] == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(m_[u] - top));
+          l = fmaf(l_[u], f, l);
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[k][e] = fmaf(x[u][e], f, acc[k][e]);
+        }
+      }
+      M = top;
+    }
+  };
+  add(std::integral_constant<int, 1>{}, pre, a.n_splits);
+  add(std::integral_constant<int, 0>{}, 0, pre);
+  // Pi^T's rows 16 wave + ln, on their way meanwhile
+  f4_t pr[NM][2];
+  if (wave < D / 16) {
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        pr[mm][e] = *reinterpret_cast<const f4_t*>(pi_t + (size_t)(16 * wave + ln) * D + 32 * mm + 8 * lg + 4 * e);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc_s[r][w][k][E * lane + e] = acc[k][e];
+  if (lane == 0) {
+    ml_s[r][w][0] = M;
+    ml_s[r][w][1] = l;
+  }
+  __syncthreads();
+  float inv = 0.f, rest[E];
+  if (w == 0) {
+    float top = M;
+#pragma unroll
+    for (int u = 1; u < NW; ++u) top = fmaxf(top, ml_s[r][u][0]);
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[0][e] = acc[1][e] = 0.f;
+#pragma unroll
+    for (int u = 0; u < NW; ++u) {
+      const float mu = ml_s[r][u][0], f = mu == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(mu - top));
+      l = fmaf(ml_s[r][u][1], f, l);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[k][e] = fmaf(acc_s[r][u][k][E * lane + e], f, acc[k][e]);
+    }
+    inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      rest[e] = acc[1][e] * inv;
+      const float y = acc[0][e] * inv;
+      const _Float16 hi = (_Float16)y;
+      c_s[r][E * lane + e] = __builtin_bit_cast(uint16_t, hi);
+      c_s[NR + r][E * lane + e] = f2h(y - (float)hi);
+    }
+  }
+  __syncthreads();
+  if (wave < D / 16) {
+    f4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm) {
+      h8_t ph, pl;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = pr[mm][e / 4][e % 4];
+        ph[e] = (_Float16)y;
+        pl[e] = (_Float16)(y - (float)ph[e]);
+      }
+      const h8_t c8 = *reinterpret_cast<const h8_t*>(&c_s[ln % (2 * NR)][32 * mm + 8 * lg]);
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8, pl, sum, 0, 0, 0);
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8, ph, sum, 0, 0, 0);
+    }
+    // rows 4 lg + e of the product: first halves in lanes of lg 0, second ones of lg 1
+#pragma unroll
+    for (int e = 0; e < NR; ++e) {
+      const float z = sum[e] + __shfl_xor(sum[e], 16, 64);
+      if (lg == 0) y_s[e][16 * wave + ln] = z;
+    }
+  }
+  __syncthreads();
+  if (row >= a.rows || w != 0) return;
+  const int t = (int)(row % a.t_len);
+  const long long bh = row / a.t_len;
+  const int hq = (int)(bh % a.n_q_heads), b = (int)(bh / a.n_q_heads);
+  const int n = min(a.seq_lens[b], a.max_len);
+  const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+  const bool any = t < m && n - m + t >= 0;
+  const long long o = b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2] + E * lane;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float y = any ? y_s[r][E * lane + e] + rest[e] : 0.f;
+    if (a.out_type == 0) static_cast<float*>(a.out)[o + e] = y;
+    else static_cast<_Float16*>(a.out)[o + e] = (_Float16)y;
+  }
+}
+
 struct WeightArgs {
   tqk_cache_desc d;
   const int32_t* seq_lens;
@@ -169,38 +302,6 @@ __global__ __launch_bounds__(256) void tqk_group_weights(WeightArgs a) {
     float* const w = a.weights + ((long long)b * Hkv + h) * d.max_groups_per_seq + g;
     *w = (float)((double)*w + y);
   }
-}
-
-template <int D, int VB, bool TILED>
-void launch_keys(const MoreArgs& a, dim3 grid, hipStream_t st) {
-  if (a.d.key_grid == 2)
-    hipLaunchKernelGGL((tqk_attend_codes<D, VB, VB, true, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
-  else if (a.d.key_bits == 4)
-    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 4, false, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
-  else if (a.d.key_bits == 3)
-    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 3, false, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL((tqk_attend_codes<D, VB, 2, false, TILED, true>), grid, dim3(kFewThreads), 0, st, a);
-}
-template <int D, bool TILED>
-void launch_values(const MoreArgs& a, dim3 grid, hipStream_t st) {
-  if (a.d.value_bits == 2)
-    launch_keys<D, 2, TILED>(a, grid, st);
-  else if (a.d.value_bits == 3)
-    launch_keys<D, 3, TILED>(a, grid, st);
-  else
-    launch_keys<D, 4, TILED>(a, grid, st);
-}
-void launch_more(const MoreArgs& a, long long groups, hipStream_t st) {
-  const dim3 grid((unsigned)groups);
-  if (a.d.head_dim == 64)
-    launch_values<64, false>(a, grid, st);
-  else if (a.d.head_dim == 256)
-    launch_values<256, false>(a, grid, st);
-  else if (v_tiled(a.d.group_tokens, a.d.page_tokens, TQK_D, 0))
-    launch_values<TQK_D, true>(a, grid, st);
-  else
-    launch_values<TQK_D, false>(a, grid, st);
 }
 
 template <int D>
@@ -357,21 +458,48 @@ size_t weight_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const Wei
 
 // ---- a shared prefix ---------------------------------------------------------
 struct SharedPlan {
-  MorePlan pre, rest;
+  long long pre_pairs;  // workgroups of a split of the prefix
+  int pre_splits;
+  MorePlan rest;
 };
 SharedPlan shared_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, int groups) {
   SharedPlan s{};
   const int gq = d->n_q_heads / d->n_kv_heads, tokens = groups * d->group_tokens;
-  s.pre.per_item = 1;
-  s.pre.q_items = (int)(((long long)t->batch * t->q_len * gq + kFewRows - 1) / kFewRows);
-  s.pre.pairs = (long long)s.pre.q_items * d->n_kv_heads;
-  s.pre.n_splits = few_splits(s.pre.pairs, (long long)groups * ((d->group_tokens + 31) / 32), 0.0);
+  s.pre_pairs = ((long long)t->batch * t->q_len * gq + 127) / 128 * d->n_kv_heads;
+  // rounds of the workgroups that fit (one a CU) times a split's tiles and the set-up,
+  // joining and rotation of about five tiles' time
+  const int tiles = (groups * ((d->group_tokens + 31) / 32) + 1) / (d->head_dim == 256 ? 1 : 2);
+  double best = 1e30;
+  for (int n = 1; n <= 64 && n <= tiles; ++n) {
+    const double rounds = (double)((s.pre_pairs * n + device_cus() - 1) / device_cus());
+    const double cost = rounds * ((tiles + n - 1) / n + 5);
+    if (cost < best - 1e-9) {
+      best = cost;
+      s.pre_splits = n;
+    }
+  }
   s.rest = more_plan(d, t->batch, t->q_len, INT32_MAX, t->max_len - tokens, 0.0);
   return s;
+}
+// Whether reading the prefix once pays: it takes launches of its own and a set-up, about
+// 28 us, and 3.2 a tile of its workgroups; each sequence for itself finds the others'
+// codes in cache, a block of 32 tokens and 16 rows 1.2 ns of the whole card (0.8 at
+// head_dim 64, 4.9 at 256).  Each for itself and once, 32 / 8 heads of 128: a prefix of
+// 32768 tokens, 4 sequences 58 and 87 us, 8 95 and 88, 32 340 and 117; 8192 tokens, 4
+// sequences 29 and 51; 2048 tokens, 32 sequences 35 and 54; head_dim 256, 16 / 8 heads,
+// 4096 tokens, 4 sequences 60 and 79, 16 117 and 93.
+bool prefix_pays(const tqk_cache_desc* d, const tqk_attend_desc* t, int groups, const SharedPlan& s) {
+  const int gq = d->n_q_heads / d->n_kv_heads, blocks = groups * ((d->group_tokens + 31) / 32);
+  const double scale = 256.0 / device_cus(), block = d->head_dim == 64 ? 0.8e-3 : d->head_dim == TQK_D ? 1.2e-3 : 4.9e-3;
+  const double each = (double)t->batch * (((long long)t->q_len * gq + 15) / 16) * d->n_kv_heads * blocks * block * scale;
+  const int tiles = d->head_dim == 256 ? blocks : (blocks + 1) / 2;
+  const double rounds = (double)((s.pre_pairs * s.pre_splits + device_cus() - 1) / device_cus());
+  return each > 28.0 + rounds * ((tiles + s.pre_splits - 1) / s.pre_splits) * 3.2 + (d->head_dim == 256 ? 10.0 : 0.0);
 }
 int check_shared(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
   const int rc = check_more(d, t, false);
   if (rc != TQK_OK) return rc;
+  if (d->key_grid == 2) return TQK_EUNSUPPORTED;
   if (groups < 1 || groups > n_groups_of(t->max_len, d->hot_window, d->group_tokens)) return TQK_EINVAL;
   return TQK_OK;
 }
@@ -476,7 +604,8 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
 size_t tqk_attend_shared_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
   if (check_shared(d, t, groups) != TQK_OK || !t->batch || !t->q_len) return 0;
   const SharedPlan s = shared_plan(d, t, groups);
-  return partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, s.pre.n_splits + s.rest.n_splits, d->head_dim);
+  if (!prefix_pays(d, t, groups, s)) return tqk_few_workspace_bytes(d, t);
+  return partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, s.pre_splits + s.rest.n_splits, d->head_dim);
 }
 
 int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, int32_t groups,
@@ -489,26 +618,31 @@ int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   if (rc != TQK_OK) return rc;
   if (workspace_bytes < tqk_attend_shared_workspace_bytes(d, t, groups)) return TQK_EWORKSPACE;
   const SharedPlan s = shared_plan(d, t, groups);
-  if (s.pre.pairs * s.pre.n_splits > kMostGroups || s.rest.pairs * s.rest.n_splits > kMostGroups) return TQK_EINVAL;
+  if (!prefix_pays(d, t, groups, s)) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, workspace_bytes, stream);
+  if (s.pre_pairs * s.pre_splits > kMostGroups || s.rest.pairs * s.rest.n_splits > kMostGroups) return TQK_EINVAL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const int splits = s.pre.n_splits + s.rest.n_splits;
+  const int splits = s.pre_splits + s.rest.n_splits;
   MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
   a.rows = (long long)t->batch * d->n_q_heads * t->q_len;
   a.part_acc = static_cast<float*>(workspace);
   a.part_ml = a.part_acc + (size_t)splits * a.rows * d->head_dim;
-  a.per_item = 1;
-  a.q_items = s.pre.q_items;
-  a.n_splits = s.pre.n_splits;
+  a.n_splits = s.pre_splits;
   a.shared = groups * d->group_tokens;
-  launch_more(a, s.pre.pairs * s.pre.n_splits, st);
+  tqk_launch_prefix(a, (unsigned)(s.pre_pairs * s.pre_splits), st);
   a.skip = a.shared;
-  a.shared = 0;
-  a.split0 = s.pre.n_splits;
+  a.split0 = s.pre_splits;
   a.per_item = s.rest.per_item;
   a.q_items = s.rest.q_items;
   a.n_splits = s.rest.n_splits;
   launch_rows(a, s.rest.pairs * s.rest.n_splits, st);
-  launch_join(join_args(a, splits, nullptr), d->head_dim, st);
+  const JoinMoreArgs j = join_args(a, splits, nullptr);
+  const dim3 grid((unsigned)((a.rows + 3) / 4));
+  if (d->head_dim == 64)
+    hipLaunchKernelGGL(tqk_join_shared<64>, grid, dim3(1024), 0, st, j, p->pi_t, s.pre_splits);
+  else if (d->head_dim == TQK_D)
+    hipLaunchKernelGGL(tqk_join_shared<TQK_D>, grid, dim3(1024), 0, st, j, p->pi_t, s.pre_splits);
+  else
+    hipLaunchKernelGGL(tqk_join_shared<256>, grid, dim3(1024), 0, st, j, p->pi_t, s.pre_splits);
   return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
 }
 

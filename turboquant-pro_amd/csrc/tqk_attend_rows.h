@@ -20,9 +20,7 @@
 // The next block's scores are computed beside this block's exponentials and values.
 #pragma once
 
-#include "tqk_attend.h"
-#include "tqk_attend_codes_kernels.h"
-#include "tqk_wave.h"
+#include "tqk_attend_few.h"
 
 namespace {
 
@@ -33,6 +31,9 @@ template <int N>
 __device__ __forceinline__ float row_ror(float x) {
   return bitsf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fbits(x), 0x120 + N, 0xF, 0xF, true));
 }
+// the value of the lane before / after (the first / last one's: 0)
+__device__ __forceinline__ int lane_before(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x138, 0xF, 0xF, true); }
+__device__ __forceinline__ int lane_after(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x130, 0xF, 0xF, true); }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t entries_of(const uint32_t* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(base), (short)0, (int)bytes, 0x00020000);
 }
@@ -84,6 +85,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
   __shared__ __align__(16) float corr_s[kFewWaves][NR][kCorr];   // scores' first values of a stretch
   __shared__ __align__(16) float zero_s[4];
   __shared__ __align__(16) uint16_t qc_s[D][NR];                 // queries by channel
+  __shared__ __align__(16) uint16_t qr_s[kRows8][D];             // and by row
   __shared__ __align__(16) float lev_s[16], cen_s[16];
   __shared__ float up_s[2][2];  // the best of the scales of a half: its loss, itself
   __shared__ float ml_s[2][kFewWaves][kRows8];
@@ -142,19 +144,26 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
   const int i1 = min(i0 + run, is_cold ? cold.n : hot.n);
 
   // Q: this column's row, channels CPL lg + 8 m .. + 7 (rows past the last: a real one's, dropped later)
-  h8_t qf[NM];
+  // (in LDS: the loop has no registers for them)
   const int t_in = min(max(t, 0), a.q_len - 1);
   const uint16_t* const qp = a.q + b * a.q_stride[0] + (h * gq + row % gq) * a.q_stride[1] + t_in * a.q_stride[2];
+  float q_top = 0.f;  // the largest |q| (what is not finite: as the largest of fp16; its rows are lost whatever the power)
+  {
+    uint16_t one = 0;
 #pragma unroll
-  for (int mm = 0; mm < NM; ++mm) qf[mm] = *reinterpret_cast<const h8_t*>(qp + CPL * lg + 8 * mm);
-  if (wave == 0 && ln < NR) {
-#pragma unroll
-    for (int mm = 0; mm < NM; ++mm)
+    for (int mm = 0; mm < NM; ++mm) {
+      const h8_t q8 = *reinterpret_cast<const h8_t*>(qp + CPL * lg + 8 * mm);
+      if (wave == 0 && !is_lo) *reinterpret_cast<h8_t*>(&qr_s[ln][CPL * lg + 8 * mm]) = q8;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const _Float16 y = qf[mm][e];
-        qc_s[CPL * lg + 8 * mm + e][ln] = __builtin_bit_cast(uint16_t, y);
+        const _Float16 y = q8[e];
+        const uint16_t bits = __builtin_bit_cast(uint16_t, y);
+        if (wave == 0 && ln < NR) qc_s[CPL * lg + 8 * mm + e][ln] = bits;
+        const uint16_t mag = bits & 0x7FFF;
+        one = mag > one ? mag : one;
       }
+    }
+    if constexpr (!PK) q_top = wave_reduce<true>(h2f(one < 0x7C00 ? one : (uint16_t)0x7BFF));
   }
   // the coded keys' weights, this column's half of an fp16 pair: q * scale group by
   // group, or for rotated keys q @ Pi^T; over a power of two, w_up, where they pass fp16
@@ -170,20 +179,6 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     bw[s].u[0] = bw[s].u[1] = v01;
     bw[s].u[2] = bw[s].u[3] = v23;
   };
-  // the wave's largest |q| (what is not finite: as the largest of fp16; its rows
-  // are lost whatever the power)
-  float q_top = 0.f;
-  if constexpr (!PK) {
-    typedef uint16_t us8_t __attribute__((ext_vector_type(8)));
-    us8_t top = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-    for (int mm = 0; mm < NM; ++mm)
-      top = __builtin_elementwise_max(top, __builtin_bit_cast(us8_t, qf[mm]) & (uint16_t)0x7FFF);
-    uint16_t one = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) one = top[e] > one ? top[e] : one;
-    q_top = wave_reduce<true>(h2f(one < 0x7C00 ? one : (uint16_t)0x7BFF));
-  }
 
   // ---- the coded blocks of this wave: state and loads
   const size_t head = (size_t)h * d.n_pages * P;
@@ -337,10 +332,12 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
       const int ch = CPL * lg + 4 * s;
       const f4_t s4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][0][ch]);
       const f4_t m4 = *reinterpret_cast<const f4_t*>(&stat_s[wave][1][ch]);
+      typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+      const h4_t qh = *reinterpret_cast<const h4_t*>(&qr_s[ln & 7][ch]);
       float q4[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        q4[k] = (float)qf[s / 2][4 * (s % 2) + k];
+        q4[k] = (float)qh[k];
         y = fmaf(q4[k], m4[k], y);
       }
       put_weights(s, q4[0] * s4[0], q4[1] * s4[1], q4[2] * s4[2], q4[3] * s4[3]);
@@ -354,11 +351,10 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
 #pragma unroll
     for (int i = 0; i < NR; ++i) br[i] = bitsf((uint32_t)__builtin_amdgcn_readlane((int)fbits(bias), i));
     {
-      constexpr int NT = kSeg * NR / 64;  // tokens of a lane: row lane % NR
+      constexpr int kStep = 256 / NR;  // tokens that the lanes fill at a time: four each, row lane % NR
       const float y = __shfl(bias, lane % NR, 64);
-      float* const to = corr + lane % NR * kCorr + lane / NR * NT;
-#pragma unroll
-      for (int i = 0; i < NT; i += 4) *reinterpret_cast<f4_t*>(to + i) = f4_t{y, y, y, y};
+      float* const to = corr + lane % NR * kCorr + lane / NR * 4;
+      for (int i = 0; i < min(kSeg, G - kSeg * sg); i += kStep) *reinterpret_cast<f4_t*>(to + i) = f4_t{y, y, y, y};
     }
     wave_sync();
     if (PK || n_ent == 0) return;
@@ -434,24 +430,22 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
 #pragma unroll
     for (int i = 0; i < NR; ++i) sv[i] = acc[i];
     const int tl = tcur, tf = tfirst >= 0 ? tfirst : tcur;
-    const int tl_up = __shfl_up(tl, 1), tf_dn = __shfl_down(tf, 1);
+    const int tl_up = lane_before(tl), tf_dn = lane_after(tf);
     const int tl_prev = lane > 0 ? tl_up : -1, tf_next = lane < 63 ? tf_dn : -1;
-    if (__builtin_amdgcn_ballot_w64(tl >= 0 && tl == tl_prev) != 0) {
+    int kd = tl_prev;  // the last run's token `o` lanes before
+    for (int o = 1; o < 64 && __builtin_amdgcn_ballot_w64(tl >= 0 && kd == tl) != 0; o <<= 1) {
+      const bool add = kd == tl && tl >= 0;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int kd = __shfl_up(tl, o);
-        // (a lane whose first run is another token's does not go on its neighbours')
-        const bool add = lane >= o && kd == tl && tl >= 0;
-#pragma unroll
-        for (int i = 0; i < NR; ++i) {
-          const float v = __shfl_up(sv[i], o);
-          sv[i] += add ? v : 0.f;
-        }
+      for (int i = 0; i < NR; ++i) {
+        const float v = o == 1 ? bitsf((uint32_t)lane_before((int)fbits(sv[i]))) : __shfl_up(sv[i], o, 64);
+        sv[i] += add ? v : 0.f;
       }
+      kd = __shfl_up(tl, 2 * o, 64);
+      kd = lane >= 2 * o ? kd : -1;
     }
     float sprev[NR];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) sprev[i] = __shfl_up(sv[i], 1);
+    for (int i = 0; i < NR; ++i) sprev[i] = bitsf((uint32_t)lane_before((int)fbits(sv[i])));
     if (tfirst >= 0) {  // the first run ends inside this lane: with what came before
       const bool cin = tl_prev == tfirst;
 #pragma unroll
@@ -483,9 +477,13 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
           const uint8_t* src = a.p.vcodes + (head + rr) * VROW + ((D == 64 ? ln / 2 : ln) + 16 * s) * VB;
           if constexpr (VB == 4)
             vw[s][e] = *reinterpret_cast<const uint32_t*>(src);
-          else if constexpr (VB == 3)
-            vw[s][e] = (uint32_t)src[0] | (uint32_t)src[1] << 8 | (uint32_t)src[2] << 16;
-          else
+          else if constexpr (VB == 3) {
+            // (a dword of the row at any byte: from the byte before, of the first piece from itself)
+            const int piece = (D == 64 ? ln / 2 : ln) + 16 * s;
+            uint32_t y;
+            __builtin_memcpy(&y, src - (piece > 0), 4);
+            vw[s][e] = piece > 0 ? y >> 8 : y;
+          } else
             vw[s][e] = *reinterpret_cast<const uint16_t*>(src);
         }
       }
@@ -561,12 +559,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     __syncthreads();
     float* const q_s = &corr_s[0][0][0];  // [8][D]
     float* const r_s = q_s + kRows8 * D;  // [8][D]
-    if (wave == 0 && !is_lo) {
-#pragma unroll
-      for (int mm = 0; mm < NM; ++mm)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q_s[ln * D + CPL * lg + 8 * mm + e] = (float)qf[mm][e];
-    }
+    for (int i = tid; i < kRows8 * D; i += kFewThreads) q_s[i] = h2f(qr_s[i / D][i % D]);
     __syncthreads();
     for (int i = tid; i < kRows8 * D; i += kFewThreads) {
       const int r = i / D, j = i % D;
@@ -659,14 +652,21 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
         S[tile] = PK ? f4_t{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const f4_t*>(init + init_step * (32 * kb + 16 * tile));
-        union { h8_t h; u32x2_t u[2]; } y[NSL];
+        // (at head_dim 256 half of the levels at a time: there are no registers for all)
+        constexpr int kAtOnce = NSL < 8 ? NSL : 8;
 #pragma unroll
-        for (int s = 0; s < NSL; ++s) {
-          y[s].u[0] = levels(kw[tile], KB * 4 * s);
-          y[s].u[1] = levels(kw[tile], KB * (4 * s + 2));
+        for (int s0 = 0; s0 < NSL; s0 += kAtOnce) {
+          union { h8_t h; u32x2_t u[2]; } y[kAtOnce];
+#pragma unroll
+          for (int s = 0; s < kAtOnce; ++s) {
+            y[s].u[0] = levels(kw[tile], KB * 4 * (s0 + s));
+            y[s].u[1] = levels(kw[tile], KB * (4 * (s0 + s) + 2));
+          }
+#pragma unroll
+          for (int s = 0; s < kAtOnce; ++s)
+            S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[s].h, bw[s0 + s].h, S[tile], 0, 0, 0);
+          if constexpr (D == 256) __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int s = 0; s < NSL; ++s) S[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[s].h, bw[s].h, S[tile], 0, 0, 0);
       }
     };
     if constexpr (!PK) {
@@ -781,6 +781,9 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     }
   } else if (!is_cold) {
     // uncoded blocks, straight from the ring
+    h8_t qf[NM];
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm) qf[mm] = *reinterpret_cast<const h8_t*>(&qr_s[ln & 7][CPL * lg + 8 * mm]);
     const size_t ring = ((size_t)b * Hkv + h) * d.hot_ring;
     const uint16_t* const hk = static_cast<const uint16_t*>(a.p.hot_k);
     const uint16_t* const hv = static_cast<const uint16_t*>(a.p.hot_v);

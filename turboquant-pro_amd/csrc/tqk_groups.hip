@@ -50,45 +50,43 @@ __device__ __forceinline__ double row_sum(double x) {
   return x;
 }
 
-constexpr int kScoreGroups = 16;  // groups of a workgroup: four waves of four
-
+// A group's levels of a lane's channels, E ln .. for ln of 16 lanes, and its score.
 template <int D>
-__global__ __launch_bounds__(256) void tqk_score_groups(ScoreArgs a) {
-  constexpr int E = D / 16;  // channels of a lane: E ln ..
-  const tqk_cache_desc& d = a.d;
-  const int Hkv = d.n_kv_heads, gq = d.n_q_heads / Hkv;
-  const int ln = threadIdx.x & 15;
-  int x = blockIdx.x;
-  const int chunks = (a.most + kScoreGroups - 1) / kScoreGroups;
-  const int g = x % chunks * kScoreGroups + threadIdx.x / 16;
-  x /= chunks;
-  const int h = x % Hkv, b = x / Hkv;
-  const int n = min(a.seq_lens[b], a.max_len), ng = n_groups_of(n, d.hot_window, d.group_tokens);
-  if (g - (int)threadIdx.x / 16 >= ng) return;  // (the whole workgroup)
-  const int slot = a.p.group_table[(size_t)b * d.max_groups_per_seq + min(g, ng - 1)];
-  const size_t at = ((size_t)slot * Hkv + h) * D + E * ln;
-  // nf4: levels -1 .. 1 of the scale; uniform: 0 .. 2^bits - 1 of the step
-  const double steps = d.key_grid == 1 ? 0.5 * (double)((1 << d.key_bits) - 1) : 0.0;
+struct GroupLevels {
+  static constexpr int E = D / 16;
+  f4_t sc[E / 4], mu[E / 4];
   double mid[E], half[E];
+  __device__ __forceinline__ void load(const ScoreArgs& a, int b, int h, int g) {
+    const int slot = a.p.group_table[(size_t)b * a.d.max_groups_per_seq + g];
+    const size_t at = ((size_t)slot * a.d.n_kv_heads + h) * D + E * (threadIdx.x & 15);
 #pragma unroll
-  for (int e = 0; e < E; e += 4) {
-    const f4_t sc = *reinterpret_cast<const f4_t*>(a.p.gscale + at + e);
-    const f4_t mu = *reinterpret_cast<const f4_t*>(a.p.gmean + at + e);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      mid[e + k] = fma((double)sc[k], steps, (double)mu[k]);
-      half[e + k] = (double)sc[k] * (d.key_grid == 1 ? steps : 1.0) * (double)a.spread;
+    for (int e = 0; e < E / 4; ++e) {
+      sc[e] = *reinterpret_cast<const f4_t*>(a.p.gscale + at + 4 * e);
+      mu[e] = *reinterpret_cast<const f4_t*>(a.p.gmean + at + 4 * e);
     }
   }
-  for (int t = a.t0; t < a.t0 + a.t_len; ++t) {
+  __device__ __forceinline__ void ready(const ScoreArgs& a) {
+    // nf4: levels -1 .. 1 of the scale; uniform: 0 .. 2^bits - 1 of the step
+    const double steps = a.d.key_grid == 1 ? 0.5 * (double)((1 << a.d.key_bits) - 1) : 0.0;
+    const double width = (a.d.key_grid == 1 ? steps : 1.0) * (double)a.spread;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      mid[e] = fma((double)sc[e / 4][e % 4], steps, (double)mu[e / 4][e % 4]);
+      half[e] = (double)sc[e / 4][e % 4] * width;
+    }
+  }
+  // query t's, in every lane of the 16
+  __device__ __forceinline__ double score(const ScoreArgs& a, int b, int h, int t) const {
+    const int gq = a.d.n_q_heads / a.d.n_kv_heads;
+    const uint16_t* const qp = a.q + b * a.q_stride[0] + (long long)h * gq * a.q_stride[1] + t * a.q_stride[2] + E * (threadIdx.x & 15);
     double best = 0.0;
+#pragma unroll 4
     for (int i = 0; i < gq; ++i) {
-      const uint16_t* const qp = a.q + b * a.q_stride[0] + (h * gq + i) * a.q_stride[1] + t * a.q_stride[2] + E * ln;
       double y = 0.0;
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
         typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-        const h4_t q4 = *reinterpret_cast<const h4_t*>(qp + e);
+        const h4_t q4 = *reinterpret_cast<const h4_t*>(qp + i * a.q_stride[1] + e);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const double q = (double)(float)q4[k];
@@ -96,11 +94,30 @@ __global__ __launch_bounds__(256) void tqk_score_groups(ScoreArgs a) {
         }
       }
       y = row_sum(y);
-      // (a NaN stays one)
-      best = i == 0 || y > best || y != y ? y : best;
+      best = i == 0 || y > best || y != y ? y : best;  // (a NaN stays one)
     }
-    if (ln == 0 && g < ng)
-      a.scores[(((size_t)b * Hkv + h) * a.t_len + t - a.t0) * a.most + g] = best;
+    return best;
+  }
+};
+
+constexpr int kScoreGroups = 16;  // groups of a workgroup: four waves of four
+
+template <int D>
+__global__ __launch_bounds__(256) void tqk_score_groups(ScoreArgs a) {
+  const int Hkv = a.d.n_kv_heads;
+  int x = blockIdx.x;
+  const int chunks = (a.most + kScoreGroups - 1) / kScoreGroups;
+  const int g0 = x % chunks * kScoreGroups, g = g0 + threadIdx.x / 16;
+  x /= chunks;
+  const int h = x % Hkv, b = x / Hkv;
+  const int n = min(a.seq_lens[b], a.max_len), ng = n_groups_of(n, a.d.hot_window, a.d.group_tokens);
+  if (g0 >= ng) return;  // (the whole workgroup)
+  GroupLevels<D> levels;
+  levels.load(a, b, h, min(g, ng - 1));
+  levels.ready(a);
+  for (int t = a.t0; t < a.t0 + a.t_len; ++t) {
+    const double y = levels.score(a, b, h, t);
+    if ((threadIdx.x & 15) == 0 && g < ng) a.scores[(((size_t)b * Hkv + h) * a.t_len + t - a.t0) * a.most + g] = y;
   }
 }
 
@@ -118,7 +135,7 @@ __device__ __forceinline__ int popcount64(uint64_t x) { return __popcll(x); }
 // emit(i, chosen, rank among the chosen, rank among the others) for every candidate,
 // ranks in the order of the candidates.
 template <int NT, int KPL, class Load, class Emit>
-__device__ void pick(int c, int top, int first, int last, int tid, int (&count_s)[2][NT / 64 + 1], Load load, Emit emit) {
+__device__ void pick(int c, int top, int first, int last, int tid, int (*count_s)[NT / 64 + 1], Load load, Emit emit) {
   constexpr int NW = NT / 64;
   const int wave = tid >> 6, lane = tid & 63;
   const int steps = (c + NT - 1) / NT;
@@ -168,8 +185,28 @@ __device__ void pick(int c, int top, int first, int last, int tid, int (&count_s
   int ties = 0;        // and that many equal to it, the first ones
   if (need > 0) {
     v = 0;
-    int at = c;  // keys from v on
-    for (int bit = 63; bit >= 0 && at != need; --bit) {
+    int at = c, bit = 63;  // keys from v on
+    if constexpr (NW == 1 && KPL > 0) {
+      // (scores are of one sign and nearly one size: the bits that all keys have are
+      // the threshold's)
+      uint64_t one = 0, diff = 0;
+#pragma unroll
+      for (int j = 0; j < KPL; ++j) one = keys[j] ? keys[j] : one;
+      const uint64_t some = __builtin_amdgcn_ballot_w64(one != 0);
+      const int from = some ? __builtin_ctzll(some) : 0;
+      one = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(one >> 32), from) << 32 |
+            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)one, from);
+#pragma unroll
+      for (int j = 0; j < KPL; ++j) diff |= keys[j] ? keys[j] ^ one : 0;
+      uint32_t hi = (uint32_t)(diff >> 32);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) hi |= (uint32_t)__shfl_xor((int)hi, o, 64);
+      if (hi) {
+        bit = 63 - __builtin_clz(hi);
+        v = bit == 63 ? 0 : one >> (bit + 1) << (bit + 1);
+      }
+    }
+    for (; bit >= 0 && at != need; --bit) {
       const uint64_t higher = v | 1ull << bit;
       const int n = count_from(higher);
       if (n >= need) {
@@ -249,6 +286,45 @@ __global__ __launch_bounds__(NT) void tqk_pick_groups(ScoreArgs a) {
   for (int i = min(c, a.top) + tid; i < a.top; i += NT) out[i] = -1;
 }
 
+// Both in one for few rows over few groups: a workgroup a kv head of a sequence, 64
+// groups at a time, the next ones on their way; then a wave a query.  127 groups, 4
+// rows, 128 workgroups 11.6 us, where the two kernels take 16.5; but 511 groups 28 to 16,
+// 187 groups of 21 rows 31 to 17: one workgroup's loads and 64-bit products then bound it.
+constexpr int kTogether = 128, kTogetherRows = 8;
+template <int D>
+__global__ __launch_bounds__(1024) void tqk_choose_groups(ScoreArgs a) {
+  __shared__ double score_s[kTogetherRows][kTogether];
+  const tqk_cache_desc& d = a.d;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int h = blockIdx.x % d.n_kv_heads, b = blockIdx.x / d.n_kv_heads;
+  const int n = min(a.seq_lens[b], a.max_len), ng = n_groups_of(n, d.hot_window, d.group_tokens);
+  if (ng > a.top) {  // (else every candidate is chosen)
+    GroupLevels<D> now, next;
+    now.load(a, b, h, min(tid / 16, ng - 1));
+    for (int g0 = 0; g0 < ng; g0 += 64) {
+      if (g0 + 64 < ng) next.load(a, b, h, min(g0 + 64 + tid / 16, ng - 1));
+      const int g = g0 + tid / 16;
+      now.ready(a);
+      for (int t = 0; t < a.q_len; ++t) {
+        const double y = now.score(a, b, h, t);
+        if ((tid & 15) == 0 && g < ng) score_s[t][g] = y;
+      }
+      now = next;
+    }
+    __syncthreads();
+  }
+  if (wave >= a.q_len) return;
+  const int t = wave, p = position(n, a.q_lens, a.q_len, b, t);
+  const int c = p < 0 ? 0 : min(ng, p / d.group_tokens + 1);
+  int32_t* const out = a.groups + ((long long)blockIdx.x * a.q_len + t) * a.top;
+  auto key = [&](int i) { return key_of(score_s[t][i]); };
+  auto emit = [&](int i, bool in, int rank, int) {
+    if (in) out[rank] = i;
+  };
+  pick<64, kTogether / 64>(c, a.top, a.first, a.last, lane, nullptr, key, emit);
+  for (int i = min(c, a.top) + lane; i < a.top; i += 64) out[i] = -1;
+}
+
 struct EvictArgs {
   tqk_cache_desc d;
   float* weights;
@@ -264,8 +340,10 @@ struct EvictArgs {
   int keep, first, last;
 };
 
-template <int NT, int KPL>
-__global__ __launch_bounds__(NT) void tqk_evict(EvictArgs a) {
+// KPL: candidates that a lane of the first wave holds; 0: all waves choose.
+template <int KPL>
+__global__ __launch_bounds__(1024) void tqk_evict(EvictArgs a) {
+  constexpr int NT = 1024, kAhead = 4;
   __shared__ int count_s[2][NT / 64 + 1];
   const tqk_cache_desc& d = a.d;
   const int b = blockIdx.x, tid = threadIdx.x, G = d.group_tokens, mg = d.max_groups_per_seq, Hkv = d.n_kv_heads;
@@ -279,41 +357,62 @@ __global__ __launch_bounds__(NT) void tqk_evict(EvictArgs a) {
   int32_t* const kept = a.kept + (size_t)b * a.keep;
   for (int i = n_in + tid; i < a.keep; i += NT) kept[i] = -1;
   float* const w = a.weights + (size_t)b * Hkv * mg;
+  const long long all = (long long)Hkv * mg;
   if (gone == 0) {
     for (int i = tid; i < n_in; i += NT) kept[i] = i;
-    for (int i = tid; i < Hkv * mg; i += NT)
+    for (long long i = tid; i < all; i += NT)
       if (i % mg >= ng) w[i] = 0.f;
     return;
   }
   double* const s = a.scores + (size_t)b * mg;
-  for (int i = tid; i < ng; i += NT) {  // (each thread its own candidates')
-    double y = 0.0;
-    for (int h = 0; h < Hkv; ++h) y += (double)w[(size_t)h * mg + i];
-    s[i] = y;
-  }
   int32_t* const bt = a.block_table + (size_t)b * d.max_pages_per_seq;
   int32_t* const gt = a.group_table + (size_t)b * mg;
   int32_t* const order = a.order + (size_t)b * mg;
   int32_t* const pages = a.pages + (size_t)b * d.max_pages_per_seq;
   int32_t* const slots = a.slots + (size_t)b * mg;
-  pick<NT, KPL>(ng, a.keep, a.first, a.last, tid, count_s, [&](int i) { return key_of(s[i]); },
-                [&](int i, bool in, int rank, int other) {
-                  order[in ? rank : n_in + other] = i;
-                  if (in) kept[rank] = i;
-                });
-  for (int i = tid; i < ng; i += NT) slots[i] = gt[i];
+  for (int i = tid; i < ng; i += NT) {
+    double y = 0.0;
+    for (int h0 = 0; h0 < Hkv; h0 += 8) {  // (eight heads' weights on their way at once; summed in order)
+      float x[8];
+#pragma unroll
+      for (int h = 0; h < 8; ++h) x[h] = w[(size_t)min(h0 + h, Hkv - 1) * mg + i];
+#pragma unroll
+      for (int h = 0; h < 8; ++h) y += h0 + h < Hkv ? (double)x[h] : 0.0;
+    }
+    s[i] = y;
+    slots[i] = gt[i];
+  }
   for (int i = tid; i < ng * per; i += NT) pages[i] = bt[i];
+  __syncthreads();
+  auto key = [&](int i) { return key_of(s[i]); };
+  auto emit = [&](int i, bool in, int rank, int other) {
+    order[in ? rank : n_in + other] = i;
+    if (in) kept[rank] = i;
+  };
+  if constexpr (KPL > 0) {
+    if (tid < 64) pick<64, KPL>(ng, a.keep, a.first, a.last, tid, nullptr, key, emit);
+  } else {
+    pick<NT, 0>(ng, a.keep, a.first, a.last, tid, count_s, key, emit);
+  }
   __syncthreads();
   for (int i = tid; i < ng; i += NT) gt[i] = slots[order[i]];
   for (int i = tid; i < ng * per; i += NT) bt[i] = pages[order[i / per] * per + i % per];
   // the weights: a place's comes from no earlier one, so a stretch at a time in order
-  for (int h = 0; h < Hkv; ++h)
-    for (int i0 = 0; i0 < mg; i0 += NT) {
-      const int i = i0 + tid;
-      const float x = i < n_in ? w[(size_t)h * mg + order[i]] : 0.f;
-      __syncthreads();
-      if (i < mg) w[(size_t)h * mg + i] = x;
+  for (long long i0 = 0; i0 < all; i0 += NT * kAhead) {
+    float x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const long long i = i0 + u * NT + tid;
+      const int g = (int)(i % mg);
+      x[u] = i < all && g < n_in ? w[i - g + order[g]] : 0.f;
     }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const long long i = i0 + u * NT + tid;
+      if (i < all) w[i] = x[u];
+    }
+  }
 }
 
 // The rings' places: token t at t % ring, after `turn` tokens less at (t - turn) % ring.
@@ -430,6 +529,16 @@ int tqk_select_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   a.most = sp.most;
   const long long pairs = (long long)s->batch * d->n_kv_heads, chunks = (sp.most + kScoreGroups - 1) / kScoreGroups;
   if (pairs * chunks > INT32_MAX / 256 || pairs * sp.t_len > INT32_MAX / 1024) return TQK_EINVAL;
+  if (sp.most <= kTogether && s->q_len * (d->n_q_heads / d->n_kv_heads) <= kTogetherRows) {
+    const dim3 grid((unsigned)pairs);
+    if (d->head_dim == 64)
+      hipLaunchKernelGGL(tqk_choose_groups<64>, grid, dim3(1024), 0, st, a);
+    else if (d->head_dim == 128)
+      hipLaunchKernelGGL(tqk_choose_groups<128>, grid, dim3(1024), 0, st, a);
+    else
+      hipLaunchKernelGGL(tqk_choose_groups<256>, grid, dim3(1024), 0, st, a);
+    return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+  }
   for (a.t0 = 0; a.t0 < s->q_len; a.t0 += sp.t_len) {
     a.t_len = s->q_len - a.t0 < sp.t_len ? s->q_len - a.t0 : sp.t_len;
     if (sp.most > s->top) {  // (else every candidate is chosen)
@@ -442,7 +551,9 @@ int tqk_select_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
         hipLaunchKernelGGL(tqk_score_groups<256>, grid, dim3(256), 0, st, a);
     }
     const dim3 rows((unsigned)(pairs * a.t_len));
-    if (sp.most <= 64 * 16)
+    if (sp.most <= 64 * 8)
+      hipLaunchKernelGGL((tqk_pick_groups<64, 8>), rows, dim3(64), 0, st, a);
+    else if (sp.most <= 64 * 16)
       hipLaunchKernelGGL((tqk_pick_groups<64, 16>), rows, dim3(64), 0, st, a);
     else if (sp.most <= 1024 * 16)
       hipLaunchKernelGGL((tqk_pick_groups<1024, 16>), rows, dim3(1024), 0, st, a);
@@ -490,10 +601,13 @@ int tqk_evict_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, int32_t b
   a.keep = keep;
   a.first = first;
   a.last = last;
-  if (d->max_groups_per_seq <= 1024 * 16)
-    hipLaunchKernelGGL((tqk_evict<1024, 16>), dim3((unsigned)batch), dim3(1024), 0, st, a);
+  const dim3 grid((unsigned)batch), block(1024);
+  if (d->max_groups_per_seq <= 64 * 2)
+    hipLaunchKernelGGL(tqk_evict<2>, grid, block, 0, st, a);
+  else if (d->max_groups_per_seq <= 64 * 8)
+    hipLaunchKernelGGL(tqk_evict<8>, grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((tqk_evict<1024, 0>), dim3((unsigned)batch), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(tqk_evict<0>, grid, block, 0, st, a);
   if (hipGetLastError() != hipSuccess) return TQK_EHIP;
   RingArgs r{};
   r.ring[0] = static_cast<uint8_t*>(p->hot_k);

@@ -33,6 +33,7 @@ PER_UNIT = {
     "tqk_attend.hip": [],
     "tqk_attend_codes.hip": [],
     "tqk_attend_more.hip": [],
+    "tqk_attend_prefix.hip": [],
     "tqk_attend_rows_64.hip": [],
     "tqk_attend_rows_128.hip": [],
     "tqk_attend_rows_256.hip": [],

@@ -538,7 +538,7 @@ class TQKVPool:
         """Whether a step of T queries reads a shared prefix once for all sequences:
         every query stands behind it and sees it whole, and the rows are as few as
         go over the codes."""
-        return (self._shared > 0 and not self.f32 and (window == 0 or window >= max_len)
+        return (self._shared > 0 and not self.f32 and self.key_grid != "polar" and (window == 0 or window >= max_len)
                 and T * (self.n_q_heads // self.n_kv_heads) <= SHARED_ROWS
                 and min(self.lengths) - T >= self._shared * self.group_tokens - 1)
 
