@@ -486,6 +486,7 @@ int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
  * weights of group g's tokens, summed over the sequence's queries and kv head h's query
  * heads.
  *   weights [batch][n_kv_heads][max_groups_per_seq] fp32 (batch * n_kv_heads at most 65535)
+ *           (read and written without atomics: calls that add to it do not overlap)
  * fp16 caches, over the codes however many queries; 256 MiB of blocks' sums at a time
  * beside the partial results.
  */
@@ -498,8 +499,9 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
 /*
  * tqk_attend (t->window and t->sinks are 0) of sequences whose first `groups` coded
  * groups are the same pages and slots in every sequence's tables: they are read
- * through the first sequence's, once for all.  Every query sees them whole (p is at
- * least groups * group_tokens - 1).  fp16 caches.
+ * through the first sequence's, once for all (or, where the batch is too small for
+ * that to be faster, as by tqk_attend).  Every query sees them whole (p is at least
+ * groups * group_tokens - 1).  fp16 caches with per-channel keys (key_grid 0 or 1).
  */
 size_t tqk_attend_shared_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups);
 

@@ -65,6 +65,7 @@ class TQKVPool:
                                key_grid=key_grid, zero_point=zero_point, rope_theta=rope_theta,
                                k_bias=k_bias, input_dtype=input_dtype)
         self._custom_table = block_table is not None
+        self._pages_twice = False  # (a caller's table may name a page in two places)
         if zero_point not in ZERO_POINTS:
             raise ValueError(f"zero_point must be one of {tuple(ZERO_POINTS)}")
         if key_grid not in KEY_GRIDS:
@@ -154,6 +155,7 @@ class TQKVPool:
             bt = np.asarray(block_table, dtype=np.int32).reshape(max_batch, max_pages)
             if bt.min() < 0 or bt.max() >= n_pages:
                 raise ValueError("block_table entries must index the page pool")
+            self._pages_twice = len(np.unique(bt)) < bt.size
         self.block_table = torch.from_numpy(bt.copy()).to(dev)
         gt = np.arange(n_slots, dtype=np.int32).reshape(max_batch, max_groups)
         self.group_table = torch.from_numpy(gt).to(dev)
@@ -458,11 +460,13 @@ class TQKVPool:
 
         ``weights`` (fp32 ``(B, Hkv, max_groups)``, contiguous) is added to: the
         softmax weights of every coded group's tokens, summed over the queries and
-        the kv head's query heads (what :meth:`evict` goes by).  Both of them fp16
-        pools, over the codes however many queries.
+        the kv head's query heads (what :meth:`evict` goes by).  Calls that add to one
+        tensor go one after another.  Both of them fp16 pools, over the codes however
+        many queries.
 
         After :meth:`share_prefix`, steps of few queries without a window read the
-        shared groups once for all sequences.
+        shared groups once for all sequences, where that is faster.  (A captured step is
+        one of the pool as it was shared then: capture again after :meth:`reset`.)
 
         Returns ``(B, Hq, T, D)`` in the queries' type (``out`` where given,
         its rows apart, else laid out ``(B, T, Hq, D)``); rows ``t >= m`` and queries before
@@ -613,6 +617,8 @@ class TQKVPool:
         B, keep, first, last = self.max_batch, int(keep), int(first), int(last)
         if self.zero_point == "bias":
             raise NotImplementedError('evict: the zero points of zero_point="bias" belong to the groups\' positions')
+        if self._pages_twice:  # (a page that one place frees would be written while another one reads it)
+            raise NotImplementedError("evict: the caller's block table names a page twice")
         if first < 0 or last < 0:
             raise ValueError("evict: first and last are not negative")
         first = max(first, self._shared)
