@@ -5,6 +5,29 @@
 #include "tqk_attend.h"
 #include "tqk_wave.h"
 
+// Division by a number that a launch has: by a product (2^32 / n, rounded up: exact while
+// x n < 2^32) where the host knows that x stays below that.  The compiler's own are some
+// 200 cycles each, ten of them in a row before the first block.
+struct FewDiv {
+  int n;
+  uint32_t mul;  // 0: a division
+  __device__ __forceinline__ int operator()(int x) const {
+    return n == 1 ? x : mul ? (int)__umulhi((uint32_t)x, mul) : x / n;
+  }
+};
+inline FewDiv few_div(long long n, long long most) {  // x from 0 to `most`
+  return FewDiv{(int)n, n > 1 && (most + 1) * n <= (1LL << 32) ? (uint32_t)(0xFFFFFFFFu / (uint32_t)n + 1) : 0u};
+}
+// What tqk_attend_rows divides by.
+struct FewDivs {
+  FewDiv splits, heads, items;  // of the workgroups
+  FewDiv heads_of;              // query heads of a kv head
+  FewDiv group, blocks;         // tokens of a group, its blocks
+  FewDiv waves;                 // of all splits
+  float per_page;               // 1 / tokens of a page
+  int group_pages;
+};
+
 // Arguments of the kernels behind tqk_attend_groups, tqk_attend_weights and
 // tqk_attend_shared: a window, or a list of groups in its place, or the tokens from one
 // on; partial results, and every coded block's maximum and sum, for launches that follow.
@@ -34,6 +57,7 @@ struct MoreArgs {
   int direct;        // one split, and its result is the output
   float* block_ml;   // [row][blocks][2]: maximum and sum of a coded block, or null
   int blocks;        // blocks of a row there
+  FewDivs by;
 };
 
 // up to eight rows of a (sequence, kv head) a workgroup (tqk_attend_rows.h)
@@ -74,6 +98,13 @@ struct BlockRuns {
     }
   }
   return splits;
+}
+
+// x / n of uniform numbers that are mostly small
+[[maybe_unused]] __device__ __forceinline__ int few_quotient(int x, int n) {
+  if (x >= 1 << 22) return x / n;
+  const int q = (int)((float)x * __builtin_amdgcn_rcpf((float)n)), r = x - q * n;  // (within one of it)
+  return q + (r >= n) - (r < 0);
 }
 
 }  // namespace

@@ -1,17 +1,22 @@
-// Attention over the codes of an fp16 cache of more kinds than a window's (gfx950):
-// over listed groups, with the weight that every coded group received, and over a
-// prefix that all sequences share (tqk_attend_codes_kernels.h has the kernel).
+// Attention over the codes of an fp16 cache of more kinds than a window's (gfx950): over
+// listed groups, with the weight that every coded group received, and over a prefix that
+// all sequences share.  The plans, joins and entry points; tqk_attend_rows.h has the
+// kernel of up to eight rows of a sequence, tqk_attend_prefix.hip that of 128 rows of any.
 //
 // Listed groups: a workgroup's blocks are those of its list, nothing else is read.
 //
 // Weights: softmax_j = 2^(s_j - M) / L with a row's maximum M and sum L, which are
 // known when its splits are joined.  A wave writes each block's own maximum and sum
-// beside its partial results (8 bytes a row and block of 32 tokens), the join writes M
-// and L, and tqk_group_weights adds 2^(m - M) l / L over a kv head's rows and a
-// group's blocks, in one order and 64 bits: no atomics.
+// beside its partial results (8 bytes a row and block of 32 tokens: 10 of the step's
+// 170 us), the join writes M and L, and tqk_group_weights adds 2^(m - M) l / L over a kv
+// head's rows and a group's blocks, in one order and 64 bits: no atomics.  6 us at 16
+// sequences of 32768 tokens, 16.8 MB of sums.
 //
-// A shared prefix: rows of all sequences are attended 16 at a time over one copy of
-// its codes, then each sequence's rows over its other tokens; the join takes both.
+// A shared prefix: rows of all sequences over one copy of its codes, then each
+// sequence's rows over its other tokens; one join takes both.
+//
+// The joins are latency: 4 to 5 us a launch, the chain lengths -> partial results ->
+// output.
 #include "tqk_attend_few.h"
 
 namespace {
@@ -36,6 +41,7 @@ struct JoinMoreArgs {
 // 23 splits 8.7 us, where four waves take 4), D / 64 channels a lane.
 template <int D, int NW>
 __global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
+  touch_args<JoinMoreArgs>();
   constexpr int E = D / 64, kAhead = 8;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % NW;
   const long long row = (long long)blockIdx.x * (4 / NW) + wave / NW;
@@ -124,6 +130,7 @@ __global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
 // pair, times Pi's, by the matrix cores.
 template <int D>
 __global__ __launch_bounds__(1024) void tqk_join_shared(JoinMoreArgs a, const float* pi_t, int pre) {
+  touch_args<JoinMoreArgs>();
   constexpr int E = D / 64, NM = D / 32, kAhead = 8, NW = 4, NR = 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, lg = lane >> 4;
   const int w = wave % NW, r = wave / NW;
@@ -269,6 +276,7 @@ struct WeightArgs {
 // weights += what the launch's queries gave every group.  A thread a block of 32
 // tokens (blockIdx.x: whole groups of them), rows one after another.
 __global__ __launch_bounds__(256) void tqk_group_weights(WeightArgs a) {
+  touch_args<WeightArgs>();
   const tqk_cache_desc& d = a.d;
   const int G = d.group_tokens, Hkv = d.n_kv_heads, gq = d.n_q_heads / Hkv;
   const int h = blockIdx.y % Hkv, b = blockIdx.y / Hkv, tid = threadIdx.x;
@@ -321,7 +329,19 @@ void launch_join(const JoinMoreArgs& a, int D, hipStream_t st) {
     launch_join_rows<256>(a, st);
 }
 
-void launch_rows(const MoreArgs& a, long long groups, hipStream_t st) {
+void launch_rows(MoreArgs a, long long groups, hipStream_t st) {
+  const tqk_cache_desc& d = a.d;
+  const long long blocks = (d.group_tokens + 31) / 32, n_waves = (long long)a.n_splits * kFewWaves;
+  const long long most = ((long long)a.max_len / d.group_tokens + 2) * blocks, listed = (long long)a.n_list * blocks;
+  a.by.splits = few_div(a.n_splits, groups);
+  a.by.heads = few_div(d.n_kv_heads, groups);
+  a.by.items = few_div(a.q_items, groups);
+  a.by.heads_of = few_div(d.n_q_heads / d.n_kv_heads, 8);
+  a.by.group = few_div(d.group_tokens, a.max_len);
+  a.by.blocks = few_div(blocks, listed > most ? listed : most);
+  a.by.waves = few_div(n_waves, listed + most + d.hot_window + n_waves);
+  a.by.per_page = 1.0f / (float)d.page_tokens;
+  a.by.group_pages = d.group_tokens / d.page_tokens;
   if (a.d.head_dim == 64)
     tqk_launch_rows_64(a, (unsigned)groups, st);
   else if (a.d.head_dim == TQK_D)
@@ -416,6 +436,25 @@ int check_more(const tqk_cache_desc* d, const tqk_attend_desc* t, bool windowed)
 }
 constexpr long long kMostGroups = 1LL << 22;  // (512 threads each: fewer than 2^32)
 
+// All rows of a call in one launch, and the join of its splits.
+size_t item_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const MorePlan& mp) {
+  return mp.n_splits > 1 ? partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, mp.n_splits, d->head_dim) : 16;
+}
+int run_items(MoreArgs a, const MorePlan& mp, void* workspace, void* stream) {
+  if (mp.pairs * mp.n_splits > kMostGroups) return TQK_EINVAL;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  a.per_item = mp.per_item;
+  a.q_items = mp.q_items;
+  a.n_splits = mp.n_splits;
+  a.direct = mp.n_splits == 1;
+  a.rows = (long long)a.batch * a.d.n_q_heads * a.q_len;
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = a.part_acc + (size_t)mp.n_splits * a.rows * a.d.head_dim;
+  launch_rows(a, mp.pairs * mp.n_splits, st);
+  if (!a.direct) launch_join(join_args(a, mp.n_splits, nullptr), a.d.head_dim, st);
+  return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+}
+
 // ---- listed groups ----------------------------------------------------------
 int check_list(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
   const int rc = check_more(d, t, false);
@@ -458,43 +497,43 @@ size_t weight_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const Wei
 
 // ---- a shared prefix ---------------------------------------------------------
 struct SharedPlan {
+  bool once;            // the prefix is read once
   long long pre_pairs;  // workgroups of a split of the prefix
   int pre_splits;
-  MorePlan rest;
+  MorePlan rest;  // what follows it, or (not `once`) every sequence for itself
 };
-SharedPlan shared_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, int groups) {
-  SharedPlan s{};
-  const int gq = d->n_q_heads / d->n_kv_heads, tokens = groups * d->group_tokens;
-  s.pre_pairs = ((long long)t->batch * t->q_len * gq + 127) / 128 * d->n_kv_heads;
-  // rounds of the workgroups that fit (one a CU) times a split's tiles and the set-up,
-  // joining and rotation of about five tiles' time
-  const int tiles = (groups * ((d->group_tokens + 31) / 32) + 1) / (d->head_dim == 256 ? 1 : 2);
-  double best = 1e30;
-  for (int n = 1; n <= 64 && n <= tiles; ++n) {
-    const double rounds = (double)((s.pre_pairs * n + device_cus() - 1) / device_cus());
-    const double cost = rounds * ((tiles + n - 1) / n + 5);
-    if (cost < best - 1e-9) {
-      best = cost;
-      s.pre_splits = n;
-    }
-  }
-  s.rest = more_plan(d, t->batch, t->q_len, INT32_MAX, t->max_len - tokens, 0.0);
-  return s;
-}
 // Whether reading the prefix once pays: it takes launches of its own and a set-up, about
 // 28 us, and 3.2 a tile of its workgroups; each sequence for itself finds the others'
-// codes in cache, a block of 32 tokens and 16 rows 1.2 ns of the whole card (0.8 at
-// head_dim 64, 4.9 at 256).  Each for itself and once, 32 / 8 heads of 128: a prefix of
-// 32768 tokens, 4 sequences 58 and 87 us, 8 95 and 88, 32 340 and 117; 8192 tokens, 4
-// sequences 29 and 51; 2048 tokens, 32 sequences 35 and 54; head_dim 256, 16 / 8 heads,
-// 4096 tokens, 4 sequences 60 and 79, 16 117 and 93.
-bool prefix_pays(const tqk_cache_desc* d, const tqk_attend_desc* t, int groups, const SharedPlan& s) {
-  const int gq = d->n_q_heads / d->n_kv_heads, blocks = groups * ((d->group_tokens + 31) / 32);
-  const double scale = 256.0 / device_cus(), block = d->head_dim == 64 ? 0.8e-3 : d->head_dim == TQK_D ? 1.2e-3 : 4.9e-3;
-  const double each = (double)t->batch * (((long long)t->q_len * gq + 15) / 16) * d->n_kv_heads * blocks * block * scale;
-  const int tiles = d->head_dim == 256 ? blocks : (blocks + 1) / 2;
-  const double rounds = (double)((s.pre_pairs * s.pre_splits + device_cus() - 1) / device_cus());
-  return each > 28.0 + rounds * ((tiles + s.pre_splits - 1) / s.pre_splits) * 3.2 + (d->head_dim == 256 ? 10.0 : 0.0);
+// codes in cache, a block of 32 tokens and 8 rows 1.0 ns of the whole card (0.7 at
+// head_dim 64, 4 at 256; 16 rows of tqk_run_few a fifth more).  Each for itself and once,
+// us, 32 / 8 heads of 128: a prefix of 32768 tokens, 4 sequences 46 and 87, 8 73 and 88,
+// 32 near 300 and 108; 4096 tokens, 64 sequences 84 and 78; 2048 tokens, 32 sequences 29
+// and 54; head_dim 256, 16 / 8 heads, 4096 tokens, 4 sequences 44 and 79, 16 81 and 79.
+SharedPlan shared_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, int groups) {
+  SharedPlan s{};
+  const int gq = d->n_q_heads / d->n_kv_heads, tokens = groups * d->group_tokens, cus = device_cus();
+  const int blocks = groups * ((d->group_tokens + 31) / 32), tiles = d->head_dim == 256 ? blocks : (blocks + 1) / 2;
+  const long long rows = (long long)t->q_len * gq;  // of a workgroup each for itself: 8, or 16 a pass
+  const double block = (d->head_dim == 64 ? 0.7e-3 : d->head_dim == TQK_D ? 1.0e-3 : 4.0e-3) * (rows > 8 ? 1.2 : 1.0);
+  const double each = (double)t->batch * ((rows + 15) / 16) * d->n_kv_heads * blocks * block * 256.0 / cus;
+  const double first = d->head_dim == 256 ? 38.0 : 28.0, tile = 3.2;
+  if (each > first + tile) {
+    s.pre_pairs = ((long long)t->batch * t->q_len * gq + 127) / 128 * d->n_kv_heads;
+    // rounds of the workgroups that fit (one a CU) times a split's tiles and the set-up
+    // and joining of about five tiles' time
+    long long best = INT64_MAX, once = 0;
+    for (int n = 1; n <= 64 && n <= tiles; ++n) {
+      const long long rounds = (s.pre_pairs * n + cus - 1) / cus, run = (tiles + n - 1) / n;
+      if (rounds * (run + 5) < best) {
+        best = rounds * (run + 5);
+        once = rounds * run;
+        s.pre_splits = n;
+      }
+    }
+    s.once = each > first + (double)once * tile;
+  }
+  s.rest = more_plan(d, t->batch, t->q_len, INT32_MAX, t->max_len - (s.once ? tokens : 0), s.once ? 0.0 : 2.0);
+  return s;
 }
 int check_shared(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
   const int rc = check_more(d, t, false);
@@ -511,7 +550,7 @@ extern "C" {
 size_t tqk_attend_groups_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
   if (check_list(d, t, l) != TQK_OK || !t->batch || !t->q_len) return 0;
   const MorePlan mp = list_plan(d, t, l);
-  return mp.n_splits > 1 ? partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, mp.n_splits, d->head_dim) : 16;
+  return item_bytes(d, t, mp);
 }
 
 int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t,
@@ -524,24 +563,12 @@ int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   if (rc != TQK_OK) return rc;
   if (l->n > 0 && !groups) return TQK_EINVAL;
   if (workspace_bytes < tqk_attend_groups_workspace_bytes(d, t, l)) return TQK_EWORKSPACE;
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const MorePlan mp = list_plan(d, t, l);
-  if (mp.pairs * mp.n_splits > kMostGroups) return TQK_EINVAL;
   MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
   // (a list of none: any pointer, which is not read)
   a.groups = groups ? groups : reinterpret_cast<const int32_t*>(seq_lens);
   for (int i = 0; i < 3; ++i) a.g_stride[i] = l->stride[i];
   a.n_list = l->n;
-  a.per_item = mp.per_item;
-  a.q_items = mp.q_items;
-  a.n_splits = mp.n_splits;
-  a.direct = mp.n_splits == 1;
-  a.rows = (long long)t->batch * d->n_q_heads * t->q_len;
-  a.part_acc = static_cast<float*>(workspace);
-  a.part_ml = a.part_acc + (size_t)mp.n_splits * a.rows * d->head_dim;
-  launch_rows(a, mp.pairs * mp.n_splits, st);
-  if (!a.direct) launch_join(join_args(a, mp.n_splits, nullptr), d->head_dim, st);
-  return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+  return run_items(a, list_plan(d, t, l), workspace, stream);
 }
 
 size_t tqk_attend_weights_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) {
@@ -604,7 +631,7 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
 size_t tqk_attend_shared_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
   if (check_shared(d, t, groups) != TQK_OK || !t->batch || !t->q_len) return 0;
   const SharedPlan s = shared_plan(d, t, groups);
-  if (!prefix_pays(d, t, groups, s)) return tqk_few_workspace_bytes(d, t);
+  if (!s.once) return s.rest.q_items > 1 ? tqk_few_workspace_bytes(d, t) : item_bytes(d, t, s.rest);
   return partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, s.pre_splits + s.rest.n_splits, d->head_dim);
 }
 
@@ -618,7 +645,10 @@ int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   if (rc != TQK_OK) return rc;
   if (workspace_bytes < tqk_attend_shared_workspace_bytes(d, t, groups)) return TQK_EWORKSPACE;
   const SharedPlan s = shared_plan(d, t, groups);
-  if (!prefix_pays(d, t, groups, s)) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, workspace_bytes, stream);
+  if (!s.once) {  // (more than eight rows: sixteen a workgroup)
+    if (s.rest.q_items > 1) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, workspace_bytes, stream);
+    return run_items(more_args(d, p, t, q, seq_lens, q_lens, out), s.rest, workspace, stream);
+  }
   if (s.pre_pairs * s.pre_splits > kMostGroups || s.rest.pairs * s.rest.n_splits > kMostGroups) return TQK_EINVAL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int splits = s.pre_splits + s.rest.n_splits;

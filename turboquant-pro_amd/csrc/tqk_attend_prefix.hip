@@ -10,6 +10,10 @@
 // V^T P^T as they are; two waves share a row group, by tokens, or at head_dim 256 by
 // channels.  Weights times norms are fp16 pairs, two products.  While a tile is
 // multiplied the next one is decoded, and the one after it is on its way.
+//
+// 32768 tokens, 32 sequences, 32 / 8 heads of 128 (8 x 32 splits of 16 tiles): 73 us, 17 of
+// them once (tables, first tiles, sums out through LDS) and 3.2 a tile: its look-ups,
+// stores and reads in LDS, 96 KB, and 0.9 us of products, at two waves a SIMD.
 #include "tqk_attend_few.h"
 
 namespace {
@@ -30,6 +34,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void tqk_attend_prefix(MoreArgs a) 
   constexpr int VROW = D * VB / 8;
   constexpr int kVThreads = TT / 4 * CQ;    // values: 4 tokens x 4 channels a thread
   static_assert(kVThreads <= kPreThreads && TPT * TG == TT, "the threads cover a tile");
+  touch_args<MoreArgs>();
   const tqk_cache_desc& d = a.d;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lc = lane & 31, hl = lane >> 5;

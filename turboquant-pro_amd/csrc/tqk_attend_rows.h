@@ -18,6 +18,17 @@
 // sparse tile of a second product cost a block 16 products, 22 LDS reads and six stores.
 //
 // The next block's scores are computed beside this block's exponentials and values.
+//
+// What bounds it: a block's chain (look-ups of levels -> products -> exponentials ->
+// look-ups of centroids -> products) at two waves a SIMD, 256 registers each; three or
+// four waves spill 190 to 320 registers (313 us for 190).  Measured, 32 / 8 heads of 128:
+// 16 sequences of 32768 tokens, every group's weight kept, 171 us (3.2 TB/s; with the
+// pages in cache some 20 less, without the blocks' sums 10 less); 16 groups of 127
+// listed, ten blocks a wave, 34 us; 64 of 511 of one sequence, three blocks a wave, 20
+// us; one block a wave 14.5.  Of a short run some 9 us are set-up (lengths -> list ->
+// tables -> codes, one load after another; the tables and the group's weights meanwhile)
+// and 3 the waves' joining and rotation.  head_dim 256: 60 to 90 registers spill, 42 us
+// for 8 groups of 30, 8 sequences.
 #pragma once
 
 #include "tqk_attend_few.h"
@@ -54,17 +65,17 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
   constexpr int kSeg = 1024 / NR < kSegMost ? 1024 / NR : kSegMost;  // tokens of a stretch
   constexpr int SB = kSeg / 32, kCorr = kSeg + 4;
   const tqk_cache_desc& d = a.d;
+  touch_args<MoreArgs>();
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int ln = lane & 15, lg = lane >> 4;
   const bool is_lo = (ln & 8) != 0;
   const float lo_sel = is_lo ? 1.f : 0.f;
-  const int G = d.group_tokens, P = d.page_tokens, Hkv = d.n_kv_heads, Hq = d.n_q_heads, gq = Hq / Hkv;
-  int x = blockIdx.x;
-  const int split = x % a.n_splits;
-  x /= a.n_splits;
-  const int h = x % Hkv;
-  x /= Hkv;
-  const int q0 = a.t0 + x % a.q_items * a.per_item, b = x / a.q_items;
+  const int G = d.group_tokens, P = d.page_tokens, Hkv = d.n_kv_heads, Hq = d.n_q_heads, gq = a.by.heads_of.n;
+  int x = blockIdx.x, y = a.by.splits(x);
+  const int split = x - y * a.n_splits;
+  x = y;
+  y = a.by.heads(x);
+  const int h = x - y * Hkv, b = a.by.items(y), q0 = a.t0 + (y - b * a.q_items) * a.per_item;
 
   // a pair of key codes -> its levels, {hi, hi} and {lo, lo}; a pair of value codes
   // -> its centroids; with 4-bit keys and values one row for both.  Copies by lane:
@@ -73,33 +84,66 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
   constexpr int kKeyLog = 8, kValLog = D == 256 && VB == 4 && !kShared ? 7 : 8;  // log2 of an entry's bytes
   constexpr int kKeyCopies = kShared ? 16 : 32, kValCopies = kShared ? 32 : (1 << kValLog) / 4;
   constexpr int kKeyEntries = 1 << (2 * KB), kValEntries = 1 << (2 * VB);
-  constexpr int kOutBytes = kFewWaves * kRows8 * D * 4, kKeyBytes = kKeyEntries << kKeyLog;
+  constexpr int OST = D + 4;  // floats of a row of the waves' accumulators
+  constexpr int kOutBytes = kFewWaves * kRows8 * OST * 4, kKeyBytes = kKeyEntries << kKeyLog;
   // Both tables in one array, values from a multiple of their size on: a value's entry
   // and copy are joined by one and-or.
   constexpr int kValBytes = kShared ? 0 : kValEntries << kValLog;
   constexpr int kKeyRoom = kOutBytes > kKeyBytes ? kOutBytes : kKeyBytes;
-  __shared__ __align__(65536) uint8_t table_s[kValBytes + kKeyRoom];
-  uint8_t* const val_s = table_s + (kShared ? 128 : 0);
-  uint8_t* const key_s = table_s + kValBytes;
-  __shared__ __align__(16) float stat_s[kFewWaves][2][D];        // the group's scale and mean
-  __shared__ __align__(16) float corr_s[kFewWaves][NR][kCorr];   // scores' first values of a stretch
-  __shared__ __align__(16) float zero_s[4];
-  __shared__ __align__(16) uint16_t qc_s[D][NR];                 // queries by channel
-  __shared__ __align__(16) uint16_t qr_s[kRows8][D];             // and by row
-  __shared__ __align__(16) float lev_s[16], cen_s[16];
-  __shared__ float up_s[2][2];  // the best of the scales of a half: its loss, itself
-  __shared__ float ml_s[2][kFewWaves][kRows8];
+  // (one struct: the tables first, no gap before them)
+  struct Lds {
+    uint8_t table[kValBytes + kKeyRoom];
+    float stat[kFewWaves][2][D];       // the group's scale and mean
+    float corr[kFewWaves][NR][kCorr];  // scores' first values of a stretch
+    float zero[4];
+    uint16_t qc[D][NR];                // queries by channel
+    uint16_t qr[kRows8][D];            // and by row
+    float ml[2][kFewWaves][kRows8];
+  };
+  __shared__ __align__(65536) Lds lds;
+  uint8_t* const val_s = lds.table + (kShared ? 128 : 0);
+  uint8_t* const key_s = lds.table + kValBytes;
+  auto& stat_s = lds.stat;
+  auto& corr_s = lds.corr;
+  auto& zero_s = lds.zero;
+  auto& qc_s = lds.qc;
+  auto& qr_s = lds.qr;
+  auto& ml_s = lds.ml;
 
-  const int n = min(a.seq_lens[b], a.max_len);
+  // What waits for nothing is asked for first: the queries, a table entry's levels and
+  // centroids (a thread fills a part of one entry of each table).
+  struct Part {
+    int entry, first, pieces;  // entry -1: none
+  };
+  auto part_of = [&](int entries, int pieces) {  // of `pieces` 16-byte pieces an entry
+    const int mine = max(entries * pieces / kFewThreads, 1), each = pieces / mine;
+    return Part{tid < entries * each ? tid / each : -1, tid % each * mine, mine};
+  };
+  const Part kp = part_of(kKeyEntries, kKeyCopies / 2), vp = part_of(kValEntries, kValCopies / 4);
+  const int ke = max(kp.entry, 0), ve = max(vp.entry, 0);
+  auto level = [&](int i) { return PK ? a.p.vcent[i] : key_level(d.key_grid, i); };
+  const float lev0 = level(k_code_even(ke, KB)), lev1 = level(k_code_odd(ke, KB));
+  const float cen0 = a.p.vcent[ve & ((1 << VB) - 1)], cen1 = a.p.vcent[ve >> VB];
+  float cen[1 << VB];
+#pragma unroll
+  for (int i = 0; i < (1 << VB); ++i) cen[i] = a.p.vcent[i];
   const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-  if (tid < 16) lev_s[tid] = PK ? a.p.vcent[tid & ((1 << VB) - 1)] : key_level(d.key_grid, tid);
-  if (tid < (1 << VB)) cen_s[tid] = a.p.vcent[tid];
-  if (tid < 4) zero_s[tid] = 0.f;
   // the rows: query q0 + row / gq, head h gq + row % gq
   const int n_rows = min(a.per_item, min(m, a.t0 + a.t_len) - q0) * gq;  // (negative: none)
-  const int row = min(ln & 7, max(n_rows, 1) - 1), t = q0 + row / gq, p = n - m + t;
+  const int row = min(ln & 7, max(n_rows, 1) - 1), row_t = a.by.heads_of(row), row_h = row - row_t * gq, t = q0 + row_t;
+  // Q: this column's row, channels CPL lg + 8 m .. + 7 (rows past the last: a real one's, dropped later)
+  h8_t q8[NM];
+  {
+    const uint16_t* const qp = a.q + b * a.q_stride[0] + (h * gq + row_h) * a.q_stride[1] + min(max(t, 0), a.q_len - 1) * a.q_stride[2];
+#pragma unroll
+    for (int mm = 0; mm < NM; ++mm) q8[mm] = *reinterpret_cast<const h8_t*>(qp + CPL * lg + 8 * mm);
+  }
+  const int32_t* const list = a.groups ? a.groups + b * a.g_stride[0] + h * a.g_stride[1] + q0 * a.g_stride[2] : nullptr;
+  const int listed0 = list && lane < a.n_list ? list[lane] : -1;
+  const int n = min(a.seq_lens[b], a.max_len), p = n - m + t;
+  if (tid < 4) zero_s[tid] = 0.f;
   const int p_lo = n - m + q0, p_hi = n - m + min(q0 + a.per_item, m) - 1;
-  const int ng = n_groups_of(n, d.hot_window, G), n_cold = ng * G;
+  const int ng = n > d.hot_window ? a.by.group(n - d.hot_window - 1) + 1 : 0, n_cold = ng * G;
   auto low = [&](int pos) { return max(a.window > 0 && a.window <= pos ? pos - a.window + 1 : 0, a.skip); };
   const int lo = low(p), lo_first = low(p_lo), lo_last = low(p_hi);
   const int sinks = min(a.sinks, max(n, 0));
@@ -120,50 +164,57 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     }
     return r;
   };
-  const int nblk = (G + 31) / 32;  // blocks of a group
+  const int nblk = a.by.blocks.n;  // blocks of a group
   BlockRuns cold{0, 0, 0};
-  const int32_t* list = nullptr;
-  if (a.groups) {  // block i: block i % nblk of group list[i / nblk], up to the last that there is
-    list = a.groups + b * a.g_stride[0] + h * a.g_stride[1] + q0 * a.g_stride[2];
+  if (list) {  // block i: block i % nblk of group list[i / nblk], up to the last that there is
     int last = 0;
-    for (int i = lane; i < a.n_list; i += 64) last = (unsigned)list[i] < (unsigned)ng ? i + 1 : last;
-    for (int o = 32; o; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
-    cold.n = n_rows > 0 ? __builtin_amdgcn_readfirstlane(last) * nblk : 0;
+    for (int i = 0; i < a.n_list; i += 64) {
+      const int g = i == 0 ? listed0 : i + lane < a.n_list ? list[i + lane] : -1;
+      const uint64_t real = __builtin_amdgcn_ballot_w64((unsigned)g < (unsigned)ng);
+      last = real ? i + 64 - __builtin_clzll(real) : last;
+    }
+    cold.n = n_rows > 0 ? last * nblk : 0;
   } else {
-    cold = runs(0, n_cold, [&](int tok) { return tok / G * nblk + tok % G / 32; });
+    cold = runs(0, n_cold, [&](int tok) {
+      const int g = a.by.group(tok);
+      return g * nblk + (tok - g * G) / 32;
+    });
   }
   const BlockRuns hot = runs(n_cold, n, [&](int tok) { return (tok - n_cold) / 32; });
   // equal runs for the waves of all splits, coded ones first
   const int n_waves = a.n_splits * kFewWaves;
-  int run = max((cold.n + hot.n + n_waves - 1) / n_waves, 1);
-  while ((cold.n + run - 1) / run + (hot.n + run - 1) / run > n_waves) ++run;
-  const int cold_waves = (cold.n + run - 1) / run;
+  int run = max(a.by.waves(cold.n + hot.n + n_waves - 1), 1), cold_waves;
+  for (;; ++run) {
+    cold_waves = few_quotient(cold.n + run - 1, run);
+    if (cold_waves + few_quotient(hot.n + run - 1, run) <= n_waves) break;
+  }
   const int gw = split * kFewWaves + wave;
   const bool is_cold = gw < cold_waves;
   const int i0 = (is_cold ? gw : gw - cold_waves) * run;
   const int i1 = min(i0 + run, is_cold ? cold.n : hot.n);
 
-  // Q: this column's row, channels CPL lg + 8 m .. + 7 (rows past the last: a real one's, dropped later)
-  // (in LDS: the loop has no registers for them)
-  const int t_in = min(max(t, 0), a.q_len - 1);
-  const uint16_t* const qp = a.q + b * a.q_stride[0] + (h * gq + row % gq) * a.q_stride[1] + t_in * a.q_stride[2];
+  // (the queries in LDS: the loop has no registers for them)
   float q_top = 0.f;  // the largest |q| (what is not finite: as the largest of fp16; its rows are lost whatever the power)
   {
-    uint16_t one = 0;
+    typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
+    us2_t two = {0, 0};
 #pragma unroll
     for (int mm = 0; mm < NM; ++mm) {
-      const h8_t q8 = *reinterpret_cast<const h8_t*>(qp + CPL * lg + 8 * mm);
-      if (wave == 0 && !is_lo) *reinterpret_cast<h8_t*>(&qr_s[ln][CPL * lg + 8 * mm]) = q8;
+      if (wave == mm && !is_lo) *reinterpret_cast<h8_t*>(&qr_s[ln][CPL * lg + 8 * mm]) = q8[mm];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const _Float16 y = q8[e];
-        const uint16_t bits = __builtin_bit_cast(uint16_t, y);
-        if (wave == 0 && ln < NR) qc_s[CPL * lg + 8 * mm + e][ln] = bits;
-        const uint16_t mag = bits & 0x7FFF;
-        one = mag > one ? mag : one;
+        const _Float16 y = q8[mm][e];
+        if (wave == mm && ln < NR) qc_s[CPL * lg + 8 * mm + e][ln] = __builtin_bit_cast(uint16_t, y);
       }
+      union { h8_t h; uint32_t u[4]; } bits;
+      bits.h = q8[mm];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) two = __builtin_elementwise_max(two, __builtin_bit_cast(us2_t, bits.u[e] & 0x7FFF7FFFu));
     }
-    if constexpr (!PK) q_top = wave_reduce<true>(h2f(one < 0x7C00 ? one : (uint16_t)0x7BFF));
+    if constexpr (!PK) {
+      const uint16_t one = max(two.x, two.y);
+      q_top = wave_reduce<true>(h2f(one < 0x7C00 ? one : (uint16_t)0x7BFF));
+    }
   }
   // the coded keys' weights, this column's half of an fp16 pair: q * scale group by
   // group, or for rotated keys q @ Pi^T; over a power of two, w_up, where they pass fp16
@@ -192,8 +243,8 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
   // Every load of the loop is issued, at an index inside its table, so that the
   // waits on them stay exact.  What the tables say of 64 blocks of the run at a
   // time, one a lane: their chain of loads is paid once.
-  const float per_page = 1.0f / (float)P;
-  const int group_pages = G / P;
+  const float per_page = a.by.per_page;
+  const int group_pages = a.by.group_pages;
   // the page row of token o of group g (pages inside a group by a product: fewer
   // than 256 tokens, exact)
   auto page_row = [&](int g, int o) {
@@ -204,8 +255,8 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
   auto load_meta = [&](int i) {
     meta_i = i;
     const int blk = cold.at(min(i + lane, i1 - 1));
-    meta_g = blk / nblk;
-    meta_k = blk % nblk;
+    meta_g = a.by.blocks(blk);
+    meta_k = blk - meta_g * nblk;
     meta_tok = meta_g * G;
     if (list) {
       const int g = list[meta_g];
@@ -359,13 +410,13 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     wave_sync();
     if (PK || n_ent == 0) return;
     // Lane L takes `each` consecutive entries of the list, which is sorted by token: a
-    // token's run that ends inside the lane and is not its first is the lane's alone and
-    // is written; first and last ones may go on in the neighbours.
+    // token's run that ends inside the lane is written; the first one may have begun in
+    // the lanes before, the last one may go on in the next.
     const int each = (n_ent + 63) >> 6, mine = n_ent - lane * each, t0 = kSeg * sg;
-    float acc[NR], facc[NR];
+    float acc[NR];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) acc[i] = facc[i] = 0.f;
-    int tcur = -1, tfirst = -1;
+    for (int i = 0; i < NR; ++i) acc[i] = 0.f;
+    int tcur = -1, tf = -1;
     struct Ops {
       float mean;
       uint32_t q[NR / 2];
@@ -389,15 +440,12 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
       const int tx = (int)((y & 0xFFFFu) / D) - t0;
       const bool valid = k < mine && (unsigned)tx < (unsigned)kSeg;
       const int tk = valid ? tx : -1;
-      const bool close = tk != tcur && tcur >= 0, first = close && tfirst < 0;
-      if (close && tfirst >= 0) {
+      const bool same = tk == tcur;
+      if (!same && tcur >= 0) {
 #pragma unroll
         for (int i = 0; i < NR; ++i) corr[i * kCorr + tcur] = acc[i] + br[i];
       }
-#pragma unroll
-      for (int i = 0; i < NR; ++i) facc[i] = first ? acc[i] : facc[i];
-      tfirst = first ? tcur : tfirst;
-      const bool same = tk == tcur;
+      tf = tf < 0 ? tk : tf;
       tcur = tk;
       const float dv = valid ? (h2f((uint16_t)(y >> 16)) - o.mean) * w_down : 0.f;
 #pragma unroll
@@ -429,7 +477,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     float sv[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) sv[i] = acc[i];
-    const int tl = tcur, tf = tfirst >= 0 ? tfirst : tcur;
+    const int tl = tcur;
     const int tl_up = lane_before(tl), tf_dn = lane_after(tf);
     const int tl_prev = lane > 0 ? tl_up : -1, tf_next = lane < 63 ? tf_dn : -1;
     int kd = tl_prev;  // the last run's token `o` lanes before
@@ -446,10 +494,9 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     float sprev[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) sprev[i] = bitsf((uint32_t)lane_before((int)fbits(sv[i])));
-    if (tfirst >= 0) {  // the first run ends inside this lane: with what came before
-      const bool cin = tl_prev == tfirst;
+    if (tf >= 0 && tf != tl && tl_prev == tf) {  // the first run ends inside this lane: and what came before
 #pragma unroll
-      for (int i = 0; i < NR; ++i) corr[i * kCorr + tfirst] = facc[i] + (cin ? sprev[i] : 0.f) + br[i];
+      for (int i = 0; i < NR; ++i) corr[i * kCorr + tf] += sprev[i];
     }
     if (tl >= 0 && tf_next != tl) {
 #pragma unroll
@@ -499,37 +546,44 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     load_values(first);
   }
 
-  lds_barrier();
-
-  // the scale of the value codebook: candidate 1 + i / 128 whose centroids lose
-  // least to fp16, the first of equals; half of them by even waves, half by odd ones
+  // ---- the tables, while the first codes are on their way
   {
-    const float g = 1.0f + (float)(2 * lane + wave % 2) * (1.0f / 128);
-    float err = 0.f;
+    const uint2 y = split_pair(lev0, lev1);
+    if (kp.entry >= 0)
 #pragma unroll
-    for (int i = 0; i < (1 << VB); ++i) {
-      const float y = cen_s[i] * g, r = y - (float)(_Float16)y;
-      err = fmaf(r, r, err);
-    }
-    err *= __builtin_amdgcn_rcpf(g * g);
-    const float best = -wave_reduce<true>(-err);
-    const uint64_t first = __builtin_amdgcn_ballot_w64(err == best);
-    if (wave < 2 && lane == 0) {
-      up_s[wave][0] = best;
-      up_s[wave][1] = 1.0f + (float)(first ? 2 * __builtin_ctzll(first) + wave : 0) * (1.0f / 128);
-    }
+      for (int k = 0; k < kp.pieces; ++k)  // (entries apart by a table row: each begins at another piece)
+        *reinterpret_cast<u32x4_t*>(key_s + (ke << kKeyLog) + 16 * (kp.first + (k + ke) % kp.pieces)) = u32x4_t{y.x, y.y, y.x, y.y};
   }
-  for (int i = tid; i < kKeyEntries * kKeyCopies / 2; i += kFewThreads) {
-    const int e = i / (kKeyCopies / 2);
-    const uint2 y = split_pair(lev_s[k_code_even(e, KB)], lev_s[k_code_odd(e, KB)]);
-    *reinterpret_cast<u32x4_t*>(key_s + (e << kKeyLog) + 16 * (i % (kKeyCopies / 2))) = u32x4_t{y.x, y.y, y.x, y.y};
+  // the scale of the value codebook: candidate 1 + i / 128 whose centroids lose least to
+  // fp16
+  float up;
+  {
+    float best = INFINITY, at = 1.f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const float g = 1.0f + (float)(2 * lane + half) * (1.0f / 128);
+      float err = 0.f;
+#pragma unroll
+      for (int i = 0; i < (1 << VB); ++i) {
+        const float y = cen[i] * g, r = y - (float)(_Float16)y;
+        err = fmaf(r, r, err);
+      }
+      err *= __builtin_amdgcn_rcpf(g * g);
+      if (err < best) {
+        best = err;
+        at = g;
+      }
+    }
+    const float least = -wave_reduce<true>(-best);
+    const uint64_t first = __builtin_amdgcn_ballot_w64(best == least);
+    up = bitsf((uint32_t)__builtin_amdgcn_readlane((int)fbits(at), first ? __builtin_ctzll(first) : 0));
   }
-  lds_barrier();
-  const float up = up_s[up_s[1][0] < up_s[0][0]][1];
-  for (int i = tid; i < kValEntries * kValCopies / 4; i += kFewThreads) {
-    const int e = i / (kValCopies / 4);
-    const uint32_t y = pk_f16(cen_s[e & ((1 << VB) - 1)] * up, cen_s[e >> VB] * up);
-    *reinterpret_cast<u32x4_t*>(val_s + (e << kValLog) + 16 * (i % (kValCopies / 4))) = u32x4_t{y, y, y, y};
+  {
+    const uint32_t y = pk_f16(cen0 * up, cen1 * up);
+    if (vp.entry >= 0)
+#pragma unroll
+      for (int k = 0; k < vp.pieces; ++k)
+        *reinterpret_cast<u32x4_t*>(val_s + (ve << kValLog) + 16 * (vp.first + (k + ve) % vp.pieces)) = u32x4_t{y, y, y, y};
   }
   // a table read: the field of `bits` bits at bit `bit` of the word array w, as an
   // entry of 2^lg bytes and this lane's copy in it
@@ -684,100 +738,111 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     int k = of(meta_k, i0), tok0 = of(meta_tok, i0), g = of(meta_g, i0);
     Rows after = next_rows;
     load_keys(i0 + 1, next_rows);
-    for (int i = i0;;) {
-      const int cnt = min(32, G - 32 * k);
-      if (i + 3 >= meta_i + 64 && i + 1 < i1) load_meta(i + 1);
-      const bool more = i + 1 < i1;
-      after = rows_of(i + 2);
+    int i = i0;
+    // The last block without a next one's scores beside it, in a copy of the loop's body
+    // (the last one's again in their place: 2 us more of every run)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = S[e / 4][e % 4], z = y + row_ror<8>(y);
-        S[e / 4][e % 4] = PK ? z * norm_of(kn_now, e) : z;  // (PK: score = |k| (q_rot . centroids))
-      }
-      if (__builtin_expect(up_now != 1.f, 0)) {
-        S[0] *= up_now;
-        S[1] *= up_now;
-      }
-      const bool whole = cnt == 32 && all_see(tok0, 32);
-      // (a hidden token's norm may be anything: its weight is zero)
-      float nv[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) nv[e] = norm_of(norm, e);
-      mask_and_max(S, tok0, cnt, whole, [&](int e, bool seen) { nv[e] = seen ? nv[e] : 0.f; });
-      const int i_n = min(i + 1, i1 - 1), k_n = of(meta_k, i_n), tok_n = of(meta_tok, i_n), g_n = of(meta_g, i_n);
-      if constexpr (!PK) {
+    for (int part = 0; part < 2; ++part) {
+      const bool more = part == 0;
+      while (!more || i + 1 < i1) {
+        const int cnt = min(32, G - 32 * k);
         if (more) {
-          const bool apart = i + 1 == cold.n0;  // (the second run may start inside a group)
-          if (k_n == 0 || apart) begin_group();
-          if (k_n % SB == 0 || apart) begin_stretch(k_n / SB);
+          if (i + 3 >= meta_i + 64) load_meta(i + 1);
+          after = rows_of(i + 2);
         }
-      }
-      f4_t N[2];
-      product(N, k_n % SB);
-      if constexpr (PK) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) kn_now[e] = kn[e];
-      }
-      up_now = w_up;
-      load_keys(i + 2, after);
-      float w[8];
-      const float sum = weights(S, w);
-      float pw[8];
+        for (int e = 0; e < 8; ++e) {
+          const float y = S[e / 4][e % 4], z = y + row_ror<8>(y);
+          S[e / 4][e % 4] = PK ? z * norm_of(kn_now, e) : z;  // (PK: score = |k| (q_rot . centroids))
+        }
+        if (__builtin_expect(up_now != 1.f, 0)) {
+          S[0] *= up_now;
+          S[1] *= up_now;
+        }
+        const bool whole = cnt == 32 && all_see(tok0, 32);
+        // (a hidden token's norm may be anything: its weight is zero)
+        float nv[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pw[e] = w[e] * nv[e];
-      }
-      const h8_t pf = halves(pw);
-      // V^T P^T: row ln of the first operand is channel NC ln + j of the piece
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        if constexpr (TILED) {
-          // a channel's token pairs side by side in the unit's bits
-#pragma unroll
-          for (int j = 0; j < NC; ++j) {
-            union { h8_t h; uint32_t u[4]; } y;
-#pragma unroll
-            for (int f = 0; f < 4; ++f) y.u[f] = centroids(vw[0] + 4 * (f / 2), (2 * j + f % 2) * 2 * VB);
-            O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, pf, O[j], 0, 0, 0);
+        for (int e = 0; e < 8; ++e) nv[e] = norm_of(norm, e);
+        mask_and_max(S, tok0, cnt, whole, [&](int e, bool seen) { nv[e] = seen ? nv[e] : 0.f; });
+        int k_n = 0, tok_n = 0, g_n = 0;
+        f4_t N[2];
+        if (more) {
+          k_n = of(meta_k, i + 1);
+          tok_n = of(meta_tok, i + 1);
+          g_n = of(meta_g, i + 1);
+          if constexpr (!PK) {
+            const bool apart = i + 1 == cold.n0;  // (the second run may start inside a group)
+            if (k_n == 0 || apart) begin_group();
+            if (k_n % SB == 0 || apart) begin_stretch(k_n / SB);
           }
-        } else {
-          // by channel pairs, the tokens of a channel then brought together
+          product(N, k_n % SB);
+          if constexpr (PK) {
 #pragma unroll
-          for (int j = 0; j < NC; j += 2) {
-            uint32_t two[8];
+            for (int e = 0; e < 8; ++e) kn_now[e] = kn[e];
+          }
+          up_now = w_up;
+          load_keys(i + 2, after);
+        }
+        float w[8];
+        const float sum = weights(S, w);
+        float pw[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t y = D == 64 ? vw[s][e] >> ((ln & 1) * 4 * VB) : vw[s][e];
-              two[e] = centroids(&y, VB * j);
+        for (int e = 0; e < 8; ++e) {
+          pw[e] = w[e] * nv[e];
+        }
+        const h8_t pf = halves(pw);
+        // V^T P^T: row ln of the first operand is channel NC ln + j of the piece
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          if constexpr (TILED) {
+            // a channel's token pairs side by side in the unit's bits
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+              union { h8_t h; uint32_t u[4]; } y;
+#pragma unroll
+              for (int f = 0; f < 4; ++f) y.u[f] = centroids(vw[0] + 4 * (f / 2), (2 * j + f % 2) * 2 * VB);
+              O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.h, pf, O[j], 0, 0, 0);
             }
-            union { h8_t h; uint32_t u[4]; } y0, y1;
+          } else {
+            // by channel pairs, the tokens of a channel then brought together
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              y0.u[f] = __builtin_amdgcn_perm(two[2 * f + 1], two[2 * f], 0x05040100u);
-              y1.u[f] = __builtin_amdgcn_perm(two[2 * f + 1], two[2 * f], 0x07060302u);
+            for (int j = 0; j < NC; j += 2) {
+              uint32_t two[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t y = D == 64 ? vw[s][e] >> ((ln & 1) * 4 * VB) : vw[s][e];
+                two[e] = centroids(&y, VB * j);
+              }
+              union { h8_t h; uint32_t u[4]; } y0, y1;
+#pragma unroll
+              for (int f = 0; f < 4; ++f) {
+                y0.u[f] = __builtin_amdgcn_perm(two[2 * f + 1], two[2 * f], 0x05040100u);
+                y1.u[f] = __builtin_amdgcn_perm(two[2 * f + 1], two[2 * f], 0x07060302u);
+              }
+              O[NC * s + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y0.h, pf, O[NC * s + j], 0, 0, 0);
+              O[NC * s + j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y1.h, pf, O[NC * s + j + 1], 0, 0, 0);
             }
-            O[NC * s + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y0.h, pf, O[NC * s + j], 0, 0, 0);
-            O[NC * s + j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y1.h, pf, O[NC * s + j + 1], 0, 0, 0);
           }
         }
-      }
-      if (a.block_ml) {
-        const float y = colgroup_sum(sum);
-        if (lg == 0 && ln < n_rows && !is_lo) {
-          const long long o = ((((long long)b * Hq + h * gq + row % gq) * a.t_len + t - a.t0) * a.blocks + g * nblk + k) * 2;
-          a.block_ml[o] = m_run;
-          a.block_ml[o + 1] = y;
+        if (a.block_ml) {
+          const float y = colgroup_sum(sum);
+          if (lg == 0 && ln < n_rows && !is_lo) {
+            const long long o = ((((long long)b * Hq + h * gq + row_h) * a.t_len + t - a.t0) * a.blocks + g * nblk + k) * 2;
+            a.block_ml[o] = m_run;
+            a.block_ml[o + 1] = y;
+          }
         }
+        if (!more) break;
+        load_values(next_rows);
+        next_rows = after;
+        S[0] = N[0];
+        S[1] = N[1];
+        k = k_n;
+        tok0 = tok_n;
+        g = g_n;
+        ++i;
       }
-      if (!more) break;
-      load_values(next_rows);
-      next_rows = after;
-      S[0] = N[0];
-      S[1] = N[1];
-      k = k_n;
-      tok0 = tok_n;
-      g = g_n;
-      ++i;
     }
   } else if (!is_cold) {
     // uncoded blocks, straight from the ring
@@ -921,15 +986,28 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
       ml_s[1][wave][ln] = l;
     }
     lds_barrier();  // (every wave has read its last levels)
+    // (the two columns of a row write two of its four stretches of channels each)
+    float* const to = out_s + (wave * kRows8 + (ln & 7)) * OST;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int j = 0; j < NC; ++j)
+      for (int j = 0; j < NC; j += 4) {
+        f4_t z[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = O[NC * s + j][e], z = y + row_ror<8>(y);
-          if (!is_lo) out_s[(wave * kRows8 + ln) * D + 128 * s + NC * (4 * lg + e) + j] = z;
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float y = O[NC * s + j + k][e];
+            z[e][k] = y + row_ror<8>(y);
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          f4_t y;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = is_lo ? z[2 + e][k] : z[e][k];
+          *reinterpret_cast<f4_t*>(to + 128 * s + NC * (4 * lg + (is_lo ? 2 : 0) + e) + j) = y;
         }
+      }
   }
   __syncthreads();
   constexpr int kRowGroups = kFewThreads / D;                 // rows side by side
@@ -947,7 +1025,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
 #pragma unroll
     for (int w = 0; w < kFewWaves; ++w) {
       const float mw = ml_s[0][w][r], f = mw == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(mw - ms[k]));
-      const float y = out_s[(w * kRows8 + r) * D + j];
+      const float y = out_s[(w * kRows8 + r) * OST + j];
       ls[k] = fmaf(ml_s[1][w][r], f, ls[k]);
       // (a state without a maximum holds zeros; a NaN among its scores leaves it one)
       if (w < first_hot) cs[k] += y * f; else hs[k] += y * f;
@@ -957,16 +1035,17 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
     __syncthreads();
     // the coded sums over their weights' sum (within fp16's range then) as an
     // fp16 pair, times Pi's
-    uint16_t* const c_s = reinterpret_cast<uint16_t*>(key_s);                 // [2][8][D]
-    float* const y_s = reinterpret_cast<float*>(key_s) + kRows8 * D;  // [8][D]
+    constexpr int CST = D + 8;
+    uint16_t* const c_s = reinterpret_cast<uint16_t*>(key_s);           // [2][8][CST]
+    float* const y_s = reinterpret_cast<float*>(key_s) + kRows8 * CST;  // [8][D]
 #pragma unroll
     for (int k = 0; k < RPT; ++k) {
       const int r = r0 + kRowGroups * k;
       if (r < kRows8) {
         const float y = ls[k] != 0.f ? cs[k] / (ls[k] * up) : 0.f;
         const _Float16 hi = (_Float16)y;
-        c_s[r * D + j] = __builtin_bit_cast(uint16_t, hi);
-        c_s[(kRows8 + r) * D + j] = f2h(y - (float)hi);
+        c_s[r * CST + j] = __builtin_bit_cast(uint16_t, hi);
+        c_s[(kRows8 + r) * CST + j] = f2h(y - (float)hi);
       }
     }
     __syncthreads();
@@ -984,7 +1063,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
             pl[e] = (_Float16)(y - (float)ph[e]);
           }
           // (rows 8 to 15 of the operand: the sums' second halves)
-          const h8_t ch = *reinterpret_cast<const h8_t*>(c_s + ln * D + 32 * mm + 8 * lg);
+          const h8_t ch = *reinterpret_cast<const h8_t*>(c_s + ln * CST + 32 * mm + 8 * lg);
           acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, pl, acc, 0, 0, 0);
           acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, ph, acc, 0, 0, 0);
         }
@@ -1008,7 +1087,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void tqk_attend_rows(MoreArgs a) {
   for (int k = 0; k < RPT; ++k) {
     const int r = r0 + kRowGroups * k;
     if (r >= all_rows) continue;
-    const int tr = q0 + r / gq, hq = h * gq + r % gq;
+    const int rt = a.by.heads_of(r), tr = q0 + rt, hq = h * gq + r - rt * gq;
     if (a.direct) {
       const long long o = b * a.o_stride[0] + hq * a.o_stride[1] + tr * a.o_stride[2] + j;
       // (a query in a coded group that is not listed may see nothing)

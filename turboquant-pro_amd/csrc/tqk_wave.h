@@ -88,4 +88,16 @@ __device__ __forceinline__ uint32_t pk_f16(float x, float y) {
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
+// A word of every line of a kernel's arguments: the lines arrive together, where the
+// loads that use them wait for one line after another (eleven lines: 2 us of a kernel).
+template <class Args>
+__device__ __forceinline__ void touch_args() {
+  typedef __attribute__((address_space(4))) const uint32_t arg_t;
+  arg_t* const args = (arg_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  uint32_t y = 0;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(Args) / 4); i += 16) y |= args[i];
+  asm volatile("" ::"s"(y));
+}
+
 }  // namespace
