@@ -551,7 +551,8 @@ int tqk_select_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
  *   seq_lens [batch] i32, rewritten;  weights [batch][n_kv_heads][max_groups_per_seq] fp32, rewritten
  *   kept [batch][keep] i32: the former index of every group that stays, ascending, then -1
  * zero_point 0 and 1 (the "bias" zero points of later groups belong to their positions:
- * TQK_EUNSUPPORTED); hot_ring * 16 bytes within 64 KiB.
+ * TQK_EUNSUPPORTED); hot_ring * 16 bytes within 64 KiB; max_pages_per_seq reaches as
+ * far as max_groups_per_seq (else TQK_EINVAL).
  */
 size_t tqk_evict_groups_workspace_bytes(const tqk_cache_desc* d, int32_t batch);
 

@@ -224,6 +224,8 @@ def test_evictions(kw, want):
 def test_evictions_of_other_caches():
     c = Call(dict(zero_point=2), null=())
     assert c.evict()[1] == c.N.TQK_EUNSUPPORTED
+    c = Call(dict(max_pages_per_seq=23))  # (a page short of six groups)
+    assert c.evict()[1] == c.N.TQK_EINVAL
     c = Call(shift=("kept",), null=())
     assert c.evict()[1] == c.N.TQK_EWORKSPACE
     for cache, want in ((dict(hot_window=4096, hot_ring=4096, group_tokens=2048), "EWORKSPACE"),

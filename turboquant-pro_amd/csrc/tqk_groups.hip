@@ -585,6 +585,8 @@ int tqk_evict_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, int32_t b
   if (rc != TQK_OK) return rc;
   if (d->zero_point == 2) return TQK_EUNSUPPORTED;
   if (batch < 0 || batch > 65535 || keep < 0 || first < 0 || last < 0 || (long long)first + last > keep) return TQK_EINVAL;
+  // (a sequence as long as its groups' table has its pages)
+  if ((long long)d->max_groups_per_seq * (d->group_tokens / d->page_tokens) > d->max_pages_per_seq) return TQK_EINVAL;
   const int cb = ring_columns(d);
   if (!cb) return TQK_EUNSUPPORTED;
   if (!batch) return TQK_OK;
