@@ -8,9 +8,8 @@
 // Weights: softmax_j = 2^(s_j - M) / L with a row's maximum M and sum L, which are
 // known when its splits are joined.  A wave writes each block's own maximum and sum
 // beside its partial results (8 bytes a row and block of 32 tokens: 10 of the step's
-// 170 us), the join writes M and L, and tqk_group_weights adds 2^(m - M) l / L over a kv
-// head's rows and a group's blocks, in one order and 64 bits: no atomics.  6 us at 16
-// sequences of 32768 tokens, 16.8 MB of sums.
+// 170 us); workgroups beside the join's add 2^(m - M) l / L over a kv head's rows and a
+// group's blocks, in one order and 64 bits: no atomics.
 //
 // A shared prefix: rows of all sequences over one copy of its codes, then each
 // sequence's rows over its other tokens; one join takes both.
@@ -30,7 +29,6 @@ struct JoinMoreArgs {
   const int32_t* seq_lens;
   const int32_t* q_lens;
   void* out;
-  float* row_ml;  // [row][2]: maximum and sum over all splits, or null
   long long rows;
   long long o_stride[3];
   int n_splits, n_q_heads, q_len, max_len, out_type, t0, t_len;
@@ -40,11 +38,10 @@ struct JoinMoreArgs {
 // eight of them on their way at a time (one after another they are a chain of loads:
 // 23 splits 8.7 us, where four waves take 4), D / 64 channels a lane.
 template <int D, int NW>
-__global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
-  touch_args<JoinMoreArgs>();
+__device__ void join_rows(const JoinMoreArgs& a, unsigned block) {
   constexpr int E = D / 64, kAhead = 8;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % NW;
-  const long long row = (long long)blockIdx.x * (4 / NW) + wave / NW;
+  const long long row = (long long)block * (4 / NW) + wave / NW;
   __shared__ float acc_s[4][D], ml_s[4][2];
   const bool real = row < a.rows;
   const long long from = real ? row : 0;
@@ -118,10 +115,12 @@ __global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
     if (a.out_type == 0) static_cast<float*>(a.out)[o + e] = y;
     else static_cast<_Float16*>(a.out)[o + e] = (_Float16)y;
   }
-  if (a.row_ml && lane == 0) {
-    a.row_ml[2 * row] = M;
-    a.row_ml[2 * row + 1] = l;
-  }
+}
+
+template <int D, int NW>
+__global__ __launch_bounds__(256) void tqk_join_more(JoinMoreArgs a) {
+  touch_args<JoinMoreArgs>();
+  join_rows<D, NW>(a, blockIdx.x);
 }
 
 // The same where the first `pre` splits hold sums of centroids (of a shared prefix): four
@@ -265,43 +264,87 @@ __global__ __launch_bounds__(1024) void tqk_join_shared(JoinMoreArgs a, const fl
 
 struct WeightArgs {
   tqk_cache_desc d;
-  const int32_t* seq_lens;
-  const int32_t* q_lens;
   const float* block_ml;  // [row][blocks][2]
-  const float* row_ml;    // [row][2]
   float* weights;         // [sequence][kv head][max_groups_per_seq]
-  int q_len, max_len, window, sinks, t0, t_len, blocks, nblk;
+  int window, sinks, blocks, nblk, chunks;
+  unsigned join_blocks;  // workgroups that join rows; those behind them add weights up
 };
 
-// weights += what the launch's queries gave every group.  A thread a block of 32
-// tokens (blockIdx.x: whole groups of them), rows one after another.
-__global__ __launch_bounds__(256) void tqk_group_weights(WeightArgs a) {
-  touch_args<WeightArgs>();
+// weights += what the launch's queries gave every group.  A thread a block of 32 tokens
+// (a workgroup: whole groups of them), rows one after another.  A row's maximum and sum
+// over its splits are found here once more, by a thread a row, so that no launch waits
+// for the join's (4.5 us of a step).
+constexpr int kWeightRows = 256;  // at a time
+__device__ void group_weights(const JoinMoreArgs& ja, const WeightArgs& a, unsigned block) {
   const tqk_cache_desc& d = a.d;
   const int G = d.group_tokens, Hkv = d.n_kv_heads, gq = d.n_q_heads / Hkv;
-  const int h = blockIdx.y % Hkv, b = blockIdx.y / Hkv, tid = threadIdx.x;
+  const int chunk = block % a.chunks, h = block / a.chunks % Hkv, b = block / a.chunks / Hkv, tid = threadIdx.x;
   const int per = 256 / a.nblk;  // groups of a workgroup
-  const int n = min(a.seq_lens[b], a.max_len), ng = n_groups_of(n, d.hot_window, G);
-  const int m = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-  const int g = blockIdx.x * per + tid / a.nblk, k = tid % a.nblk;
+  const int n = min(ja.seq_lens[b], ja.max_len), ng = n_groups_of(n, d.hot_window, G);
+  const int m = ja.q_lens ? min(max(ja.q_lens[b], 0), ja.q_len) : ja.q_len;
+  const int g = chunk * per + tid / a.nblk, k = tid % a.nblk;
   const int first = g * G + 32 * k, last = first + min(32, G - 32 * k) - 1;
   const bool mine = tid < per * a.nblk && g < ng;
-  const int t_end = min(m, a.t0 + a.t_len), sinks = min(a.sinks, max(n, 0));
+  const int t_begin = max(ja.t0, m - n), t_end = min(m, ja.t0 + ja.t_len), sinks = min(a.sinks, max(n, 0));
+  const int each = max(t_end - t_begin, 0), rows = gq * each;
+  if (chunk * per >= ng || rows == 0) return;  // (the whole workgroup)
+  const long long at = mine ? g * a.nblk + k : 0;
+  __shared__ float M_s[kWeightRows], L_s[kWeightRows];
+  __shared__ double sum_s[256];
   double sum = 0.0;
-  for (int i = 0; i < gq; ++i) {
-    const long long row0 = ((long long)b * d.n_q_heads + h * gq + i) * a.t_len - a.t0;
-    for (int t = max(a.t0, m - n); t < t_end; ++t) {
-      const int p = n - m + t, lo = a.window > 0 && a.window <= p ? p - a.window + 1 : 0;
-      // (only blocks that this row sees were visited)
-      if (mine && first <= p && (min(last, p) >= lo || first < sinks)) {
-        const float* x = a.block_ml + ((row0 + t) * a.blocks + g * a.nblk + k) * 2;
-        const float* r = a.row_ml + 2 * (row0 + t);
-        const float l = x[1];
-        if (l != 0.f) sum += (double)(__builtin_amdgcn_exp2f(x[0] - r[0]) * l / r[1]);
+  for (int r0 = 0; r0 < rows; r0 += kWeightRows) {
+    const int n_rows = min(kWeightRows, rows - r0);
+    __syncthreads();  // (the rows before are read)
+    if (tid < n_rows) {
+      const int i = (r0 + tid) / each, t = t_begin + (r0 + tid) % each;
+      const float* const ml = ja.part_ml + 2 * (((long long)b * d.n_q_heads + h * gq + i) * ja.t_len + t - ja.t0);
+      float M = -INFINITY, L = 0.f;
+      for (int s0 = 0; s0 < ja.n_splits; s0 += 8) {
+        float m_[8], l_[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float* const y = ml + 2 * min(s0 + u, ja.n_splits - 1) * ja.rows;
+          m_[u] = y[0];
+          l_[u] = s0 + u < ja.n_splits ? y[1] : 0.f;
+        }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) top = fmaxf(top, m_[u]);
+        L *= M == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(M - top));
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          L = fmaf(l_[u], m_[u] == -INFINITY ? 0.f : above_zero(__builtin_amdgcn_exp2f(m_[u] - top)), L);
+        M = top;
+      }
+      M_s[tid] = M;
+      L_s[tid] = L;
+    }
+    __syncthreads();
+    int i = r0 / each, t = t_begin + r0 % each;
+    for (int j0 = 0; j0 < n_rows; j0 += 8) {  // (eight rows' numbers on their way at once, summed in order)
+      float m_[8], l_[8];
+      int p[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const long long row = ((long long)b * d.n_q_heads + h * gq + i) * ja.t_len + t - ja.t0;
+        p[u] = j0 + u < n_rows ? n - m + t : -1;
+        m_[u] = a.block_ml[(row * a.blocks + at) * 2];
+        l_[u] = a.block_ml[(row * a.blocks + at) * 2 + 1];
+        if (j0 + u + 1 < n_rows && ++t == t_end) {
+          t = t_begin;
+          ++i;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int lo = a.window > 0 && a.window <= p[u] ? p[u] - a.window + 1 : 0;
+        // (only blocks that this row sees were visited)
+        const bool seen = mine && first <= p[u] && (min(last, p[u]) >= lo || first < sinks);
+        const int j = min(j0 + u, kWeightRows - 1);
+        if (seen && l_[u] != 0.f) sum += (double)(__builtin_amdgcn_exp2f(m_[u] - M_s[j]) * l_[u] / L_s[j]);
       }
     }
   }
-  __shared__ double sum_s[256];
   sum_s[tid] = sum;
   __syncthreads();
   if (mine && k == 0) {
@@ -312,21 +355,44 @@ __global__ __launch_bounds__(256) void tqk_group_weights(WeightArgs a) {
   }
 }
 
-template <int D>
-void launch_join_rows(const JoinMoreArgs& a, hipStream_t st) {
-  // (few rows: a workgroup each; many, whose waves hide each other's loads, four)
-  if (a.n_splits > 4 && a.rows <= 4096)
-    hipLaunchKernelGGL((tqk_join_more<D, 4>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((tqk_join_more<D, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+struct JoinWeightArgs {
+  JoinMoreArgs j;
+  WeightArgs w;
+};
+template <int D, int NW>
+__global__ __launch_bounds__(256) void tqk_join_weights(JoinWeightArgs a) {
+  touch_args<JoinWeightArgs>();
+  if (blockIdx.x < a.w.join_blocks) join_rows<D, NW>(a.j, blockIdx.x);
+  else group_weights(a.j, a.w, blockIdx.x - a.w.join_blocks);
 }
-void launch_join(const JoinMoreArgs& a, int D, hipStream_t st) {
+
+// (few rows: a workgroup each; many, whose waves hide each other's loads, four)
+bool join_apart(const JoinMoreArgs& a) { return a.n_splits > 4 && a.rows <= 4096; }
+unsigned join_blocks(const JoinMoreArgs& a) { return (unsigned)(join_apart(a) ? a.rows : (a.rows + 3) / 4); }
+
+// `w`: with the weights of `blocks` workgroups, or null
+template <int D>
+void launch_join_rows(const JoinMoreArgs& a, const WeightArgs* w, unsigned blocks, hipStream_t st) {
+  if (w) {
+    const JoinWeightArgs x{a, *w};
+    const dim3 grid(w->join_blocks + blocks);
+    if (join_apart(a))
+      hipLaunchKernelGGL((tqk_join_weights<D, 4>), grid, dim3(256), 0, st, x);
+    else
+      hipLaunchKernelGGL((tqk_join_weights<D, 1>), grid, dim3(256), 0, st, x);
+  } else if (join_apart(a)) {
+    hipLaunchKernelGGL((tqk_join_more<D, 4>), dim3(join_blocks(a)), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((tqk_join_more<D, 1>), dim3(join_blocks(a)), dim3(256), 0, st, a);
+  }
+}
+void launch_join(const JoinMoreArgs& a, const WeightArgs* w, unsigned blocks, int D, hipStream_t st) {
   if (D == 64)
-    launch_join_rows<64>(a, st);
+    launch_join_rows<64>(a, w, blocks, st);
   else if (D == TQK_D)
-    launch_join_rows<TQK_D>(a, st);
+    launch_join_rows<TQK_D>(a, w, blocks, st);
   else
-    launch_join_rows<256>(a, st);
+    launch_join_rows<256>(a, w, blocks, st);
 }
 
 void launch_rows(MoreArgs a, long long groups, hipStream_t st) {
@@ -400,14 +466,13 @@ MoreArgs more_args(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_a
   return a;
 }
 
-JoinMoreArgs join_args(const MoreArgs& a, int splits, float* row_ml) {
+JoinMoreArgs join_args(const MoreArgs& a, int splits) {
   JoinMoreArgs j{};
   j.part_acc = a.part_acc;
   j.part_ml = a.part_ml;
   j.seq_lens = a.seq_lens;
   j.q_lens = a.q_lens;
   j.out = a.out;
-  j.row_ml = row_ml;
   j.rows = a.rows;
   for (int i = 0; i < 3; ++i) j.o_stride[i] = a.o_stride[i];
   j.n_splits = splits;
@@ -451,7 +516,7 @@ int run_items(MoreArgs a, const MorePlan& mp, void* workspace, void* stream) {
   a.part_acc = static_cast<float*>(workspace);
   a.part_ml = a.part_acc + (size_t)mp.n_splits * a.rows * a.d.head_dim;
   launch_rows(a, mp.pairs * mp.n_splits, st);
-  if (!a.direct) launch_join(join_args(a, mp.n_splits, nullptr), a.d.head_dim, st);
+  if (!a.direct) launch_join(join_args(a, mp.n_splits), nullptr, 0, a.d.head_dim, st);
   return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
 }
 
@@ -492,7 +557,7 @@ WeightPlan weight_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
 }
 size_t weight_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const WeightPlan& w) {
   const long long rows = (long long)t->batch * d->n_q_heads * w.t_len;
-  return partial_bytes(rows, w.mp.n_splits, d->head_dim) + (size_t)rows * 8 + (size_t)rows * w.blocks * 8;
+  return partial_bytes(rows, w.mp.n_splits, d->head_dim) + (size_t)rows * w.blocks * 8;
 }
 
 // ---- a shared prefix ---------------------------------------------------------
@@ -590,6 +655,8 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
   if (w.mp.pairs * w.mp.n_splits > kMostGroups) return TQK_EINVAL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int nblk = (d->group_tokens + 31) / 32, per = 256 / nblk, ng = w.blocks / nblk;
+  const int chunks = (ng + per - 1) / per;
+  if ((long long)chunks * t->batch * d->n_kv_heads >= 1 << 23) return TQK_EINVAL;  // (and the join's: fewer than 2^24)
   MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
   a.per_item = w.mp.per_item;
   a.n_splits = w.mp.n_splits;
@@ -600,29 +667,20 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
     a.q_items = (a.t_len + a.per_item - 1) / a.per_item;
     a.rows = (long long)t->batch * d->n_q_heads * a.t_len;
     a.part_ml = a.part_acc + (size_t)a.n_splits * a.rows * d->head_dim;
-    float* const row_ml = a.part_ml + (size_t)a.n_splits * a.rows * 2;
-    a.block_ml = row_ml + (size_t)a.rows * 2;
+    a.block_ml = a.part_ml + (size_t)a.n_splits * a.rows * 2;
     launch_rows(a, (long long)t->batch * a.q_items * d->n_kv_heads * a.n_splits, st);
-    launch_join(join_args(a, a.n_splits, row_ml), d->head_dim, st);
-    if (ng > 0) {
-      WeightArgs g{};
-      g.d = *d;
-      g.seq_lens = seq_lens;
-      g.q_lens = q_lens;
-      g.block_ml = a.block_ml;
-      g.row_ml = row_ml;
-      g.weights = weights;
-      g.q_len = t->q_len;
-      g.max_len = t->max_len;
-      g.window = t->window;
-      g.sinks = t->sinks;
-      g.t0 = a.t0;
-      g.t_len = a.t_len;
-      g.blocks = w.blocks;
-      g.nblk = nblk;
-      hipLaunchKernelGGL(tqk_group_weights, dim3((unsigned)((ng + per - 1) / per), (unsigned)(t->batch * d->n_kv_heads)),
-                         dim3(256), 0, st, g);
-    }
+    const JoinMoreArgs j = join_args(a, a.n_splits);
+    WeightArgs g{};
+    g.d = *d;
+    g.block_ml = a.block_ml;
+    g.weights = weights;
+    g.window = t->window;
+    g.sinks = t->sinks;
+    g.blocks = w.blocks;
+    g.nblk = nblk;
+    g.chunks = chunks;
+    g.join_blocks = join_blocks(j);
+    launch_join(j, chunks ? &g : nullptr, (unsigned)(chunks * t->batch * d->n_kv_heads), d->head_dim, st);
     if (hipGetLastError() != hipSuccess) return TQK_EHIP;
   }
   return TQK_OK;
@@ -665,7 +723,7 @@ int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   a.q_items = s.rest.q_items;
   a.n_splits = s.rest.n_splits;
   launch_rows(a, s.rest.pairs * s.rest.n_splits, st);
-  const JoinMoreArgs j = join_args(a, splits, nullptr);
+  const JoinMoreArgs j = join_args(a, splits);
   const dim3 grid((unsigned)((a.rows + 3) / 4));
   if (d->head_dim == 64)
     hipLaunchKernelGGL(tqk_join_shared<64>, grid, dim3(1024), 0, st, j, p->pi_t, s.pre_splits);

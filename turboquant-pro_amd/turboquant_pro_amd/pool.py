@@ -635,7 +635,8 @@ class TQKVPool:
         self.check()
         self._keep_tables("evict")
         kept = torch.empty((B, keep), dtype=torch.int32, device=weights.device)
-        gone = [max(0, self.n_groups(b) - keep) * self.group_tokens for b in range(B)]
+        W, G = self.hot_window, self.group_tokens
+        gone = [max(0, (n - W - 1) // G + 1 - keep) * G if n > W else 0 for n in self.lengths]
         lib = N.lib()
         with on_device(weights.device):
             need = lib.tqk_evict_groups_workspace_bytes(ctypes.byref(self.desc), B)
