@@ -199,6 +199,8 @@ class TQKVPool:
         self._evicted = [0] * max_batch
         self._evicted_dev = None
         self._made_tables = None
+        # positions of the first tokens of the groups in every slot, once groups were evicted
+        self._slot_starts = None
 
     # ------------------------------------------------------------------ #
     @staticmethod
@@ -234,7 +236,7 @@ class TQKVPool:
         self.lengths = [0] * self.max_batch
         self.seq_lens.zero_()
         self._shared = 0
-        self._evicted, self._evicted_dev = [0] * self.max_batch, None
+        self._evicted, self._evicted_dev, self._slot_starts = [0] * self.max_batch, None, None
         if self._made_tables is not None:
             self.block_table.copy_(self._made_tables[0])
             self.group_table.copy_(self._made_tables[1])
@@ -309,6 +311,9 @@ class TQKVPool:
         new.hot_v.copy_(self.hot_v)
         new.lengths = list(self.lengths)
         new._evicted = list(self._evicted)
+        if self._slot_starts is not None:
+            new._keep_starts()
+            new._slot_starts[sn] = self._slot_starts[so]
         new.seq_lens.copy_(self.seq_lens)
         torch.cuda.synchronize(dev)
         return new
@@ -340,6 +345,9 @@ class TQKVPool:
         n_items = sum(g1 - g0 for g0, g1 in spans)
         L = N.lib()
         st = self._stream()
+        if n_items and self._slot_starts is not None:
+            self._label([(b, g, g * self.group_tokens + self._evicted[b])
+                         for b, (g0, g1) in enumerate(spans) if self._evicted[b] for g in range(g0, g1)])
         if n_items:
             self._overflow.zero_()
         if T > 0 and B <= N.APPEND_SEQS and n_items <= N.APPEND_GROUPS:
@@ -637,6 +645,8 @@ class TQKVPool:
         kept = torch.empty((B, keep), dtype=torch.int32, device=weights.device)
         W, G = self.hot_window, self.group_tokens
         gone = [max(0, (n - W - 1) // G + 1 - keep) * G if n > W else 0 for n in self.lengths]
+        if any(gone):
+            self._keep_starts()
         lib = N.lib()
         with on_device(weights.device):
             need = lib.tqk_evict_groups_workspace_bytes(ctypes.byref(self.desc), B)
@@ -656,6 +666,28 @@ class TQKVPool:
         """Tokens that :meth:`evict` took from every sequence: the next token's position
         is ``lengths[b] + evicted_tokens[b]``."""
         return list(self._evicted)
+
+    def _keep_starts(self) -> None:
+        """Groups' positions go with their slots from here on (a slot keeps its group while
+        the tables are reordered; without evictions a group's is ``g * group_tokens``)."""
+        torch = _torch()
+        if self._slot_starts is None:
+            starts = torch.arange(self.max_groups, dtype=torch.int32, device=self.kcodes.device) * self.group_tokens
+            self._slot_starts = torch.zeros(self.max_batch * self.max_groups, dtype=torch.int32, device=starts.device)
+            self._slot_starts[self.group_table.long()] = starts.expand(self.max_batch, -1)
+
+    def _label(self, groups) -> None:
+        """Positions of groups of sequences that lost tokens: ``[(b, g, position), ...]``."""
+        if groups:
+            x = _torch().tensor(groups, dtype=_torch().int64).pin_memory().to(self.kcodes.device, non_blocking=True)
+            self._slot_starts[self.group_table[x[:, 0], x[:, 1]].long()] = x[:, 2].int()
+
+    def position_start(self, b: int, g: int) -> int:
+        """The position of the first token of sequence b's group g: ``g * group_tokens``
+        unless groups before it were evicted (:meth:`evict`)."""
+        if self._slot_starts is None:
+            return g * self.group_tokens
+        return int(self._slot_starts[self.group_table[b, g].long()])
 
     def share_prefix(self, source: int = 0) -> None:
         """Every other sequence (all of them empty) gets the tokens of ``source``: its
@@ -784,7 +816,7 @@ class TQKVPool:
             return {
                 "kpacked": pack_values(codes, self.key_bits).reshape(-1),
                 "knorms": self.knorm[:, phys, off].contiguous().cpu().numpy(),
-                "position_start": g * G,
+                "position_start": self.position_start(b, g),
                 "vpacked": np.ascontiguousarray(vp).reshape(-1),
                 "vnorms": vn.cpu().numpy(),
             }
@@ -821,7 +853,7 @@ class TQKVPool:
             "nf4_scale": scale,
             "nf4_mean": stored_mean,
             "zp_mode": "calibrated" if self.zero_point == "symmetric" else self.zero_point,
-            "position_start": g * G,
+            "position_start": self.position_start(b, g),
             "outlier_idx": oidx.astype(np.int32),
             "outlier_val": oval,
             "outlier_count": cnt.astype(np.int64),
@@ -923,13 +955,18 @@ class TQKVPool:
             self.vnorm[:, phys, off] = torch.from_numpy(
                 np.asarray(values["vnorms"], np.float32).reshape(H, G)).to(self.device)
 
-    def load_sequence(self, b: int, groups, hot_k, hot_v) -> None:
+    def load_sequence(self, b: int, groups, hot_k, hot_v, evicted_tokens: int | None = None) -> None:
         """Restore sequence ``b`` (empty) from coded groups and hot tokens:
         ``groups`` = ``[(keys, values), ...]`` in :meth:`import_group`'s
         layout, written as they are (no re-encode), then ``hot_k``/``hot_v``
         ``(Hkv, n_hot, D)`` into the hot ring (in the pool's input dtype).  The split must be the
         flush cadence's: ``n_groups_for(len(groups) * G + n_hot)`` is
-        ``len(groups)``."""
+        ``len(groups)``.
+
+        A sequence that groups were evicted from (:meth:`evict`) comes with its
+        ``evicted_tokens``, so that its positions count on, and every group's
+        ``position_start`` in its keys, as :meth:`export_group` gives them; without the
+        number, groups that stand behind tokens which are not here are refused."""
         torch = _torch()
         if self.lengths[b] != 0:
             raise ValueError(f"sequence {b} is not empty")
@@ -941,11 +978,29 @@ class TQKVPool:
         if n_groups_for(L, W) != len(groups) or L > self.max_seq_len:
             raise ValueError(f"{len(groups)} groups + {n_hot} hot tokens is not a state of the "
                              f"flush cadence (hot window {W}, group {G}) within {self.max_seq_len} tokens")
+        starts = [None if keys is None else keys.get("position_start") for keys, _ in groups]
+        gone = 0 if evicted_tokens is None else int(evicted_tokens)
+        if gone < 0 or gone % G or gone + L >= 2 ** 31:
+            raise ValueError(f"evicted_tokens are whole groups of {G} tokens, not {evicted_tokens}")
+        if gone:
+            if self.zero_point == "bias":
+                raise NotImplementedError('load_sequence: the zero points of zero_point="bias" belong to the groups\' positions')
+            if any(x is None for x in starts):
+                raise ValueError("groups of a sequence that lost tokens come with their position_start")
+            starts = [int(x) for x in starts]
+            if any(x % G for x in starts) or any(y <= x for x, y in zip([-1] + starts, starts + [len(groups) * G + gone])):
+                raise ValueError(f"groups at {starts} are not {len(groups)} of the first {len(groups) + gone // G} of a sequence")
+        elif evicted_tokens is None and any(x is not None and int(x) > g * G for g, x in enumerate(starts)):
+            raise ValueError("the groups' positions are those of a sequence that lost tokens: its evicted_tokens are needed")
         for g, (keys, values) in enumerate(groups):
             self.import_group(b, g, keys=keys, values=values)
         if n_hot:
             idx = torch.arange(L - n_hot, L, device=self.device) % W
             self.hot_k[b][:, idx] = hot_k.to(device=self.device, dtype=self.dtype)
             self.hot_v[b][:, idx] = hot_v.to(device=self.device, dtype=self.dtype)
+        if gone:
+            self._keep_starts()
+            self._evicted[b], self._evicted_dev = gone, None
+            self._label([(b, g, x) for g, x in enumerate(starts)])
         self.lengths[b] = L
         self.seq_lens[b] = L
