@@ -552,7 +552,9 @@ int tqk_select_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
  *   kept [batch][keep] i32: the former index of every group that stays, ascending, then -1
  * zero_point 0 and 1 (the "bias" zero points of later groups belong to their positions:
  * TQK_EUNSUPPORTED); hot_ring * 16 bytes within 64 KiB; max_pages_per_seq reaches as
- * far as max_groups_per_seq (else TQK_EINVAL).
+ * far as max_groups_per_seq and the rings are fewer than 2^23 columns (batch * n_kv_heads
+ * * 2 * a row's bytes over those of a column, the most of 128, 64, 32 and 16 that
+ * are within 64 KiB for hot_ring rows; else TQK_EINVAL).
  */
 size_t tqk_evict_groups_workspace_bytes(const tqk_cache_desc* d, int32_t batch);
 

@@ -499,6 +499,10 @@ int ring_columns(const tqk_cache_desc* d) {  // bytes of a column, 0: none fits
     if ((long long)cb * d->hot_ring <= kRingBytes) return cb;
   return 0;
 }
+// Workgroups that turn the rings.
+long long ring_groups(const tqk_cache_desc* d, int batch, int cb) {
+  return (long long)batch * d->n_kv_heads * 2 * (d->head_dim * (d->input_f32 ? 4 : 2) / cb);
+}
 
 }  // namespace
 
@@ -589,6 +593,8 @@ int tqk_evict_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, int32_t b
   if ((long long)d->max_groups_per_seq * (d->group_tokens / d->page_tokens) > d->max_pages_per_seq) return TQK_EINVAL;
   const int cb = ring_columns(d);
   if (!cb) return TQK_EUNSUPPORTED;
+  // (before anything is rewritten)
+  if (ring_groups(d, batch, cb) > INT32_MAX / 256) return TQK_EINVAL;
   if (!batch) return TQK_OK;
   if (!p || !p->hot_k || !p->hot_v || !weights || !seq_lens || !block_table || !group_table || (keep > 0 && !kept))
     return TQK_EINVAL;
@@ -628,9 +634,7 @@ int tqk_evict_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, int32_t b
   r.row_bytes = d->head_dim * (d->input_f32 ? 4 : 2);
   r.cb = cb;
   r.heads = d->n_kv_heads;
-  const long long groups = (long long)batch * d->n_kv_heads * 2 * (r.row_bytes / cb);
-  if (groups > INT32_MAX / 256) return TQK_EINVAL;
-  hipLaunchKernelGGL(tqk_rotate_ring, dim3((unsigned)groups), dim3(256), 0, st, r);
+  hipLaunchKernelGGL(tqk_rotate_ring, dim3((unsigned)ring_groups(d, batch, cb)), dim3(256), 0, st, r);
   return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
 }
 
