@@ -470,7 +470,7 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
  * whose decode reads every group (turboquant_pro/kv_kernel.py:319-381).
  */
 typedef struct tqk_group_list {
-  int32_t n;          /* entries of a list */
+  int32_t n;          /* entries of a list, at most 2^24 */
   int64_t stride[3];  /* entries between sequences, kv heads and queries */
 } tqk_group_list;
 
@@ -526,7 +526,7 @@ typedef struct tqk_select_desc {
   int32_t batch;
   int32_t q_len;
   int32_t max_len;
-  int32_t top;    /* at least 1 */
+  int32_t top;    /* 1 to 2^24 */
   int32_t first;  /* first + last <= top */
   int32_t last;
   float spread;
@@ -550,6 +550,7 @@ int tqk_select_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
  *   block_table, group_table  the cache's own (p->block_table, p->group_table), rewritten
  *   seq_lens [batch] i32, rewritten;  weights [batch][n_kv_heads][max_groups_per_seq] fp32, rewritten
  *   kept [batch][keep] i32: the former index of every group that stays, ascending, then -1
+ *        (keep is at most 2^24)
  * zero_point 0 and 1 (the "bias" zero points of later groups belong to their positions:
  * TQK_EUNSUPPORTED); hot_ring * 16 bytes within 64 KiB; max_pages_per_seq reaches as
  * far as max_groups_per_seq and the rings are fewer than 2^23 columns (batch * n_kv_heads

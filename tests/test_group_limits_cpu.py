@@ -26,3 +26,10 @@ def test_more_rings_than_a_launch_are_refused_first(heads, ring, columns):
     for batch, want in ((min(most, 65535), "EWORKSPACE"), (most + 1, "EINVAL")):
         c = Call(cache)
         assert c.evict(batch=batch)[1] == getattr(c.N, "TQK_" + want), batch
+
+
+@pytest.mark.parametrize("n,want", [(1 << 24, "EWORKSPACE"), ((1 << 24) + 1, "EINVAL"), (2 ** 31 - 1, "EINVAL")])
+def test_lists_past_their_counters_are_refused(n, want):
+    """A thread's next place in a list of nearly 2^31 entries would pass 32 bits."""
+    c = Call()
+    assert c.select(top=n)[1] == c.evict(keep=n)[1] == getattr(c.N, "TQK_" + want)

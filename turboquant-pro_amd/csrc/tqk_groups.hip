@@ -457,6 +457,7 @@ __global__ __launch_bounds__(256) void tqk_rotate_ring(RingArgs a) {
 }
 
 // ---- plans and checks ---------------------------------------------------------
+constexpr int kMostListed = 1 << 24;  // entries of a list (its places are counted in 32 bits)
 constexpr long long kMostScoreBytes = (long long)256 << 20;  // scores at a time: more queries go in slices
 
 int check_select(const tqk_cache_desc* d, const tqk_select_desc* s) {
@@ -470,7 +471,7 @@ int check_select(const tqk_cache_desc* d, const tqk_select_desc* s) {
   const int rc = tqk_check_attend(d, &t);
   if (rc != TQK_OK) return rc;
   if (d->input_f32 || d->key_grid == 2) return TQK_EUNSUPPORTED;
-  if (s->top < 1 || s->first < 0 || s->last < 0 || (long long)s->first + s->last > s->top) return TQK_EINVAL;
+  if (s->top < 1 || s->top > kMostListed || s->first < 0 || s->last < 0 || (long long)s->first + s->last > s->top) return TQK_EINVAL;
   if (!(s->spread >= 0.f) || s->spread > 3.0e38f) return TQK_EINVAL;
   return TQK_OK;
 }
@@ -588,7 +589,7 @@ int tqk_evict_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, int32_t b
   const int rc = tqk_check_desc(d);
   if (rc != TQK_OK) return rc;
   if (d->zero_point == 2) return TQK_EUNSUPPORTED;
-  if (batch < 0 || batch > 65535 || keep < 0 || first < 0 || last < 0 || (long long)first + last > keep) return TQK_EINVAL;
+  if (batch < 0 || batch > 65535 || keep < 0 || keep > kMostListed || first < 0 || last < 0 || (long long)first + last > keep) return TQK_EINVAL;
   // (a sequence as long as its groups' table has its pages)
   if ((long long)d->max_groups_per_seq * (d->group_tokens / d->page_tokens) > d->max_pages_per_seq) return TQK_EINVAL;
   const int cb = ring_columns(d);

@@ -632,6 +632,8 @@ class TQKVPool:
         first = max(first, self._shared)
         if keep < first + last:
             raise ValueError(f"evict keeps the first {first} and the last {last} groups: keep is at least that, not {keep}")
+        if keep > 2 ** 24:
+            raise ValueError(f"evict keeps at most {2 ** 24} groups of a sequence, not {keep}")
         if tuple(weights.shape) != (B, self.n_kv_heads, self.max_groups) or weights.dtype != torch.float32 or \
                 not weights.is_contiguous():
             raise ValueError(f"weights are contiguous fp32 ({B}, {self.n_kv_heads}, {self.max_groups}), not "
