@@ -520,7 +520,9 @@ int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
  * product with the levels' centre.  In 64 bits; a score that is no number ranks above
  * all, equal ones by the lower index.
  *   groups [batch][n_kv_heads][q_len][top] i32, ascending, then -1
- * fp16 caches with per-channel keys (key_grid 0 or 1).  No counterpart in the reference.
+ * fp16 caches with per-channel keys (key_grid 0 or 1), however many queries; batch *
+ * n_kv_heads fewer than 2^21, and times the groups of the longest sequence over 16
+ * fewer than 2^23 (else TQK_EINVAL).  No counterpart in the reference.
  */
 typedef struct tqk_select_desc {
   int32_t batch;

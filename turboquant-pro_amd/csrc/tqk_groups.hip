@@ -458,7 +458,12 @@ __global__ __launch_bounds__(256) void tqk_rotate_ring(RingArgs a) {
 
 // ---- plans and checks ---------------------------------------------------------
 constexpr int kMostListed = 1 << 24;  // entries of a list (its places are counted in 32 bits)
-constexpr long long kMostScoreBytes = (long long)256 << 20;  // scores at a time: more queries go in slices
+// Scores and workgroups of a launch: more queries go in slices.
+constexpr long long kMostScoreBytes = (long long)256 << 20, kMostRows = INT32_MAX / 1024, kMostScoreGroups = INT32_MAX / 256;
+
+long long score_chunks(const tqk_cache_desc* d, int max_len) {
+  return (n_groups_of(max_len, d->hot_window, d->group_tokens) + kScoreGroups - 1) / kScoreGroups;
+}
 
 int check_select(const tqk_cache_desc* d, const tqk_select_desc* s) {
   if (!s) return TQK_EINVAL;
@@ -473,6 +478,8 @@ int check_select(const tqk_cache_desc* d, const tqk_select_desc* s) {
   if (d->input_f32 || d->key_grid == 2) return TQK_EUNSUPPORTED;
   if (s->top < 1 || s->top > kMostListed || s->first < 0 || s->last < 0 || (long long)s->first + s->last > s->top) return TQK_EINVAL;
   if (!(s->spread >= 0.f) || s->spread > 3.0e38f) return TQK_EINVAL;
+  const long long pairs = (long long)s->batch * d->n_kv_heads;  // (a launch has at least one query of each)
+  if (pairs > kMostRows || pairs * score_chunks(d, s->max_len) > kMostScoreGroups) return TQK_EINVAL;
   return TQK_OK;
 }
 
@@ -483,8 +490,9 @@ struct SelectPlan {
 SelectPlan select_plan(const tqk_cache_desc* d, const tqk_select_desc* s) {
   SelectPlan sp{};
   sp.most = n_groups_of(s->max_len, d->hot_window, d->group_tokens);
-  const long long one = (long long)s->batch * d->n_kv_heads * sp.most * 8;
+  const long long pairs = (long long)s->batch * d->n_kv_heads, one = pairs * sp.most * 8;
   long long fit = one ? kMostScoreBytes / one : s->q_len;
+  fit = fit < kMostRows / pairs ? fit : kMostRows / pairs;
   fit = fit < 1 ? 1 : fit;
   sp.t_len = fit < s->q_len ? (int)fit : s->q_len;
   sp.ws_bytes = (size_t)one * sp.t_len + 16;
@@ -541,8 +549,7 @@ int tqk_select_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   a.last = s->last;
   a.spread = s->spread;
   a.most = sp.most;
-  const long long pairs = (long long)s->batch * d->n_kv_heads, chunks = (sp.most + kScoreGroups - 1) / kScoreGroups;
-  if (pairs * chunks > INT32_MAX / 256 || pairs * sp.t_len > INT32_MAX / 1024) return TQK_EINVAL;
+  const long long pairs = (long long)s->batch * d->n_kv_heads, chunks = score_chunks(d, s->max_len);
   if (sp.most <= kTogether && s->q_len * (d->n_q_heads / d->n_kv_heads) <= kTogetherRows) {
     const dim3 grid((unsigned)pairs);
     if (d->head_dim == 64)
