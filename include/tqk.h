@@ -466,8 +466,9 @@ int tqk_attend(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atten
  * [0, groups of the sequence) are none; a group listed twice counts twice.
  *   groups [batch][n_kv_heads][q_len][n] i32 by the list's strides, entries side by
  *   side; a query stride of 0: one list for all queries of a (sequence, kv head)
- * fp16 caches, over the codes however many queries.  No counterpart in the reference,
- * whose decode reads every group (turboquant_pro/kv_kernel.py:319-381).
+ * fp16 caches, over the codes however many queries (batch * n_q_heads * q_len up to
+ * 2^30 rows, batch * n_kv_heads up to 2^22; else TQK_EINVAL).  No counterpart in the
+ * reference, whose decode reads every group (turboquant_pro/kv_kernel.py:319-381).
  */
 typedef struct tqk_group_list {
   int32_t n;          /* entries of a list, at most 2^24 */
@@ -485,10 +486,11 @@ int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
  * tqk_attend that keeps account of the groups' weight: weights[b][h][g] += the softmax
  * weights of group g's tokens, summed over the sequence's queries and kv head h's query
  * heads.
- *   weights [batch][n_kv_heads][max_groups_per_seq] fp32 (batch * n_kv_heads at most 65535)
+ *   weights [batch][n_kv_heads][max_groups_per_seq] fp32 (batch * n_kv_heads at most 65535,
+ *           and times the longest sequence's coded blocks of 32 tokens over 256 fewer than 2^23)
  *           (read and written without atomics: calls that add to it do not overlap)
- * fp16 caches, over the codes however many queries; 256 MiB of blocks' sums at a time
- * beside the partial results.
+ * fp16 caches, over the codes however many queries (up to 2^30 rows); 256 MiB of blocks'
+ * sums at a time beside the partial results.
  */
 size_t tqk_attend_weights_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t);
 
@@ -501,7 +503,9 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
  * groups are the same pages and slots in every sequence's tables: they are read
  * through the first sequence's, once for all (or, where the batch is too small for
  * that to be faster, as by tqk_attend).  Every query sees them whole (p is at least
- * groups * group_tokens - 1).  fp16 caches with per-channel keys (key_grid 0 or 1).
+ * groups * group_tokens - 1).  fp16 caches with per-channel keys (key_grid 0 or 1); steps
+ * of few queries: more workgroups than one launch takes (2^22, of 8 to 128 rows) are
+ * refused (TQK_EINVAL).
  */
 size_t tqk_attend_shared_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups);
 

@@ -56,3 +56,28 @@ def test_choices_for_any_batch_up_to_a_launch(heads, batch, max_len, want):
     c = Call({**MANY, "n_kv_heads": heads, "n_q_heads": heads})
     need, rc = c.select(batch=batch, max_len=max_len)
     assert rc == getattr(c.N, "TQK_" + want) and (need > 0) == (want == "EWORKSPACE")
+
+
+def test_weights_of_more_rows_than_a_launch():
+    """Short caches, many queries: slices of 2^22 workgroups (one query of 8 heads each), one split."""
+    cache = {**MANY, "n_kv_heads": 8, "n_q_heads": 64}
+    for batch, q_len, slice_ in ((2048, 512, 256), (1024, 512, 512), (1024, 513, 512), (3, 512, 512)):
+        c = Call(cache, dict(batch=batch, q_len=q_len, max_len=512))
+        need, rc = c.weights()
+        assert rc == c.N.TQK_EWORKSPACE
+        # (a split's sums of 130 floats a row; blocks: none)
+        assert need == 256 + batch * 64 * slice_ * 130 * 4 * (1 if batch > 3 else (need - 256) // (batch * 64 * slice_ * 520))
+
+
+@pytest.mark.parametrize("kind", ["groups", "weights", "shared"])
+@pytest.mark.parametrize("batch,q_len,heads", [(1 << 22, 1, 2), (1 << 20, 2, 8), (4096, 256, 8), (1 << 19, 1, 8), (1 << 13, 7, 8),
+                                               (1024, 512, 8), (65535, 60, 1), (1 << 16, 1, 1), (64, 1 << 17, 1)])
+def test_a_workspace_is_given_where_the_call_is_taken(kind, batch, q_len, heads):
+    c = Call({**MANY, "n_kv_heads": heads, "n_q_heads": heads * 8}, dict(batch=batch, q_len=q_len))
+    need, rc = getattr(c, kind)()
+    assert (need > 0) == (rc == c.N.TQK_EWORKSPACE) and rc in (c.N.TQK_EWORKSPACE, c.N.TQK_EINVAL)
+    rows, pairs = batch * heads * 8 * q_len, batch * heads
+    if kind == "groups":
+        assert (need > 0) == (rows < 2 ** 30 and pairs <= 2 ** 22)
+    elif kind == "weights":
+        assert (need > 0) == (rows < 2 ** 30 and pairs <= 65535)

@@ -897,6 +897,7 @@ struct FewPlan {
   size_t ws_bytes;
 };
 
+constexpr long long kMostFewGroups = 1LL << 22;  // workgroups of a launch (512 threads each: fewer than 2^32)
 FewPlan few_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   FewPlan fp{};
   const int gq = d->n_q_heads / d->n_kv_heads;
@@ -953,6 +954,7 @@ void launch_few(const FewArgs& a, dim3 grid, hipStream_t st) {
 }  // namespace
 
 size_t tqk_few_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) { return few_plan(d, t).ws_bytes; }
+bool tqk_few_fits(const tqk_cache_desc* d, const tqk_attend_desc* t) { return few_plan(d, t).groups <= kMostFewGroups; }
 
 int tqk_run_few(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
                 const int32_t* seq_lens, const int32_t* q_lens, void* out, void* workspace, size_t workspace_bytes,
@@ -960,7 +962,7 @@ int tqk_run_few(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_atte
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const FewPlan fp = few_plan(d, t);
   if (workspace_bytes < fp.ws_bytes) return TQK_EWORKSPACE;
-  if (fp.groups > (1LL << 22)) return TQK_EINVAL;  // (512 threads each: fewer than 2^32)
+  if (fp.groups > kMostFewGroups) return TQK_EINVAL;
   FewArgs a{};
   a.d = *d;
   a.p = *p;

@@ -418,11 +418,18 @@ void launch_rows(MoreArgs a, long long groups, hipStream_t st) {
 
 size_t partial_bytes(long long rows, int splits, int D) { return (size_t)splits * rows * (D + 2) * sizeof(float) + 256; }
 
+constexpr long long kMostGroups = 1LL << 22;  // workgroups of a launch (512 threads each: fewer than 2^32)
+
 // Queries, kv heads and sequences of a launch, and its splits.
 struct MorePlan {
   int per_item, q_items, n_splits;
   long long pairs;  // workgroups of a split
 };
+// Queries of a launch, `per_item` of them a workgroup: more go in slices.
+int launch_queries(const tqk_cache_desc* d, const tqk_attend_desc* t, int per_item) {
+  const long long fit = kMostGroups / ((long long)t->batch * d->n_kv_heads) * per_item;
+  return fit < t->q_len ? (int)fit : t->q_len;
+}
 MorePlan more_plan(const tqk_cache_desc* d, long long batch, int queries, int most_per_item, long long tokens, double join) {
   MorePlan mp{};
   const int gq = d->n_q_heads / d->n_kv_heads;
@@ -431,6 +438,7 @@ MorePlan more_plan(const tqk_cache_desc* d, long long batch, int queries, int mo
   mp.q_items = (queries + mp.per_item - 1) / mp.per_item;
   mp.pairs = batch * mp.q_items * d->n_kv_heads;
   mp.n_splits = few_splits(mp.pairs, (tokens + 31) / 32 + 1, join);
+  if (mp.pairs * mp.n_splits > kMostGroups && mp.n_splits > 1) mp.n_splits = mp.pairs < kMostGroups ? (int)(kMostGroups / mp.pairs) : 1;
   return mp;
 }
 
@@ -497,27 +505,30 @@ int check_more(const tqk_cache_desc* d, const tqk_attend_desc* t, bool windowed)
   if (d->input_f32) return TQK_EUNSUPPORTED;
   if (!windowed && (t->window || t->sinks)) return TQK_EINVAL;
   if ((long long)t->batch * d->n_q_heads * t->q_len > INT32_MAX / 2) return TQK_EINVAL;
+  if ((long long)t->batch * d->n_kv_heads > kMostGroups) return TQK_EINVAL;  // (a launch has a query of each)
   return TQK_OK;
 }
-constexpr long long kMostGroups = 1LL << 22;  // (512 threads each: fewer than 2^32)
 
-// All rows of a call in one launch, and the join of its splits.
-size_t item_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const MorePlan& mp) {
-  return mp.n_splits > 1 ? partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, mp.n_splits, d->head_dim) : 16;
+// The rows of t_len queries at a time (mp: the plan of so many), and the join of their splits.
+size_t item_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const MorePlan& mp, int t_len) {
+  return mp.n_splits > 1 ? partial_bytes((long long)t->batch * d->n_q_heads * t_len, mp.n_splits, d->head_dim) : 16;
 }
-int run_items(MoreArgs a, const MorePlan& mp, void* workspace, void* stream) {
-  if (mp.pairs * mp.n_splits > kMostGroups) return TQK_EINVAL;
+int run_items(MoreArgs a, const MorePlan& mp, int t_len, void* workspace, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   a.per_item = mp.per_item;
-  a.q_items = mp.q_items;
   a.n_splits = mp.n_splits;
   a.direct = mp.n_splits == 1;
-  a.rows = (long long)a.batch * a.d.n_q_heads * a.q_len;
   a.part_acc = static_cast<float*>(workspace);
-  a.part_ml = a.part_acc + (size_t)mp.n_splits * a.rows * a.d.head_dim;
-  launch_rows(a, mp.pairs * mp.n_splits, st);
-  if (!a.direct) launch_join(join_args(a, mp.n_splits), nullptr, 0, a.d.head_dim, st);
-  return hipGetLastError() == hipSuccess ? TQK_OK : TQK_EHIP;
+  for (a.t0 = 0; a.t0 < a.q_len; a.t0 += t_len) {
+    a.t_len = a.q_len - a.t0 < t_len ? a.q_len - a.t0 : t_len;
+    a.q_items = (a.t_len + a.per_item - 1) / a.per_item;
+    a.rows = (long long)a.batch * a.d.n_q_heads * a.t_len;
+    a.part_ml = a.part_acc + (size_t)mp.n_splits * a.rows * a.d.head_dim;
+    launch_rows(a, (long long)a.batch * a.q_items * a.d.n_kv_heads * a.n_splits, st);
+    if (!a.direct) launch_join(join_args(a, mp.n_splits), nullptr, 0, a.d.head_dim, st);
+    if (hipGetLastError() != hipSuccess) return TQK_EHIP;
+  }
+  return TQK_OK;
 }
 
 // ---- listed groups ----------------------------------------------------------
@@ -527,12 +538,18 @@ int check_list(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_grou
   if (!l || l->n < 0 || l->n > (1 << 24)) return TQK_EINVAL;
   return TQK_OK;
 }
-MorePlan list_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
+struct ListPlan {
+  int t_len;  // queries of a slice
+  MorePlan mp;
+};
+ListPlan list_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
   const int G = d->group_tokens, nblk = (G + 31) / 32;
   const long long groups = n_groups_of(t->max_len, d->hot_window, G);
   const long long listed = l->n < groups ? l->n : groups;  // (more: of one twice)
   const long long hot = t->max_len < d->hot_window ? t->max_len : d->hot_window;
-  return more_plan(d, t->batch, t->q_len, l->stride[2] ? 1 : INT32_MAX, 32 * listed * nblk + hot, 2.0);
+  const int most = l->stride[2] ? 1 : INT32_MAX;  // (a list a query: a workgroup each)
+  const int t_len = launch_queries(d, t, l->stride[2] ? 1 : 8 / (d->n_q_heads / d->n_kv_heads));
+  return ListPlan{t_len, more_plan(d, t->batch, t_len, most, 32 * listed * nblk + hot, 2.0)};
 }
 
 // ---- weights ----------------------------------------------------------------
@@ -548,12 +565,24 @@ WeightPlan weight_plan(const tqk_cache_desc* d, const tqk_attend_desc* t) {
   const long long one = (long long)t->batch * d->n_q_heads * w.blocks * 8;  // bytes of a query
   long long fit = one ? kMostBlockBytes / one : t->q_len;
   fit = fit < 1 ? 1 : fit;
-  w.t_len = fit < t->q_len ? (int)fit : t->q_len;
+  const int gq = d->n_q_heads / d->n_kv_heads, per = 8 / gq, most = launch_queries(d, t, per);
+  w.t_len = fit < most ? (int)fit : most;
   // (whole workgroups where a slice ends)
-  const int gq = d->n_q_heads / d->n_kv_heads, per = 8 / gq;
   if (w.t_len < t->q_len && w.t_len > per) w.t_len = w.t_len / per * per;
   w.mp = more_plan(d, t->batch, w.t_len, INT32_MAX, window_tokens(t, per), 0.0);
   return w;
+}
+int weight_chunks(const tqk_cache_desc* d, const tqk_attend_desc* t) {  // workgroups of a (sequence, kv head)'s sums
+  const int nblk = (d->group_tokens + 31) / 32, per = 256 / nblk;
+  return (n_groups_of(t->max_len, d->hot_window, d->group_tokens) + per - 1) / per;
+}
+int check_weights(const tqk_cache_desc* d, const tqk_attend_desc* t) {
+  const int rc = check_more(d, t, true);
+  if (rc != TQK_OK) return rc;
+  const long long pairs = (long long)t->batch * d->n_kv_heads;
+  // (and the join's workgroups: fewer than 2^24)
+  if (pairs > 65535 || pairs * weight_chunks(d, t) >= 1 << 23) return TQK_EINVAL;
+  return TQK_OK;
 }
 size_t weight_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const WeightPlan& w) {
   const long long rows = (long long)t->batch * d->n_q_heads * w.t_len;
@@ -600,6 +629,10 @@ SharedPlan shared_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, int gr
   s.rest = more_plan(d, t->batch, t->q_len, INT32_MAX, t->max_len - (s.once ? tokens : 0), s.once ? 0.0 : 2.0);
   return s;
 }
+bool shared_fits(const tqk_cache_desc* d, const tqk_attend_desc* t, const SharedPlan& s) {
+  if (!s.once && s.rest.q_items > 1) return tqk_few_fits(d, t);
+  return s.pre_pairs * s.pre_splits <= kMostGroups && s.rest.pairs * s.rest.n_splits <= kMostGroups;
+}
 int check_shared(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
   const int rc = check_more(d, t, false);
   if (rc != TQK_OK) return rc;
@@ -614,8 +647,8 @@ extern "C" {
 
 size_t tqk_attend_groups_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, const tqk_group_list* l) {
   if (check_list(d, t, l) != TQK_OK || !t->batch || !t->q_len) return 0;
-  const MorePlan mp = list_plan(d, t, l);
-  return item_bytes(d, t, mp);
+  const ListPlan lp = list_plan(d, t, l);
+  return item_bytes(d, t, lp.mp, lp.t_len);
 }
 
 int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t,
@@ -633,30 +666,28 @@ int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   a.groups = groups ? groups : reinterpret_cast<const int32_t*>(seq_lens);
   for (int i = 0; i < 3; ++i) a.g_stride[i] = l->stride[i];
   a.n_list = l->n;
-  return run_items(a, list_plan(d, t, l), workspace, stream);
+  const ListPlan lp = list_plan(d, t, l);
+  return run_items(a, lp.mp, lp.t_len, workspace, stream);
 }
 
 size_t tqk_attend_weights_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t) {
-  if (check_more(d, t, true) != TQK_OK || !t->batch || !t->q_len) return 0;
+  if (check_weights(d, t) != TQK_OK || !t->batch || !t->q_len) return 0;
   return weight_bytes(d, t, weight_plan(d, t));
 }
 
 int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tqk_attend_desc* t, const void* q,
                        const int32_t* seq_lens, const int32_t* q_lens, void* out, float* weights, void* workspace,
                        size_t workspace_bytes, void* stream) {
-  int rc = check_more(d, t, true);
+  int rc = check_weights(d, t);
   if (rc != TQK_OK) return rc;
   if (!t->batch || !t->q_len) return TQK_OK;
   rc = checked(d, p, t, q, seq_lens, out, workspace);
   if (rc != TQK_OK) return rc;
-  if (!weights || (long long)t->batch * d->n_kv_heads > 65535) return TQK_EINVAL;
+  if (!weights) return TQK_EINVAL;
   const WeightPlan w = weight_plan(d, t);
   if (workspace_bytes < weight_bytes(d, t, w)) return TQK_EWORKSPACE;
-  if (w.mp.pairs * w.mp.n_splits > kMostGroups) return TQK_EINVAL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const int nblk = (d->group_tokens + 31) / 32, per = 256 / nblk, ng = w.blocks / nblk;
-  const int chunks = (ng + per - 1) / per;
-  if ((long long)chunks * t->batch * d->n_kv_heads >= 1 << 23) return TQK_EINVAL;  // (and the join's: fewer than 2^24)
+  const int nblk = (d->group_tokens + 31) / 32, chunks = weight_chunks(d, t);
   MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
   a.per_item = w.mp.per_item;
   a.n_splits = w.mp.n_splits;
@@ -689,7 +720,8 @@ int tqk_attend_weights(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const t
 size_t tqk_attend_shared_workspace_bytes(const tqk_cache_desc* d, const tqk_attend_desc* t, int32_t groups) {
   if (check_shared(d, t, groups) != TQK_OK || !t->batch || !t->q_len) return 0;
   const SharedPlan s = shared_plan(d, t, groups);
-  if (!s.once) return s.rest.q_items > 1 ? tqk_few_workspace_bytes(d, t) : item_bytes(d, t, s.rest);
+  if (!shared_fits(d, t, s)) return 0;
+  if (!s.once) return s.rest.q_items > 1 ? tqk_few_workspace_bytes(d, t) : item_bytes(d, t, s.rest, t->q_len);
   return partial_bytes((long long)t->batch * d->n_q_heads * t->q_len, s.pre_splits + s.rest.n_splits, d->head_dim);
 }
 
@@ -701,13 +733,13 @@ int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
   if (!t->batch || !t->q_len) return TQK_OK;
   rc = checked(d, p, t, q, seq_lens, out, workspace);
   if (rc != TQK_OK) return rc;
-  if (workspace_bytes < tqk_attend_shared_workspace_bytes(d, t, groups)) return TQK_EWORKSPACE;
   const SharedPlan s = shared_plan(d, t, groups);
+  if (!shared_fits(d, t, s)) return TQK_EINVAL;
+  if (workspace_bytes < tqk_attend_shared_workspace_bytes(d, t, groups)) return TQK_EWORKSPACE;
   if (!s.once) {  // (more than eight rows: sixteen a workgroup)
     if (s.rest.q_items > 1) return tqk_run_few(d, p, t, q, seq_lens, q_lens, out, workspace, workspace_bytes, stream);
-    return run_items(more_args(d, p, t, q, seq_lens, q_lens, out), s.rest, workspace, stream);
+    return run_items(more_args(d, p, t, q, seq_lens, q_lens, out), s.rest, t->q_len, workspace, stream);
   }
-  if (s.pre_pairs * s.pre_splits > kMostGroups || s.rest.pairs * s.rest.n_splits > kMostGroups) return TQK_EINVAL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int splits = s.pre_splits + s.rest.n_splits;
   MoreArgs a = more_args(d, p, t, q, seq_lens, q_lens, out);
