@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from attn_ref import visible  # noqa: E402
-from more_ref import cached, check_rows, listed, make_pool, queries  # noqa: E402
+from more_ref import cached, check_rows, listed, make_pool, queries, tokens  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,76 @@ def test_weights_of_more_rows_than_a_launch():
         for h in (0, H - 1):
             s = slice(5 * h, 5 * h + 5)
             check_rows(out[b, s], q[b, s], k[h], v[h], sees, f"seq {b} head {h}")
+
+
+def ringed(ring, lens, Hq, H, D, room, **kw):
+    """A pool whose rings are longer than the hot window."""
+    import ctypes
+
+    from turboquant_pro_amd import TQKVPool
+    pool = TQKVPool(n_kv_heads=H, n_q_heads=Hq, head_dim=D, max_batch=len(lens), max_seq_len=max(lens) + room, seed=3, **kw)
+    pool.hot_k, pool.hot_v = (torch.full((len(lens), H, ring, D), 7.0, dtype=pool.dtype, device="cuda") for _ in range(2))
+    pool.ptrs.hot_k, pool.ptrs.hot_v, pool.desc.hot_ring = pool.hot_k.data_ptr(), pool.hot_v.data_ptr(), ring
+    assert pool.ptrs.hot_k == ctypes.c_void_p(pool.hot_k.data_ptr()).value
+    k, v = tokens(3, len(lens), H, max(lens), D, pool.dtype)
+    pool.append(k, v, n_new=lens)
+    pool.check()
+    return pool
+
+
+@pytest.mark.parametrize("ring,D,form", [(512, 128, dict()), (513, 128, dict()), (1024, 64, dict()), (2048, 128, dict()),
+                                         (4096, 128, dict()), (4095, 64, dict()), (4096, 256, dict(input_dtype="float32")),
+                                         (100, 64, dict(hot_window=64))])
+def test_evictions_turn_rings_of_any_length(ring, D, form):
+    """Columns of 128 to 16 bytes: the cache after evictions and appends as with a ring of
+    the hot window's size."""
+    print(f"[limits] ring {ring} D={D} {form}", flush=True)
+    lens, H = [2900, 1500, 40], 2
+    one, two = ringed(ring, lens, 2 * H, H, D, 1500, **form), make_pool(3, lens, 2 * H, H, D, room=1500, **form)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    for step in range(3):
+        weights = torch.rand((3, H, one.max_groups), generator=gen, device="cuda")
+        other = weights.clone()
+        keep = (9, 5, 3)[step]
+        assert torch.equal(one.evict(weights, keep), two.evict(other, keep))
+        assert torch.equal(weights, other) and one.lengths == two.lengths
+        for i in range(2):
+            for b, (x, y) in enumerate(zip(zip(*one.dense()), zip(*two.dense()))):
+                n = one.lengths[b]
+                assert torch.equal(x[0][:, :n], y[0][:, :n]) and torch.equal(x[1][:, :n], y[1][:, :n]), f"step {step} seq {b}"
+            q = queries(step, one, 1)
+            assert torch.equal(one.attend(q), two.attend(q))
+            k, v = tokens(20 + step, 3, H, 400, D, one.dtype)
+            one.append(k, v, n_new=[400, 37, 1])
+            two.append(k, v, n_new=[400, 37, 1])
+
+
+@pytest.mark.parametrize("D,Hq,H,form", [(128, 8, 2, dict()), (64, 4, 4, dict(hot_window=64)), (256, 7, 1, dict(value_bits=4))])
+def test_infinite_values_of_uncoded_tokens(D, Hq, H, form):
+    """Their channel of the rows that see them, however small their weight is; a row that
+    does not see them, and every other number, stays as it is."""
+    print(f"[limits] infinities D={D} {Hq}/{H}", flush=True)
+    pool, gq, T = make_pool(10, [1500, 700], Hq, H, D, **form), Hq // H, 3
+    q = queries(11, pool, T)
+    q[..., 3] = 1.0
+    groups = pool.select_groups(q, 2)
+    b, h, token = 1, H - 1, pool.lengths[1] - 2  # (the first query stands before it)
+    at = token % pool.hot_window
+    pool.hot_k[b, h, at] = 0.0
+    pool.hot_k[b, h, at, 3] = -60000.0
+    pool.hot_v[b, h, at, 11] = 0.0
+
+    def runs():
+        w = torch.zeros((2, H, pool.max_groups), device="cuda")
+        return [pool.attend(q, groups=groups), pool.attend(q, weights=w), pool.attend(q, window=9, sinks=3, weights=w)], w
+
+    want, weights = runs()
+    for x in (float("inf"), float("-inf"), float("nan")):
+        pool.hot_v[b, h, at, 11] = x
+        got, w = runs()
+        assert torch.equal(w, weights)
+        for y, was in zip(got, want):
+            rows = y[b, h * gq:(h + 1) * gq, 1:, 11].clone()
+            assert bool((rows.isnan() if x != x else rows == x).all())
+            y[b, h * gq:(h + 1) * gq, 1:, 11] = was[b, h * gq:(h + 1) * gq, 1:, 11]
+            assert torch.equal(y, was)
