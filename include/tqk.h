@@ -519,9 +519,9 @@ int tqk_attend_shared(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
  * for candidates the c groups with a token j <= p.  All of them where c <= top; else
  * the first `first` and last `last` ones and those of the largest
  *   score = max over the kv head's query heads of sum_i q_i mid_i + spread |q_i| half_i
- * where mid +- half are the ends of channel i's key levels in the group (a side-list's
- * values may lie outside): at spread 1 a bound on the products with its keys, at 0 the
- * product with the levels' centre.  In 64 bits; a score that is no number ranks above
+ * where mid +- half are the ends of channel i's key levels in the group (the encode's
+ * reach over every value, a side-list's too; another writer's need not): at spread 1 a
+ * bound on the products with its keys, at 0 the product with the levels' centre.  In 64 bits; a score that is no number ranks above
  * all, equal ones by the lower index.
  *   groups [batch][n_kv_heads][q_len][top] i32, ascending, then -1
  * fp16 caches with per-channel keys (key_grid 0 or 1), however many queries; batch *

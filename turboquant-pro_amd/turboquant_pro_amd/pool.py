@@ -561,9 +561,9 @@ class TQKVPool:
         ``q`` and ``q_lens`` as for :meth:`attend`.  Of the groups that begin at or
         before a query the ``first`` and ``last`` ones are always chosen, and those with
         the largest ``max over the kv head's query heads of sum_i q_i mid_i + spread
-        |q_i| half_i``, ``mid +- half`` the ends of channel i's key levels in the group
-        (a side-list's values may lie outside).  ``spread=1``: a bound on the products
-        with its keys; 0: the product with the levels' centre.  Only the groups' scales
+        |q_i| half_i``, ``mid +- half`` the ends of channel i's key levels in the group,
+        which reach over all its values, a side-list's among them (only an imported
+        group's may lie outside).  ``spread=1``: a bound on the products with its keys; 0: the product with the levels' centre.  Only the groups' scales
         and zero points are read; 64 bits, equal scores by the lower index, a score
         that is no number above all.  fp16 pools with per-channel keys."""
         torch = _torch()
