@@ -14,8 +14,14 @@
 // A shared prefix: rows of all sequences over one copy of its codes, then each
 // sequence's rows over its other tokens; one join takes both.
 //
-// The joins are latency: 4 to 5 us a launch, the chain lengths -> partial results ->
-// output.
+// The joins are latency, the chain lengths -> partial results -> output: 4 to 5 us a
+// launch, 6 to 8 with the groups' weights (their chain is one longer), 9 for a shared
+// prefix (the rotation).  In launches of their own, so that nothing has to be zero
+// before a call; an arrival counter a row would save part of that.
+//
+// An ordinary tqk_attend step stays with tqk_attend_codes, whose outputs it has had;
+// up to eight rows tqk_attend_rows is faster (32 / 8 heads of 128, 16 sequences of 32768
+// tokens: 175 for 189 us) and closer, and more rows go sixteen a workgroup there.
 #include "tqk_attend_few.h"
 
 namespace {
@@ -599,10 +605,13 @@ struct SharedPlan {
 // Whether reading the prefix once pays: it takes launches of its own and a set-up, about
 // 28 us, and 3.2 a tile of its workgroups; each sequence for itself finds the others'
 // codes in cache, a block of 32 tokens and 8 rows 1.0 ns of the whole card (0.7 at
-// head_dim 64, 4 at 256; 16 rows of tqk_run_few a fifth more).  Each for itself and once,
-// us, 32 / 8 heads of 128: a prefix of 32768 tokens, 4 sequences 46 and 87, 8 73 and 88,
-// 32 near 300 and 108; 4096 tokens, 64 sequences 84 and 78; 2048 tokens, 32 sequences 29
-// and 54; head_dim 256, 16 / 8 heads, 4096 tokens, 4 sequences 44 and 79, 16 81 and 79.
+// head_dim 64, 4 at 256; 16 rows of tqk_run_few a fifth more, whose weights are single
+// fp16 numbers, 2.9e-4 of the result for 2.1e-4).  Each for itself and once, us, 32 / 8
+// heads of 128: a prefix of 32768 tokens, 4 sequences 46 and 87, 8 73 and 88, 32 near
+// 300 and 108; 4096 tokens, 64 sequences 84 and 78; 2048 tokens, 32 sequences 29 and 54;
+// head_dim 256, 16 / 8 heads, 4096 tokens, 4 sequences 44 and 79, 16 81 and 79.
+// (Measured with 3- and 4-bit values, 4-bit keys and a side-list of 2 %: other forms of
+// the cache are taken to cost the same.)
 SharedPlan shared_plan(const tqk_cache_desc* d, const tqk_attend_desc* t, int groups) {
   SharedPlan s{};
   const int gq = d->n_q_heads / d->n_kv_heads, tokens = groups * d->group_tokens, cus = device_cus();

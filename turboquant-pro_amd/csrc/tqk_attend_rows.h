@@ -22,8 +22,11 @@
 // What bounds it: a block's chain (look-ups of levels -> products -> exponentials ->
 // look-ups of centroids -> products) at two waves a SIMD, 256 registers each; three or
 // four waves spill 190 to 320 registers (313 us for 190).  Measured, 32 / 8 heads of 128:
-// 16 sequences of 32768 tokens, every group's weight kept, 171 us (3.2 TB/s; with the
-// pages in cache some 20 less, without the blocks' sums 10 less); 16 groups of 127
+// 16 sequences of 32768 tokens, every group's weight kept, 175 us (3.2 TB/s; with the
+// pages in cache some 20 less, without the blocks' sums 10 less): the waves wait 48 % of
+// their cycles, vector issue half of the time, LDS 32 %, the matrix cores 14 %
+// (tqk_decode_split_mfma over the same cache, one query: 135 us, a fifth fewer vector
+// instructions, 33 % waiting); 16 groups of 127
 // listed, ten blocks a wave, 34 us; 64 of 511 of one sequence, three blocks a wave, 20
 // us; one block a wave 14.5.  Of a short run some 9 us are set-up (lengths -> list ->
 // tables -> codes, one load after another; the tables and the group's weights meanwhile)

@@ -13,7 +13,7 @@
 // All of them are chains of a few dependent loads and of the search's counts, not
 // bytes.  Measured: 127 groups of 16 sequences and 8 heads (16.6 MB of levels) chosen in
 // 11 us by one launch; 511 groups of one sequence 5 and 8 us; an eviction from the same
-// 16 sequences 7.7, their rings (134 MB moved) 10.
+// 16 sequences 8, their rings (33.5 MB, read and written) 10.
 #include "tqk_attend.h"
 #include "tqk_wave.h"
 

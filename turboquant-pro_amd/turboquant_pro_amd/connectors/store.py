@@ -157,8 +157,8 @@ class TurboQuantBlockStore:
 
     def save_sequence(self, request_id: str, layer_name: str, keys: Any, values: Any,
                       group_tokens: int, hot_window: int) -> int:
-        """Store one sequence's layer K/V ``(H, L, D)`` the way a paged pool
-        holds it: one record per coded group of the flush cadence
+        """Store one sequence's layer K/V ``(H, L, D)``, from its first token on,
+        the way a paged pool holds it: one record per coded group of the flush cadence
         (``<layer>#g<i>``, ``group_tokens`` tokens each, so each is exactly the
         pool's group) and the hot window as it is (``<layer>#hot0``, a
         :class:`RawTokens` payload: fp16 for fp16 K/V, fp32 otherwise, the
