@@ -138,3 +138,22 @@ def test_a_whole_sequence_is_restored_as_ever():
             assert other.evicted_tokens == [0] and starts(other, 0) == starts(pool, 0)
             for x, y in zip(cached(pool, 0), cached(other, 0)):
                 assert torch.equal(x, y)
+
+
+def test_inference_mode():
+    """Evictions and shares inside of it, appends, exports and resets outside."""
+    print("[positions] inference mode", flush=True)
+    pool = make_pool(9, [0, 2600], 4, 2, room=1500)
+    with torch.inference_mode():
+        want = evicted(pool, [[], [g * 256 for g in range(pool.n_groups(1))]], 1, 4)
+        pool.share_prefix(1)
+    want = grow(pool, [want[1]] * 2, 3, [700, 300])
+    assert [starts(pool, b) for b in range(2)] == want
+    q = queries(1, pool, 1)
+    with torch.inference_mode():
+        got = pool.attend(q)
+        want = grow(pool, want, 4, [300, 700])
+    assert torch.isfinite(got).all() and [starts(pool, b) for b in range(2)] == want
+    assert torch.isfinite(grown_out := pool.grown(9000).attend(q)).all() and grown_out.shape == got.shape
+    pool.reset()
+    assert pool.lengths == [0, 0]

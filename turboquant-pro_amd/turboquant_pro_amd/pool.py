@@ -674,9 +674,10 @@ class TQKVPool:
         the tables are reordered; without evictions a group's is ``g * group_tokens``)."""
         torch = _torch()
         if self._slot_starts is None:
-            starts = torch.arange(self.max_groups, dtype=torch.int32, device=self.kcodes.device) * self.group_tokens
-            self._slot_starts = torch.zeros(self.max_batch * self.max_groups, dtype=torch.int32, device=starts.device)
-            self._slot_starts[self.group_table.long()] = starts.expand(self.max_batch, -1)
+            with torch.inference_mode(False):  # (an append outside of it writes there too)
+                starts = torch.arange(self.max_groups, dtype=torch.int32, device=self.kcodes.device) * self.group_tokens
+                self._slot_starts = torch.zeros(self.max_batch * self.max_groups, dtype=torch.int32, device=starts.device)
+                self._slot_starts[self.group_table.long()] = starts.expand(self.max_batch, -1)
 
     def _label(self, groups) -> None:
         """Positions of groups of sequences that lost tokens: ``[(b, g, position), ...]``."""
