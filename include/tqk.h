@@ -485,7 +485,7 @@ int tqk_attend_groups(const tqk_cache_desc* d, const tqk_cache_ptrs* p, const tq
 /*
  * tqk_attend that keeps account of the groups' weight: weights[b][h][g] += the softmax
  * weights of group g's tokens, summed over the sequence's queries and kv head h's query
- * heads.
+ * heads (what they received while they were uncoded is not in it).
  *   weights [batch][n_kv_heads][max_groups_per_seq] fp32 (batch * n_kv_heads at most 65535,
  *           and times the longest sequence's coded blocks of 32 tokens over 256 fewer than 2^23)
  *           (read and written without atomics: calls that add to it do not overlap)

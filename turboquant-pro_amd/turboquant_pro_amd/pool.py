@@ -468,8 +468,9 @@ class TQKVPool:
 
         ``weights`` (fp32 ``(B, Hkv, max_groups)``, contiguous) is added to: the
         softmax weights of every coded group's tokens, summed over the queries and
-        the kv head's query heads (what :meth:`evict` goes by).  Calls that add to one
-        tensor go one after another.  Both of them fp16 pools, over the codes however
+        the kv head's query heads (what :meth:`evict` goes by; what tokens received before
+        their group was coded is not counted).  Calls that add to one tensor go one after
+        another.  Both of them fp16 pools, over the codes however
         many queries.
 
         After :meth:`share_prefix`, steps of few queries without a window read the
@@ -613,7 +614,8 @@ class TQKVPool:
 
         ``weights`` (fp32 ``(B, Hkv, max_groups)``, as ``attend(weights=...)`` adds it
         up): a group's is its sum over the heads, in 64 bits; equal ones by the lower
-        index, a sum that is no number above all.  The weights move along with their
+        index, a sum that is no number above all.  (A group coded lately has had few steps
+        to add to its weight: ``last`` keeps those coded since the last call.)  The weights move along with their
         groups, the rest become zero.  No code moves: the sequences' table rows are
         reordered, their lengths shortened and their rings turned; the freed pages take
         the sequence's next groups.  A shared prefix stays whole.
